@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define KITTY_ABI_VERSION 7
+#define KITTY_ABI_VERSION 8
 
 /* Element type of 16-bit data (the *_dtype fields below). */
 #define KITTY_DTYPE_F16 0
@@ -510,6 +510,113 @@ typedef struct {
 
 int kitty_channel_scores(const kitty_score_layer *layers, int32_t n, int32_t num_kv_heads, int32_t head_dim,
                          int32_t d_boost, int32_t sentinel, float *scores, uint8_t *boost_idx, kitty_stream_t stream);
+
+/* ------------------------------------------------------ 8-bit paged cache
+ * Pages of page_tokens tokens of one sequence, all KV heads, in 8 bits (ABI
+ * version 8; no counterpart in the reference, whose only cache is the 2-bit
+ * one).  Code c (e4m3: 4 exponent and 3 mantissa bits, no infinities, 0x7f and
+ * 0xff NaN) of page p, head h stands for c * scale[p, h, s], s = 0 for keys and
+ * 1 for values; any finite positive float scale is read, kitty_cache8_write
+ * makes powers of two.  Strides are in elements: bytes for the codes (multiples
+ * of 16, the channel stride 1, bases 16-byte aligned), floats for the scales
+ * (even, the two streams next to each other, base 8-byte aligned). */
+typedef struct {
+    uint8_t *key;   /* (P, H, G, D); the pools may be NULL where P is 0 */
+    uint8_t *value; /* (P, H, G, D) */
+    float *scale;   /* (P, H, 2) */
+    int64_t key_s_page, key_s_head, key_s_tok;
+    int64_t value_s_page, value_s_head, value_s_tok;
+    int64_t scale_s_page, scale_s_head;
+    int64_t num_pages;    /* ids outside [0, num_pages) are never dereferenced */
+    int32_t num_kv_heads; /* H */
+    int32_t head_dim;     /* D: a multiple of 16, 16 to 256 */
+    int32_t page_tokens;  /* G: 16, 32, 64, 128 or 256 */
+} kitty_cache8;
+
+#define KITTY_SRC_F16 0  /* element types of the 16- and 32-bit side of the cache */
+#define KITTY_SRC_BF16 1
+#define KITTY_SRC_F32 2
+
+/* Quantises tokens as they are written: row t < lens[b] (all `tokens` rows where
+ * lens is NULL) of key and value becomes token start[b] + t of sequence b, in
+ * row (start[b] + t) % G of page block_table[b * bt_stride + (start[b] + t) / G].
+ * Per page, head and stream with m the largest finite |x| of its new rows:
+ *   need   = the smallest power of two >= 2^-64 with m <= 448 * need
+ *   scale' = max(scale, need) where the page holds tokens before start[b], else need
+ *   new codes = e4m3(x / scale'), NaN and infinities -> NaN
+ *   codes of its tokens before start[b] = e4m3(code * scale / scale') where scale' != scale
+ * (e4m3: nearest, ties to even; exact quotients where the scales are powers of
+ * two).  Rows behind the last new one keep their bytes, pages without a new row
+ * their scales.  Not written: tokens of a sequence whose start is negative, and
+ * tokens whose page number is table_pages or more or whose page id is outside
+ * the pool.  A page named for two sequences of one call, both of which write to
+ * it, holds a mixture of the two. */
+typedef struct {
+    const void *key, *value; /* (B, H, tokens, D), channel stride 1 */
+    int64_t key_s_seq, key_s_head, key_s_tok, value_s_seq, value_s_head, value_s_tok;
+    const int32_t *block_table; /* (B, table_pages) page ids */
+    int64_t bt_stride;
+    const int32_t *start;    /* (B,) tokens each sequence holds before the call */
+    const int32_t *lens;     /* (B,) rows of each sequence, clamped to [0, tokens]; NULL: tokens */
+    int32_t batch, tokens, table_pages;
+    int32_t src_dtype;       /* KITTY_SRC_*: key and value */
+} kitty_cache8_write_args;
+
+int kitty_cache8_write(const kitty_cache8 *cache, const kitty_cache8_write_args *args, kitty_stream_t stream);
+
+/* Reads tokens back: row t < tokens of key and value becomes token start[b] + t
+ * of sequence b (start NULL: from 0), code * scale in fp32 rounded once to
+ * out_dtype; 0 where start[b] + t >= lens[b], NaN where the token has no page
+ * (a negative position, a page number >= table_pages, an id outside the pool). */
+typedef struct {
+    void *key, *value;       /* (B, H, tokens, D), channel stride 1, 16-byte aligned rows */
+    int64_t key_s_seq, key_s_head, key_s_tok, value_s_seq, value_s_head, value_s_tok;
+    const int32_t *block_table;
+    int64_t bt_stride;
+    const int32_t *start;    /* (B,) or NULL */
+    const int32_t *lens;     /* (B,) tokens of each sequence in the cache */
+    int32_t batch, tokens, table_pages;
+    int32_t out_dtype;       /* KITTY_SRC_* */
+} kitty_cache8_read_args;
+
+int kitty_cache8_read(const kitty_cache8 *cache, const kitty_cache8_read_args *args, kitty_stream_t stream);
+
+/* Attention over the cache: for query row i < q_lens[b] (tokens where NULL) of
+ * head h, whose keys and values are head h / (num_q_heads / H)'s,
+ *   out[b, h, i] = sum_j softmax_j(q[b, h, i] . k_j * sm_scale) v_j
+ * over the tokens j < lens[b] of sequence b; with causal, row i is token
+ * lens[b] - q_lens[b] + i and sees j up to itself.  lse (optional) receives
+ * log sum_j exp(score_j) in fp32.  Rows that see nothing, and rows i >=
+ * q_lens[b], are 0 with lse -infinity.  A sequence whose lens is negative or
+ * more than table_pages pages hold, or whose q_lens is outside [0, tokens],
+ * gives NaN rows, and so does a page id outside the pool to the rows that see
+ * one of its tokens; masked tokens, whatever they hold, reach no row.
+ * Scores, softmax and sums are fp32, the 8-bit codes enter their products
+ * exactly, weights in two bf16 terms (16 bits); |q . code| must stay finite.
+ * block_table entries behind a sequence's last page are not read.
+ * plan_tokens: what the caller knows of the largest lens[b] (0: table_pages *
+ * G); it only chooses how the work is split, results differ by rounding.
+ * Calls may overlap on different streams given workspaces of their own. */
+typedef struct {
+    const uint16_t *q; /* (B, Hq, T, D), 16-byte aligned rows */
+    uint16_t *out;     /* (B, Hq, T, D), 16-byte aligned rows, q's type */
+    float *lse;        /* (B, Hq, T) contiguous, or NULL */
+    int64_t q_s_seq, q_s_head, q_s_tok, o_s_seq, o_s_head, o_s_tok;
+    const int32_t *block_table;
+    int64_t bt_stride;
+    const int32_t *lens;   /* (B,) tokens in the cache, those of the queries included */
+    const int32_t *q_lens; /* (B,) or NULL */
+    int32_t batch, num_q_heads, tokens, table_pages, plan_tokens;
+    int32_t causal;
+    int32_t dtype;         /* KITTY_DTYPE_F16 or KITTY_DTYPE_BF16: q and out */
+    float sm_scale;
+    void *workspace;       /* kitty_cache8_attention_workspace_size bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} kitty_cache8_attention_args;
+
+int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
+                                          size_t *bytes);
+int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, kitty_stream_t stream);
 
 #ifdef __cplusplus
 }

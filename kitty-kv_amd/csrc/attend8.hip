@@ -1,0 +1,627 @@
+// Attention of few query rows over the 8-bit paged cache, on gfx950: the
+// decode step, and the few tokens of a draft.
+//
+// Bound by HBM: every code is read once for all the query rows of its KV head
+// (head of the group fastest, up to 16 RT rows), at two bytes per token and
+// channel.  The work of a batch is its (sequence, KV head) pairs in units of
+// 128 tokens, cut into equal runs of units for the workgroups by lengths read
+// on the device, so ragged batches stay even.  A workgroup's four waves take 32
+// tokens of a unit each, independently (codes HBM -> registers, one step
+// ahead), and join in LDS at the end of a pair's run; runs that are not the
+// whole of a pair leave a partial that cache8_merge_kernel joins.
+//
+//  S^T = K Q^T, 16x16x32 MFMAs: A row = token, reduction slot (g, j) of step
+//  2c + u = channel 64c + 16g + 8u + j, so a lane reads 16 contiguous codes per
+//  64 channels, widened to q's type (exact).  Lane (n = query l & 15, g = l / 16)
+//  ends with its query's scores of tokens 4g .. 4g + 3 of each 16-token half.
+//  O^T += V^T P^T: the scores' registers are the B operand as they stand, slot
+//  8g + e standing for token 4g + e (e < 4) of the first half, 4g + e - 4 of the
+//  second.  A lane reads those eight tokens' rows at D / 16 contiguous channels,
+//  so A row m of product dt is channel (D / 16) m + dt, and a byte permute
+//  pairs two tokens' codes before they are widened to bf16.
+//
+// Scales: the key's is a factor of the scores, the value's of the weights,
+// which go in two bf16 terms: 16 bits with fp32's range, where a page's scale
+// may be anything.  The running maximum is raised only when a score passes it
+// by 2^8.
+#include <algorithm>
+
+#include "attend8.h"
+
+namespace kitty {
+
+constexpr int kWaves = 4;
+
+template <int DP, int RT>
+struct RowBuf {
+    u32x4 k[2][DP / 64];
+    unsigned v[8][DP / 64];
+    float2 sc[2];
+};
+
+template <int DP, int RT>
+struct RowState {
+    u32x4 q[RT][DP / 32];
+    f32x4 o[RT][DP / 16];
+    float m[RT], l[RT];
+    int vis[RT];
+};
+
+// Max and sum over the four lanes of one query (16 apart).
+__device__ __forceinline__ float quad_max(float v)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    v = fmaxf(__builtin_bit_cast(float, (int)a[0]), __builtin_bit_cast(float, (int)a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (int)b[0]), __builtin_bit_cast(float, (int)b[1]));
+}
+__device__ __forceinline__ float quad_sum(float v)
+{
+    const auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    v = __builtin_bit_cast(float, (int)a[0]) + __builtin_bit_cast(float, (int)a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    return __builtin_bit_cast(float, (int)b[0]) + __builtin_bit_cast(float, (int)b[1]);
+}
+
+// Value operand of product dt: the lane's eight tokens at channel dt of its
+// D / 16, each byte picked by (tokens 2e, 2e + 1) pairs and widened.
+template <int DP>
+__device__ __forceinline__ u32x4 value_operand(const unsigned (&v)[8][DP / 64], int dt)
+{
+    u32x4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const unsigned a = v[2 * e][dt >> 2], b = v[2 * e + 1][dt >> 2];
+        // bytes (a.c, b.c, a.c + 1, b.c + 1) with c = dt & 2; both channels of the pair share the permute
+        const unsigned w = __builtin_amdgcn_perm(b, a, dt & 2 ? 0x07030602u : 0x05010400u);
+        r[e] = dt & 1 ? widen<true, true>(w) : widen<true, false>(w);
+    }
+    return r;
+}
+
+// 32 tokens from `tok` on, in `buf`, folded into the wave's rows.  MASK: some
+// row may not see all of them.
+template <int DP, int RT, bool BF16, bool MASK>
+__device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &buf, int tok, int vis_max, float cs, int g)
+{
+    f32x4 S[RT][2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+            S[rt][hf] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const unsigned w0 = buf.k[hf][c][2 * u], w1 = buf.k[hf][c][2 * u + 1];
+                const u32x4 a = {widen<BF16, false>(w0), widen<BF16, true>(w0), widen<BF16, false>(w1), widen<BF16, true>(w1)};
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    S[rt][hf] = mfma16<BF16>(a, W.q[rt][2 * c + u], S[rt][hf]);
+            }
+    }
+    // a token's row in the registers: half e / 4, token 4g + e % 4 of it
+    bool odd = false;
+    if constexpr (MASK) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
+#pragma unroll
+            for (int w = 0; w < DP / 64; ++w) {
+                buf.v[e][w] = t < vis_max ? buf.v[e][w] : 0;   // rows no query sees hold anything
+                odd |= nan_codes(buf.v[e][w]) != 0;
+            }
+        }
+        odd = __ballot(odd) != 0;
+    }
+    u32x4 hi[RT], lo[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        float s[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            s[e] = S[rt][e >> 2][e & 3] * (cs * buf.sc[e >> 2].x);
+            if constexpr (MASK)
+                s[e] = tok + 16 * (e >> 2) + 4 * g + (e & 3) < W.vis[rt] ? s[e] : -__builtin_inff();
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e)
+            mx = fmaxf(mx, s[e]);
+        if (__ballot(mx > W.m[rt] + 8.0f)) {
+            mx = quad_max(mx);
+            const float mn = mx > W.m[rt] + 8.0f ? mx : W.m[rt], alpha = __builtin_amdgcn_exp2f(W.m[rt] - mn);
+            W.m[rt] = mn;
+            W.l[rt] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt)
+                W.o[rt][dt] *= alpha;
+        }
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            s[e] = __builtin_amdgcn_exp2f(s[e] - W.m[rt]);
+            sum += s[e];
+            s[e] *= buf.sc[e >> 2].y;
+        }
+        W.l[rt] += sum;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            unsigned h, l;
+            split_bf16(s[2 * e], s[2 * e + 1], h, l);
+            hi[rt][e] = h, lo[rt][e] = l;
+        }
+    }
+    if (MASK && odd) {
+        // NaN values that not every row sees: count them by row and channel
+        // (products of 0 / 1), give those rows NaN and take them out of the codes.
+        unsigned ind[8][DP / 64];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int w = 0; w < DP / 64; ++w) {
+                const unsigned nn = nan_codes(buf.v[e][w]), byte = (nn >> 7) * 0xffu;
+                ind[e][w] = byte & 0x38383838u;   // 1.0
+                buf.v[e][w] &= ~byte;
+            }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            u32x4 see;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int t = tok + 16 * (e >> 1) + 4 * g + 2 * (e & 1);
+                see[e] = (t < W.vis[rt] ? 0x3f80u : 0u) | (t + 1 < W.vis[rt] ? 0x3f800000u : 0u);
+            }
+#pragma unroll
+            for (int dt = 0; dt < DP / 16; ++dt) {
+                const f32x4 cnt = mfma16<true>(value_operand<DP>(ind, dt), see, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    W.o[rt][dt][i] = cnt[i] > 0.0f ? __builtin_nanf("") : W.o[rt][dt][i];
+            }
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; ++dt) {
+        const u32x4 vf = value_operand<DP>(buf.v, dt);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            W.o[rt][dt] = mfma16<true>(vf, hi[rt], W.o[rt][dt]);
+            W.o[rt][dt] = mfma16<true>(vf, lo[rt], W.o[rt][dt]);
+        }
+    }
+}
+
+// Units of sequence b for one (KV head, row block).
+__device__ __forceinline__ int units8(const Attend8 &p, int b)
+{
+    const Seq8 s = seq8(p, b);
+    return s.bad ? 0 : (s.n + kUnit - 1) / kUnit;
+}
+
+// CUT: D is below DP, and the lanes beyond it read nothing.
+template <int DP, int RT, bool BF16, bool CUT>
+__global__ __launch_bounds__(64 * kWaves, DP <= 128 && RT == 1 ? 2 : 1) void cache8_rows_kernel(Attend8 p)
+{
+    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4;
+    __shared__ __attribute__((aligned(16))) float lds_o[kWaves][RM][LD];
+    __shared__ float2 lds_ml[kWaves][RM];
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int per_seq = p.c.H * p.nrb;
+
+    // this workgroup's run [u, u1) of all units, and the sequence it starts in
+    int total = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        int x = b0 + lane < p.B ? units8(p, b0 + lane) : 0;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1)
+            x += __shfl_xor(x, off);
+        total += x * per_seq;
+    }
+    total = __builtin_amdgcn_readfirstlane(total);
+    const int N = min(p.n_wg, total), wg = blockIdx.x;
+    if (wg >= N)
+        return;
+    auto start_of = [&](int w) { return (int)((int64_t)w * total / N); };
+    int u = start_of(wg);
+    const int u0 = u, u1 = start_of(wg + 1);
+    int b = 0, pre = 0;     // first unit of sequence b
+    for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
+        const int x = b0 + lane < p.B ? units8(p, b0 + lane) * per_seq : 0;
+        int inc = x;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(inc, off);
+            inc += lane >= off ? y : 0;
+        }
+        const unsigned long long past = __ballot(base + inc > u);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            b = b0 + l;
+            pre = base + __shfl(inc - x, l);
+            break;
+        }
+        base += __shfl(inc, 63);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    pre = __builtin_amdgcn_readfirstlane(pre);
+
+    while (u < u1) {
+        const Seq8 sq = seq8(p, b);
+        const int nt = units8(p, b);
+        if (u >= pre + nt * per_seq) {
+            pre += nt * per_seq;
+            ++b;
+            continue;
+        }
+        const int item = (u - pre) / nt, tile = (u - pre) - item * nt, tile1 = min(nt, tile + (u1 - u));
+        const int kh = item / p.nrb, rb = item - kh * p.nrb, r0 = rb * RM;
+        const int t_lo = r0 / p.gq, t_hi = min((r0 + RM - 1) / p.gq, sq.tq - 1);   // query tokens of the block
+        const int vis_min = visible8(p, sq, t_lo), vis_max = t_hi < t_lo ? 0 : visible8(p, sq, t_hi);
+        const int end = min(tile1 * kUnit, vis_max);
+
+        RowState<DP, RT> W;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int r = r0 + 16 * rt + n, t = r / p.gq, h = kh * p.gq + r - t * p.gq;
+            W.vis[rt] = visible8(p, sq, t);
+            W.m[rt] = kLowest;
+            W.l[rt] = 0.0f;
+            const uint16_t *q = p.q + b * p.q_s_seq + h * p.q_s_head + t * p.q_s_tok;
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                const int ch = 64 * (c >> 1) + 16 * g + 8 * (c & 1);
+                W.q[rt][c] = u32x4{0, 0, 0, 0};
+                if (t < sq.tq && (!CUT || ch < p.c.D))
+                    W.q[rt][c] = *(const u32x4 *)(q + ch);
+            }
+#pragma unroll
+            for (int dt = 0; dt < CB; ++dt)
+                W.o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        const int32_t *table = p.table + b * p.bt_stride;
+        const int last = (sq.n - 1) >> p.c.lg, lg = p.c.lg;
+        const uint8_t *kp = p.c.key + kh * p.c.key_s_head, *vp = p.c.value + kh * p.c.value_s_head;
+        const float *sp = p.c.scale + kh * p.c.scale_s_head;
+        const uint32_t k_lane = (uint32_t)n * p.c.key_s_tok + 16 * g;
+        const uint32_t v_ch = CUT && CB * n >= p.c.D ? 0 : CB * n;
+        const uint32_t v_lane = (uint32_t)(4 * g) * p.c.value_s_tok + v_ch;
+        auto ids = [&](int tok, int (&id)[2]) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+                id[hf] = table[min((tok + 16 * hf) >> lg, last)];
+        };
+        auto load = [&](int tok, const int (&id)[2], RowBuf<DP, RT> &buf) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const bool bad = bad_page(p.c, id[hf]);
+                const int64_t page = bad ? 0 : id[hf];
+                const uint32_t row = (uint32_t)(tok + 16 * hf) & ((1u << lg) - 1);
+                const uint8_t *k = kp + page * p.c.key_s_page + (row * p.c.key_s_tok + k_lane);
+#pragma unroll
+                for (int c = 0; c < DP / 64; ++c)
+                    buf.k[hf][c] = CUT && 64 * c + 16 * g >= p.c.D ? u32x4{0, 0, 0, 0} : *(const u32x4 *)(k + 64 * c);
+                const uint8_t *v = vp + page * p.c.value_s_page + (row * p.c.value_s_tok + v_lane);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint8_t *src = v + (uint32_t)e * p.c.value_s_tok;
+                    unsigned(&d)[DP / 64] = buf.v[4 * hf + e];
+                    if constexpr (DP == 64) {
+                        d[0] = *(const unsigned *)src;
+                    } else if constexpr (DP == 128) {
+                        const uint2 x = *(const uint2 *)src;
+                        d[0] = x.x, d[1] = x.y;
+                    } else {
+                        const u32x4 x = *(const u32x4 *)src;
+                        d[0] = x[0], d[1] = x[1], d[2] = x[2], d[3] = x[3];
+                    }
+                }
+                buf.sc[hf] = *(const float2 *)(sp + page * p.c.scale_s_page);
+                if (bad)
+                    buf.sc[hf].x = __builtin_nanf("");
+            }
+        };
+        auto step = [&](int tok, RowBuf<DP, RT> &buf) {
+            if (tok + 32 <= vis_min)
+                row_step<DP, RT, BF16, false>(W, buf, tok, vis_max, p.cs, g);
+            else
+                row_step<DP, RT, BF16, true>(W, buf, tok, vis_max, p.cs, g);
+        };
+        int tok = tile * kUnit + 32 * wave;
+        if (tok < end) {
+            RowBuf<DP, RT> a, c;
+            int id[2];
+            ids(tok, id);
+            load(tok, id, a);
+            ids(tok + kUnit, id);
+            while (true) {
+                if (tok + kUnit < end) {
+                    load(tok + kUnit, id, c);
+                    ids(tok + 2 * kUnit, id);
+                }
+                step(tok, a);
+                if ((tok += kUnit) >= end)
+                    break;
+                if (tok + kUnit < end) {
+                    load(tok + kUnit, id, a);
+                    ids(tok + 2 * kUnit, id);
+                }
+                step(tok, c);
+                if ((tok += kUnit) >= end)
+                    break;
+            }
+        }
+
+        // the waves' rows joined
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const float l = quad_sum(W.l[rt]);
+            if (g == 0)
+                lds_ml[wave][16 * rt + n] = make_float2(W.m[rt], l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int d4 = 0; d4 < CB / 4; ++d4)
+                    *(float4 *)&lds_o[wave][16 * rt + n][CB * (4 * g + i) + 4 * d4] =
+                        make_float4(W.o[rt][4 * d4][i], W.o[rt][4 * d4 + 1][i], W.o[rt][4 * d4 + 2][i], W.o[rt][4 * d4 + 3][i]);
+        }
+        __syncthreads();
+        const bool whole = tile == 0 && tile1 == nt;
+        const int slot = 2 * wg + (u == u0 ? 0 : 1), rows = min(RM, p.gq * p.T - r0);
+        if (tile == 0 && threadIdx.x == 0) {
+            const int64_t last_unit = (int64_t)u + nt;   // one past the item's last
+            p.ws_tab[b * per_seq + item] = whole ? make_int2(-1, 0) : make_int2(slot, (int)((last_unit * N - 1) / total));
+        }
+        for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * kWaves) {
+            const int r = i / (DP / 4), ch = 4 * (i - r * (DP / 4));
+            float m = kLowest, l = 0.0f;
+            float2 ml[kWaves];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                ml[w] = lds_ml[w][r];
+                m = fmaxf(m, ml[w].x);
+            }
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float f = __builtin_amdgcn_exp2f(ml[w].x - m);
+                const float4 x = *(const float4 *)&lds_o[w][r][ch];
+                l += f * ml[w].y;
+                acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+            }
+            if (!whole) {
+                *(float4 *)(p.ws_o + ((int64_t)slot * RM + r) * DP + ch) = acc;
+                if (ch == 0)
+                    p.ws_ml[slot * RM + r] = make_float2(m, l);
+                continue;
+            }
+            const int t = (r0 + r) / p.gq, h = kh * p.gq + (r0 + r) - t * p.gq;
+            const bool none = visible8(p, sq, t) == 0;
+            const float inv = none ? 0.0f : 1.0f / l;
+            if (!CUT || ch < p.c.D)
+                *(uint2 *)(p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok + ch) =
+                    make_uint2((uint32_t)f2x(acc.x * inv, BF16) | (uint32_t)f2x(acc.y * inv, BF16) << 16,
+                               (uint32_t)f2x(acc.z * inv, BF16) | (uint32_t)f2x(acc.w * inv, BF16) << 16);
+            if (ch == 0 && p.lse)
+                p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
+        }
+        __syncthreads();
+        u += tile1 - tile;
+    }
+}
+
+// Joins the partials of one row; also the rows no workgroup touched: of
+// sequences without tokens (0) and of broken lengths (NaN).
+template <int DP, bool BF16>
+__global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, int RM)
+{
+    constexpr int CPL = DP / 64;   // channels per lane
+    __shared__ float lds_o[kWaves][DP];
+    __shared__ float2 lds_ml[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int rows = p.gq * p.T, pair = blockIdx.x / rows, row = blockIdx.x - pair * rows;
+    const int b = pair / p.c.H, kh = pair - b * p.c.H, rb = row / RM, r = row - rb * RM;
+    const int t = row / p.gq, h = kh * p.gq + row - t * p.gq;
+    const Seq8 sq = seq8(p, b);
+    float m = kLowest, l = 0.0f, o[CPL];
+#pragma unroll
+    for (int e = 0; e < CPL; ++e)
+        o[e] = sq.bad ? __builtin_nanf("") : 0.0f;
+    if (sq.bad)
+        m = l = __builtin_nanf("");
+    else if (sq.n > 0) {
+        const int2 tab = p.ws_tab[pair * p.nrb + rb];
+        if (tab.x < 0)
+            return;
+        const int first = tab.x >> 1, count = tab.y - first + 1;
+        auto slot = [&](int i) { return (int64_t)(i == 0 ? tab.x : 2 * (first + i)) * RM + r; };
+        for (int i = wave; i < count; i += 4 * kWaves) {
+            float2 ml[4];
+            float x[4][CPL];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t s = slot(min(i + j * kWaves, count - 1));
+                ml[j] = p.ws_ml[s];
+#pragma unroll
+                for (int e = 0; e < CPL; ++e)
+                    x[j][e] = p.ws_o[s * DP + CPL * lane + e];
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (i + j * kWaves >= count)
+                    break;
+                const float mn = fmaxf(m, ml[j].x);
+                const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml[j].x - mn);
+                m = mn;
+                l = f0 * l + f1 * ml[j].y;
+#pragma unroll
+                for (int e = 0; e < CPL; ++e)
+                    o[e] = f0 * o[e] + f1 * x[j][e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < CPL; ++e)
+        lds_o[wave][CPL * lane + e] = o[e];
+    if (lane == 0)
+        lds_ml[wave] = make_float2(m, l);
+    __syncthreads();
+    const bool none = !sq.bad && visible8(p, sq, t) == 0;
+    const int ch = threadIdx.x;
+    if (ch >= p.c.D)
+        return;
+    float M = kLowest, L = 0.0f, acc = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w)
+        M = fmaxf(M, lds_ml[w].x);
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f(lds_ml[w].x - M);
+        L += f * lds_ml[w].y;
+        acc += f * lds_o[w][ch];
+    }
+    p.out[b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok + ch] = f2x(none ? 0.0f : acc / L, BF16);
+    if (ch == 0 && p.lse)
+        p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (M + __builtin_log2f(L)) / kLog2e;
+}
+
+static int device_cus()
+{
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+        cus = 256;
+    return cus;
+}
+
+static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+struct Plan8 {
+    int DP, RT, nrb, n_wg;
+    size_t o_bytes, ml_bytes, bytes;
+};
+
+static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &pl)
+{
+    const int64_t rows = (int64_t)a.num_q_heads / c.H * a.tokens;
+    pl.DP = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
+    pl.RT = rows <= 16 ? 1 : 2;
+    const int RM = 16 * pl.RT;
+    const int64_t nrb = (rows + RM - 1) / RM;
+    const int64_t items = (int64_t)a.batch * c.H * nrb;
+    const int64_t units = (((int64_t)a.table_pages << c.lg) + kUnit - 1) / kUnit;
+    if (rows > kMaxBlocks || (int64_t)a.batch * c.H * rows > kMaxBlocks || items * std::max<int64_t>(units, 1) > 0x7fffffff)
+        return fail(KITTY_E_UNSUPPORTED, "too many rows or pages for one launch");
+    pl.nrb = (int)nrb;
+    pl.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus(), items * units));
+    pl.o_bytes = up16((size_t)2 * pl.n_wg * RM * pl.DP * 4);
+    pl.ml_bytes = up16((size_t)2 * pl.n_wg * RM * 8);
+    pl.bytes = pl.o_bytes + pl.ml_bytes + up16((size_t)items * 8);
+    return KITTY_OK;
+}
+
+static int check_attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, Cache8 &c)
+{
+    if (!args)
+        return fail(KITTY_E_INVALID, "args is NULL");
+    if (const int rc = check_cache8(cache, c))
+        return rc;
+    const kitty_cache8_attention_args &a = *args;
+    if (a.batch < 0 || a.tokens < 0 || a.table_pages < 0 || a.plan_tokens < 0)
+        return fail(KITTY_E_INVALID, "batch, tokens, table_pages and plan_tokens must not be negative");
+    if (a.num_q_heads <= 0 || a.num_q_heads % c.H)
+        return fail(KITTY_E_INVALID, "num_q_heads must be a positive multiple of num_kv_heads");
+    if (a.dtype != KITTY_DTYPE_F16 && a.dtype != KITTY_DTYPE_BF16)
+        return fail(KITTY_E_INVALID, "dtype must be KITTY_DTYPE_F16 or KITTY_DTYPE_BF16");
+    if (!(a.sm_scale > 0.0f) || a.sm_scale > 1e30f)
+        return fail(KITTY_E_INVALID, "sm_scale must be positive and finite");
+    if ((int64_t)a.table_pages << c.lg > 0x7fffffff)
+        return fail(KITTY_E_UNSUPPORTED, "a sequence is limited to 2^31 - 1 tokens");
+    return KITTY_OK;
+}
+
+} // namespace kitty
+
+using namespace kitty;
+
+extern "C" int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
+                                                     size_t *bytes)
+{
+    Cache8 c;
+    Plan8 pl;
+    if (!bytes)
+        return fail(KITTY_E_INVALID, "bytes is NULL");
+    if (const int rc = check_attend8(cache, args, c))
+        return rc;
+    if (const int rc = plan8(c, *args, pl))
+        return rc;
+    *bytes = pl.bytes;
+    return KITTY_OK;
+}
+
+extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
+                                      kitty_stream_t stream)
+{
+    Attend8 p;
+    Plan8 pl;
+    if (const int rc = check_attend8(cache, args, p.c))
+        return rc;
+    const kitty_cache8_attention_args &a = *args;
+    if (a.batch == 0 || a.tokens == 0)
+        return KITTY_OK;
+    if (!a.q || !a.out || !a.lens || (!a.block_table && a.table_pages))
+        return fail(KITTY_E_INVALID, "NULL q, out, lens or block_table");
+    if (!aligned(a.q, 16) || !aligned(a.out, 16))
+        return fail(KITTY_E_INVALID, "q and out must be 16-byte aligned");
+    for (int64_t s : {a.q_s_seq, a.q_s_head, a.q_s_tok, a.o_s_seq, a.o_s_head, a.o_s_tok})
+        if (s % 8)
+            return fail(KITTY_E_INVALID, "strides of q and out must be multiples of 8 elements (16-byte rows)");
+    if (const int rc = plan8(p.c, a, pl))
+        return rc;
+    if (!a.workspace || !aligned(a.workspace, 16) || a.workspace_bytes < pl.bytes)
+        return fail(KITTY_E_INVALID, "workspace is NULL, misaligned or smaller than kitty_cache8_attention_workspace_size");
+    p.q = a.q, p.out = a.out, p.lse = a.lse;
+    p.q_s_seq = a.q_s_seq, p.q_s_head = a.q_s_head, p.q_s_tok = a.q_s_tok;
+    p.o_s_seq = a.o_s_seq, p.o_s_head = a.o_s_head, p.o_s_tok = a.o_s_tok;
+    p.table = a.block_table, p.bt_stride = a.bt_stride, p.lens = a.lens, p.q_lens = a.q_lens;
+    p.B = a.batch, p.Hq = a.num_q_heads, p.T = a.tokens, p.gq = a.num_q_heads / p.c.H;
+    p.table_pages = a.table_pages, p.causal = a.causal ? 1 : 0;
+    p.nrb = pl.nrb, p.n_wg = pl.n_wg;
+    p.cs = a.sm_scale * kLog2e;
+    char *ws = (char *)a.workspace;
+    p.ws_o = (float *)ws, p.ws_ml = (float2 *)(ws + pl.o_bytes), p.ws_tab = (int2 *)(ws + pl.o_bytes + pl.ml_bytes);
+
+    const dim3 block(64 * kWaves), grid((unsigned)p.n_wg);
+    const dim3 merge((unsigned)((int64_t)p.B * p.c.H * p.gq * p.T));
+    auto rows = [&](auto dp, auto rt, auto bf) {
+        constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
+        constexpr bool BF = decltype(bf)::value;
+        if (p.c.D == DP)
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false>), grid, block, 0, (hipStream_t)stream, p);
+        else
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true>), grid, block, 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL((cache8_merge_kernel<DP, BF>), merge, block, 0, (hipStream_t)stream, p, 16 * RT);
+    };
+    auto by_type = [&](auto dp, auto rt) {
+        if (a.dtype == KITTY_DTYPE_BF16)
+            rows(dp, rt, std::true_type{});
+        else
+            rows(dp, rt, std::false_type{});
+    };
+    auto by_rows = [&](auto dp) {
+        if (pl.RT == 1)
+            by_type(dp, std::integral_constant<int, 1>{});
+        else
+            by_type(dp, std::integral_constant<int, 2>{});
+    };
+    if (pl.DP == 64)
+        by_rows(std::integral_constant<int, 64>{});
+    else if (pl.DP == 128)
+        by_rows(std::integral_constant<int, 128>{});
+    else
+        by_rows(std::integral_constant<int, 256>{});
+    return check_launch("cache8_rows_kernel");
+}

@@ -19,7 +19,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # KITTY_HIP_LIBRARY selects another build of the same ABI (e.g. a tuning variant).
 LIB_PATH = os.environ.get("KITTY_HIP_LIBRARY") or os.path.join(_HERE, "libkitty_hip.so")
 
-KITTY_ABI_VERSION = 7
+KITTY_ABI_VERSION = 8
 KITTY_OK = 0
 KITTY_E_INVALID = -1
 KITTY_E_HIP = -2
@@ -29,6 +29,7 @@ KITTY_E_NOT_FOUND = -5
 KITTY_DECODE_UNIQUE_BOOST_ROWS = 1
 KITTY_DTYPE_F16 = 0
 KITTY_DTYPE_BF16 = 1
+KITTY_SRC_F16, KITTY_SRC_BF16, KITTY_SRC_F32 = 0, 1, 2
 KITTY_OUT_F16, KITTY_OUT_F32, KITTY_OUT_BF16 = 0, 1, 2
 KITTY_DECODE_PATH_GENERIC, KITTY_DECODE_PATH_MFMA = 0, 1
 
@@ -154,6 +155,42 @@ class PrefillArgs(ctypes.Structure):
     ]
 
 
+class Cache8(ctypes.Structure):
+    """kitty_cache8: the pools of an 8-bit paged cache."""
+    _fields_ = [
+        ("key", _vp), ("value", _vp), ("scale", _vp),
+        ("key_s_page", _i64), ("key_s_head", _i64), ("key_s_tok", _i64),
+        ("value_s_page", _i64), ("value_s_head", _i64), ("value_s_tok", _i64),
+        ("scale_s_page", _i64), ("scale_s_head", _i64),
+        ("num_pages", _i64), ("num_kv_heads", _i32), ("head_dim", _i32), ("page_tokens", _i32),
+    ]
+
+
+class Cache8RowsArgs(ctypes.Structure):
+    """kitty_cache8_write_args and kitty_cache8_read_args: the same fields in the
+    same order (dtype: src_dtype and out_dtype)."""
+    _fields_ = [
+        ("key", _vp), ("value", _vp),
+        ("key_s_seq", _i64), ("key_s_head", _i64), ("key_s_tok", _i64),
+        ("value_s_seq", _i64), ("value_s_head", _i64), ("value_s_tok", _i64),
+        ("block_table", _vp), ("bt_stride", _i64), ("start", _vp), ("lens", _vp),
+        ("batch", _i32), ("tokens", _i32), ("table_pages", _i32), ("dtype", _i32),
+    ]
+
+
+class Cache8AttentionArgs(ctypes.Structure):
+    """kitty_cache8_attention_args."""
+    _fields_ = [
+        ("q", _vp), ("out", _vp), ("lse", _vp),
+        ("q_s_seq", _i64), ("q_s_head", _i64), ("q_s_tok", _i64),
+        ("o_s_seq", _i64), ("o_s_head", _i64), ("o_s_tok", _i64),
+        ("block_table", _vp), ("bt_stride", _i64), ("lens", _vp), ("q_lens", _vp),
+        ("batch", _i32), ("num_q_heads", _i32), ("tokens", _i32), ("table_pages", _i32), ("plan_tokens", _i32),
+        ("causal", _i32), ("dtype", _i32), ("sm_scale", ctypes.c_float),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "kitty_abi_version", "kitty_last_error", "kitty_quantize_kv_blocks",
     "kitty_dequantize_key_page", "kitty_dequantize_value_page",
@@ -162,7 +199,8 @@ EXPORTED_SYMBOLS = (
     "kitty_channel_abs_sum_workspace_size", "kitty_channel_abs_sum_deferred_size", "kitty_channel_abs_sum_deferred",
     "kitty_channel_abs_sum_flush", "kitty_store_i32", "kitty_prefill_attention",
     "kitty_store_prompt", "kitty_zero_regions", "kitty_decode_step", "kitty_channel_abs_sum_first",
-    "kitty_channel_scores",
+    "kitty_channel_scores", "kitty_cache8_write", "kitty_cache8_read", "kitty_cache8_attention_workspace_size",
+    "kitty_cache8_attention",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -208,6 +246,11 @@ def load() -> ctypes.CDLL:
     L.kitty_store_prompt.argtypes = [ctypes.POINTER(PromptArgs), _vp]
     L.kitty_zero_regions.argtypes = [ctypes.POINTER(ZeroRegion), _i32, _vp]
     L.kitty_prefill_attention.argtypes = [ctypes.POINTER(PrefillArgs), _vp]
+    L.kitty_cache8_write.argtypes = [ctypes.POINTER(Cache8), ctypes.POINTER(Cache8RowsArgs), _vp]
+    L.kitty_cache8_read.argtypes = L.kitty_cache8_write.argtypes
+    L.kitty_cache8_attention_workspace_size.argtypes = [ctypes.POINTER(Cache8), ctypes.POINTER(Cache8AttentionArgs),
+                                                        ctypes.POINTER(ctypes.c_size_t)]
+    L.kitty_cache8_attention.argtypes = [ctypes.POINTER(Cache8), ctypes.POINTER(Cache8AttentionArgs), _vp]
     if L.kitty_abi_version() != KITTY_ABI_VERSION:
         raise ImportError(f"libkitty_hip ABI {L.kitty_abi_version()} != {KITTY_ABI_VERSION}")
     _lib = L
