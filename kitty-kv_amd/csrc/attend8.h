@@ -23,12 +23,27 @@ struct Attend8 {
     int64_t bt_stride;
     int B, Hq, T, gq, table_pages, causal;
     int nrb;            // row blocks per (sequence, KV head)
-    int n_wg;           // workgroups of the split
+    int n_wg;           // row kernel: workgroups that share the work
+    int splits;         // tile kernel: parts of a row block's tokens
     float cs;           // sm_scale * log2(e)
     float *ws_o;        // partials: (slots, rows of a block, D padded)
     float2 *ws_ml;      // (slots, rows of a block): maximum (log2 units) and sum
-    int2 *ws_tab;       // (items): first slot (-1: written whole), last workgroup
+    int2 *ws_tab;       // row kernel, (items): first slot (-1: written whole), last workgroup
 };
+
+constexpr int kTileRows = 128;   // query rows of the tile kernel's workgroup
+
+// The tile kernel (attend8_tile.hip) on row blocks of kTileRows, p.splits parts each.
+void launch_tiles(const Attend8 &p, int DP, bool bf16, hipStream_t stream);
+
+// Reads that are the same for a wave and that no kernel of the call writes:
+// through the scalar unit, so that waits for them do not wait for the vector
+// loads in flight.
+template <typename T>
+__device__ __forceinline__ T uniform_load(const T *p)
+{
+    return *(const __attribute__((address_space(4))) T *)p;
+}
 
 // A sequence of the batch as the kernels read it.
 struct Seq8 {

@@ -30,6 +30,8 @@
 
 namespace kitty {
 
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kWaves = 4;
 
 template <int DP, int RT>
@@ -64,8 +66,9 @@ __device__ __forceinline__ float quad_sum(float v)
 }
 
 // Value operand of product dt: the lane's eight tokens at channel dt of its
-// D / 16, each byte picked by (tokens 2e, 2e + 1) pairs and widened.
-template <int DP>
+// D / 16, each byte picked by (tokens 2e, 2e + 1) pairs and widened.  COUNT: 1
+// in the place of NaN codes and 0 elsewhere.
+template <int DP, bool COUNT>
 __device__ __forceinline__ u32x4 value_operand(const unsigned (&v)[8][DP / 64], int dt)
 {
     u32x4 r;
@@ -73,16 +76,18 @@ __device__ __forceinline__ u32x4 value_operand(const unsigned (&v)[8][DP / 64], 
     for (int e = 0; e < 4; ++e) {
         const unsigned a = v[2 * e][dt >> 2], b = v[2 * e + 1][dt >> 2];
         // bytes (a.c, b.c, a.c + 1, b.c + 1) with c = dt & 2; both channels of the pair share the permute
-        const unsigned w = __builtin_amdgcn_perm(b, a, dt & 2 ? 0x07030602u : 0x05010400u);
+        unsigned w = __builtin_amdgcn_perm(b, a, dt & 2 ? 0x07030602u : 0x05010400u);
+        if constexpr (COUNT)
+            w = (nan_codes(w) >> 7) * 0x38u;
         r[e] = dt & 1 ? widen<true, true>(w) : widen<true, false>(w);
     }
     return r;
 }
 
-// 32 tokens from `tok` on, in `buf`, folded into the wave's rows.  MASK: some
+// 32 tokens from `tok` on, in `buf`, folded into the wave's rows.  mask: some
 // row may not see all of them.
-template <int DP, int RT, bool BF16, bool MASK>
-__device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &buf, int tok, int vis_max, float cs, int g)
+template <int DP, int RT, bool BF16>
+__device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &buf, int tok, int vis_max, float cs, int g, bool mask)
 {
     f32x4 S[RT][2];
 #pragma unroll
@@ -103,7 +108,7 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
     }
     // a token's row in the registers: half e / 4, token 4g + e % 4 of it
     bool odd = false;
-    if constexpr (MASK) {
+    if (mask) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int t = tok + 16 * (e >> 2) + 4 * g + (e & 3);
@@ -120,11 +125,12 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
     for (int rt = 0; rt < RT; ++rt) {
         float s[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
+        for (int e = 0; e < 8; ++e)
             s[e] = S[rt][e >> 2][e & 3] * (cs * buf.sc[e >> 2].x);
-            if constexpr (MASK)
+        if (mask)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
                 s[e] = tok + 16 * (e >> 2) + 4 * g + (e & 3) < W.vis[rt] ? s[e] : -__builtin_inff();
-        }
         float mx = s[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e)
@@ -153,18 +159,9 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
             hi[rt][e] = h, lo[rt][e] = l;
         }
     }
-    if (MASK && odd) {
+    if (odd) {
         // NaN values that not every row sees: count them by row and channel
         // (products of 0 / 1), give those rows NaN and take them out of the codes.
-        unsigned ind[8][DP / 64];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-#pragma unroll
-            for (int w = 0; w < DP / 64; ++w) {
-                const unsigned nn = nan_codes(buf.v[e][w]), byte = (nn >> 7) * 0xffu;
-                ind[e][w] = byte & 0x38383838u;   // 1.0
-                buf.v[e][w] &= ~byte;
-            }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             u32x4 see;
@@ -175,16 +172,21 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
             }
 #pragma unroll
             for (int dt = 0; dt < DP / 16; ++dt) {
-                const f32x4 cnt = mfma16<true>(value_operand<DP>(ind, dt), see, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                const f32x4 cnt = mfma16<true>(value_operand<DP, true>(buf.v, dt), see, f32x4{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     W.o[rt][dt][i] = cnt[i] > 0.0f ? __builtin_nanf("") : W.o[rt][dt][i];
             }
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int w = 0; w < DP / 64; ++w)
+                buf.v[e][w] &= ~((nan_codes(buf.v[e][w]) >> 7) * 0xffu);
     }
 #pragma unroll
     for (int dt = 0; dt < DP / 16; ++dt) {
-        const u32x4 vf = value_operand<DP>(buf.v, dt);
+        const u32x4 vf = value_operand<DP, false>(buf.v, dt);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             W.o[rt][dt] = mfma16<true>(vf, hi[rt], W.o[rt][dt]);
@@ -200,11 +202,14 @@ __device__ __forceinline__ int units8(const Attend8 &p, int b)
     return s.bad ? 0 : (s.n + kUnit - 1) / kUnit;
 }
 
+// Steps of a wave's ring of codes.
+constexpr int ring_steps(int DP, int RT) { return DP == 64 ? 4 : DP == 128 ? (RT == 1 ? 4 : 2) : 3; }
+
 // CUT: D is below DP, and the lanes beyond it read nothing.
 template <int DP, int RT, bool BF16, bool CUT>
-__global__ __launch_bounds__(64 * kWaves, DP <= 128 && RT == 1 ? 2 : 1) void cache8_rows_kernel(Attend8 p)
+__global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_kernel(Attend8 p)
 {
-    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4;
+    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NB = ring_steps(DP, RT);
     __shared__ __attribute__((aligned(16))) float lds_o[kWaves][RM][LD];
     __shared__ float2 lds_ml[kWaves][RM];
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
@@ -292,7 +297,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 && RT == 1 ? 2 : 1) void cac
         auto ids = [&](int tok, int (&id)[2]) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
-                id[hf] = table[min((tok + 16 * hf) >> lg, last)];
+                id[hf] = uniform_load(table + min((tok + 16 * hf) >> lg, last));
         };
         auto load = [&](int tok, const int (&id)[2], RowBuf<DP, RT> &buf) {
 #pragma unroll
@@ -303,55 +308,54 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 && RT == 1 ? 2 : 1) void cac
                 const uint8_t *k = kp + page * p.c.key_s_page + (row * p.c.key_s_tok + k_lane);
 #pragma unroll
                 for (int c = 0; c < DP / 64; ++c)
-                    buf.k[hf][c] = CUT && 64 * c + 16 * g >= p.c.D ? u32x4{0, 0, 0, 0} : *(const u32x4 *)(k + 64 * c);
+                    buf.k[hf][c] = CUT && 64 * c + 16 * g >= p.c.D ? u32x4{0, 0, 0, 0} : __builtin_nontemporal_load((const u32x4 *)(k + 64 * c));
                 const uint8_t *v = vp + page * p.c.value_s_page + (row * p.c.value_s_tok + v_lane);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const uint8_t *src = v + (uint32_t)e * p.c.value_s_tok;
                     unsigned(&d)[DP / 64] = buf.v[4 * hf + e];
                     if constexpr (DP == 64) {
-                        d[0] = *(const unsigned *)src;
+                        d[0] = __builtin_nontemporal_load((const unsigned *)src);
                     } else if constexpr (DP == 128) {
-                        const uint2 x = *(const uint2 *)src;
-                        d[0] = x.x, d[1] = x.y;
+                        const u32x2 x = __builtin_nontemporal_load((const u32x2 *)src);
+                        d[0] = x[0], d[1] = x[1];
                     } else {
-                        const u32x4 x = *(const u32x4 *)src;
+                        const u32x4 x = __builtin_nontemporal_load((const u32x4 *)src);
                         d[0] = x[0], d[1] = x[1], d[2] = x[2], d[3] = x[3];
                     }
                 }
-                buf.sc[hf] = *(const float2 *)(sp + page * p.c.scale_s_page);
-                if (bad)
-                    buf.sc[hf].x = __builtin_nanf("");
+                const uint64_t sc = uniform_load((const uint64_t *)(sp + page * p.c.scale_s_page));
+                buf.sc[hf] = make_float2(bad ? __builtin_nanf("") : __builtin_bit_cast(float, (uint32_t)sc),
+                                         __builtin_bit_cast(float, (uint32_t)(sc >> 32)));
             }
         };
-        auto step = [&](int tok, RowBuf<DP, RT> &buf) {
-            if (tok + 32 <= vis_min)
-                row_step<DP, RT, BF16, false>(W, buf, tok, vis_max, p.cs, g);
-            else
-                row_step<DP, RT, BF16, true>(W, buf, tok, vis_max, p.cs, g);
-        };
+        // A ring of NB steps' codes, NB - 1 in flight while one is computed; the page
+        // ids of the next load are fetched a step before it.  Loads past the wave's
+        // last step repeat that step's: a branch around them would make every wait
+        // one for all loads.
         int tok = tile * kUnit + 32 * wave;
         if (tok < end) {
-            RowBuf<DP, RT> a, c;
+            const int final = tok + (end - 1 - tok) / kUnit * kUnit;
+            RowBuf<DP, RT> ring[NB];
             int id[2];
             ids(tok, id);
-            load(tok, id, a);
-            ids(tok + kUnit, id);
-            while (true) {
-                if (tok + kUnit < end) {
-                    load(tok + kUnit, id, c);
-                    ids(tok + 2 * kUnit, id);
+#pragma unroll
+            for (int j = 0; j < NB - 1; ++j) {
+                load(min(tok + j * kUnit, final), id, ring[j]);
+                ids(min(tok + (j + 1) * kUnit, final), id);
+            }
+            bool more = true;
+            while (more) {
+#pragma unroll
+                for (int j = 0; j < NB; ++j) {
+                    if (!more)
+                        break;
+                    load(min(tok + (NB - 1) * kUnit, final), id, ring[(j + NB - 1) % NB]);
+                    ids(min(tok + NB * kUnit, final), id);
+                    row_step<DP, RT, BF16>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min);
+                    tok += kUnit;
+                    more = tok < end;
                 }
-                step(tok, a);
-                if ((tok += kUnit) >= end)
-                    break;
-                if (tok + kUnit < end) {
-                    load(tok + kUnit, id, a);
-                    ids(tok + 2 * kUnit, id);
-                }
-                step(tok, c);
-                if ((tok += kUnit) >= end)
-                    break;
             }
         }
 
@@ -413,37 +417,48 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 && RT == 1 ? 2 : 1) void cac
     }
 }
 
-// Joins the partials of one row; also the rows no workgroup touched: of
-// sequences without tokens (0) and of broken lengths (NaN).
-template <int DP, bool BF16>
+// Joins the partials of ROWS rows (4: one a wave, 1: one for the four waves, where
+// rows are too few to fill the device); also, after the row kernel, the rows no
+// workgroup touched: of sequences without tokens (0) and of broken lengths (NaN).
+// TILES: the partials are the tile kernel's p.splits parts.
+template <int DP, bool BF16, bool TILES, int ROWS>
 __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, int RM)
 {
-    constexpr int CPL = DP / 64;   // channels per lane
-    __shared__ float lds_o[kWaves][DP];
-    __shared__ float2 lds_ml[kWaves];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int rows = p.gq * p.T, pair = blockIdx.x / rows, row = blockIdx.x - pair * rows;
+    constexpr int CPL = DP / 64, STEP = ROWS == 1 ? kWaves : 1;   // channels per lane, partials between a wave's
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rows = p.gq * p.T, all = ROWS == 1 ? blockIdx.x : blockIdx.x * ROWS + wave;
+    const int pair = all / rows, row = all - pair * rows;
+    if (ROWS > 1 && pair >= p.B * p.c.H)
+        return;
     const int b = pair / p.c.H, kh = pair - b * p.c.H, rb = row / RM, r = row - rb * RM;
     const int t = row / p.gq, h = kh * p.gq + row - t * p.gq;
     const Seq8 sq = seq8(p, b);
     float m = kLowest, l = 0.0f, o[CPL];
 #pragma unroll
     for (int e = 0; e < CPL; ++e)
-        o[e] = sq.bad ? __builtin_nanf("") : 0.0f;
-    if (sq.bad)
-        m = l = __builtin_nanf("");
-    else if (sq.n > 0) {
-        const int2 tab = p.ws_tab[pair * p.nrb + rb];
+        o[e] = 0.0f;
+    if (sq.bad) {
+        l = __builtin_nanf("");
+    } else if (sq.n > 0) {
+        const int item = pair * p.nrb + rb;
+        int2 tab = make_int2(0, 0);
+        if constexpr (!TILES)
+            tab = p.ws_tab[item];
         if (tab.x < 0)
             return;
-        const int first = tab.x >> 1, count = tab.y - first + 1;
-        auto slot = [&](int i) { return (int64_t)(i == 0 ? tab.x : 2 * (first + i)) * RM + r; };
-        for (int i = wave; i < count; i += 4 * kWaves) {
+        const int first = tab.x >> 1, count = TILES ? p.splits : tab.y - first + 1;
+        auto slot = [&](int i) {
+            if constexpr (TILES)
+                return ((int64_t)item * p.splits + i) * RM + r;
+            else
+                return (int64_t)(i == 0 ? tab.x : 2 * (first + i)) * RM + r;
+        };
+        for (int i = ROWS == 1 ? wave : 0; i < count; i += 4 * STEP) {
             float2 ml[4];
             float x[4][CPL];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int64_t s = slot(min(i + j * kWaves, count - 1));
+                const int64_t s = slot(min(i + j * STEP, count - 1));
                 ml[j] = p.ws_ml[s];
 #pragma unroll
                 for (int e = 0; e < CPL; ++e)
@@ -451,7 +466,7 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if (i + j * kWaves >= count)
+                if (i + j * STEP >= count)
                     break;
                 const float mn = fmaxf(m, ml[j].x);
                 const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml[j].x - mn);
@@ -463,29 +478,40 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
             }
         }
     }
-#pragma unroll
-    for (int e = 0; e < CPL; ++e)
-        lds_o[wave][CPL * lane + e] = o[e];
-    if (lane == 0)
-        lds_ml[wave] = make_float2(m, l);
-    __syncthreads();
     const bool none = !sq.bad && visible8(p, sq, t) == 0;
-    const int ch = threadIdx.x;
-    if (ch >= p.c.D)
-        return;
-    float M = kLowest, L = 0.0f, acc = 0.0f;
+    uint16_t *out = p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok;
+    if constexpr (ROWS == 1) {
+        __shared__ float lds_o[kWaves][DP];
+        __shared__ float2 lds_ml[kWaves];
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-        M = fmaxf(M, lds_ml[w].x);
+        for (int e = 0; e < CPL; ++e)
+            lds_o[wave][CPL * lane + e] = o[e];
+        if (lane == 0)
+            lds_ml[wave] = make_float2(m, l);
+        __syncthreads();
+        const int ch = threadIdx.x;
+        if (ch >= p.c.D)
+            return;
+        float M = kLowest, L = 0.0f, acc = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(lds_ml[w].x - M);
-        L += f * lds_ml[w].y;
-        acc += f * lds_o[w][ch];
+        for (int w = 0; w < kWaves; ++w)
+            M = fmaxf(M, lds_ml[w].x);
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(lds_ml[w].x - M);
+            L += f * lds_ml[w].y;
+            acc += f * lds_o[w][ch];
+        }
+        out[ch] = f2x(none ? 0.0f : acc / L, BF16);
+        m = M, l = L;
+    } else {
+#pragma unroll
+        for (int e = 0; e < CPL; ++e)
+            if (CPL * lane + e < p.c.D)
+                out[CPL * lane + e] = f2x(none ? 0.0f : o[e] / l, BF16);
     }
-    p.out[b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok + ch] = f2x(none ? 0.0f : acc / L, BF16);
-    if (ch == 0 && p.lse)
-        p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (M + __builtin_log2f(L)) / kLog2e;
+    if ((ROWS == 1 ? threadIdx.x : lane) == 0 && p.lse)
+        p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
 }
 
 static int device_cus()
@@ -500,26 +526,44 @@ static int device_cus()
 static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 struct Plan8 {
-    int DP, RT, nrb, n_wg;
+    bool tiles;
+    int DP, RT, nrb, n_wg, splits;
     size_t o_bytes, ml_bytes, bytes;
 };
 
+// Rows from which the merge gives each a wave instead of four.
+constexpr int64_t kMergeRows = 2048;
+// Rows that the row kernel takes: two blocks of 16, whose codes are read once.
+constexpr int kRowKernelRows = 32;
+
 static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &pl)
 {
-    const int64_t rows = (int64_t)a.num_q_heads / c.H * a.tokens;
+    const int64_t rows = (int64_t)a.num_q_heads / c.H * a.tokens, pairs = (int64_t)a.batch * c.H;
     pl.DP = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
-    pl.RT = rows <= 16 ? 1 : 2;
-    const int RM = 16 * pl.RT;
-    const int64_t nrb = (rows + RM - 1) / RM;
-    const int64_t items = (int64_t)a.batch * c.H * nrb;
-    const int64_t units = (((int64_t)a.table_pages << c.lg) + kUnit - 1) / kUnit;
-    if (rows > kMaxBlocks || (int64_t)a.batch * c.H * rows > kMaxBlocks || items * std::max<int64_t>(units, 1) > 0x7fffffff)
+    pl.tiles = rows > kRowKernelRows;
+    pl.RT = rows <= 16 || pl.DP == 256 ? 1 : 2;   // at 256 channels two blocks' registers do not fit
+    const int RM = pl.tiles ? kTileRows : 16 * pl.RT;
+    const int64_t nrb = (rows + RM - 1) / RM, items = pairs * nrb;
+    const int64_t cap = (int64_t)a.table_pages << c.lg;   // tokens of the longest sequence, as far as the host knows
+    const int64_t tokens = a.plan_tokens > 0 ? std::min<int64_t>(a.plan_tokens, cap) : cap;
+    const int64_t units = (cap + kUnit - 1) / kUnit;
+    if (rows > kMaxBlocks || pairs * rows > kMaxBlocks || items * std::max<int64_t>(units, 1) > 0x7fffffff)
         return fail(KITTY_E_UNSUPPORTED, "too many rows or pages for one launch");
     pl.nrb = (int)nrb;
-    pl.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus(), items * units));
-    pl.o_bytes = up16((size_t)2 * pl.n_wg * RM * pl.DP * 4);
-    pl.ml_bytes = up16((size_t)2 * pl.n_wg * RM * 8);
-    pl.bytes = pl.o_bytes + pl.ml_bytes + up16((size_t)items * 8);
+    pl.n_wg = pl.splits = 1;
+    int64_t slots = 0;
+    if (pl.tiles) {
+        // parts of at least four tiles, until there are two workgroups a CU (one at 256 channels)
+        const int64_t want = (pl.DP == 256 ? 1 : 2) * (int64_t)device_cus() / std::max<int64_t>(items, 1);
+        pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tokens / 256));
+        slots = pl.splits > 1 ? items * pl.splits : 0;
+    } else {
+        pl.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus(), items * units));
+        slots = 2 * pl.n_wg;
+    }
+    pl.o_bytes = up16((size_t)slots * RM * pl.DP * 4);
+    pl.ml_bytes = up16((size_t)slots * RM * 8);
+    pl.bytes = pl.o_bytes + pl.ml_bytes + (pl.tiles ? 0 : up16((size_t)items * 8));
     return KITTY_OK;
 }
 
@@ -581,7 +625,7 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
             return fail(KITTY_E_INVALID, "strides of q and out must be multiples of 8 elements (16-byte rows)");
     if (const int rc = plan8(p.c, a, pl))
         return rc;
-    if (!a.workspace || !aligned(a.workspace, 16) || a.workspace_bytes < pl.bytes)
+    if ((!a.workspace && pl.bytes) || !aligned(a.workspace, 16) || a.workspace_bytes < pl.bytes)
         return fail(KITTY_E_INVALID, "workspace is NULL, misaligned or smaller than kitty_cache8_attention_workspace_size");
     p.q = a.q, p.out = a.out, p.lse = a.lse;
     p.q_s_seq = a.q_s_seq, p.q_s_head = a.q_s_head, p.q_s_tok = a.q_s_tok;
@@ -589,39 +633,61 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
     p.table = a.block_table, p.bt_stride = a.bt_stride, p.lens = a.lens, p.q_lens = a.q_lens;
     p.B = a.batch, p.Hq = a.num_q_heads, p.T = a.tokens, p.gq = a.num_q_heads / p.c.H;
     p.table_pages = a.table_pages, p.causal = a.causal ? 1 : 0;
-    p.nrb = pl.nrb, p.n_wg = pl.n_wg;
+    p.nrb = pl.nrb, p.n_wg = pl.n_wg, p.splits = pl.splits;
     p.cs = a.sm_scale * kLog2e;
     char *ws = (char *)a.workspace;
     p.ws_o = (float *)ws, p.ws_ml = (float2 *)(ws + pl.o_bytes), p.ws_tab = (int2 *)(ws + pl.o_bytes + pl.ml_bytes);
 
-    const dim3 block(64 * kWaves), grid((unsigned)p.n_wg);
-    const dim3 merge((unsigned)((int64_t)p.B * p.c.H * p.gq * p.T));
+    const hipStream_t st = (hipStream_t)stream;
+    const bool bf16 = a.dtype == KITTY_DTYPE_BF16;
+    const dim3 block(64 * kWaves);
+    auto merge = [&](auto dp, auto bf, auto tiles) {
+        constexpr int DP = decltype(dp)::value;
+        constexpr bool BF = decltype(bf)::value, TILES = decltype(tiles)::value;
+        const int64_t rows = (int64_t)p.B * p.Hq * p.T;
+        const int RM = TILES ? kTileRows : 16 * pl.RT;
+        if (rows < kMergeRows)
+            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, 1>), dim3((unsigned)rows), block, 0, st, p, RM);
+        else
+            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, 4>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, p, RM);
+    };
     auto rows = [&](auto dp, auto rt, auto bf) {
         constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
         constexpr bool BF = decltype(bf)::value;
         if (p.c.D == DP)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false>), grid, block, 0, (hipStream_t)stream, p);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false>), dim3((unsigned)p.n_wg), block, 0, st, p);
         else
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true>), grid, block, 0, (hipStream_t)stream, p);
-        hipLaunchKernelGGL((cache8_merge_kernel<DP, BF>), merge, block, 0, (hipStream_t)stream, p, 16 * RT);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true>), dim3((unsigned)p.n_wg), block, 0, st, p);
     };
-    auto by_type = [&](auto dp, auto rt) {
-        if (a.dtype == KITTY_DTYPE_BF16)
-            rows(dp, rt, std::true_type{});
-        else
-            rows(dp, rt, std::false_type{});
+    auto go = [&](auto dp, auto bf) {
+        constexpr int DP = decltype(dp)::value;
+        if (pl.tiles) {
+            launch_tiles(p, DP, bf16, st);
+            if (p.splits > 1)
+                merge(dp, bf, std::true_type{});
+            return;
+        }
+        if constexpr (DP <= 128) {
+            if (pl.RT == 2)
+                rows(dp, std::integral_constant<int, 2>{}, bf);
+            else
+                rows(dp, std::integral_constant<int, 1>{}, bf);
+        } else {
+            rows(dp, std::integral_constant<int, 1>{}, bf);
+        }
+        merge(dp, bf, std::false_type{});
     };
-    auto by_rows = [&](auto dp) {
-        if (pl.RT == 1)
-            by_type(dp, std::integral_constant<int, 1>{});
+    auto by_type = [&](auto dp) {
+        if (bf16)
+            go(dp, std::true_type{});
         else
-            by_type(dp, std::integral_constant<int, 2>{});
+            go(dp, std::false_type{});
     };
     if (pl.DP == 64)
-        by_rows(std::integral_constant<int, 64>{});
+        by_type(std::integral_constant<int, 64>{});
     else if (pl.DP == 128)
-        by_rows(std::integral_constant<int, 128>{});
+        by_type(std::integral_constant<int, 128>{});
     else
-        by_rows(std::integral_constant<int, 256>{});
-    return check_launch("cache8_rows_kernel");
+        by_type(std::integral_constant<int, 256>{});
+    return check_launch("8-bit cache attention");
 }

@@ -1,0 +1,393 @@
+// Attention of many query rows over the 8-bit paged cache, on gfx950: a
+// prompt's chunk behind what the cache holds, or decoder rows over an encoder's
+// states.
+//
+// Bound by the matrix cores and the softmax's vector instructions.  One wave
+// takes 32 query rows (head of the group fastest), a 256-thread workgroup four
+// waves of one (sequence, KV head) pair, and each tile of 64 tokens is widened
+// once for all of them: codes HBM -> registers (the next tile's, while one is
+// computed) -> 16-bit floats in one of two LDS stages, keys in q's type and
+// values in bf16, both exact.  Chunks are swizzled so that neither the key reads
+// nor the transposing value reads conflict.
+//
+//  S^T = K Q^T with 32x32x16 MFMAs: lane (n = query row l & 31, g = l / 32) ends
+//  with its row's scores of tokens 8j + 4g + 0..3, so the softmax needs one
+//  exchange between lanes l and l + 32 per tile.
+//  O^T += V^T P^T: the scores' registers are the B operand as they stand; slots
+//  8g + e of a 16-token step stand for tokens 4g + e (e < 4) and 8 + 4g + e - 4,
+//  and ds_read_b64_tr_b16 fetches the value rows in that order.
+//
+// Scales belong to 16-token steps (a page holds 16 tokens or more): the key's is
+// a factor of the scores, the value's of the weights, which go in two bf16
+// terms, 16 bits with fp32's range.  The running maximum is raised only when a
+// tile passes it by 2^8.  Where the row blocks are too few for the device, the
+// tokens of each are split evenly, and cache8_merge_kernel joins the parts.
+#include <type_traits>
+
+#include "attend8.h"
+
+namespace kitty {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTile = 64, kTileWaves = kTileRows / 32;
+
+template <bool BF16>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c)
+{
+    if constexpr (BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// max / sum of a value with the lane 32 apart
+__device__ __forceinline__ float other_max(float v)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, (int)s[0]), __builtin_bit_cast(float, (int)s[1]));
+}
+__device__ __forceinline__ float other_sum(float v)
+{
+    const auto s = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(int, v), __builtin_bit_cast(int, v), false, false);
+    return __builtin_bit_cast(float, (int)s[0]) + __builtin_bit_cast(float, (int)s[1]);
+}
+
+// Where 16-byte chunk c of a tile's row lies in the row's DP / 8 chunks.
+template <int DP>
+__device__ __forceinline__ int key_slot(int row, int c) { return c ^ (row & (DP == 64 ? 7 : 15)); }
+template <int DP>
+__device__ __forceinline__ int value_slot(int row, int c) { return c ^ (4 * (DP == 64 ? row >> 1 & 1 : row & 3)); }
+
+// 16 codes as two chunks of 16-bit floats.
+template <bool BF16>
+__device__ __forceinline__ void widen16(u32x4 w, u32x4 (&r)[2])
+{
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        r[e >> 1][2 * (e & 1)] = widen<BF16, false>(w[e]);
+        r[e >> 1][2 * (e & 1) + 1] = widen<BF16, true>(w[e]);
+    }
+}
+
+// NaNs of a pair of bf16 values, as 1 in each half.
+__device__ __forceinline__ unsigned nan_pairs(unsigned w)
+{
+    return (((w & 0x7fff7fffu) + 0x007f007fu) & 0x80008000u) >> 15;
+}
+
+template <int DP>
+struct TileState {
+    u32x4 q[DP / 16];    // k-step s: channels 16s + 8g .. + 7
+    f32x16 o[DP / 32];   // O^T: channels 32dt + 8 (i / 4) + 4g + i % 4
+    float m, l;          // running maximum (log2 units), this lane's half of the sum
+    int vis;             // tokens the row sees
+    int k_base, v_base[DP / 32];
+};
+
+// Tokens t0 .. t0 + 63 in a stage folded into the wave's rows.  sc: (key, value)
+// scales of its four 16-token steps, the key's times sm_scale * log2(e); lost: bits
+// of the steps that have no page.  mask: some row does not see them all; odd: and
+// there are NaN values among them.
+template <int DP, bool BF16>
+__device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char *kst, const unsigned char *vst, int t0,
+                                          const float2 (&sc)[4], unsigned lost, int lane, bool mask, bool odd)
+{
+    const int g = lane >> 5, n = lane & 31;
+    f32x16 S[2];
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            S[mt][i] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) {
+        const int off = W.k_base + 16 * key_slot<DP>(n, 2 * s + g);
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+            S[mt] = mfma32<BF16>(*(const u32x4 *)(kst + off + 64 * DP * mt), W.q[s], S[mt]);
+    }
+    if (lost) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                S[mt][i] = lost >> (2 * mt + (i >> 3)) & 1 ? __builtin_nanf("") : S[mt][i];
+    }
+    if (mask) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                S[mt][i] = t0 + 32 * mt + 8 * (i >> 2) + 4 * g + (i & 3) < W.vis ? S[mt][i] : -__builtin_inff();
+    }
+    float mx = -__builtin_inff();
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+        float a = S[st >> 1][8 * (st & 1)];
+#pragma unroll
+        for (int i = 1; i < 8; ++i)
+            a = fmaxf(a, S[st >> 1][8 * (st & 1) + i]);
+        mx = fmaxf(mx, a * sc[st].x);
+    }
+    mx = other_max(mx);
+    const bool raise = mx > W.m + 8.0f;
+    if (__ballot(raise)) {
+        const float mn = raise ? mx : W.m;
+        const float alpha = __builtin_amdgcn_exp2f(W.m - mn);
+        W.m = mn;
+        W.l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                W.o[dt][i] *= alpha;
+    }
+    unsigned hi[2][8], lo[2][8];
+    float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = sc[2 * mt + (i >> 2)];
+            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(S[mt][2 * i], f.x, -W.m));
+            const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[mt][2 * i + 1], f.x, -W.m));
+            ls[(2 * i) & 3] += a;
+            ls[(2 * i + 1) & 3] += b;
+            split_bf16(a * f.y, b * f.y, hi[mt][i], lo[mt][i]);
+        }
+    W.l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+        const int mt = s >> 1, r = 4 * (s & 1);
+        const u32x4 ph = {hi[mt][r], hi[mt][r + 1], hi[mt][r + 2], hi[mt][r + 3]};
+        const u32x4 pl = {lo[mt][r], lo[mt][r + 1], lo[mt][r + 2], lo[mt][r + 3]};
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt) {
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const unsigned char *src = vst + W.v_base[dt] + 32 * DP * s;
+            const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)src);
+            const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src + 16 * DP));
+            const uint2 a = __builtin_bit_cast(uint2, v0), b = __builtin_bit_cast(uint2, v1);
+            u32x4 vf = {a.x, a.y, b.x, b.y};
+            if (odd) {
+                // NaN values reach the rows that see them, and no others: counted by
+                // products of 0 / 1, then taken out of the operand
+                u32x4 ind, see;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned nn = nan_pairs(vf[e]);
+                    ind[e] = nn * 0x3f80u;
+                    vf[e] &= ~(nn * 0xffffu);
+                    const int t = t0 + 16 * s + 8 * (e >> 1) + 4 * g + 2 * (e & 1);
+                    see[e] = (t < W.vis ? 0x3f80u : 0u) | (t + 1 < W.vis ? 0x3f800000u : 0u);
+                }
+                f32x16 cnt;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    cnt[i] = 0.0f;
+                cnt = mfma32<true>(ind, see, cnt);
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    W.o[dt][i] = cnt[i] > 0.0f ? __builtin_nanf("") : W.o[dt][i];
+            }
+            W.o[dt] = mfma32<true>(vf, ph, W.o[dt]);
+            W.o[dt] = mfma32<true>(vf, pl, W.o[dt]);
+        }
+    }
+}
+
+template <int DP, bool BF16, bool CUT>
+__global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_tile_kernel(Attend8 p)
+{
+    constexpr int RM = kTileRows, TPR = DP / 16, PASS = 64 * kTileWaves / TPR, NP = kTile / PASS;
+    __shared__ __attribute__((aligned(16))) unsigned char ks[2][kTile * DP * 2], vs[2][kTile * DP * 2];
+    __shared__ int odd_tile[2];
+    const int lane = threadIdx.x & 63, g = lane >> 5, n = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // pairs vary fastest, so with a multiple of eight pairs a pair's pages stay in
+    // one XCD's L2; the last row blocks, with the most tokens, start first
+    const int pairs = p.B * p.c.H, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+    const int split = rest % p.splits, rb = p.nrb - 1 - rest / p.splits;
+    const int b = pair / p.c.H, kh = pair - b * p.c.H, r0 = rb * RM;
+    const Seq8 sq = seq8(p, b);
+    const int rows = min(RM, p.gq * p.T - r0);
+    const int t_lo = r0 / p.gq, t_hi = min((r0 + rows - 1) / p.gq, sq.tq - 1);
+    const int vis_max = sq.bad || t_hi < t_lo ? 0 : visible8(p, sq, t_hi), vis_min = visible8(p, sq, t_lo);
+    const int nt = (vis_max + kTile - 1) / kTile;
+    const int first = (int)((int64_t)nt * split / p.splits), end = (int)((int64_t)nt * (split + 1) / p.splits);
+
+    TileState<DP> W;
+    const int w0 = r0 + 32 * wave, r = w0 + n, t = r / p.gq, h = kh * p.gq + r - t * p.gq;
+    const bool row = r < p.gq * p.T;
+    W.vis = sq.bad ? 0 : visible8(p, sq, t);
+    const int w_lo = w0 / p.gq, w_hi = min((w0 + 31) / p.gq, sq.tq - 1);
+    const int wave_min = visible8(p, sq, w_lo), wave_max = sq.bad || w_hi < w_lo ? 0 : visible8(p, sq, w_hi);
+    {
+        const uint16_t *q = p.q + b * p.q_s_seq + h * p.q_s_head + t * p.q_s_tok;
+#pragma unroll
+        for (int s = 0; s < DP / 16; ++s) {
+            W.q[s] = u32x4{0, 0, 0, 0};
+            if (!sq.bad && t < sq.tq && (!CUT || 16 * s < p.c.D))
+                W.q[s] = *(const u32x4 *)(q + 16 * s + 8 * g);
+        }
+    }
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            W.o[dt][i] = 0.0f;
+    W.m = kLowest;
+    W.l = 0.0f;
+    W.k_base = n * 2 * DP;
+    {
+        const int i = lane & 15, hs = lane >> 4 & 1, tr = 4 * g + (i >> 2);   // the lane's token row of a 16-token step
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+            W.v_base[dt] = tr * 2 * DP + 16 * value_slot<DP>(tr, 4 * dt + 2 * hs) + 8 * (i & 3);
+    }
+
+    // loads: thread x brings chunk x % TPR (16 codes) of rows x / TPR + PASS j; the rows
+    // of a wave and j lie in one 16-token step, so their page is the wave's
+    const int32_t *table = p.table + b * p.bt_stride;
+    const int lg = p.c.lg, last = (sq.n - 1) >> lg;
+    const int lr = threadIdx.x / TPR, lc = threadIdx.x % TPR;
+    const bool cut = CUT && 16 * lc >= p.c.D;
+    const uint8_t *kp = p.c.key + kh * p.c.key_s_head + (cut ? 0 : 16 * lc);
+    const uint8_t *vp = p.c.value + kh * p.c.value_s_head + (cut ? 0 : 16 * lc);
+    const float *sp = p.c.scale + kh * p.c.scale_s_head;
+    u32x4 kr[NP], vr[NP];
+    float2 sc[4], sc_next[4];
+    unsigned lost = 0, lost_next = 0;
+    auto load = [&](int tile) {
+        int64_t page[4];
+        lost_next = 0;
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+            const int id = uniform_load(table + min((tile * kTile + 16 * st) >> lg, last));
+            const bool bad = bad_page(p.c, id);
+            page[st] = bad ? 0 : id;
+            lost_next |= (bad ? 1u : 0u) << st;
+            const uint64_t x = uniform_load((const uint64_t *)(sp + page[st] * p.c.scale_s_page));
+            sc_next[st] = make_float2(__builtin_bit_cast(float, (uint32_t)x) * p.cs, __builtin_bit_cast(float, (uint32_t)(x >> 32)));
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            // step of this wave's rows in pass j
+            const int st = (64 / TPR * wave + PASS * j) >> 4;
+            const int64_t pg = st == 0 ? page[0] : st == 1 ? page[1] : st == 2 ? page[2] : page[3];
+            const uint32_t rw = (uint32_t)(tile * kTile + lr + PASS * j) & ((1u << lg) - 1);
+            kr[j] = *(const u32x4 *)(kp + pg * p.c.key_s_page + rw * p.c.key_s_tok);
+            vr[j] = *(const u32x4 *)(vp + pg * p.c.value_s_page + rw * p.c.value_s_tok);
+        }
+    };
+    auto store = [&](int tile, int stage) {
+        bool odd = false;
+        const bool ragged = (tile + 1) * kTile > vis_min;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int rw = lr + PASS * j;
+            if (ragged) {   // rows no query sees hold anything
+                if (tile * kTile + rw >= vis_max)
+                    vr[j] = u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    odd |= nan_codes(vr[j][e]) != 0;
+            }
+            u32x4 x[2];
+            widen16<BF16>(cut ? u32x4{0, 0, 0, 0} : kr[j], x);
+            unsigned char *k = ks[stage] + rw * 2 * DP;
+            *(u32x4 *)(k + 16 * key_slot<DP>(rw, 2 * lc)) = x[0];
+            *(u32x4 *)(k + 16 * key_slot<DP>(rw, 2 * lc + 1)) = x[1];
+            widen16<true>(vr[j], x);
+            unsigned char *v = vs[stage] + rw * 2 * DP;
+            *(u32x4 *)(v + 16 * value_slot<DP>(rw, 2 * lc)) = x[0];
+            *(u32x4 *)(v + 16 * value_slot<DP>(rw, 2 * lc + 1)) = x[1];
+        }
+        if (__ballot(odd) && lane == 0)
+            odd_tile[stage] = tile;
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+            sc[st] = sc_next[st];
+        lost = lost_next;
+    };
+    if (threadIdx.x < 2)
+        odd_tile[threadIdx.x] = -1;
+    __syncthreads();
+    if (first < end) {
+        load(first);
+        store(first, 0);
+    }
+    for (int tile = first; tile < end; ++tile) {
+        const int stage = (tile - first) & 1, t0 = tile * kTile;
+        __syncthreads();   // the tile is in its stage; every wave is done with the other one
+        const bool more = tile + 1 < end;
+        if (more)
+            load(tile + 1);
+        if (t0 < wave_max) {
+            const bool mask = t0 + kTile > wave_min;
+            tile_step<DP, BF16>(W, ks[stage], vs[stage], t0, sc, lost, lane, mask, mask && odd_tile[stage] == tile);
+        }
+        if (more)
+            store(tile + 1, stage ^ 1);
+    }
+
+    const float l = other_sum(W.l);
+    if (!row)
+        return;
+    if (p.splits > 1) {
+        const int64_t at = ((int64_t)(pair * p.nrb + rb) * p.splits + split) * RM + 32 * wave + n;
+        if (g == 0)
+            p.ws_ml[at] = make_float2(W.m, l);
+#pragma unroll
+        for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(float4 *)(p.ws_o + at * DP + 32 * dt + 8 * j + 4 * g) =
+                    make_float4(W.o[dt][4 * j], W.o[dt][4 * j + 1], W.o[dt][4 * j + 2], W.o[dt][4 * j + 3]);
+        return;
+    }
+    const bool none = !sq.bad && W.vis == 0;
+    const float inv = sq.bad ? __builtin_nanf("") : none ? 0.0f : 1.0f / l;
+    uint16_t *o = p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int ch = 32 * dt + 8 * j + 4 * g;
+            if (!CUT || ch < p.c.D)
+                *(uint2 *)(o + ch) = make_uint2((uint32_t)f2x(W.o[dt][4 * j] * inv, BF16) | (uint32_t)f2x(W.o[dt][4 * j + 1] * inv, BF16) << 16,
+                                                (uint32_t)f2x(W.o[dt][4 * j + 2] * inv, BF16) | (uint32_t)f2x(W.o[dt][4 * j + 3] * inv, BF16) << 16);
+        }
+    if (g == 0 && p.lse)
+        p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
+            sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (W.m + __builtin_log2f(l)) / kLog2e;
+}
+
+void launch_tiles(const Attend8 &p, int DP, bool bf16, hipStream_t stream)
+{
+    const dim3 grid((unsigned)(p.B * p.c.H * p.nrb * p.splits)), block(64 * kTileWaves);
+    auto go = [&](auto dp, auto bf) {
+        constexpr int N = decltype(dp)::value;
+        constexpr bool BF = decltype(bf)::value;
+        if (p.c.D == N)
+            hipLaunchKernelGGL((cache8_tile_kernel<N, BF, false>), grid, block, 0, stream, p);
+        else
+            hipLaunchKernelGGL((cache8_tile_kernel<N, BF, true>), grid, block, 0, stream, p);
+    };
+    auto by_size = [&](auto bf) {
+        if (DP == 64)
+            go(std::integral_constant<int, 64>{}, bf);
+        else if (DP == 128)
+            go(std::integral_constant<int, 128>{}, bf);
+        else
+            go(std::integral_constant<int, 256>{}, bf);
+    };
+    if (bf16)
+        by_size(std::true_type{});
+    else
+        by_size(std::false_type{});
+}
+
+} // namespace kitty
