@@ -202,14 +202,11 @@ __device__ __forceinline__ int units8(const Attend8 &p, int b)
     return s.bad ? 0 : (s.n + kUnit - 1) / kUnit;
 }
 
-// Steps of a wave's ring of codes.
-constexpr int ring_steps(int DP, int RT) { return DP == 64 ? 4 : DP == 128 ? (RT == 1 ? 4 : 2) : 3; }
-
 // CUT: D is below DP, and the lanes beyond it read nothing.
 template <int DP, int RT, bool BF16, bool CUT>
 __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_kernel(Attend8 p)
 {
-    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NB = ring_steps(DP, RT);
+    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NB = 2;
     __shared__ __attribute__((aligned(16))) float lds_o[kWaves][RM][LD];
     __shared__ float2 lds_ml[kWaves][RM];
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
@@ -337,21 +334,21 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
         if (tok < end) {
             const int final = tok + (end - 1 - tok) / kUnit * kUnit;
             RowBuf<DP, RT> ring[NB];
-            int id[2];
-            ids(tok, id);
+            int id[NB][2];
 #pragma unroll
-            for (int j = 0; j < NB - 1; ++j) {
-                load(min(tok + j * kUnit, final), id, ring[j]);
-                ids(min(tok + (j + 1) * kUnit, final), id);
-            }
+            for (int j = 0; j < NB; ++j)
+                ids(min(tok + j * kUnit, final), id[j]);
+#pragma unroll
+            for (int j = 0; j < NB - 1; ++j)
+                load(min(tok + j * kUnit, final), id[j], ring[j]);
             bool more = true;
             while (more) {
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     if (!more)
                         break;
-                    load(min(tok + (NB - 1) * kUnit, final), id, ring[(j + NB - 1) % NB]);
-                    ids(min(tok + NB * kUnit, final), id);
+                    load(min(tok + (NB - 1) * kUnit, final), id[NB - 1], ring[(j + NB - 1) % NB]);
+                    ids(min(tok + NB * kUnit, final), id[NB - 1]);
                     row_step<DP, RT, BF16>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min);
                     tok += kUnit;
                     more = tok < end;
