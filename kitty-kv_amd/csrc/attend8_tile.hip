@@ -18,9 +18,14 @@
 //  and ds_read_b64_tr_b16 fetches the value rows in that order.
 //
 // Scales belong to 16-token steps (a page holds 16 tokens or more): the key's is
-// a factor of the scores, the value's of the weights, which go in two bf16
-// terms, 16 bits with fp32's range.  The running maximum is raised only when a
-// tile passes it by 2^8.  Where the row blocks are too few for the device, the
+// a factor of the scores, the logarithm of the value's is added to them, so that
+// the running maximum m is that of weight times scale, the exponential gives
+// w = p * scale in one step, and p's sum is that of w by 1 / scale.  It is raised
+// only when a tile passes it by 2^8.
+// Weights: for fp16 results two bf16 terms (16 bits, error 2^-18), as a third of
+// the products' time buys the error of fp32 weights; for bf16 results, which keep
+// 8 bits, one fp16 term (11 bits, error 2^-11 of a weight, 2^-25 of the largest
+// where that is more; w is at most 2^8 and the largest at least 1).  Where the row blocks are too few for the device, the
 // tokens of each are split evenly, and cache8_merge_kernel joins the parts.
 #include <type_traits>
 
@@ -71,28 +76,35 @@ __device__ __forceinline__ void widen16(u32x4 w, u32x4 (&r)[2])
     }
 }
 
-// NaNs of a pair of bf16 values, as 1 in each half.
-__device__ __forceinline__ unsigned nan_pairs(unsigned w)
+// (a, b) as fp16, rounded to nearest.
+__device__ __forceinline__ unsigned pack_f16(float a, float b)
 {
-    return (((w & 0x7fff7fffu) + 0x007f007fu) & 0x80008000u) >> 15;
+    typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+    half2v h;
+    h[0] = (_Float16)a, h[1] = (_Float16)b;
+    return __builtin_bit_cast(unsigned, h);
 }
 
 template <int DP>
 struct TileState {
     u32x4 q[DP / 16];    // k-step s: channels 16s + 8g .. + 7
     f32x16 o[DP / 32];   // O^T: channels 32dt + 8 (i / 4) + 4g + i % 4
-    float m, l;          // running maximum (log2 units), this lane's half of the sum
+    float m, l;          // running maximum of score + log2(value scale), this lane's half of the sum
     int vis;             // tokens the row sees
     int k_base, v_base[DP / 32];
 };
 
-// Tokens t0 .. t0 + 63 in a stage folded into the wave's rows.  sc: (key, value)
-// scales of its four 16-token steps, the key's times sm_scale * log2(e); lost: bits
-// of the steps that have no page.  mask: some row does not see them all; odd: and
-// there are NaN values among them.
+// Scales of a 16-token step: the key's times sm_scale * log2(e), and of the value's
+// the logarithm and the reciprocal.
+struct StepScale {
+    float key, log_v, inv_v;
+};
+
+// Tokens t0 .. t0 + 63 in a stage folded into the wave's rows.  mask: some row does
+// not see them all.
 template <int DP, bool BF16>
 __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char *kst, const unsigned char *vst, int t0,
-                                          const float2 (&sc)[4], unsigned lost, int lane, bool mask, bool odd)
+                                          const StepScale (&sc)[4], int lane, bool mask)
 {
     const int g = lane >> 5, n = lane & 31;
     f32x16 S[2];
@@ -108,14 +120,8 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
         for (int mt = 0; mt < 2; ++mt)
             S[mt] = mfma32<BF16>(*(const u32x4 *)(kst + off + 64 * DP * mt), W.q[s], S[mt]);
     }
-    if (lost) {
-#pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                S[mt][i] = lost >> (2 * mt + (i >> 3)) & 1 ? __builtin_nanf("") : S[mt][i];
-    }
     if (mask) {
+        asm volatile("");   // a branch, not 32 selects in every tile
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -129,7 +135,7 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
 #pragma unroll
         for (int i = 1; i < 8; ++i)
             a = fmaxf(a, S[st >> 1][8 * (st & 1) + i]);
-        mx = fmaxf(mx, a * sc[st].x);
+        mx = fmaxf(mx, __builtin_fmaf(a, sc[st].key, sc[st].log_v));
     }
     mx = other_max(mx);
     const bool raise = mx > W.m + 8.0f;
@@ -144,25 +150,29 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
             for (int i = 0; i < 16; ++i)
                 W.o[dt][i] *= alpha;
     }
-    unsigned hi[2][8], lo[2][8];
-    float ls[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int TERMS = BF16 ? 1 : 2;
+    unsigned pt[TERMS][2][8];
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
+    for (int st = 0; st < 4; ++st) {
+        const float add = sc[st].log_v - W.m;
+        float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 f = sc[2 * mt + (i >> 2)];
-            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(S[mt][2 * i], f.x, -W.m));
-            const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[mt][2 * i + 1], f.x, -W.m));
-            ls[(2 * i) & 3] += a;
-            ls[(2 * i + 1) & 3] += b;
-            split_bf16(a * f.y, b * f.y, hi[mt][i], lo[mt][i]);
+        for (int i = 4 * (st & 1); i < 4 * (st & 1) + 4; ++i) {
+            const float a = __builtin_amdgcn_exp2f(__builtin_fmaf(S[st >> 1][2 * i], sc[st].key, add));
+            const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[st >> 1][2 * i + 1], sc[st].key, add));
+            sum[0] += a;
+            sum[1] += b;
+            if constexpr (BF16)
+                pt[0][st >> 1][i] = pack_f16(a, b);
+            else
+                split_bf16(a, b, pt[0][st >> 1][i], pt[1][st >> 1][i]);
         }
-    W.l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+        W.l = __builtin_fmaf(sum[0] + sum[1], sc[st].inv_v, W.l);
+    }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
         const int mt = s >> 1, r = 4 * (s & 1);
-        const u32x4 ph = {hi[mt][r], hi[mt][r + 1], hi[mt][r + 2], hi[mt][r + 3]};
-        const u32x4 pl = {lo[mt][r], lo[mt][r + 1], lo[mt][r + 2], lo[mt][r + 3]};
+        u32x4 vf[DP / 32];
 #pragma unroll
         for (int dt = 0; dt < DP / 32; ++dt) {
             typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
@@ -170,30 +180,14 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
             const s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)src);
             const s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(src + 16 * DP));
             const uint2 a = __builtin_bit_cast(uint2, v0), b = __builtin_bit_cast(uint2, v1);
-            u32x4 vf = {a.x, a.y, b.x, b.y};
-            if (odd) {
-                // NaN values reach the rows that see them, and no others: counted by
-                // products of 0 / 1, then taken out of the operand
-                u32x4 ind, see;
+            vf[dt] = u32x4{a.x, a.y, b.x, b.y};
+        }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const unsigned nn = nan_pairs(vf[e]);
-                    ind[e] = nn * 0x3f80u;
-                    vf[e] &= ~(nn * 0xffffu);
-                    const int t = t0 + 16 * s + 8 * (e >> 1) + 4 * g + 2 * (e & 1);
-                    see[e] = (t < W.vis ? 0x3f80u : 0u) | (t + 1 < W.vis ? 0x3f800000u : 0u);
-                }
-                f32x16 cnt;
+        for (int k = 0; k < TERMS; ++k) {
+            const u32x4 w = {pt[k][mt][r], pt[k][mt][r + 1], pt[k][mt][r + 2], pt[k][mt][r + 3]};
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    cnt[i] = 0.0f;
-                cnt = mfma32<true>(ind, see, cnt);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    W.o[dt][i] = cnt[i] > 0.0f ? __builtin_nanf("") : W.o[dt][i];
-            }
-            W.o[dt] = mfma32<true>(vf, ph, W.o[dt]);
-            W.o[dt] = mfma32<true>(vf, pl, W.o[dt]);
+            for (int dt = 0; dt < DP / 32; ++dt)
+                W.o[dt] = mfma32<!BF16>(vf[dt], w, W.o[dt]);
         }
     }
 }
@@ -203,7 +197,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
 {
     constexpr int RM = kTileRows, TPR = DP / 16, PASS = 64 * kTileWaves / TPR, NP = kTile / PASS;
     __shared__ __attribute__((aligned(16))) unsigned char ks[2][kTile * DP * 2], vs[2][kTile * DP * 2];
-    __shared__ int odd_tile[2];
+    __shared__ int met_nan;
     const int lane = threadIdx.x & 63, g = lane >> 5, n = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // pairs vary fastest, so with a multiple of eight pairs a pair's pages stay in
@@ -258,19 +252,20 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
     const uint8_t *vp = p.c.value + kh * p.c.value_s_head + (cut ? 0 : 16 * lc);
     const float *sp = p.c.scale + kh * p.c.scale_s_head;
     u32x4 kr[NP], vr[NP];
-    float2 sc[4], sc_next[4];
-    unsigned lost = 0, lost_next = 0;
+    StepScale sc[4], sc_next[4];
+    unsigned lost = 0;   // bits of the next tile's steps that have no page
     auto load = [&](int tile) {
         int64_t page[4];
-        lost_next = 0;
+        lost = 0;
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
             const int id = uniform_load(table + min((tile * kTile + 16 * st) >> lg, last));
             const bool bad = bad_page(p.c, id);
             page[st] = bad ? 0 : id;
-            lost_next |= (bad ? 1u : 0u) << st;
+            lost |= (bad ? 1u : 0u) << st;
             const uint64_t x = uniform_load((const uint64_t *)(sp + page[st] * p.c.scale_s_page));
-            sc_next[st] = make_float2(__builtin_bit_cast(float, (uint32_t)x) * p.cs, __builtin_bit_cast(float, (uint32_t)(x >> 32)));
+            const float vs = fmaxf(__builtin_bit_cast(float, (uint32_t)(x >> 32)), 1.175494351e-38f);
+            sc_next[st] = StepScale{__builtin_bit_cast(float, (uint32_t)x) * p.cs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
@@ -288,32 +283,40 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int rw = lr + PASS * j;
-            if (ragged) {   // rows no query sees hold anything
+            if (ragged) {
+                // tokens that not every row sees: rows no query sees hold anything, and
+                // a NaN would reach the others as 0 * NaN (it is put back at the end)
                 if (tile * kTile + rw >= vis_max)
                     vr[j] = u32x4{0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    odd |= nan_codes(vr[j][e]) != 0;
+                for (int e = 0; e < 4; ++e) {
+                    const unsigned nn = nan_codes(vr[j][e]);
+                    odd |= nn != 0;
+                    vr[j][e] &= ~((nn >> 7) * 0xffu);
+                }
             }
             u32x4 x[2];
+            if (lost) {   // keys of a missing page are NaN: so are the scores of rows that see them
+                const unsigned c = lost >> ((64 / TPR * wave + PASS * j) >> 4) & 1 ? 0x7f7f7f7fu : 0u;
+                kr[j] = kr[j] | c;
+            }
             widen16<BF16>(cut ? u32x4{0, 0, 0, 0} : kr[j], x);
             unsigned char *k = ks[stage] + rw * 2 * DP;
             *(u32x4 *)(k + 16 * key_slot<DP>(rw, 2 * lc)) = x[0];
             *(u32x4 *)(k + 16 * key_slot<DP>(rw, 2 * lc + 1)) = x[1];
-            widen16<true>(vr[j], x);
+            widen16<!BF16>(vr[j], x);
             unsigned char *v = vs[stage] + rw * 2 * DP;
             *(u32x4 *)(v + 16 * value_slot<DP>(rw, 2 * lc)) = x[0];
             *(u32x4 *)(v + 16 * value_slot<DP>(rw, 2 * lc + 1)) = x[1];
         }
-        if (__ballot(odd) && lane == 0)
-            odd_tile[stage] = tile;
+        if (odd)
+            met_nan = 1;
 #pragma unroll
         for (int st = 0; st < 4; ++st)
             sc[st] = sc_next[st];
-        lost = lost_next;
     };
-    if (threadIdx.x < 2)
-        odd_tile[threadIdx.x] = -1;
+    if (threadIdx.x == 0)
+        met_nan = 0;
     __syncthreads();
     if (first < end) {
         load(first);
@@ -326,11 +329,35 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
         if (more)
             load(tile + 1);
         if (t0 < wave_max) {
-            const bool mask = t0 + kTile > wave_min;
-            tile_step<DP, BF16>(W, ks[stage], vs[stage], t0, sc, lost, lane, mask, mask && odd_tile[stage] == tile);
+            tile_step<DP, BF16>(W, ks[stage], vs[stage], t0, sc, lane, t0 + kTile > wave_min);
         }
         if (more)
             store(tile + 1, stage ^ 1);
+    }
+
+    __syncthreads();
+    if (met_nan) {
+        // the NaN values taken out above, to the rows that see them
+        for (int tok = max(first, vis_min / kTile) * kTile; tok < min(end * kTile, vis_max); ++tok) {
+            const int id = uniform_load(table + (tok >> lg));
+            if (bad_page(p.c, id))
+                continue;   // its rows' scores are NaN already
+            const uint8_t *v = p.c.value + id * p.c.value_s_page + kh * p.c.value_s_head +
+                               ((uint32_t)tok & ((1u << lg) - 1)) * p.c.value_s_tok;
+#pragma unroll
+            for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int ch = 32 * dt + 8 * j + 4 * g;
+                    if (CUT && ch >= p.c.D)
+                        continue;
+                    const unsigned nn = nan_codes(*(const unsigned *)(v + ch));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (nn >> (8 * e + 7) & 1 && tok < W.vis)
+                            W.o[dt][4 * j + e] = __builtin_nanf("");
+                }
+        }
     }
 
     const float l = other_sum(W.l);

@@ -98,12 +98,13 @@ class Ref:
         return out
 
     def attend(self, q, table, lens, q_lens=None, causal=True, sm_scale=None):
-        """(out, lse, spread): spread = softmax @ |v|, the size of what the sums add up;
-        and the largest sum of |q k| * sm_scale of a row."""
+        """(out, lse, spread, mag, small): spread = softmax @ |v|, the size of what the sums
+        add up; mag the largest sum of |q k| * sm_scale of a row; small = the largest weight
+        times value scale, times the sum of |code|, of a channel."""
         B, Hq, T, D = q.shape
         sm = D ** -0.5 if sm_scale is None else sm_scale
         gq = Hq // self.H
-        out, spread = np.zeros((2, B, Hq, T, D))
+        out, spread, small = np.zeros((3, B, Hq, T, D))
         lse = np.full((B, Hq, T), -np.inf)
         mag = np.zeros((B, Hq, T))
         for b in range(B):
@@ -112,8 +113,9 @@ class Ref:
                 out[b], lse[b] = np.nan, np.nan
                 continue
             kv = self.tokens(table, b, 0, n)
+            ids = [self.page(table, b, i // self.G) for i in range(n)]
             for h in range(Hq):
-                k, v = kv[0, h // gq], kv[1, h // gq]
+                k, v, vs = kv[0, h // gq], kv[1, h // gq], self.scale[ids, h // gq, 1]
                 for i in range(t):
                     e = n - t + i + 1 if causal else n
                     if e <= 0:
@@ -125,20 +127,27 @@ class Ref:
                         w /= w.sum()
                         out[b, h, i] = w @ v[:e]
                         spread[b, h, i] = w @ np.abs(v[:e])
+                        small[b, h, i] = np.max(w * vs[:e]) * (np.abs(v[:e]) / vs[:e, None]).sum(0)
                         mag[b, h, i] = np.nanmax(np.abs(k[:e]) @ np.abs(q[b, h, i]) * sm, initial=0.0)
-        return out, lse, spread, mag
+        return out, lse, spread, mag, small
 
 
-def tolerance(dtype, ref, spread, mag, D, n):
-    """How far an attention output may be off: half a step of its type; and of what the
-    sums add up, twice (weight and total) the error of a weight: 2^-17 of its two bf16
-    terms, fp32 scores (D products and sums and 4 factors, 2^-24 of `mag` each, an
-    exponent's absolute error being the weight's relative one; log2(e) * 2^-24 of `mag`
-    for the exponent's own rounding), exp2 to 2^-22, and fp32 sums of n weights (n 2^-24,
-    in the weighted sum too)."""
+def tolerance(dtype, ref, spread, mag, small, rows, D, n):
+    """How far an attention output may be off: half a step of its type, and of what the
+    sums add up the errors of the weights:
+    * twice (weight and total) fp32's: scores of D products and sums and 6 factors, 2^-24
+      of `mag` each, an exponent's absolute error being the weight's relative one; exp2 and
+      the logarithm of a scale, 2^-20 together (log2 of 2^-64 .. 2^120 to 2^-24 of it);
+      sums of n weights, n 2^-24;
+    * the weights' own: two bf16 terms, each rounded to nearest by 2^-9: 2^-18, 2^-17 with
+      the remainder's own rounding; for bf16 and more than 32 rows of a KV head one fp16
+      term, 2^-11, and where a weight lies below fp16's normal numbers 2^-25 of the largest
+      weight times its scale, on every code."""
     half = torch.finfo(dtype).eps / 2
-    w = 2 * (2.0 ** -17 + (D + 6) * 2.0 ** -24 * mag + 2.0 ** -22 + n * 2.0 ** -24)
-    return half * np.abs(ref) + w[..., None] * spread + float(torch.finfo(dtype).smallest_normal) * half * 2
+    one = dtype == torch.bfloat16 and rows > 32
+    w = 2 * ((D + 6) * 2.0 ** -24 * mag + 2.0 ** -20 + n * 2.0 ** -24) + (2.0 ** -11 if one else 2.0 ** -17)
+    return (half * np.abs(ref) + w[..., None] * spread + (2.0 ** -25 * small if one else 0.0)
+            + float(torch.finfo(dtype).smallest_normal) * half * 2)
 
 
 def numpy(t):

@@ -212,8 +212,9 @@ def check_attend(cache, q, table, lens, q_lens=None, causal=True, sm_scale=None,
     out, lse = cache.attend(q.to(dev), table, i32(lens, dev), q_lens=None if q_lens is None else i32(q_lens, dev),
                             causal=causal, sm_scale=sm_scale, return_lse=True, **kw)
     assert out.dtype == q.dtype and out.shape == q.shape
-    want, wlse, spread, mag = Ref(cache).attend(numpy(q), table.cpu().numpy(), lens, q_lens, causal, sm_scale)
-    tol = tolerance(q.dtype, want, spread, mag, q.shape[3], max(max(lens), 1))
+    want, wlse, spread, mag, small = Ref(cache).attend(numpy(q), table.cpu().numpy(), lens, q_lens, causal, sm_scale)
+    tol = tolerance(q.dtype, want, spread, mag, small, q.shape[1] // cache.num_kv_heads * q.shape[2], q.shape[3],
+                    max(max(lens), 1))
     got, glse = numpy(out), numpy(lse)
     np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
     bad = np.abs(got - want) > tol
