@@ -252,20 +252,24 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
     const uint8_t *vp = p.c.value + kh * p.c.value_s_head + (cut ? 0 : 16 * lc);
     const float *sp = p.c.scale + kh * p.c.scale_s_head;
     u32x4 kr[NP], vr[NP];
-    StepScale sc[4], sc_next[4];
-    unsigned lost = 0;   // bits of the next tile's steps that have no page
+    StepScale sc[4];
+    uint64_t raw[4];         // the next tile's scales
+    int ids[4];              // page ids of the tile that load() takes
+    unsigned lost = 0;       // bits of the next tile's steps that have no page
+    auto fetch_ids = [&](int tile) {
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+            ids[st] = uniform_load(table + min((tile * kTile + 16 * st) >> lg, last));
+    };
     auto load = [&](int tile) {
         int64_t page[4];
         lost = 0;
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
-            const int id = uniform_load(table + min((tile * kTile + 16 * st) >> lg, last));
-            const bool bad = bad_page(p.c, id);
-            page[st] = bad ? 0 : id;
+            const bool bad = bad_page(p.c, ids[st]);
+            page[st] = bad ? 0 : ids[st];
             lost |= (bad ? 1u : 0u) << st;
-            const uint64_t x = uniform_load((const uint64_t *)(sp + page[st] * p.c.scale_s_page));
-            const float vs = fmaxf(__builtin_bit_cast(float, (uint32_t)(x >> 32)), 1.175494351e-38f);
-            sc_next[st] = StepScale{__builtin_bit_cast(float, (uint32_t)x) * p.cs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+            raw[st] = uniform_load((const uint64_t *)(sp + page[st] * p.c.scale_s_page));
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
@@ -276,6 +280,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
             kr[j] = *(const u32x4 *)(kp + pg * p.c.key_s_page + rw * p.c.key_s_tok);
             vr[j] = *(const u32x4 *)(vp + pg * p.c.value_s_page + rw * p.c.value_s_tok);
         }
+        fetch_ids(tile + 1);   // a step ahead: the loads above wait for no scalar load of their own
     };
     auto store = [&](int tile, int stage) {
         bool odd = false;
@@ -312,13 +317,16 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
         if (odd)
             met_nan = 1;
 #pragma unroll
-        for (int st = 0; st < 4; ++st)
-            sc[st] = sc_next[st];
+        for (int st = 0; st < 4; ++st) {
+            const float vs = fmaxf(__builtin_bit_cast(float, (uint32_t)(raw[st] >> 32)), 1.175494351e-38f);
+            sc[st] = StepScale{__builtin_bit_cast(float, (uint32_t)raw[st]) * p.cs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+        }
     };
     if (threadIdx.x == 0)
         met_nan = 0;
     __syncthreads();
     if (first < end) {
+        fetch_ids(first);
         load(first);
         store(first, 0);
     }
