@@ -414,26 +414,33 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
     }
 }
 
-// Joins the partials of ROWS rows (4: one a wave, 1: one for the four waves, where
-// rows are too few to fill the device); also, after the row kernel, the rows no
+// Joins the partials of each row; also, after the row kernel, the rows no
 // workgroup touched: of sequences without tokens (0) and of broken lengths (NaN).
-// TILES: the partials are the tile kernel's p.splits parts.
-template <int DP, bool BF16, bool TILES, int ROWS>
+// DP / 4 lanes take a row, four channels each.  ALONE: a workgroup per row, whose
+// lane groups share its partials and join in LDS (few rows, many partials);
+// otherwise a row per lane group.  TILES: the partials are the tile kernel's
+// p.splits parts.
+template <int DP, bool BF16, bool TILES, bool ALONE>
 __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, int RM)
 {
-    constexpr int CPL = DP / 64, STEP = ROWS == 1 ? kWaves : 1;   // channels per lane, partials between a wave's
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int rows = p.gq * p.T, all = ROWS == 1 ? blockIdx.x : blockIdx.x * ROWS + wave;
+    constexpr int LPR = DP / 4, GROUPS = 64 * kWaves / LPR, STEP = ALONE ? GROUPS : 1;
+    const int group = threadIdx.x / LPR, ch = 4 * (threadIdx.x % LPR);
+    const int rows = p.gq * p.T, all = ALONE ? blockIdx.x : blockIdx.x * GROUPS + group;
     const int pair = all / rows, row = all - pair * rows;
-    if (ROWS > 1 && pair >= p.B * p.c.H)
+    if (!ALONE && pair >= p.B * p.c.H)
         return;
     const int b = pair / p.c.H, kh = pair - b * p.c.H, rb = row / RM, r = row - rb * RM;
     const int t = row / p.gq, h = kh * p.gq + row - t * p.gq;
     const Seq8 sq = seq8(p, b);
-    float m = kLowest, l = 0.0f, o[CPL];
-#pragma unroll
-    for (int e = 0; e < CPL; ++e)
-        o[e] = 0.0f;
+    float m = kLowest, l = 0.0f;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto fold = [&](float m1, float l1, float4 x) {
+        const float mn = fmaxf(m, m1);
+        const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(m1 - mn);
+        m = mn;
+        l = f0 * l + f1 * l1;
+        o.x = f0 * o.x + f1 * x.x, o.y = f0 * o.y + f1 * x.y, o.z = f0 * o.z + f1 * x.z, o.w = f0 * o.w + f1 * x.w;
+    };
     if (sq.bad) {
         l = __builtin_nanf("");
     } else if (sq.n > 0) {
@@ -444,70 +451,44 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
         if (tab.x < 0)
             return;
         const int first = tab.x >> 1, count = TILES ? p.splits : tab.y - first + 1;
-        auto slot = [&](int i) {
-            if constexpr (TILES)
-                return ((int64_t)item * p.splits + i) * RM + r;
-            else
-                return (int64_t)(i == 0 ? tab.x : 2 * (first + i)) * RM + r;
-        };
-        for (int i = ROWS == 1 ? wave : 0; i < count; i += 4 * STEP) {
+        for (int i = ALONE ? group : 0; i < count; i += 4 * STEP) {
             float2 ml[4];
-            float x[4][CPL];
+            float4 x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int64_t s = slot(min(i + j * STEP, count - 1));
+                const int k = min(i + j * STEP, count - 1);
+                const int64_t s = TILES ? ((int64_t)item * p.splits + k) * RM + r
+                                        : (int64_t)(k == 0 ? tab.x : 2 * (first + k)) * RM + r;
                 ml[j] = p.ws_ml[s];
-#pragma unroll
-                for (int e = 0; e < CPL; ++e)
-                    x[j][e] = p.ws_o[s * DP + CPL * lane + e];
+                x[j] = *(const float4 *)(p.ws_o + s * DP + ch);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (i + j * STEP >= count)
-                    break;
-                const float mn = fmaxf(m, ml[j].x);
-                const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(ml[j].x - mn);
-                m = mn;
-                l = f0 * l + f1 * ml[j].y;
-#pragma unroll
-                for (int e = 0; e < CPL; ++e)
-                    o[e] = f0 * o[e] + f1 * x[j][e];
-            }
+            for (int j = 0; j < 4; ++j)
+                if (i + j * STEP < count)
+                    fold(ml[j].x, ml[j].y, x[j]);
         }
     }
-    const bool none = !sq.bad && visible8(p, sq, t) == 0;
-    uint16_t *out = p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok;
-    if constexpr (ROWS == 1) {
-        __shared__ float lds_o[kWaves][DP];
-        __shared__ float2 lds_ml[kWaves];
-#pragma unroll
-        for (int e = 0; e < CPL; ++e)
-            lds_o[wave][CPL * lane + e] = o[e];
-        if (lane == 0)
-            lds_ml[wave] = make_float2(m, l);
+    if constexpr (ALONE) {
+        __shared__ __attribute__((aligned(16))) float lds_o[GROUPS][DP];
+        __shared__ float2 lds_ml[GROUPS];
+        *(float4 *)&lds_o[group][ch] = o;
+        if (ch == 0)
+            lds_ml[group] = make_float2(m, l);
         __syncthreads();
-        const int ch = threadIdx.x;
-        if (ch >= p.c.D)
+        if (group != 0)
             return;
-        float M = kLowest, L = 0.0f, acc = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w)
-            M = fmaxf(M, lds_ml[w].x);
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(lds_ml[w].x - M);
-            L += f * lds_ml[w].y;
-            acc += f * lds_o[w][ch];
-        }
-        out[ch] = f2x(none ? 0.0f : acc / L, BF16);
-        m = M, l = L;
-    } else {
-#pragma unroll
-        for (int e = 0; e < CPL; ++e)
-            if (CPL * lane + e < p.c.D)
-                out[CPL * lane + e] = f2x(none ? 0.0f : o[e] / l, BF16);
+        for (int k = 1; k < GROUPS; ++k)
+            fold(lds_ml[k].x, lds_ml[k].y, *(const float4 *)&lds_o[k][ch]);
     }
-    if ((ROWS == 1 ? threadIdx.x : lane) == 0 && p.lse)
+    if (ch >= p.c.D)
+        return;
+    const bool none = !sq.bad && visible8(p, sq, t) == 0;
+    const float inv = none ? 0.0f : 1.0f / l;
+    *(uint2 *)(p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok + ch) =
+        make_uint2((uint32_t)f2x(o.x * inv, BF16) | (uint32_t)f2x(o.y * inv, BF16) << 16,
+                   (uint32_t)f2x(o.z * inv, BF16) | (uint32_t)f2x(o.w * inv, BF16) << 16);
+    if (ch == 0 && p.lse)
         p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
 }
 
@@ -528,7 +509,7 @@ struct Plan8 {
     size_t o_bytes, ml_bytes, bytes;
 };
 
-// Rows from which the merge gives each a wave instead of four.
+// Rows from which the merge gives each a lane group instead of a workgroup.
 constexpr int64_t kMergeRows = 2048;
 // Rows that the row kernel takes: two blocks of 16, whose codes are read once.
 constexpr int kRowKernelRows = 32;
@@ -643,10 +624,13 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
         constexpr bool BF = decltype(bf)::value, TILES = decltype(tiles)::value;
         const int64_t rows = (int64_t)p.B * p.Hq * p.T;
         const int RM = TILES ? kTileRows : 16 * pl.RT;
-        if (rows < kMergeRows)
-            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, 1>), dim3((unsigned)rows), block, 0, st, p, RM);
-        else
-            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, 4>), dim3((unsigned)((rows + 3) / 4)), block, 0, st, p, RM);
+        if (rows < kMergeRows) {
+            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, true>), dim3((unsigned)rows), block, 0, st, p, RM);
+        } else {
+            const int64_t groups = 256 * kWaves / DP;
+            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, false>), dim3((unsigned)((rows + groups - 1) / groups)), block,
+                               0, st, p, RM);
+        }
     };
     auto rows = [&](auto dp, auto rt, auto bf) {
         constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
