@@ -246,11 +246,11 @@ def load() -> ctypes.CDLL:
     L.kitty_store_prompt.argtypes = [ctypes.POINTER(PromptArgs), _vp]
     L.kitty_zero_regions.argtypes = [ctypes.POINTER(ZeroRegion), _i32, _vp]
     L.kitty_prefill_attention.argtypes = [ctypes.POINTER(PrefillArgs), _vp]
-    L.kitty_cache8_write.argtypes = [ctypes.POINTER(Cache8), ctypes.POINTER(Cache8RowsArgs), _vp]
+    # the argument structures as packed bytes or by reference
+    L.kitty_cache8_write.argtypes = [ctypes.POINTER(Cache8), _vp, _vp]
     L.kitty_cache8_read.argtypes = L.kitty_cache8_write.argtypes
-    L.kitty_cache8_attention_workspace_size.argtypes = [ctypes.POINTER(Cache8), ctypes.POINTER(Cache8AttentionArgs),
-                                                        ctypes.POINTER(ctypes.c_size_t)]
-    L.kitty_cache8_attention.argtypes = [ctypes.POINTER(Cache8), ctypes.POINTER(Cache8AttentionArgs), _vp]
+    L.kitty_cache8_attention_workspace_size.argtypes = [ctypes.POINTER(Cache8), _vp, ctypes.POINTER(ctypes.c_size_t)]
+    L.kitty_cache8_attention.argtypes = L.kitty_cache8_write.argtypes
     if L.kitty_abi_version() != KITTY_ABI_VERSION:
         raise ImportError(f"libkitty_hip ABI {L.kitty_abi_version()} != {KITTY_ABI_VERSION}")
     _lib = L

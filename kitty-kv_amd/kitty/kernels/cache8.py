@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional, Tuple, Union
 
 import torch
@@ -26,37 +27,15 @@ from .ops import _need, calls_followed
 
 _SRC = {torch.float16: _hip.KITTY_SRC_F16, torch.bfloat16: _hip.KITTY_SRC_BF16, torch.float32: _hip.KITTY_SRC_F32}
 _PAGE_TOKENS = (16, 32, 64, 128, 256)
+# kitty_cache8_write_args / _read_args and kitty_cache8_attention_args as the C
+# compiler lays them out (packing one takes a quarter of a ctypes structure's time)
+_ROWS = struct.Struct("2P6qPq2P4i")
+_ATTENTION = struct.Struct("3P6qPq2P7ifPN")
 
 
-def _i32(t: Optional[torch.Tensor], B: int, name: str, dev: torch.device) -> int:
-    """Address of an int32 (B,) tensor on the cache's device (0 for None)."""
-    if t is None:
-        return 0
-    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == B and (B <= 1 or t.stride(0) == 1),
-          f"{name} must be int32 ({B},)")
-    if t.device != dev:
-        raise RuntimeError(f"{name} is on {t.device}, the cache on {dev}")
-    return t.data_ptr()
-
-
-def _table(t: torch.Tensor, B: int, dev: torch.device) -> Tuple[int, int, int]:
-    """(address, row stride, page numbers) of a block table."""
-    _need(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == B and (t.shape[1] <= 1 or t.stride(1) == 1),
-          f"block_table must be int32 ({B}, W) with contiguous rows")
-    if t.device != dev:
-        raise RuntimeError(f"block_table is on {t.device}, the cache on {dev}")
-    return t.data_ptr(), t.stride(0) if B > 1 else 0, t.shape[1]
-
-
-def _plain(t: torch.Tensor, name: str, dev: torch.device) -> torch.Tensor:
-    """`t` as a kernel may read it by pointer, channels next to each other."""
-    if t.device != dev:
-        raise RuntimeError(f"{name} is on {t.device}, the cache on {dev}")
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{name} needs a gradient and the 8-bit cache has no backward: call under torch.no_grad()")
-    if t.is_neg():
-        t = t.resolve_neg()
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+def _sig(t: Optional[torch.Tensor]):
+    """What the checks of a tensor depend on, but for its address."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 def _strides(t: torch.Tensor) -> Tuple[int, ...]:
@@ -64,13 +43,15 @@ def _strides(t: torch.Tensor) -> Tuple[int, ...]:
     return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
 
 
-def _rows16(t: torch.Tensor) -> Tuple[torch.Tensor, Tuple[int, ...]]:
-    """A 16-bit tensor with 16-byte aligned rows (a copy if it has none), and its strides."""
-    s = _strides(t)
-    if s[0] % 8 or s[1] % 8 or s[2] % 8 or t.data_ptr() % 16:
-        t = t.clone(memory_format=torch.contiguous_format)
-        s = _strides(t)
-    return t, s
+def _aligned16(t: torch.Tensor) -> bool:
+    return all(s * t.element_size() % 16 == 0 for s in _strides(t))
+
+
+def _given(t: torch.Tensor, name: str) -> torch.Tensor:
+    """A tensor of values as a kernel may read it by pointer."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{name} needs a gradient and the 8-bit cache has no backward: call under torch.no_grad()")
+    return t.resolve_neg() if t.is_neg() else t
 
 
 class Cache8:
@@ -117,9 +98,11 @@ class Cache8:
         self._c = _hip.Cache8(key.data_ptr(), value.data_ptr(), scale.data_ptr(), *_strides(key)[:2], key.stride(2),
                               *_strides(value)[:2], value.stride(2), *_strides(scale)[:2], P, H, D, G)
         self._ref = ctypes.byref(self._c)
-        self._ws: dict = {}      # workspace bytes by the shapes they depend on
+        # what a call of these shapes, strides and types was found to need (the
+        # checks of a signature run once; addresses are looked at in every call)
+        self._known: dict = {}
         # a batch of none: what the library refuses of the pools, it refuses here
-        _hip.check(self._lib.kitty_cache8_write(self._ref, ctypes.byref(_hip.Cache8RowsArgs()), None))
+        _hip.check(self._lib.kitty_cache8_write(self._ref, _ROWS.pack(*[0] * 16), None))
 
     @classmethod
     def empty(cls, num_pages: int, num_kv_heads: int, head_dim: int, page_tokens: int = 128,
@@ -129,20 +112,45 @@ class Cache8:
         k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2))
         return cls(k, v, torch.ones(num_pages, num_kv_heads, 2, device=device))
 
-    # ------------------------------------------------------------------ calls
-    def _launch(self, fn, args) -> None:
-        """`fn` on the current stream of the pools' device."""
-        if torch._C._cuda_getDevice() != self._index:
-            with torch.cuda.device(self._index):
-                _hip.check(fn(self._ref, ctypes.byref(args), _hip.stream_ptr(self.device)))
-        else:
-            _hip.check(fn(self._ref, ctypes.byref(args), _hip.stream_ptr(self.device)))
+    # ----------------------------------------------------------------- checks
+    def _here(self, name: str, t: torch.Tensor) -> None:
+        if t.device != self.device:
+            raise RuntimeError(f"{name} is on {t.device}, the cache on {self.device}")
+
+    def _i32(self, name: str, t: Optional[torch.Tensor], B: int, optional: bool = False) -> None:
+        if t is None and optional:
+            return
+        _need(t is not None and t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == B and (B <= 1 or t.stride(0) == 1),
+              f"{name} must be int32 ({B},)")
+        self._here(name, t)
+
+    def _check_table(self, t: torch.Tensor, B: int) -> None:
+        _need(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == B and (t.shape[1] <= 1 or t.stride(1) == 1),
+              f"block_table must be int32 ({B}, W) with contiguous rows")
+        self._here("block_table", t)
+
+    def _keep(self, sig, found):
+        if len(self._known) >= 512:
+            self._known.clear()
+        self._known[sig] = found
+        return found
 
     @staticmethod
     def _followed() -> None:
         if calls_followed():
             raise NotImplementedError("calls of the 8-bit cache cannot be traced, compiled or transformed")
 
+    def _launch(self, fn, args: bytes) -> None:
+        """`fn` on the current stream of the pools' device."""
+        if torch._C._cuda_getDevice() != self._index:
+            with torch.cuda.device(self._index):
+                rc = fn(self._ref, args, _hip.stream_ptr(self.device))
+        else:
+            rc = fn(self._ref, args, _hip.stream_ptr(self.device))
+        if rc:
+            _hip.check(rc)
+
+    # ------------------------------------------------------------------ calls
     def write(self, key: torch.Tensor, value: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
               lens: Optional[torch.Tensor] = None) -> None:
         """Rows t < lens[b] (all T where lens is None) of key and value (B, H, T, D)
@@ -156,24 +164,33 @@ class Cache8:
         Tokens without a page (a negative start, a page number past the table, an
         id outside the pool) are dropped."""
         self._followed()
-        _need(key.dim() == 4 and key.shape[1] == self.num_kv_heads and key.shape[3] == self.head_dim,
-              f"key must be (B, {self.num_kv_heads}, T, {self.head_dim})")
-        _need(value.shape == key.shape and value.dtype == key.dtype, "value must have key's shape and dtype")
-        _need(key.dtype in _SRC, "key and value must be float16, bfloat16 or float32")
-        B, _, T, _ = key.shape
-        dev = self.device
-        key, value = _plain(key, "key", dev), _plain(value, "value", dev)
-        bt, bt_stride, W = _table(block_table, B, dev)
-        _need(start is not None, "start must be given")
-        start_p, lens_p = _i32(start, B, "start", dev), _i32(lens, B, "lens", dev)
-        if B == 0 or T == 0:
-            return
-        if not self._on_device:
-            cpu8.write(self.key, self.value, self.scale, key, value, block_table, start, lens)
-            return
-        self._launch(self._lib.kitty_cache8_write, _hip.Cache8RowsArgs(
-            key.data_ptr(), value.data_ptr(), *_strides(key), *_strides(value), bt, bt_stride, start_p, lens_p, B, T, W,
-            _SRC[key.dtype]))
+        key, value = _given(key, "key"), _given(value, "value")
+        sig = ("write", _sig(key), _sig(value), _sig(block_table), _sig(start), _sig(lens))
+        found = self._known.get(sig) if self._on_device else None
+        if found is None:
+            _need(key.dim() == 4 and key.shape[1] == self.num_kv_heads and key.shape[3] == self.head_dim,
+                  f"key must be (B, {self.num_kv_heads}, T, {self.head_dim})")
+            _need(value.shape == key.shape and value.dtype == key.dtype, "value must have key's shape and dtype")
+            _need(key.dtype in _SRC, "key and value must be float16, bfloat16 or float32")
+            self._here("key", key)
+            self._here("value", value)
+            B, _, T, _ = key.shape
+            self._check_table(block_table, B)
+            self._i32("start", start, B)
+            self._i32("lens", lens, B, optional=True)
+            if key.stride(3) != 1 or value.stride(3) != 1:
+                return self.write(key.contiguous(), value.contiguous(), block_table, start, lens)
+            if B == 0 or T == 0:
+                return
+            if not self._on_device:
+                cpu8.write(self.key, self.value, self.scale, key, value, block_table, start, lens)
+                return
+            found = self._keep(sig, ((*_strides(key), *_strides(value)), block_table.stride(0) if B > 1 else 0,
+                                     (B, T, block_table.shape[1], _SRC[key.dtype])))
+        strides, bt_stride, rest = found
+        self._launch(self._lib.kitty_cache8_write, _ROWS.pack(
+            key.data_ptr(), value.data_ptr(), *strides, block_table.data_ptr(), bt_stride, start.data_ptr(),
+            0 if lens is None else lens.data_ptr(), *rest))
 
     def read(self, block_table: torch.Tensor, lens: torch.Tensor, tokens: int, start: Optional[torch.Tensor] = None,
              dtype: torch.dtype = torch.float16,
@@ -184,29 +201,47 @@ class Cache8:
         token has no page."""
         self._followed()
         tokens = int(tokens)
-        _need(tokens >= 0, "tokens must not be negative")
-        _need(block_table.dim() == 2, "block_table must be int32 (B, W)")
-        B, dev = block_table.shape[0], self.device
-        bt, bt_stride, W = _table(block_table, B, dev)
-        _need(lens is not None, "lens must be given")
-        lens_p, start_p = _i32(lens, B, "lens", dev), _i32(start, B, "start", dev)
-        shape = (B, self.num_kv_heads, tokens, self.head_dim)
+        sig = ("read", tokens, dtype, _sig(block_table), _sig(lens), _sig(start),
+               None if out is None else (_sig(out[0]), _sig(out[1])))
+        found = self._known.get(sig) if self._on_device else None
+        if found is None:
+            _need(tokens >= 0, "tokens must not be negative")
+            _need(block_table.dim() == 2, "block_table must be int32 (B, W)")
+            B = block_table.shape[0]
+            self._check_table(block_table, B)
+            self._i32("lens", lens, B)
+            self._i32("start", start, B, optional=True)
+            shape = (B, self.num_kv_heads, tokens, self.head_dim)
+            if out is None:
+                _need(dtype in _SRC, "dtype must be float16, bfloat16 or float32")
+                k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
+            else:
+                k, v = out
+                for t in out:
+                    _need(tuple(t.shape) == shape and t.dtype == k.dtype and t.dtype in _SRC and t.stride(3) == 1,
+                          f"out must be two {shape} tensors of one type with contiguous channels")
+                    self._here("out", t)
+                dtype = k.dtype
+            if B == 0 or tokens == 0:
+                return k, v
+            if not self._on_device:
+                cpu8.read(self.key, self.value, self.scale, block_table, lens, start, (k, v))
+                return k, v
+            found = self._keep(sig, (shape, _aligned16(k) and _aligned16(v), (*_strides(k), *_strides(v)),
+                                     block_table.stride(0) if B > 1 else 0, (B, tokens, block_table.shape[1], _SRC[dtype])))
+        shape, aligned, strides, bt_stride, rest = found
         if out is None:
-            _need(dtype in _SRC, "dtype must be float16, bfloat16 or float32")
-            out = (torch.empty(shape, dtype=dtype, device=dev), torch.empty(shape, dtype=dtype, device=dev))
+            k = torch.empty(shape, dtype=dtype, device=self.device)
+            v = torch.empty_like(k)
         else:
-            for t in out:
-                _need(tuple(t.shape) == shape and t.dtype == out[0].dtype and t.dtype in _SRC and t.device == dev
-                      and t.stride(3) == 1, f"out must be two {shape} tensors of one type with contiguous channels")
-        k, v = out
-        if B == 0 or tokens == 0:
-            return k, v
-        if not self._on_device:
-            cpu8.read(self.key, self.value, self.scale, block_table, lens, start, (k, v))
-        else:
-            self._launch(self._lib.kitty_cache8_read, _hip.Cache8RowsArgs(
-                k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v), bt, bt_stride, start_p, lens_p, B, tokens, W,
-                _SRC[k.dtype]))
+            k, v = out
+            if not aligned or k.data_ptr() % 16 or v.data_ptr() % 16:      # rows the kernel does not write in place
+                for t, x in zip(out, self.read(block_table, lens, tokens, start, k.dtype)):
+                    t.copy_(x)
+                return k, v
+        self._launch(self._lib.kitty_cache8_read, _ROWS.pack(
+            k.data_ptr(), v.data_ptr(), *strides, block_table.data_ptr(), bt_stride,
+            0 if start is None else start.data_ptr(), lens.data_ptr(), *rest))
         return k, v
 
     def attend(self, q: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor,
@@ -225,55 +260,61 @@ class Cache8:
         sees nothing.  max_tokens: the largest lens[b] where the program knows it
         (default: what the table can hold); it only chooses how the work is split."""
         self._followed()
-        _need(q.dim() == 4 and q.shape[3] == self.head_dim, f"q must be (B, Hq, T, {self.head_dim})")
-        _need(q.dtype in (torch.float16, torch.bfloat16), "q must be float16 or bfloat16")
-        B, Hq, T, D = q.shape
-        _need(Hq > 0 and Hq % self.num_kv_heads == 0, f"q heads must be a positive multiple of {self.num_kv_heads}")
-        dev = self.device
-        q = _plain(q, "q", dev)
-        bt, bt_stride, W = _table(block_table, B, dev)
-        _need(lens is not None, "lens must be given")
-        lens_p, q_lens_p = _i32(lens, B, "lens", dev), _i32(q_lens, B, "q_lens", dev)
-        scale = 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale)
-        _need(0.0 < scale <= 1e30, "sm_scale must be positive and finite")
-        plan = 0 if max_tokens is None else int(max_tokens)
-        _need(0 <= plan < 1 << 31, "max_tokens must be in [0, 2^31)")
-        if out is None:
-            out = torch.empty((B, Hq, T, D), dtype=q.dtype, device=dev)
-        _need(out.shape == q.shape and out.dtype == q.dtype and out.device == dev and out.stride(3) == 1,
-              "out must have q's shape, dtype and device and contiguous channels")
-        lse = torch.empty((B, Hq, T), dtype=torch.float32, device=dev) if return_lse else None
-        if B and T:
-            if not self._on_device:
-                cpu8.attend(self.key, self.value, self.scale, q, block_table, lens, q_lens, bool(causal), scale, out,
-                            torch.empty(B, Hq, T) if lse is None else lse)
-            else:
-                self._attend(q, out, lse, bt, bt_stride, W, lens_p, q_lens_p, plan, bool(causal), scale)
-        return (out, lse) if return_lse else out
-
-    def _attend(self, q: torch.Tensor, out: torch.Tensor, lse: Optional[torch.Tensor], bt: int, bt_stride: int, W: int,
-                lens: int, q_lens: int, plan: int, causal: bool, scale: float) -> None:
-        B, Hq, T, _ = q.shape
-        q, qs = _rows16(q)
-        o, os = out, _strides(out)
-        if os[0] % 8 or os[1] % 8 or os[2] % 8 or o.data_ptr() % 16:
-            o = torch.empty(out.shape, dtype=out.dtype, device=out.device)
-            os = _strides(o)
-        a = _hip.Cache8AttentionArgs(
-            q.data_ptr(), o.data_ptr(), _hip.ptr(lse), *qs, *os, bt, bt_stride, lens, q_lens, B, Hq, T, W, plan,
-            causal, _hip.KITTY_DTYPE_F16 if q.dtype == torch.float16 else _hip.KITTY_DTYPE_BF16, scale)
-        shape = (B, Hq, T, W, plan)
-        need = self._ws.get(shape)
-        if need is None:
+        q = _given(q, "q")
+        causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
+        max_tokens = 0 if max_tokens is None else int(max_tokens)
+        sig = (_sig(q), _sig(block_table), _sig(lens), _sig(q_lens), causal, sm_scale, _sig(out), max_tokens)
+        found = self._known.get(sig) if self._on_device else None
+        if found is None:
+            _need(q.dim() == 4 and q.shape[3] == self.head_dim, f"q must be (B, Hq, T, {self.head_dim})")
+            _need(q.dtype in (torch.float16, torch.bfloat16), "q must be float16 or bfloat16")
+            self._here("q", q)
+            B, Hq, T, D = q.shape
+            _need(Hq > 0 and Hq % self.num_kv_heads == 0, f"q heads must be a positive multiple of {self.num_kv_heads}")
+            self._check_table(block_table, B)
+            self._i32("lens", lens, B)
+            self._i32("q_lens", q_lens, B, optional=True)
+            scale = 1.0 / math.sqrt(D) if sm_scale is None else sm_scale
+            _need(0.0 < scale <= 1e30, "sm_scale must be positive and finite")
+            _need(0 <= max_tokens < 1 << 31, "max_tokens must be in [0, 2^31)")
+            if out is not None:
+                _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(3) == 1,
+                      "out must have q's shape and dtype and contiguous channels")
+                self._here("out", out)
+            if B == 0 or T == 0 or not self._on_device:
+                if out is None:
+                    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+                lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
+                if B and T:
+                    cpu8.attend(self.key, self.value, self.scale, q, block_table, lens, q_lens, causal, scale, out, lse)
+                return (out, lse) if return_lse else out
+            in_place = q.stride(3) == 1 and _aligned16(q) and (out is None or _aligned16(out))
+            o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+            W = block_table.shape[1]
+            head = (*_strides(q), *_strides(o))
+            rest = (B, Hq, T, W, max_tokens, causal,
+                    _hip.KITTY_DTYPE_F16 if q.dtype == torch.float16 else _hip.KITTY_DTYPE_BF16, scale)
+            bt_stride = block_table.stride(0) if B > 1 else 0
             size = ctypes.c_size_t(0)
-            _hip.check(self._lib.kitty_cache8_attention_workspace_size(self._ref, ctypes.byref(a), ctypes.byref(size)))
-            if len(self._ws) >= 256:
-                self._ws.clear()
-            need = self._ws[shape] = size.value
+            _hip.check(self._lib.kitty_cache8_attention_workspace_size(
+                self._ref, _ATTENTION.pack(0, 0, 0, *[0] * 6, 0, bt_stride, 0, 0, *rest, 0, 0), ctypes.byref(size)))
+            found = self._keep(sig, (in_place, q.is_contiguous(), head, bt_stride, rest, size.value))
+        in_place, like_q, head, bt_stride, rest, need = found
+        if not in_place or q.data_ptr() % 16 or (out is not None and out.data_ptr() % 16):
+            # rows the kernel does not read or write in place
+            got = self.attend(q.clone(memory_format=torch.contiguous_format), block_table, lens, q_lens, causal, sm_scale,
+                              None, return_lse, max_tokens)
+            if out is None:
+                return got
+            out.copy_(got[0] if return_lse else got)
+            return (out, got[1]) if return_lse else out
+        if out is None:
+            out = torch.empty_like(q) if like_q else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
         # a workspace of the call's own, from torch's allocator on its stream: calls
         # on other streams and in captured graphs never share one
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-        self._launch(self._lib.kitty_cache8_attention, a)
-        if o is not out:
-            out.copy_(o)
+        ws = q.new_empty((need + 1) // 2)
+        self._launch(self._lib.kitty_cache8_attention, _ATTENTION.pack(
+            q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, block_table.data_ptr(), bt_stride,
+            lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), *rest, ws.data_ptr(), need))
+        return (out, lse) if return_lse else out

@@ -509,3 +509,15 @@ def test_abi_refusals():
     assert need.value > 0
     a.tokens = 1 << 28
     assert L.kitty_cache8_attention_workspace_size(ctypes.byref(cache()), ctypes.byref(a), ctypes.byref(need)) == _hip.KITTY_E_UNSUPPORTED
+
+
+def test_packed_arguments_are_the_structures():
+    """The packed bytes of a call hold the fields of the C structures in their places."""
+    import ctypes
+    from kitty import _hip
+    from kitty.kernels import cache8
+    for packed, cls in ((cache8._ROWS, _hip.Cache8RowsArgs), (cache8._ATTENTION, _hip.Cache8AttentionArgs)):
+        values = list(range(3, 3 + len(cls._fields_)))
+        assert packed.size == ctypes.sizeof(cls)
+        got = cls.from_buffer_copy(packed.pack(*values))
+        assert [getattr(got, f[0]) for f in cls._fields_] == values
