@@ -202,18 +202,16 @@ __device__ __forceinline__ int units8(const Attend8 &p, int b)
     return s.bad ? 0 : (s.n + kUnit - 1) / kUnit;
 }
 
-// CUT: D is below DP, and the lanes beyond it read nothing.
-template <int DP, int RT, bool BF16, bool CUT>
-__global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_kernel(Attend8 p)
-{
-    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NB = 2;
-    __shared__ __attribute__((aligned(16))) float lds_o[kWaves][RM][LD];
-    __shared__ float2 lds_ml[kWaves][RM];
-    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int per_seq = p.c.H * p.nrb;
+// This workgroup's run of the batch's units.
+struct Run8 {
+    int total, N;      // all units, workgroups that share them
+    int u, u1;         // the run's next unit and its end
+    int b, pre;        // the sequence of unit u and its first unit
+};
 
-    // this workgroup's run [u, u1) of all units, and the sequence it starts in
+__device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
+{
+    const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb;
     int total = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
         int x = b0 + lane < p.B ? units8(p, b0 + lane) : 0;
@@ -222,14 +220,14 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
             x += __shfl_xor(x, off);
         total += x * per_seq;
     }
-    total = __builtin_amdgcn_readfirstlane(total);
-    const int N = min(p.n_wg, total), wg = blockIdx.x;
-    if (wg >= N)
-        return;
-    auto start_of = [&](int w) { return (int)((int64_t)w * total / N); };
-    int u = start_of(wg);
-    const int u0 = u, u1 = start_of(wg + 1);
-    int b = 0, pre = 0;     // first unit of sequence b
+    R.total = __builtin_amdgcn_readfirstlane(total);
+    R.N = min(p.n_wg, R.total);
+    const int wg = blockIdx.x;
+    if (wg >= R.N)
+        return false;
+    R.u = (int)((int64_t)wg * R.total / R.N);
+    R.u1 = (int)((int64_t)(wg + 1) * R.total / R.N);
+    int b = 0, pre = 0;
     for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
         const int x = b0 + lane < p.B ? units8(p, b0 + lane) * per_seq : 0;
         int inc = x;
@@ -238,7 +236,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
             const int y = __shfl_up(inc, off);
             inc += lane >= off ? y : 0;
         }
-        const unsigned long long past = __ballot(base + inc > u);
+        const unsigned long long past = __ballot(base + inc > R.u);
         if (past) {
             const int l = __builtin_ctzll(past);
             b = b0 + l;
@@ -247,21 +245,48 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
         }
         base += __shfl(inc, 63);
     }
-    b = __builtin_amdgcn_readfirstlane(b);
-    pre = __builtin_amdgcn_readfirstlane(pre);
+    R.b = __builtin_amdgcn_readfirstlane(b);
+    R.pre = __builtin_amdgcn_readfirstlane(pre);
+    return true;
+}
+
+// CUT: D is below DP, and the lanes beyond it read nothing.  NW waves: 4 for the
+// runs of the split, 8 (DIRECT) where a workgroup takes the whole of one (pair,
+// row block) and writes its rows, so that no merge follows.
+template <int DP, int RT, bool BF16, bool CUT, bool DIRECT>
+__global__ __launch_bounds__(DIRECT ? 512 : 256, DP <= 128 ? 2 : 1) void cache8_rows_kernel(Attend8 p)
+{
+    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NB = 2, NW = DIRECT ? 8 : kWaves, STRIDE = 32 * NW;
+    __shared__ __attribute__((aligned(16))) float lds_o[NW][RM][LD];
+    __shared__ float2 lds_ml[NW][RM];
+    const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int per_seq = p.c.H * p.nrb, wg = blockIdx.x;
+    Run8 R;
+    if constexpr (DIRECT) {
+        R.b = wg / per_seq;
+        R.pre = 0, R.u = wg - R.b * per_seq, R.u1 = R.u + 1;
+    } else {
+        if (!find_run(p, R))
+            return;
+    }
+    const int u0 = R.u, u1 = R.u1;
+    int u = R.u, b = R.b, pre = R.pre;
 
     while (u < u1) {
         const Seq8 sq = seq8(p, b);
-        const int nt = units8(p, b);
-        if (u >= pre + nt * per_seq) {
-            pre += nt * per_seq;
-            ++b;
-            continue;
+        int nt = units8(p, b), item = u, tile = 0, tile1 = nt;
+        if constexpr (!DIRECT) {
+            if (u >= pre + nt * per_seq) {
+                pre += nt * per_seq;
+                ++b;
+                continue;
+            }
+            item = (u - pre) / nt, tile = (u - pre) - item * nt, tile1 = min(nt, tile + (u1 - u));
         }
-        const int item = (u - pre) / nt, tile = (u - pre) - item * nt, tile1 = min(nt, tile + (u1 - u));
         const int kh = item / p.nrb, rb = item - kh * p.nrb, r0 = rb * RM;
         const int t_lo = r0 / p.gq, t_hi = min((r0 + RM - 1) / p.gq, sq.tq - 1);   // query tokens of the block
-        const int vis_min = visible8(p, sq, t_lo), vis_max = t_hi < t_lo ? 0 : visible8(p, sq, t_hi);
+        const int vis_min = visible8(p, sq, t_lo), vis_max = sq.bad || t_hi < t_lo ? 0 : visible8(p, sq, t_hi);
         const int end = min(tile1 * kUnit, vis_max);
 
         RowState<DP, RT> W;
@@ -276,7 +301,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
             for (int c = 0; c < DP / 32; ++c) {
                 const int ch = 64 * (c >> 1) + 16 * g + 8 * (c & 1);
                 W.q[rt][c] = u32x4{0, 0, 0, 0};
-                if (t < sq.tq && (!CUT || ch < p.c.D))
+                if (!sq.bad && t < sq.tq && (!CUT || ch < p.c.D))
                     W.q[rt][c] = *(const u32x4 *)(q + ch);
             }
 #pragma unroll
@@ -332,25 +357,25 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
         // one for all loads.
         int tok = tile * kUnit + 32 * wave;
         if (tok < end) {
-            const int final = tok + (end - 1 - tok) / kUnit * kUnit;
+            const int final = tok + (end - 1 - tok) / STRIDE * STRIDE;
             RowBuf<DP, RT> ring[NB];
             int id[NB][2];
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-                ids(min(tok + j * kUnit, final), id[j]);
+                ids(min(tok + j * STRIDE, final), id[j]);
 #pragma unroll
             for (int j = 0; j < NB - 1; ++j)
-                load(min(tok + j * kUnit, final), id[j], ring[j]);
+                load(min(tok + j * STRIDE, final), id[j], ring[j]);
             bool more = true;
             while (more) {
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
                     if (!more)
                         break;
-                    load(min(tok + (NB - 1) * kUnit, final), id[NB - 1], ring[(j + NB - 1) % NB]);
-                    ids(min(tok + NB * kUnit, final), id[NB - 1]);
+                    load(min(tok + (NB - 1) * STRIDE, final), id[NB - 1], ring[(j + NB - 1) % NB]);
+                    ids(min(tok + NB * STRIDE, final), id[NB - 1]);
                     row_step<DP, RT, BF16>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min);
-                    tok += kUnit;
+                    tok += STRIDE;
                     more = tok < end;
                 }
             }
@@ -370,24 +395,24 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
                         make_float4(W.o[rt][4 * d4][i], W.o[rt][4 * d4 + 1][i], W.o[rt][4 * d4 + 2][i], W.o[rt][4 * d4 + 3][i]);
         }
         __syncthreads();
-        const bool whole = tile == 0 && tile1 == nt;
+        const bool whole = DIRECT || (tile == 0 && tile1 == nt);
         const int slot = 2 * wg + (u == u0 ? 0 : 1), rows = min(RM, p.gq * p.T - r0);
-        if (tile == 0 && threadIdx.x == 0) {
+        if (!DIRECT && tile == 0 && threadIdx.x == 0) {
             const int64_t last_unit = (int64_t)u + nt;   // one past the item's last
-            p.ws_tab[b * per_seq + item] = whole ? make_int2(-1, 0) : make_int2(slot, (int)((last_unit * N - 1) / total));
+            p.ws_tab[b * per_seq + item] = whole ? make_int2(-1, 0) : make_int2(slot, (int)((last_unit * R.N - 1) / R.total));
         }
-        for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * kWaves) {
+        for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
             const int r = i / (DP / 4), ch = 4 * (i - r * (DP / 4));
             float m = kLowest, l = 0.0f;
-            float2 ml[kWaves];
+            float2 ml[NW];
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 ml[w] = lds_ml[w][r];
                 m = fmaxf(m, ml[w].x);
             }
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
+            for (int w = 0; w < NW; ++w) {
                 const float f = __builtin_amdgcn_exp2f(ml[w].x - m);
                 const float4 x = *(const float4 *)&lds_o[w][r][ch];
                 l += f * ml[w].y;
@@ -400,15 +425,18 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_rows_ke
                 continue;
             }
             const int t = (r0 + r) / p.gq, h = kh * p.gq + (r0 + r) - t * p.gq;
-            const bool none = visible8(p, sq, t) == 0;
-            const float inv = none ? 0.0f : 1.0f / l;
+            const bool none = !sq.bad && visible8(p, sq, t) == 0;
+            const float inv = sq.bad ? __builtin_nanf("") : none ? 0.0f : 1.0f / l;
             if (!CUT || ch < p.c.D)
                 *(uint2 *)(p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok + ch) =
                     make_uint2((uint32_t)f2x(acc.x * inv, BF16) | (uint32_t)f2x(acc.y * inv, BF16) << 16,
                                (uint32_t)f2x(acc.z * inv, BF16) | (uint32_t)f2x(acc.w * inv, BF16) << 16);
             if (ch == 0 && p.lse)
-                p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
+                p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
+                    sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
         }
+        if constexpr (DIRECT)
+            return;
         __syncthreads();
         u += tile1 - tile;
     }
@@ -504,13 +532,26 @@ static int device_cus()
 static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 struct Plan8 {
-    bool tiles;
+    bool tiles, direct;
     int DP, RT, nrb, n_wg, splits;
     size_t o_bytes, ml_bytes, bytes;
 };
 
 // Rows from which the merge gives each a lane group instead of a workgroup.
 constexpr int64_t kMergeRows = 2048;
+// The row kernel on whole pairs, one launch of eight waves each, where a stream of a
+// pair is at most kDirectBytes and there are at most kDirectItems of them; it saves
+// the merge and reads lengths less often, and loses where its eight waves leave the
+// device idle, or where many pairs fill it anyway.  us, one launch / split and merge,
+// 8 KV heads, groups of 4, fp16:
+//   channels 128, tokens    128          512          1,024        2,048
+//   1 sequence              4.9 /  9.3   7.9 / 10.1   10.7 / 10.3  16.4 / 10.9
+//   16 sequences            5.1 /  9.6   8.3 / 12.9   11.8 / 15.2  20.6 / 20.4
+//   64 sequences            8.2 / 11.5  18.0 / 19.0   28.6 / 29.4  48.4 / 50.4
+//   256 sequences          31.9 / 35.8  70.4 / 62.9  108.7 / 103
+//   channels 64: 1 sequence 512 tokens 6.0 / 9.6, 2,048 11.9 / 9.8; 64 sequences 26.0 / 28.8
+//   channels 256 (two waves' registers spill): 1 sequence 512 tokens 13.3 / 11.8
+constexpr int64_t kDirectBytes = 1024 * 128, kDirectItems = 1024;
 // Rows that the row kernel takes: two blocks of 16, whose codes are read once.
 constexpr int kRowKernelRows = 32;
 
@@ -529,19 +570,20 @@ static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &p
         return fail(KITTY_E_UNSUPPORTED, "too many rows or pages for one launch");
     pl.nrb = (int)nrb;
     pl.n_wg = pl.splits = 1;
+    pl.direct = !pl.tiles && pl.DP <= 128 && tokens * pl.DP <= kDirectBytes && items <= kDirectItems;
     int64_t slots = 0;
     if (pl.tiles) {
         // parts of at least four tiles, until there are two workgroups a CU (one at 256 channels)
         const int64_t want = (pl.DP == 256 ? 1 : 2) * (int64_t)device_cus() / std::max<int64_t>(items, 1);
         pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tokens / 256));
         slots = pl.splits > 1 ? items * pl.splits : 0;
-    } else {
+    } else if (!pl.direct) {
         pl.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus(), items * units));
         slots = 2 * pl.n_wg;
     }
     pl.o_bytes = up16((size_t)slots * RM * pl.DP * 4);
     pl.ml_bytes = up16((size_t)slots * RM * 8);
-    pl.bytes = pl.o_bytes + pl.ml_bytes + (pl.tiles ? 0 : up16((size_t)items * 8));
+    pl.bytes = pl.o_bytes + pl.ml_bytes + (pl.tiles || pl.direct ? 0 : up16((size_t)items * 8));
     return KITTY_OK;
 }
 
@@ -635,10 +677,19 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
     auto rows = [&](auto dp, auto rt, auto bf) {
         constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
         constexpr bool BF = decltype(bf)::value;
+        const dim3 pairs((unsigned)(p.B * p.c.H * p.nrb)), runs((unsigned)p.n_wg), waves8(512);
+        if constexpr (DP <= 128) {
+            if (pl.direct && p.c.D == DP)
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true>), pairs, waves8, 0, st, p);
+            else if (pl.direct)
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true>), pairs, waves8, 0, st, p);
+            if (pl.direct)
+                return;
+        }
         if (p.c.D == DP)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false>), dim3((unsigned)p.n_wg), block, 0, st, p);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, false>), runs, block, 0, st, p);
         else
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true>), dim3((unsigned)p.n_wg), block, 0, st, p);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, false>), runs, block, 0, st, p);
     };
     auto go = [&](auto dp, auto bf) {
         constexpr int DP = decltype(dp)::value;
@@ -656,7 +707,8 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
         } else {
             rows(dp, std::integral_constant<int, 1>{}, bf);
         }
-        merge(dp, bf, std::false_type{});
+        if (!pl.direct)
+            merge(dp, bf, std::false_type{});
     };
     auto by_type = [&](auto dp) {
         if (bf16)
