@@ -250,11 +250,14 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
     return true;
 }
 
+// Whether two workgroups' registers and LDS fit a CU.
+constexpr bool two_per_cu(int DP, int RT) { return DP <= 128 && DP * RT <= 256; }
+
 // CUT: D is below DP, and the lanes beyond it read nothing.  NW waves: 4 for the
 // runs of the split, 8 (DIRECT) where a workgroup takes the whole of one (pair,
 // row block) and writes its rows, so that no merge follows.
 template <int DP, int RT, bool BF16, bool CUT, bool DIRECT>
-__global__ __launch_bounds__(DIRECT ? 512 : 256, DP <= 128 ? 2 : 1) void cache8_rows_kernel(Attend8 p)
+__global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
 {
     constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NB = 2, NW = DIRECT ? 8 : kWaves, STRIDE = 32 * NW;
     __shared__ __attribute__((aligned(16))) float lds_o[NW][RM][LD];
@@ -531,19 +534,15 @@ static int device_cus()
 
 static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
-struct Plan8 {
-    bool tiles, direct;
-    int DP, RT, nrb, n_wg, splits;
-    size_t o_bytes, ml_bytes, bytes;
-};
-
-// Rows from which the merge gives each a lane group instead of a workgroup.
-constexpr int64_t kMergeRows = 2048;
-// The row kernel on whole pairs, one launch of eight waves each, where a stream of a
-// pair is at most kDirectBytes and there are at most kDirectItems of them; it saves
-// the merge and reads lengths less often, and loses where its eight waves leave the
-// device idle, or where many pairs fill it anyway.  us, one launch / split and merge,
-// 8 KV heads, groups of 4, fp16:
+// Which kernel takes a call, by its sizes alone (rows: of a KV head, its group's
+// heads times the queries; tokens: of the longest sequence, as far as the host knows).
+//
+// 1. The row kernel on whole (pair, row block)s, one launch of eight waves each,
+// where a stream of a pair is at most kDirectBytes and there are at most
+// kDirectItems of them, or a workgroup a CU where a pair has several row blocks.  It
+// saves the merge and reads lengths less often, and loses where its eight waves leave
+// the device idle, or where the items fill it anyway.  us, one launch / split and
+// merge, 8 KV heads, one query, groups of 4, fp16:
 //   channels 128, tokens    128          512          1,024        2,048
 //   1 sequence              4.9 /  9.3   7.9 / 10.1   10.7 / 10.3  16.4 / 10.9
 //   16 sequences            5.1 /  9.6   8.3 / 12.9   11.8 / 15.2  20.6 / 20.4
@@ -551,34 +550,59 @@ constexpr int64_t kMergeRows = 2048;
 //   256 sequences          31.9 / 35.8  70.4 / 62.9  108.7 / 103
 //   channels 64: 1 sequence 512 tokens 6.0 / 9.6, 2,048 11.9 / 9.8; 64 sequences 26.0 / 28.8
 //   channels 256 (two waves' registers spill): 1 sequence 512 tokens 13.3 / 11.8
+// and of several row blocks against the tile kernel, bf16:
+//   128 rows, 128 channels, 1 sequence of 1,024 15.6 / 17.0, 8 (256 items) 19.1 / 26.1, 32 75.5 / 44.3
+//   100 rows, 64 channels, 1 sequence of 1,500 13.8 / 14.6, 8 (256 items) 14.5 / 21.5, 32 55.0 / 35.7
+//   256 rows, 128 channels, 8 sequences of 512 (512 items) 27.0 / 26.8
+//
+// 2. The row kernel's split, up to four blocks of 16 rows (two at 256 channels), whose
+// codes are read once: beyond 32 rows its registers allow one wave a SIMD, which still
+// beats the tile kernel's half-empty workgroups.  us, row / tile kernel, 32 sequences
+// of 8,192 tokens, 8 KV heads, fp16:
+//   128 channels, 36 rows 141 / 195, 64 rows 175 / 199;  64 channels, 64 rows 97 / 153
+//   256 channels, 20 rows 281 in two blocks / 331 in one at a time
+// 8 sequences: 49 / 62, 62 / 61, 39 / 48.
+//
+// 3. The tile kernel beyond.
 constexpr int64_t kDirectBytes = 1024 * 128, kDirectItems = 1024;
-// Rows that the row kernel takes: two blocks of 16, whose codes are read once.
-constexpr int kRowKernelRows = 32;
+
+struct Plan8 {
+    bool tiles, direct;
+    int DP, RT, nrb, n_wg, splits;
+    size_t o_bytes, ml_bytes, bytes;
+};
+
+// Rows from which the merge gives each a lane group instead of a workgroup (12,800
+// rows of four parts 5.6 us / 9.0 with a wave a row; 1,280 rows of nine 6.5 / 4.6).
+constexpr int64_t kMergeRows = 2048;
 
 static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &pl)
 {
     const int64_t rows = (int64_t)a.num_q_heads / c.H * a.tokens, pairs = (int64_t)a.batch * c.H;
+    const int64_t cap = (int64_t)a.table_pages << c.lg, units = (cap + kUnit - 1) / kUnit;
+    if (rows > kMaxBlocks || pairs > kMaxBlocks || pairs * rows > kMaxBlocks)
+        return fail(KITTY_E_UNSUPPORTED, "too many rows for one launch");
+    const int64_t tokens = a.plan_tokens > 0 ? std::min<int64_t>(a.plan_tokens, cap) : cap;
+    const int cus = device_cus();
     pl.DP = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
-    pl.tiles = rows > kRowKernelRows;
-    pl.RT = rows <= 16 || pl.DP == 256 ? 1 : 2;   // at 256 channels two blocks' registers do not fit
+    pl.direct = pl.DP <= 128 && tokens * pl.DP <= kDirectBytes &&
+                (rows <= 32 ? pairs <= kDirectItems : pairs * ((rows + 31) / 32) <= cus);
+    pl.tiles = !pl.direct && rows > (pl.DP == 256 ? 32 : 64);
+    pl.RT = rows <= 16 ? 1 : rows <= 32 || pl.direct || pl.DP == 256 ? 2 : rows <= 48 ? 3 : 4;
     const int RM = pl.tiles ? kTileRows : 16 * pl.RT;
     const int64_t nrb = (rows + RM - 1) / RM, items = pairs * nrb;
-    const int64_t cap = (int64_t)a.table_pages << c.lg;   // tokens of the longest sequence, as far as the host knows
-    const int64_t tokens = a.plan_tokens > 0 ? std::min<int64_t>(a.plan_tokens, cap) : cap;
-    const int64_t units = (cap + kUnit - 1) / kUnit;
-    if (rows > kMaxBlocks || pairs * rows > kMaxBlocks || items * std::max<int64_t>(units, 1) > 0x7fffffff)
-        return fail(KITTY_E_UNSUPPORTED, "too many rows or pages for one launch");
+    if (items * std::max<int64_t>(units, 1) > 0x7fffffff)
+        return fail(KITTY_E_UNSUPPORTED, "too many rows and pages for one launch");
     pl.nrb = (int)nrb;
     pl.n_wg = pl.splits = 1;
-    pl.direct = !pl.tiles && pl.DP <= 128 && tokens * pl.DP <= kDirectBytes && items <= kDirectItems;
     int64_t slots = 0;
     if (pl.tiles) {
         // parts of at least four tiles, until there are two workgroups a CU (one at 256 channels)
-        const int64_t want = (pl.DP == 256 ? 1 : 2) * (int64_t)device_cus() / std::max<int64_t>(items, 1);
+        const int64_t want = (pl.DP == 256 ? 1 : 2) * (int64_t)cus / std::max<int64_t>(items, 1);
         pl.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tokens / 256));
         slots = pl.splits > 1 ? items * pl.splits : 0;
     } else if (!pl.direct) {
-        pl.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus(), items * units));
+        pl.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>((two_per_cu(pl.DP, pl.RT) ? 2 : 1) * cus, items * units));
         slots = 2 * pl.n_wg;
     }
     pl.o_bytes = up16((size_t)slots * RM * pl.DP * 4);
@@ -678,7 +702,7 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
         constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
         constexpr bool BF = decltype(bf)::value;
         const dim3 pairs((unsigned)(p.B * p.c.H * p.nrb)), runs((unsigned)p.n_wg), waves8(512);
-        if constexpr (DP <= 128) {
+        if constexpr (DP <= 128 && RT <= 2) {
             if (pl.direct && p.c.D == DP)
                 hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true>), pairs, waves8, 0, st, p);
             else if (pl.direct)
@@ -699,13 +723,15 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
                 merge(dp, bf, std::true_type{});
             return;
         }
-        if constexpr (DP <= 128) {
-            if (pl.RT == 2)
-                rows(dp, std::integral_constant<int, 2>{}, bf);
-            else
-                rows(dp, std::integral_constant<int, 1>{}, bf);
-        } else {
+        if (pl.RT == 1)
             rows(dp, std::integral_constant<int, 1>{}, bf);
+        else if (pl.RT == 2)
+            rows(dp, std::integral_constant<int, 2>{}, bf);
+        else if constexpr (DP <= 128) {
+            if (pl.RT == 3)
+                rows(dp, std::integral_constant<int, 3>{}, bf);
+            else
+                rows(dp, std::integral_constant<int, 4>{}, bf);
         }
         if (!pl.direct)
             merge(dp, bf, std::false_type{});
