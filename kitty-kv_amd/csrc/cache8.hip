@@ -7,18 +7,21 @@
 // is the rescale of codes that were there, which would otherwise round twice.
 // Power-of-two scales cost e4m3 no relative precision (its steps are relative);
 // the largest code lies in (224, 448].
-// read: a thread takes 16 codes of four rows; the codes' fp32 products with the
-// scale round once.
+// read: a thread takes 16 bytes of output in each of four rows; the codes' fp32
+// products with the scale round once.
 // Both are bound by memory, and by launch latency where few tokens are written.
 #include "cache8.h"
 
 namespace kitty {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kKeep = 8;       // pieces of a thread that stay in registers between the two passes
 constexpr int kReadRows = 4;   // rows per thread of the read kernel
+// Codes of a thread and row: 16 bytes of output, so that a wave stores 1 KB in a run.
+constexpr int read_codes(int out) { return out == KITTY_SRC_F32 ? 4 : 8; }
 
 int check_cache8(const kitty_cache8 *cache, Cache8 &c)
 {
@@ -263,14 +266,15 @@ struct ReadParams {
 template <int OUT>
 __global__ __launch_bounds__(256) void cache8_read_kernel(ReadParams p)
 {
+    constexpr int CPT = read_codes(OUT), NW = CPT / 4;
     uint32_t i = blockIdx.x;
     const int tile = (int)(i % (uint32_t)p.tiles);
     i /= (uint32_t)p.tiles;
     const int st = (int)(i & 1);
     i >>= 1;
     const int h = (int)(i % (uint32_t)p.c.H), b = (int)(i / (uint32_t)p.c.H);
-    const int cpr = p.c.D >> 4, rpp = 256 / cpr;
-    const int r0 = (int)threadIdx.x / cpr, ch = 16 * ((int)threadIdx.x - r0 * cpr);
+    const int cpr = p.c.D / CPT, rpp = 256 / cpr;
+    const int r0 = (int)threadIdx.x / cpr, ch = CPT * ((int)threadIdx.x - r0 * cpr);
     if (r0 >= rpp)
         return;
     const int lg = p.c.lg, mask = (1 << lg) - 1;
@@ -278,13 +282,15 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(ReadParams p)
     const uint8_t *pool = (st ? p.c.value + h * p.c.value_s_head : p.c.key + h * p.c.key_s_head) + ch;
     const int64_t s_page = st ? p.c.value_s_page : p.c.key_s_page;
     const uint32_t s_tok = st ? p.c.value_s_tok : p.c.key_s_tok;
-    u32x4 code[kReadRows];
+    uint32_t code[kReadRows][NW];
     float s[kReadRows];
 #pragma unroll
     for (int j = 0; j < kReadRows; ++j) {
         const int t = (tile * kReadRows + j) * rpp + r0;
         const int64_t pos = first + t;
-        code[j] = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int e = 0; e < NW; ++e)
+            code[j][e] = 0;
         s[j] = 0.0f;
         if (t < p.tokens && pos < len) {
             const int64_t page = pos >> lg;
@@ -295,7 +301,13 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(ReadParams p)
                 s[j] = __builtin_nanf("");
             } else {
                 s[j] = p.c.scale[id * p.c.scale_s_page + h * p.c.scale_s_head + st];
-                code[j] = *(const u32x4 *)(pool + id * s_page + (uint32_t)(pos & mask) * s_tok);
+                const uint8_t *src = pool + id * s_page + (uint32_t)(pos & mask) * s_tok;
+                if constexpr (NW == 2) {
+                    const u32x2 x = __builtin_nontemporal_load((const u32x2 *)src);
+                    code[j][0] = x[0], code[j][1] = x[1];
+                } else {
+                    code[j][0] = __builtin_nontemporal_load((const uint32_t *)src);
+                }
             }
         }
     }
@@ -307,28 +319,24 @@ __global__ __launch_bounds__(256) void cache8_read_kernel(ReadParams p)
         const int t = (tile * kReadRows + j) * rpp + r0;
         if (t >= p.tokens)
             continue;
-        float x[16];
+        float x[CPT];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+        for (int e = 0; e < NW; ++e) {
             const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[j][e], false);
             const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[j][e], true);
             x[4 * e] = lo[0] * s[j], x[4 * e + 1] = lo[1] * s[j];
             x[4 * e + 2] = hi[0] * s[j], x[4 * e + 3] = hi[1] * s[j];
         }
         const int64_t o = o0 + t * o_tok;
-        if constexpr (OUT == KITTY_SRC_F32) {
+        u32x4 w;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                *(float4 *)((float *)out + o + 4 * e) = make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
-        } else {
-            constexpr bool BF = OUT == KITTY_SRC_BF16;
-            u32x4 w[2];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                w[e >> 2][e & 3] = (uint32_t)f2x(x[2 * e], BF) | (uint32_t)f2x(x[2 * e + 1], BF) << 16;
-            u32x4 *d = (u32x4 *)((uint16_t *)out + o);
-            d[0] = w[0], d[1] = w[1];
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (OUT == KITTY_SRC_F32)
+                w[e] = __builtin_bit_cast(uint32_t, x[e]);
+            else
+                w[e] = (uint32_t)f2x(x[2 * e], OUT == KITTY_SRC_BF16) | (uint32_t)f2x(x[2 * e + 1], OUT == KITTY_SRC_BF16) << 16;
         }
+        __builtin_nontemporal_store(w, (u32x4 *)((char *)out + o * (OUT == KITTY_SRC_F32 ? 4 : 2)));
     }
 }
 
@@ -416,7 +424,7 @@ extern "C" int kitty_cache8_read(const kitty_cache8 *cache, const kitty_cache8_r
         vec = vec && s * size % 16 == 0;
     if (!vec)
         return fail(KITTY_E_INVALID, "key and value rows must be 16-byte aligned");
-    const int rows = kReadRows * (256 / (p.c.D >> 4));
+    const int rows = kReadRows * (256 / (p.c.D / read_codes(a.out_dtype)));
     const int64_t tiles = ((int64_t)a.tokens + rows - 1) / rows, blocks = (int64_t)a.batch * p.c.H * 2 * tiles;
     if (blocks > kMaxBlocks || a.tokens > 1 << 30)
         return fail(KITTY_E_UNSUPPORTED, "too many tokens for one launch");
