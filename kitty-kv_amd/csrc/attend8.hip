@@ -209,45 +209,57 @@ struct Run8 {
     int b, pre;        // the sequence of unit u and its first unit
 };
 
+// First unit of workgroup w: total units shared evenly, the first total % N
+// workgroups taking one more.
+__device__ __forceinline__ int run_start(int total, int N, int w)
+{
+    const int each = total / N, more = total - each * N;
+    return w * each + min(w, more);
+}
+
+// The workgroup that has unit u.
+__device__ __forceinline__ int run_of(int total, int N, int u)
+{
+    const int each = total / N, more = total - each * N, cut = more * (each + 1);
+    return u < cut ? u / (each + 1) : more + (u - cut) / each;
+}
+
 __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
 {
-    const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb;
-    int total = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        int x = b0 + lane < p.B ? units8(p, b0 + lane) : 0;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1)
-            x += __shfl_xor(x, off);
-        total += x * per_seq;
-    }
-    R.total = __builtin_amdgcn_readfirstlane(total);
-    R.N = min(p.n_wg, R.total);
-    const int wg = blockIdx.x;
-    if (wg >= R.N)
-        return false;
-    R.u = (int)((int64_t)wg * R.total / R.N);
-    R.u1 = (int)((int64_t)(wg + 1) * R.total / R.N);
-    int b = 0, pre = 0;
-    for (int b0 = 0, base = 0; b0 < p.B; b0 += 64) {
-        const int x = b0 + lane < p.B ? units8(p, b0 + lane) * per_seq : 0;
+    const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb, wg = blockIdx.x;
+    // 64 sequences at a time: units of each and the sum up to it
+    auto sums = [&](int b0, int &x) {
+        x = b0 + lane < p.B ? units8(p, b0 + lane) * per_seq : 0;
         int inc = x;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
             const int y = __shfl_up(inc, off);
             inc += lane >= off ? y : 0;
         }
+        return inc;
+    };
+    int x, inc = sums(0, x), total = __builtin_amdgcn_readlane(inc, 63);
+    for (int b0 = 64; b0 < p.B; b0 += 64) {
+        int y;
+        total += __builtin_amdgcn_readlane(sums(b0, y), 63);
+    }
+    R.total = total;
+    R.N = min(p.n_wg, total);
+    if (wg >= R.N)
+        return false;
+    R.u = run_start(total, R.N, wg);
+    R.u1 = run_start(total, R.N, wg + 1);
+    for (int b0 = 0, base = 0;;) {
         const unsigned long long past = __ballot(base + inc > R.u);
         if (past) {
             const int l = __builtin_ctzll(past);
-            b = b0 + l;
-            pre = base + __shfl(inc - x, l);
-            break;
+            R.b = b0 + l;
+            R.pre = base + __builtin_amdgcn_readlane(inc - x, l);
+            return true;
         }
-        base += __shfl(inc, 63);
+        base += __builtin_amdgcn_readlane(inc, 63);
+        inc = sums(b0 += 64, x);
     }
-    R.b = __builtin_amdgcn_readfirstlane(b);
-    R.pre = __builtin_amdgcn_readfirstlane(pre);
-    return true;
 }
 
 // Whether two workgroups' registers and LDS fit a CU.
@@ -401,8 +413,7 @@ __global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) voi
         const bool whole = DIRECT || (tile == 0 && tile1 == nt);
         const int slot = 2 * wg + (u == u0 ? 0 : 1), rows = min(RM, p.gq * p.T - r0);
         if (!DIRECT && tile == 0 && threadIdx.x == 0) {
-            const int64_t last_unit = (int64_t)u + nt;   // one past the item's last
-            p.ws_tab[b * per_seq + item] = whole ? make_int2(-1, 0) : make_int2(slot, (int)((last_unit * R.N - 1) / R.total));
+            p.ws_tab[b * per_seq + item] = whole ? make_int2(-1, 0) : make_int2(slot, run_of(R.total, R.N, u + nt - 1));
         }
         for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
             const int r = i / (DP / 4), ch = 4 * (i - r * (DP / 4));
@@ -461,7 +472,10 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
     if (!ALONE && pair >= p.B * p.c.H)
         return;
     const int b = pair / p.c.H, kh = pair - b * p.c.H, rb = row / RM, r = row - rb * RM;
-    const int t = row / p.gq, h = kh * p.gq + row - t * p.gq;
+    const int t = row / p.gq, h = kh * p.gq + row - t * p.gq, item = pair * p.nrb + rb;
+    int2 tab = make_int2(0, 0);
+    if constexpr (!TILES)
+        tab = p.ws_tab[item];   // of a sequence without tokens it holds anything and is not used
     const Seq8 sq = seq8(p, b);
     float m = kLowest, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -475,10 +489,6 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
     if (sq.bad) {
         l = __builtin_nanf("");
     } else if (sq.n > 0) {
-        const int item = pair * p.nrb + rb;
-        int2 tab = make_int2(0, 0);
-        if constexpr (!TILES)
-            tab = p.ws_tab[item];
         if (tab.x < 0)
             return;
         const int first = tab.x >> 1, count = TILES ? p.splits : tab.y - first + 1;

@@ -73,14 +73,15 @@ template <int SRC>
 struct Piece {
     u32x4 w[SRC == KITTY_SRC_F32 ? 2 : 1];
 
-    template <bool VEC>
+    // ONCE: not read again, and kept from displacing what is
+    template <bool VEC, bool ONCE>
     __device__ __forceinline__ void load(const void *base, int64_t off)
     {
         if constexpr (VEC) {
             const u32x4 *s = (const u32x4 *)((const char *)base + off * (SRC == KITTY_SRC_F32 ? 4 : 2));
-            w[0] = s[0];
+            w[0] = ONCE ? __builtin_nontemporal_load(s) : s[0];
             if constexpr (SRC == KITTY_SRC_F32)
-                w[1] = s[1];
+                w[1] = ONCE ? __builtin_nontemporal_load(s + 1) : s[1];
         } else if constexpr (SRC == KITTY_SRC_F32) {
             const uint32_t *s = (const uint32_t *)base + off;
 #pragma unroll
@@ -199,7 +200,7 @@ __global__ __launch_bounds__(NT) void cache8_write_kernel(WriteParams p)
 #pragma unroll
     for (int j = 0; j < kKeep; ++j)
         if (in && r0 + j * rpp < rows)
-            keep[j].template load<VEC>(src, src0 + (r0 + j * rpp) * s_tok);
+            keep[j].template load<VEC, true>(src, src0 + (r0 + j * rpp) * s_tok);
 #pragma unroll
     for (int j = 0; j < kKeep; ++j)
         if (in && r0 + j * rpp < rows)
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(NT) void cache8_write_kernel(WriteParams p)
     if (in)
         for (int r = r0 + kKeep * rpp; r < rows; r += rpp) {
             Piece<SRC> x;
-            x.template load<VEC>(src, src0 + r * s_tok);
+            x.template load<VEC, false>(src, src0 + r * s_tok);
             m = x.top(m);
         }
 #pragma unroll
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(NT) void cache8_write_kernel(WriteParams p)
     if (in)
         for (int r = r0 + kKeep * rpp; r < rows; r += rpp) {
             Piece<SRC> x;
-            x.template load<VEC>(src, src0 + r * s_tok);
+            x.template load<VEC, false>(src, src0 + r * s_tok);
             *(uint2 *)(out + (uint32_t)r * d_tok) = encode(x, s, inv, pow2);
         }
     if (row0 > 0 && s != old && in) {   // the codes of earlier tokens, at the raised scale
