@@ -10,6 +10,7 @@ from .config import KittyConfig
 from .layout import Page, PageCentricKVLayoutManager
 from .pipeline import KittyInferencePipeline
 from .attention import KittyPagedAttention, KittyAttentionFactory
+from .attention8 import KittyCache8, KittyPagedAttention8
 from .sensitivity import KittySensitivityProfiler
 
 __version__ = "0.1.0"
@@ -24,5 +25,7 @@ __all__ = [
     "KittyInferencePipeline",
     "KittyPagedAttention",
     "KittyAttentionFactory",
+    "KittyCache8",
+    "KittyPagedAttention8",
     "KittySensitivityProfiler",
 ]

@@ -38,6 +38,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .attention8 import KittyCache8, KittyPagedAttention8
 from .config import KittyConfig
 from .layout import PageCentricKVLayoutManager
 from .pipeline import KittyInferencePipeline
@@ -140,10 +141,21 @@ class KittyAttentionFactory:
     """Builds the layout, the pipeline and one module per layer (attention.py:198-257)."""
 
     @classmethod
-    def from_config(cls, config: KittyConfig, boost_idx_uint8: torch.Tensor,
-                    num_q_heads: int) -> Tuple[PageCentricKVLayoutManager, KittyInferencePipeline,
-                                               List[KittyPagedAttention]]:
+    def from_config(cls, config: KittyConfig, boost_idx_uint8: torch.Tensor, num_q_heads: int,
+                    eight_bit_layers: Sequence[int] = ()) -> Tuple[PageCentricKVLayoutManager, KittyInferencePipeline,
+                                                                   List[nn.Module]]:
+        """One module per layer.  Layers in eight_bit_layers (numbers, not in the
+        reference) keep their keys and values in 8 bits: ``KittyPagedAttention8``
+        modules over one ``KittyCache8``, theirs to reset with the pipeline's
+        sequences."""
         layout = PageCentricKVLayoutManager(config, boost_idx_uint8)
         pipeline = KittyInferencePipeline(config, layout, boost_idx_uint8)
-        layers = [KittyPagedAttention(config, num_q_heads, layout, pipeline, i) for i in range(config.num_layers)]
+        layers: List[nn.Module] = [KittyPagedAttention(config, num_q_heads, layout, pipeline, i)
+                                   for i in range(config.num_layers)]
+        chosen = sorted({int(i) for i in eight_bit_layers})
+        if chosen and not (0 <= chosen[0] and chosen[-1] < config.num_layers):
+            raise ValueError(f"eight_bit_layers must be in [0, {config.num_layers})")
+        cache = KittyCache8(config, len(chosen)) if chosen else None
+        for n, i in enumerate(chosen):
+            layers[i] = KittyPagedAttention8(config, num_q_heads, cache, n)
         return layout, pipeline, layers

@@ -1,0 +1,195 @@
+"""Layers whose keys and values stay in 8 bits: the cache of all their sequences
+and an attention module with ``KittyPagedAttention``'s ``forward``.
+
+No counterpart in the reference, whose only cache is the 2-bit one.  It is for
+layers that 2 bits cost too much (often the first and the last of a model):
+``KittyAttentionFactory.from_config(..., eight_bit_layers=(0, 31))`` builds them
+next to the 2-bit ones.  At head_dim 128 a token takes 256 bytes a KV head against
+76 in 2 bits and 512 in 16.
+
+A page holds ``q_buffer_size`` tokens (16, 32, 64, 128 or 256) of one sequence and
+stands at the same place in every layer's pools, so one block table serves all
+layers; ``max_pages`` (or ``pool_pages_override``) pages are allocated per layer.
+Tokens are quantised as they are written (``kernels.cache8``), there are no 16-bit
+sinks or windows, and a chunk of any length attends over everything its sequence
+holds, itself included.  No step waits for the GPU: lengths live on the device and
+in a host copy, and only new pages send their ids over.
+"""
+from __future__ import annotations
+
+import heapq
+import math
+from typing import Dict, List, Optional, Sequence, Union
+
+import numpy as np
+import torch
+import torch.nn as nn
+
+from .config import KittyConfig
+from .kernels.cache8 import Cache8
+from .kernels.ops import stage_i32
+
+
+class KittyCache8:
+    """8-bit pools of `num_layers` layers and the sequences in them."""
+
+    def __init__(self, config: KittyConfig, num_layers: Optional[int] = None) -> None:
+        self.config = config
+        L = config.num_layers if num_layers is None else int(num_layers)
+        H, G, D, P, n = config.num_kv_heads, config.q_buffer_size, config.head_dim, config.pool_pages, config.max_batch_size
+        self.dtype = torch.float16 if config.dtype == "float16" else torch.bfloat16
+        self.layers: List[Cache8] = [Cache8.empty(P, H, D, G, device=config.device) for _ in range(L)]
+        self.device = self.layers[0].device if L else torch.device(config.device)
+        self.max_pages_per_seq = -(-config.max_seq_len // G)
+        self.block_table = torch.zeros(n, self.max_pages_per_seq, dtype=torch.int32, device=self.device)
+        self.lens = torch.zeros(L, n, dtype=torch.int32, device=self.device)     # tokens by layer and slot
+        self._held = np.zeros((L, n), np.int64)                                  # the same on the host
+        self._pages: List[List[int]] = [[] for _ in range(n)]
+        self._fresh, self._freed, self._num_pages = 0, [], P
+        self._slot_of: Dict[int, int] = {}
+        self._free_slots = list(range(n))
+        self._slots_dev: Dict[tuple, torch.Tensor] = {}
+
+    # -------------------------------------------------------------- bookkeeping
+    def slot(self, seq_id: int) -> int:
+        """Slot of a sequence, assigned (lowest free) on first use."""
+        s = self._slot_of.get(seq_id)
+        if s is None:
+            if not self._free_slots:
+                raise RuntimeError(f"all {len(self._pages)} sequence slots are in use; "
+                                   "raise KittyConfig.max_batch_size or reset finished sequences")
+            s = self._slot_of[seq_id] = heapq.heappop(self._free_slots)
+        return s
+
+    def tokens(self, seq_id: int, layer: int = 0) -> int:
+        """Tokens a sequence holds in a layer."""
+        return int(self._held[layer, self._slot_of[seq_id]]) if seq_id in self._slot_of else 0
+
+    @property
+    def pages_free(self) -> int:
+        return self._num_pages - self._fresh + len(self._freed)
+
+    def _i32(self, values: Sequence[int]) -> torch.Tensor:
+        if self.device.type == "cpu":
+            return torch.tensor(list(values), dtype=torch.int32)
+        return stage_i32(np.asarray(values, np.int32), self.device)
+
+    def _room(self, layer: int, slots: Sequence[int], tokens: int) -> None:
+        """Pages for `tokens` more tokens of each slot, all or nothing."""
+        G = self.config.q_buffer_size
+        need = [-(-(int(self._held[layer, s]) + tokens) // G) - len(self._pages[s]) for s in slots]
+        for s, n in zip(slots, need):
+            if len(self._pages[s]) + n > self.max_pages_per_seq:
+                raise RuntimeError(f"a sequence exceeds max_seq_len={self.config.max_seq_len}")
+        if sum(max(n, 0) for n in need) > self.pages_free:
+            raise RuntimeError(f"KV Cache page pool exhausted! {self.pages_free} free pages, "
+                               f"{sum(max(n, 0) for n in need)} needed.")
+        for s, n in zip(slots, need):
+            if n <= 0:
+                continue
+            new = []
+            for _ in range(n):
+                if self._freed:
+                    new.append(heapq.heappop(self._freed))
+                else:
+                    new.append(self._fresh)
+                    self._fresh += 1
+            at = len(self._pages[s])
+            self._pages[s] += new
+            self.block_table[s, at:at + n].copy_(self._i32(new))
+
+    def reset_sequence(self, seq_id: int) -> None:
+        """Drops a sequence: its pages and its slot are free again."""
+        s = self._slot_of.pop(seq_id, None)
+        if s is None:
+            return
+        for p in self._pages[s]:
+            heapq.heappush(self._freed, p)
+        self._pages[s] = []
+        self._held[:, s] = 0
+        self.lens[:, s].zero_()
+        heapq.heappush(self._free_slots, s)
+
+    # -------------------------------------------------------------------- calls
+    def _batch(self, layer: int, seq_ids: Sequence[int]):
+        """(slots, block table and lengths of the batch, slots on the device where they are no run)."""
+        slots = [self.slot(i) for i in seq_ids]
+        if len(set(slots)) != len(slots):
+            raise ValueError("a sequence appears twice in one batch")
+        s0 = slots[0]
+        if slots == list(range(s0, s0 + len(slots))):
+            return slots, self.block_table[s0:s0 + len(slots)], self.lens[layer, s0:s0 + len(slots)], None
+        key = tuple(slots)
+        idx = self._slots_dev.get(key)
+        if idx is None:
+            if len(self._slots_dev) >= 64:
+                self._slots_dev.clear()
+            idx = self._slots_dev[key] = self._i32(slots).long()
+        return slots, self.block_table[idx], self.lens[layer][idx], idx
+
+    def push(self, layer: int, keys: torch.Tensor, values: torch.Tensor, seq_ids: Sequence[int]) -> None:
+        """T tokens for each of B sequences: keys / values (B, H, T, D)."""
+        if keys.shape[0] != len(seq_ids):
+            raise ValueError(f"{len(seq_ids)} sequence ids for a batch of {keys.shape[0]}")
+        if keys.shape[0] == 0 or keys.shape[2] == 0:
+            return
+        slots = self._batch(layer, seq_ids)[0]
+        self._room(layer, slots, keys.shape[2])
+        _, table, lens, idx = self._batch(layer, seq_ids)
+        self.layers[layer].write(keys.to(self.device), values.to(self.device), table, lens)
+        if idx is None:
+            lens.add_(keys.shape[2])
+        else:
+            self.lens[layer].index_add_(0, idx, torch.full_like(lens, keys.shape[2]))
+        self._held[layer, slots] += keys.shape[2]
+
+    def attend(self, layer: int, q: torch.Tensor, seq_ids: Sequence[int], sm_scale: Optional[float] = None) -> torch.Tensor:
+        """Causal attention of the last T tokens of each sequence, q (B, Hq, T, D)."""
+        slots, table, lens, _ = self._batch(layer, seq_ids)
+        longest = int(self._held[layer, slots].max())
+        return self.layers[layer].attend(q, table, lens, sm_scale=sm_scale, max_tokens=_bucket(longest))
+
+    def read(self, layer: int, seq_ids: Sequence[int], dtype: Optional[torch.dtype] = None):
+        """(keys, values) of the sequences, (B, H, longest, D), zeros behind the shorter ones."""
+        slots, table, lens, _ = self._batch(layer, seq_ids)
+        return self.layers[layer].read(table, lens, int(self._held[layer, slots].max()), dtype=dtype or self.dtype)
+
+
+def _bucket(tokens: int) -> int:
+    """A length rounded up to a power of two, so that calls of growing sequences share their checks."""
+    return 1 << max(tokens - 1, 0).bit_length()
+
+
+class KittyPagedAttention8(nn.Module):
+    """``KittyPagedAttention``'s constructor order and ``forward`` over a ``KittyCache8``."""
+
+    def __init__(self, config: KittyConfig, num_q_heads: int, cache: KittyCache8, layer: int) -> None:
+        super().__init__()
+        self.config = config
+        self.num_q_heads = num_q_heads
+        self.num_kv_heads = config.num_kv_heads
+        self.head_dim = config.head_dim
+        self.cache = cache
+        self.layer = layer
+        self.scale = 1.0 / math.sqrt(config.head_dim)
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                seq_id: Union[int, Sequence[int]] = 0, attention_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q (B, Hq, T, D), k and v (B, Hkv, T, D): the tokens join the cache, and each
+        attends over what its sequence holds up to itself; (B, Hq, T, D) in q's type.
+        There is no backward: call under torch.no_grad()."""
+        B, nqh, T, D = q.shape
+        assert nqh == self.num_q_heads
+        assert D == self.head_dim
+        ids = [seq_id + b for b in range(B)] if isinstance(seq_id, int) else [int(s) for s in seq_id]
+        if len(ids) != B:
+            raise ValueError(f"{len(ids)} sequence ids for a batch of {B}")
+        if B == 0 or T == 0:
+            return torch.empty_like(q)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+            raise RuntimeError("the 8-bit cache has no backward: call under torch.no_grad()")
+        x = q.to(self.cache.device)
+        if x.dtype not in (torch.float16, torch.bfloat16):
+            x = x.to(self.cache.dtype)
+        self.cache.push(self.layer, k, v, ids)
+        return self.cache.attend(self.layer, x, ids, self.scale).to(q.device, q.dtype)

@@ -254,6 +254,27 @@ def test_attend_matches_float64(dev, dtype, causal, B, Hq, H, T, D, G, lens):
     check_attend(cache, q, tables(gen, B, W, B * W + 1, dev), lens, causal=causal)
 
 
+# the same rows with a table that could hold far more (entries behind the last page are
+# no ids): work shared by the lengths on the device instead of a workgroup a pair, more
+# than 64 sequences, blocks of 16 to 64 rows, runs that end in the middle of a pair
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,Hq,H,T,D,G,lens", [
+    (1, 4, 1, 1, 64, 16, [300]), (3, 16, 2, 1, 128, 64, [0, 127, 700]), (2, 3, 3, 1, 256, 256, [5, 511]),
+    (70, 2, 1, 1, 32, 16, list(range(70))), (130, 1, 1, 1, 16, 16, [3 * (b % 7) for b in range(130)]), (2, 4, 2, 9, 128, 16, [9, 1000]),
+    (1, 8, 2, 4, 128, 128, [300]), (2, 5, 1, 8, 96, 32, [400, 0]), (2, 4, 1, 15, 64, 16, [50, 333]), (2, 6, 2, 9, 256, 16, [3, 290]),
+    (1, 2, 1, 40, 256, 64, [600]), (1, 16, 1, 4, 128, 64, [1500]), (1, 8, 1, 33, 64, 64, [1500]), (1, 1, 1, 1, 128, 16, [1])])
+def test_attend_shared_by_lengths(dev, dtype, causal, B, Hq, H, T, D, G, lens):
+    gen = torch.Generator().manual_seed(B * 100 + Hq * 10 + T + D)
+    W = (max(lens) + G - 1) // G
+    cache = filled(gen, B * W + 1, H, D, G, dev)
+    cache.scale[::3] *= 1.61
+    wide = torch.full((B, 8192 // G), 1 << 30, dtype=torch.int32, device=dev)
+    wide[:, :W] = tables(gen, B, W, B * W + 1, dev)
+    check_attend(cache, torch.randn(B, Hq, T, D, generator=gen).to(dtype), wide, lens, causal=causal)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("causal", [True, False])
@@ -269,15 +290,16 @@ def test_attend_padded(dev, dtype, causal, T, q_lens):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("Hq,T", [(4, 1), (2, 6), (4, 50)])
-def test_attend_masked_places_reach_no_row(dev, Hq, T):
+@pytest.mark.parametrize("wide", [0, 600])
+@pytest.mark.parametrize("Hq,T", [(4, 1), (2, 6), (4, 50), (4, 80)])
+def test_attend_masked_places_reach_no_row(dev, Hq, T, wide):
     """NaN codes and wild page ids behind the last token, NaN keys and values of later
     tokens, a missing page: only the rows that see them change."""
     gen = torch.Generator().manual_seed(T)
     D, G, n = 128, 16, 150
     cache = filled(gen, 24, 2, D, G, dev)
-    table = tables(gen, 1, 12, 24, dev)
-    table[0, 10:] = torch.tensor([1 << 30, -5], dtype=torch.int32)
+    table = torch.cat([tables(gen, 1, 12, 24, dev), torch.full((1, wide), -9, dtype=torch.int32, device=dev)], 1)
+    table[0, 10:12] = torch.tensor([1 << 30, -5], dtype=torch.int32)
     last = int(table[0, 9])
     for pool in (cache.key, cache.value):        # rows 6 .. of the page that ends inside a tile
         pool.view(torch.uint8)[last, :, n % G:] = 0xFF
@@ -300,19 +322,21 @@ def test_attend_masked_places_reach_no_row(dev, Hq, T):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("T", [1, 4, 48])
-def test_attend_broken_lengths(dev, T):
+@pytest.mark.parametrize("G", [16, 256])
+@pytest.mark.parametrize("T", [1, 4, 20, 48, 300])
+def test_attend_broken_lengths(dev, T, G):
     """Lengths that break the rules give NaN rows to their sequence alone."""
     gen = torch.Generator().manual_seed(T)
-    cache = filled(gen, 12, 1, 64, 16, dev)
+    cache = filled(gen, 60, 1, 64, G, dev)
     q = torch.randn(5, 2, T, 64, generator=gen).half()
-    table = tables(gen, 5, 2, 12, dev)
-    check_attend(cache, q, table, [32, 33, -1, 20, 1 << 30])
-    check_attend(cache, q, table, [32, 30, 1, 20, 0], q_lens=[T, T + 1, 0, -1, 1])
+    table = tables(gen, 5, 2 if G == 16 else 10, 60, dev)
+    most = table.shape[1] * G
+    check_attend(cache, q, table, [32, most + 1, -1, 20, 1 << 30])
+    check_attend(cache, q, table, [most, 30, 1, 20, 0], q_lens=[T, T + 1, 0, -1, 1])
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("T", [1, 20, 40, 100])
 def test_attend_wide_scales(dev, T):
     """Value scales 2^-60 to 2^60 in one sequence, in bf16: weights keep the range of fp32."""
     gen = torch.Generator().manual_seed(T)
