@@ -33,6 +33,9 @@ _ROWS = struct.Struct("2P6qPq2P4i")
 _ATTENTION = struct.Struct("3P6qPq2P7ifPN")
 
 
+_FOLLOWED = "calls of the 8-bit cache cannot be traced, compiled or transformed"
+
+
 def _sig(t: Optional[torch.Tensor]):
     """What the checks of a tensor depend on, but for its address."""
     return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
@@ -135,11 +138,6 @@ class Cache8:
         self._known[sig] = found
         return found
 
-    @staticmethod
-    def _followed() -> None:
-        if calls_followed():
-            raise NotImplementedError("calls of the 8-bit cache cannot be traced, compiled or transformed")
-
     def _launch(self, fn, args: bytes) -> None:
         """`fn` on the current stream of the pools' device."""
         if torch._C._cuda_getDevice() != self._index:
@@ -149,6 +147,9 @@ class Cache8:
             rc = fn(self._ref, args, _hip.stream_ptr(self.device))
         if rc:
             _hip.check(rc)
+
+    # The calls below run their checks once per signature (_known) and spend their time
+    # on the host in tensor attributes, so they ask for each once.
 
     # ------------------------------------------------------------------ calls
     def write(self, key: torch.Tensor, value: torch.Tensor, block_table: torch.Tensor, start: torch.Tensor,
@@ -163,9 +164,11 @@ class Cache8:
         infinities become NaN.  Rows behind the last token keep their bytes.
         Tokens without a page (a negative start, a page number past the table, an
         id outside the pool) are dropped."""
-        self._followed()
-        key, value = _given(key, "key"), _given(value, "value")
-        sig = ("write", _sig(key), _sig(value), _sig(block_table), _sig(start), _sig(lens))
+        if calls_followed():
+            raise NotImplementedError(_FOLLOWED)
+        if key.requires_grad or value.requires_grad or key.is_neg() or value.is_neg():
+            key, value = _given(key, "key"), _given(value, "value")
+        sig = (key.shape, key.stride(), key.dtype, key.device, _sig(value), _sig(block_table), _sig(start), _sig(lens))
         found = self._known.get(sig) if self._on_device else None
         if found is None:
             _need(key.dim() == 4 and key.shape[1] == self.num_kv_heads and key.shape[3] == self.head_dim,
@@ -199,7 +202,8 @@ class Cache8:
         `out`): row t is token start[b] + t (start None: from 0) of sequence b,
         code * scale rounded once; 0 behind its lens[b] tokens, NaN where the
         token has no page."""
-        self._followed()
+        if calls_followed():
+            raise NotImplementedError(_FOLLOWED)
         tokens = int(tokens)
         sig = ("read", tokens, dtype, _sig(block_table), _sig(lens), _sig(start),
                None if out is None else (_sig(out[0]), _sig(out[1])))
@@ -227,11 +231,12 @@ class Cache8:
             if not self._on_device:
                 cpu8.read(self.key, self.value, self.scale, block_table, lens, start, (k, v))
                 return k, v
-            found = self._keep(sig, (shape, _aligned16(k) and _aligned16(v), (*_strides(k), *_strides(v)),
+            like = k.new_empty(1).expand(shape)      # what new outputs look like, of one element
+            found = self._keep(sig, (like, _aligned16(k) and _aligned16(v), (*_strides(k), *_strides(v)),
                                      block_table.stride(0) if B > 1 else 0, (B, tokens, block_table.shape[1], _SRC[dtype])))
-        shape, aligned, strides, bt_stride, rest = found
+        like, aligned, strides, bt_stride, rest = found
         if out is None:
-            k = torch.empty(shape, dtype=dtype, device=self.device)
+            k = torch.empty_like(like, memory_format=torch.contiguous_format)
             v = torch.empty_like(k)
         else:
             k, v = out
@@ -259,11 +264,14 @@ class Cache8:
         rows' log of the sum of exp(score), float32 (B, Hq, T), -inf where a row
         sees nothing.  max_tokens: the largest lens[b] where the program knows it
         (default: what the table can hold); it only chooses how the work is split."""
-        self._followed()
-        q = _given(q, "q")
+        if calls_followed():
+            raise NotImplementedError(_FOLLOWED)
+        if q.requires_grad or q.is_neg():
+            q = _given(q, "q")
         causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
         max_tokens = 0 if max_tokens is None else int(max_tokens)
-        sig = (_sig(q), _sig(block_table), _sig(lens), _sig(q_lens), causal, sm_scale, _sig(out), max_tokens)
+        sig = (q.shape, q.stride(), q.dtype, q.device, _sig(block_table), _sig(lens), None if q_lens is None else _sig(q_lens),
+               causal, sm_scale, None if out is None else _sig(out), max_tokens)
         found = self._known.get(sig) if self._on_device else None
         if found is None:
             _need(q.dim() == 4 and q.shape[3] == self.head_dim, f"q must be (B, Hq, T, {self.head_dim})")
@@ -313,8 +321,8 @@ class Cache8:
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
         # a workspace of the call's own, from torch's allocator on its stream: calls
         # on other streams and in captured graphs never share one
-        ws = q.new_empty((need + 1) // 2)
+        ws = q.new_empty((need + 1) // 2) if need else None
         self._launch(self._lib.kitty_cache8_attention, _ATTENTION.pack(
             q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, block_table.data_ptr(), bt_stride,
-            lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), *rest, ws.data_ptr(), need))
+            lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), *rest, 0 if ws is None else ws.data_ptr(), need))
         return (out, lse) if return_lse else out
