@@ -592,11 +592,15 @@ int kitty_cache8_read(const kitty_cache8 *cache, const kitty_cache8_read_args *a
  * gives NaN rows, and so does a page id outside the pool to the rows that see
  * one of its tokens; masked tokens, whatever they hold, reach no row.
  * Scores, softmax and sums are fp32, the 8-bit codes enter their products
- * exactly, weights in two bf16 terms (16 bits); |q . code| must stay finite.
- * block_table entries behind a sequence's last page are not read.
+ * exactly.  Weights enter theirs in two bf16 terms (16 bits); for bf16 results of
+ * more than 64 rows a KV head (32 where head_dim is above 128; rows: heads of the
+ * group times tokens) in one fp16 term (11 bits).  |q . code| must stay finite.
+ * block_table entries behind a sequence's last page are not read; a row of it may
+ * name up to 2^30 tokens.
  * plan_tokens: what the caller knows of the largest lens[b] (0: table_pages *
- * G); it only chooses how the work is split, results differ by rounding.
- * Calls may overlap on different streams given workspaces of their own. */
+ * G); it only chooses how the work is split, results differ by rounding.  The same
+ * call gives the same bits.  out may be q.  Calls may overlap on different streams
+ * given workspaces of their own (a size of 0 needs none). */
 typedef struct {
     const uint16_t *q; /* (B, Hq, T, D), 16-byte aligned rows */
     uint16_t *out;     /* (B, Hq, T, D), 16-byte aligned rows, q's type */

@@ -636,8 +636,8 @@ static int check_attend8(const kitty_cache8 *cache, const kitty_cache8_attention
         return fail(KITTY_E_INVALID, "dtype must be KITTY_DTYPE_F16 or KITTY_DTYPE_BF16");
     if (!(a.sm_scale > 0.0f) || a.sm_scale > 1e30f)
         return fail(KITTY_E_INVALID, "sm_scale must be positive and finite");
-    if ((int64_t)a.table_pages << c.lg > 0x7fffffff)
-        return fail(KITTY_E_UNSUPPORTED, "a sequence is limited to 2^31 - 1 tokens");
+    if ((int64_t)a.table_pages << c.lg > 1 << 30)
+        return fail(KITTY_E_UNSUPPORTED, "a block table is limited to 2^30 tokens a sequence");
     return KITTY_OK;
 }
 

@@ -84,6 +84,7 @@ def attend(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch
     B, Hq, T, D = q.shape
     P, H, G = key.shape[:3]
     gq = Hq // H
+    q = q.float()       # a copy: out may be q
     out.zero_()
     lse.fill_(-math.inf)
     rows = [T] * B if q_lens is None else q_lens.tolist()
@@ -105,7 +106,7 @@ def attend(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch
         sees = torch.ones(t, n, dtype=torch.bool)
         if causal:
             sees = torch.arange(n) <= torch.arange(n - t, n)[:, None]
-        s = (q[b, :, :t].float().reshape(H, gq * t, D) @ kv[0].transpose(1, 2)).view(H, gq, t, n) * sm_scale
+        s = (q[b, :, :t].reshape(H, gq * t, D) @ kv[0].transpose(1, 2)).view(H, gq, t, n) * sm_scale
         s = s.masked_fill(~sees, -math.inf)
         l = torch.logsumexp(s, -1)
         none = ~sees.any(-1)                                   # rows that see nothing

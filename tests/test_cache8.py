@@ -348,6 +348,28 @@ def test_attend_wide_scales(dev, T):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T,wide", [(1, 0), (1, 500), (5, 0), (40, 500), (100, 0)])
+def test_attend_infinite_queries(dev, T, wide):
+    """Infinite scores as the softmax has them: +inf (and inf - inf) make the row NaN, -inf
+    weighs nothing, a row of nothing else is NaN; the other rows keep their numbers."""
+    gen = torch.Generator().manual_seed(T)
+    cache = filled(gen, 12, 1, 64, 16, dev)
+    cache.key.view(torch.uint8)[..., 7] = 0x38                      # 1.0
+    cache.key.view(torch.uint8)[..., 9].bitwise_or_(1).bitwise_and_(0x77)   # positive, not 0
+    table = torch.cat([tables(gen, 1, 12, 12, dev), torch.zeros(1, wide, dtype=torch.int32, device=dev)], 1)
+    q = torch.randn(1, 4, T, 64, generator=gen).half()
+    clean, _, _, _, _ = Ref(cache).attend(numpy(q), table.cpu().numpy(), [180])
+    q[0, 1, :, 7] = math.inf
+    q[0, 2, :, 7] = -math.inf
+    q[0, 3, 0, 9] = math.inf
+    out, lse = cache.attend(q.to(dev), table, i32([180], dev), return_lse=True)
+    assert out[0, 1].isnan().all() and out[0, 2].isnan().all() and out[0, 3, 0].isnan().all()
+    assert (lse[0, 2] == -math.inf).all()
+    keep = np.abs(numpy(out)[0, 0] - clean[0, 0]) <= 2.0 ** -10 * np.abs(clean[0, 0]) + 1e-3 * np.abs(clean).max()
+    assert keep.all() and out[0, 3, 1:].isfinite().all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
 def test_attend_layouts(dev):
     """Views of fused projections, outputs in (B, T, H, D) memory, shared pages, unaligned
     rows, single-entry dimensions of odd strides: the same numbers."""
@@ -371,6 +393,8 @@ def test_attend_layouts(dev):
     one = x[:1, :1, 3:3 + D].unsqueeze(1)        # (1, 1, 1, D), strides of the fused row
     wide = cache.attend(one.expand(1, Hq, 1, D), table[:1], lens[:1])
     assert torch.equal(wide, cache.attend(one.expand(1, Hq, 1, D).contiguous(), table[:1], lens[:1]))
+    same = q.contiguous()
+    assert cache.attend(same, table, lens, out=same) is same and torch.equal(same, want)
     neg = torch._neg_view(q)
     assert torch.equal(cache.attend(neg, table, lens), cache.attend((-q).contiguous(), table, lens))
     assert torch.equal(cache.attend(q, table, lens, max_tokens=70), want)
@@ -531,7 +555,9 @@ def test_abi_refusals():
     need = ctypes.c_size_t(0)
     assert L.kitty_cache8_attention_workspace_size(ctypes.byref(cache()), ctypes.byref(a), ctypes.byref(need)) == _hip.KITTY_OK
     assert need.value > 0
-    a.tokens = 1 << 28
+    a.table_pages = (1 << 26) + 1
+    assert L.kitty_cache8_attention(ctypes.byref(cache()), ctypes.byref(a), None) == _hip.KITTY_E_UNSUPPORTED
+    a.table_pages, a.tokens = 4000, 1 << 28
     assert L.kitty_cache8_attention_workspace_size(ctypes.byref(cache()), ctypes.byref(a), ctypes.byref(need)) == _hip.KITTY_E_UNSUPPORTED
 
 
