@@ -195,12 +195,8 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
     }
 }
 
-// Units of sequence b for one (KV head, row block).
-__device__ __forceinline__ int units8(const Attend8 &p, int b)
-{
-    const Seq8 s = seq8(p, b);
-    return s.bad ? 0 : (s.n + kUnit - 1) / kUnit;
-}
+// Units of a sequence for one (KV head, row block).
+__device__ __forceinline__ int units8(const Seq8 &s) { return s.bad ? 0 : (s.n + kUnit - 1) / kUnit; }
 
 // This workgroup's run of the batch's units.
 struct Run8 {
@@ -229,7 +225,7 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
     const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb, wg = blockIdx.x;
     // 64 sequences at a time: units of each and the sum up to it
     auto sums = [&](int b0, int &x) {
-        x = b0 + lane < p.B ? units8(p, b0 + lane) * per_seq : 0;
+        x = b0 + lane < p.B ? units8(seq8(p, b0 + lane)) * per_seq : 0;
         int inc = x;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -249,7 +245,9 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
         return false;
     R.u = run_start(total, R.N, wg);
     R.u1 = run_start(total, R.N, wg + 1);
-    for (int b0 = 0, base = 0;;) {
+    // (the bounds here and below are for lengths that another stream changes under the
+    // call: it then gives anything, and ends)
+    for (int b0 = 0, base = 0; b0 < p.B;) {
         const unsigned long long past = __ballot(base + inc > R.u);
         if (past) {
             const int l = __builtin_ctzll(past);
@@ -260,6 +258,7 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
         base += __builtin_amdgcn_readlane(inc, 63);
         inc = sums(b0 += 64, x);
     }
+    return false;
 }
 
 // Whether two workgroups' registers and LDS fit a CU.
@@ -288,9 +287,9 @@ __global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) voi
     const int u0 = R.u, u1 = R.u1;
     int u = R.u, b = R.b, pre = R.pre;
 
-    while (u < u1) {
+    while (u < u1 && b < p.B) {
         const Seq8 sq = seq8(p, b);
-        int nt = units8(p, b), item = u, tile = 0, tile1 = nt;
+        int nt = units8(sq), item = u, tile = 0, tile1 = nt;
         if constexpr (!DIRECT) {
             if (u >= pre + nt * per_seq) {
                 pre += nt * per_seq;
@@ -491,7 +490,8 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
     } else if (sq.n > 0) {
         if (tab.x < 0)
             return;
-        const int first = tab.x >> 1, count = TILES ? p.splits : tab.y - first + 1;
+        tab.x = min(tab.x, 2 * p.n_wg - 1);
+        const int first = tab.x >> 1, count = TILES ? p.splits : min(tab.y, p.n_wg - 1) - first + 1;
         for (int i = ALONE ? group : 0; i < count; i += 4 * STEP) {
             float2 ml[4];
             float4 x[4];
