@@ -195,14 +195,22 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
     }
 }
 
-// Units of a sequence for one (KV head, row block).
-__device__ __forceinline__ int units8(const Seq8 &s) { return s.bad ? 0 : (s.n + kUnit - 1) / kUnit; }
+// Tiles of kUnit tokens of a sequence.
+__device__ __forceinline__ int tiles8(const Seq8 &s) { return s.bad ? 0 : (s.n + kUnit - 1) / kUnit; }
+
+// Units of one (KV head, row block) of a sequence: its tiles, and what beginning it
+// costs a run that has another part already, `start` tiles' time: 2 (64 ragged
+// sequences 206 -> 199 us, 8 with five queries 54.6 -> 52.4; 1, 3 and 4 take 199.2,
+// 199.5, 200.9 and 53.1, 52.2, 52.3), 0 where the runs end with the pairs anyway.
+constexpr int kStart = 2;
+__device__ __forceinline__ int units8(int tiles, int start) { return tiles ? tiles + start : 0; }
 
 // This workgroup's run of the batch's units.
 struct Run8 {
     int total, N;      // all units, workgroups that share them
     int u, u1;         // the run's next unit and its end
     int b, pre;        // the sequence of unit u and its first unit
+    int start;         // units that beginning a (KV head, row block) counts
 };
 
 // First unit of workgroup w: total units shared evenly, the first total % N
@@ -223,9 +231,10 @@ __device__ __forceinline__ int run_of(int total, int N, int u)
 __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
 {
     const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb, wg = blockIdx.x;
-    // 64 sequences at a time: units of each and the sum up to it
-    auto sums = [&](int b0, int &x) {
-        x = b0 + lane < p.B ? units8(seq8(p, b0 + lane)) * per_seq : 0;
+    // 64 sequences at a time: tiles of each, units of each and the sum up to it
+    auto tiles = [&](int b0) { return b0 + lane < p.B ? tiles8(seq8(p, b0 + lane)) : 0; };
+    auto sums = [&](int t, int &x) {
+        x = units8(t, R.start) * per_seq;
         int inc = x;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -234,10 +243,17 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
         }
         return inc;
     };
-    int x, inc = sums(0, x), total = __builtin_amdgcn_readlane(inc, 63);
+    // equal sequences whose pairs the workgroups divide evenly: no run begins a second one
+    int t = tiles(0);
+    const int each = __builtin_amdgcn_readlane(t, 0), items = p.B * per_seq;
+    const int N0 = (int)min((int64_t)p.n_wg, (int64_t)each * items);
+    R.start = kStart;
+    if (p.B <= 64 && N0 > 0 && N0 % items == 0 && !__ballot(lane < p.B && t != each))
+        R.start = 0;
+    int x, inc = sums(t, x), total = __builtin_amdgcn_readlane(inc, 63);
     for (int b0 = 64; b0 < p.B; b0 += 64) {
         int y;
-        total += __builtin_amdgcn_readlane(sums(b0, y), 63);
+        total += __builtin_amdgcn_readlane(sums(tiles(b0), y), 63);
     }
     R.total = total;
     R.N = min(p.n_wg, total);
@@ -256,7 +272,7 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
             return true;
         }
         base += __builtin_amdgcn_readlane(inc, 63);
-        inc = sums(b0 += 64, x);
+        inc = sums(tiles(b0 += 64), x);
     }
     return false;
 }
@@ -279,7 +295,7 @@ __global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) voi
     Run8 R;
     if constexpr (DIRECT) {
         R.b = wg / per_seq;
-        R.pre = 0, R.u = wg - R.b * per_seq, R.u1 = R.u + 1;
+        R.pre = 0, R.start = 0, R.u = wg - R.b * per_seq, R.u1 = R.u + 1;
     } else {
         if (!find_run(p, R))
             return;
@@ -289,14 +305,24 @@ __global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) voi
 
     while (u < u1 && b < p.B) {
         const Seq8 sq = seq8(p, b);
-        int nt = units8(sq), item = u, tile = 0, tile1 = nt;
+        const int tiles = tiles8(sq), units = DIRECT ? tiles : units8(tiles, R.start);
+        int item = u, seg = units, tile = 0, tile1 = tiles;                     // seg: units of this run's part
+        bool first = true, last_part = true;                                    // whether it has the first and last tile
         if constexpr (!DIRECT) {
-            if (u >= pre + nt * per_seq) {
-                pre += nt * per_seq;
+            if (u >= pre + units * per_seq) {
+                pre += units * per_seq;
                 ++b;
                 continue;
             }
-            item = (u - pre) / nt, tile = (u - pre) - item * nt, tile1 = min(nt, tile + (u1 - u));
+            item = (u - pre) / units;
+            const int off = (u - pre) - item * units;
+            seg = min(units - off, u1 - u);
+            if (off + seg <= R.start) {   // none of its tiles
+                u += seg;
+                continue;
+            }
+            first = off <= R.start, last_part = off + seg == units;
+            tile = max(off - R.start, 0), tile1 = off + seg - R.start;
         }
         const int kh = item / p.nrb, rb = item - kh * p.nrb, r0 = rb * RM;
         const int t_lo = r0 / p.gq, t_hi = min((r0 + RM - 1) / p.gq, sq.tq - 1);   // query tokens of the block
@@ -409,11 +435,11 @@ __global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) voi
                         make_float4(W.o[rt][4 * d4][i], W.o[rt][4 * d4 + 1][i], W.o[rt][4 * d4 + 2][i], W.o[rt][4 * d4 + 3][i]);
         }
         __syncthreads();
-        const bool whole = DIRECT || (tile == 0 && tile1 == nt);
+        const bool whole = first && last_part;
         const int slot = 2 * wg + (u == u0 ? 0 : 1), rows = min(RM, p.gq * p.T - r0);
-        if (!DIRECT && tile == 0 && threadIdx.x == 0) {
-            p.ws_tab[b * per_seq + item] = whole ? make_int2(-1, 0) : make_int2(slot, run_of(R.total, R.N, u + nt - 1));
-        }
+        if (!DIRECT && first && threadIdx.x == 0)
+            p.ws_tab[b * per_seq + item] =
+                whole ? make_int2(-1, 0) : make_int2(slot, run_of(R.total, R.N, pre + (item + 1) * units - 1));
         for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
             const int r = i / (DP / 4), ch = 4 * (i - r * (DP / 4));
             float m = kLowest, l = 0.0f;
@@ -451,7 +477,7 @@ __global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) voi
         if constexpr (DIRECT)
             return;
         __syncthreads();
-        u += tile1 - tile;
+        u += seg;
     }
 }
 
@@ -589,7 +615,7 @@ constexpr int64_t kMergeRows = 2048;
 static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &pl)
 {
     const int64_t rows = (int64_t)a.num_q_heads / c.H * a.tokens, pairs = (int64_t)a.batch * c.H;
-    const int64_t cap = (int64_t)a.table_pages << c.lg, units = (cap + kUnit - 1) / kUnit;
+    const int64_t cap = (int64_t)a.table_pages << c.lg, units = kStart + (cap + kUnit - 1) / kUnit;
     if (rows > kMaxBlocks || pairs > kMaxBlocks || pairs * rows > kMaxBlocks)
         return fail(KITTY_E_UNSUPPORTED, "too many rows for one launch");
     const int64_t tokens = a.plan_tokens > 0 ? std::min<int64_t>(a.plan_tokens, cap) : cap;
@@ -601,7 +627,7 @@ static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &p
     pl.RT = rows <= 16 ? 1 : rows <= 32 || pl.direct || pl.DP == 256 ? 2 : rows <= 48 ? 3 : 4;
     const int RM = pl.tiles ? kTileRows : 16 * pl.RT;
     const int64_t nrb = (rows + RM - 1) / RM, items = pairs * nrb;
-    if (items * std::max<int64_t>(units, 1) > 0x7fffffff)
+    if (items * units > 0x7fffffff)
         return fail(KITTY_E_UNSUPPORTED, "too many rows and pages for one launch");
     pl.nrb = (int)nrb;
     pl.n_wg = pl.splits = 1;

@@ -264,13 +264,14 @@ def test_attend_matches_float64(dev, dtype, causal, B, Hq, H, T, D, G, lens):
     (1, 4, 1, 1, 64, 16, [300]), (3, 16, 2, 1, 128, 64, [0, 127, 700]), (2, 3, 3, 1, 256, 256, [5, 511]),
     (70, 2, 1, 1, 32, 16, list(range(70))), (130, 1, 1, 1, 16, 16, [3 * (b % 7) for b in range(130)]), (2, 4, 2, 9, 128, 16, [9, 1000]),
     (1, 8, 2, 4, 128, 128, [300]), (2, 5, 1, 8, 96, 32, [400, 0]), (2, 4, 1, 15, 64, 16, [50, 333]), (2, 6, 2, 9, 256, 16, [3, 290]),
-    (1, 2, 1, 40, 256, 64, [600]), (1, 16, 1, 4, 128, 64, [1500]), (1, 8, 1, 33, 64, 64, [1500]), (1, 1, 1, 1, 128, 16, [1])])
+    (1, 2, 1, 40, 256, 64, [600]), (1, 16, 1, 4, 128, 64, [1500]), (1, 8, 1, 33, 64, 64, [1500]), (1, 1, 1, 1, 128, 16, [1]),
+    (3, 4, 2, 1, 16, 256, [20000, 15001, 37]), (5, 1, 1, 3, 16, 256, [30000, 0, 40000, 129, 9000])])
 def test_attend_shared_by_lengths(dev, dtype, causal, B, Hq, H, T, D, G, lens):
     gen = torch.Generator().manual_seed(B * 100 + Hq * 10 + T + D)
     W = (max(lens) + G - 1) // G
     cache = filled(gen, B * W + 1, H, D, G, dev)
     cache.scale[::3] *= 1.61
-    wide = torch.full((B, 8192 // G), 1 << 30, dtype=torch.int32, device=dev)
+    wide = torch.full((B, max(8192 // G, W)), 1 << 30, dtype=torch.int32, device=dev)
     wide[:, :W] = tables(gen, B, W, B * W + 1, dev)
     check_attend(cache, torch.randn(B, Hq, T, D, generator=gen).to(dtype), wide, lens, causal=causal)
 
