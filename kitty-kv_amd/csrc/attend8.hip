@@ -277,16 +277,21 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
     return false;
 }
 
+// Waves of the row kernel's workgroup: 4 for the runs of the split; where it takes the
+// whole of one (pair, row block) (DIRECT), 16 of one block of rows, each with one step's
+// codes in its 128 registers (8 waves with two steps: 1 x 512 tokens 7.9 us against 7.0,
+// 64 x 512 18.0 against 16.1), 8 of two.
+constexpr int row_waves(int RT, bool direct) { return !direct ? kWaves : RT == 1 ? 16 : 8; }
+
 // Whether two workgroups' registers and LDS fit a CU.
 constexpr bool two_per_cu(int DP, int RT) { return DP <= 128 && DP * RT <= 256; }
 
-// CUT: D is below DP, and the lanes beyond it read nothing.  NW waves: 4 for the
-// runs of the split, 8 (DIRECT) where a workgroup takes the whole of one (pair,
-// row block) and writes its rows, so that no merge follows.
+// CUT: D is below DP, and the lanes beyond it read nothing.  DIRECT: a workgroup takes
+// the whole of one (pair, row block) and writes its rows, so that no merge follows.
 template <int DP, int RT, bool BF16, bool CUT, bool DIRECT>
-__global__ __launch_bounds__(DIRECT ? 512 : 256, two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
+__global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 : two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
 {
-    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NB = 2, NW = DIRECT ? 8 : kWaves, STRIDE = 32 * NW;
+    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NW = row_waves(RT, DIRECT), NB = NW == 16 ? 1 : 2, STRIDE = 32 * NW;
     __shared__ __attribute__((aligned(16))) float lds_o[NW][RM][LD];
     __shared__ float2 lds_ml[NW][RM];
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
@@ -573,19 +578,18 @@ static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 // Which kernel takes a call, by its sizes alone (rows: of a KV head, its group's
 // heads times the queries; tokens: of the longest sequence, as far as the host knows).
 //
-// 1. The row kernel on whole (pair, row block)s, one launch of eight waves each,
-// where a stream of a pair is at most kDirectBytes and there are at most
-// kDirectItems of them, or a workgroup a CU where a pair has several row blocks.  It
-// saves the merge and reads lengths less often, and loses where its eight waves leave
-// the device idle, or where the items fill it anyway.  us, one launch / split and
-// merge, 8 KV heads, one query, groups of 4, fp16:
+// 1. The row kernel on whole (pair, row block)s, one launch, where a stream of a pair
+// is at most kDirectBytes and there are at most kDirectItems of them, or a workgroup
+// a CU where a pair has several row blocks.  It saves the merge (on the host too) and
+// reads lengths less often, and loses where its few workgroups leave the device idle.
+// us, one launch / split and merge, 8 KV heads, one query, groups of 4, fp16:
 //   channels 128, tokens    128          512          1,024        2,048
-//   1 sequence              4.9 /  9.3   7.9 / 10.1   10.7 / 10.3  16.4 / 10.9
-//   16 sequences            5.1 /  9.6   8.3 / 12.9   11.8 / 15.2  20.6 / 20.4
-//   64 sequences            8.2 / 11.5  18.0 / 19.0   28.6 / 29.4  48.4 / 50.4
-//   256 sequences          31.9 / 35.8  70.4 / 62.9  108.7 / 103
-//   channels 64: 1 sequence 512 tokens 6.0 / 9.6, 2,048 11.9 / 9.8; 64 sequences 26.0 / 28.8
-//   channels 256 (two waves' registers spill): 1 sequence 512 tokens 13.3 / 11.8
+//   1 sequence              5.0 /  8.5   7.0 /  9.6    9.9 /  9.6  15.8 / 10.0
+//   16 sequences            5.2 /  9.0   7.6 / 12.2   11.4 / 14.5  20.0 / 20.1
+//   64 sequences            9.1 / 10.6  16.2 / 18.4   26.9 / 28.6  46.6 / 48.7
+//   256 sequences          34.8 / 34.1  61.2 / 62.2   99.9 / 101.4
+//   channels 64: 1 sequence 512 tokens 5.8 / 9.1, 2,048 10.8 / 9.2; 16 of 2,048 12.4 / 15.0
+//   channels 256 (its registers would spill): 1 sequence 512 tokens 13.3 / 11.8
 // and of several row blocks against the tile kernel, bf16:
 //   128 rows, 128 channels, 1 sequence of 1,024 15.6 / 17.0, 8 (256 items) 19.1 / 26.1, 32 75.5 / 44.3
 //   100 rows, 64 channels, 1 sequence of 1,500 13.8 / 14.6, 8 (256 items) 14.5 / 21.5, 32 55.0 / 35.7
@@ -600,7 +604,7 @@ static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 // 8 sequences: 49 / 62, 62 / 61, 39 / 48.
 //
 // 3. The tile kernel beyond.
-constexpr int64_t kDirectBytes = 1024 * 128, kDirectItems = 1024;
+constexpr int64_t kDirectBytes = 1024 * 128, kDirectItems = 4096;
 
 struct Plan8 {
     bool tiles, direct;
@@ -737,12 +741,12 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
     auto rows = [&](auto dp, auto rt, auto bf) {
         constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
         constexpr bool BF = decltype(bf)::value;
-        const dim3 pairs((unsigned)(p.B * p.c.H * p.nrb)), runs((unsigned)p.n_wg), waves8(512);
+        const dim3 pairs((unsigned)(p.B * p.c.H * p.nrb)), runs((unsigned)p.n_wg), waves(64 * row_waves(RT, true));
         if constexpr (DP <= 128 && RT <= 2) {
             if (pl.direct && p.c.D == DP)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true>), pairs, waves8, 0, st, p);
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true>), pairs, waves, 0, st, p);
             else if (pl.direct)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true>), pairs, waves8, 0, st, p);
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true>), pairs, waves, 0, st, p);
             if (pl.direct)
                 return;
         }
