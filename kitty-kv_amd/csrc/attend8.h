@@ -87,7 +87,8 @@ __device__ __forceinline__ unsigned widen(unsigned codes)
         return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.0f, HI));
 }
 
-// (a, b) as packed bf16 terms hi + lo: 16 bits of each, fp32's range.
+// (a, b) as packed bf16 terms hi + lo: 16 bits of each (a rounding to bf16 is off by
+// 2^-8 at most, that of the rest by as much of it), fp32's range.
 __device__ __forceinline__ void split_bf16(float a, float b, unsigned &hi, unsigned &lo)
 {
     bf16x2 h, r;

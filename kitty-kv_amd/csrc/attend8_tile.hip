@@ -22,11 +22,20 @@
 // the running maximum m is that of weight times scale, the exponential gives
 // w = p * scale in one step, and p's sum is that of w by 1 / scale.  It is raised
 // only when a tile passes it by 2^8.
-// Weights: for fp16 results two bf16 terms (16 bits, error 2^-18), as a third of
-// the products' time buys the error of fp32 weights; for bf16 results, which keep
-// 8 bits, one fp16 term (11 bits, error 2^-11 of a weight, 2^-25 of the largest
-// where that is more; w is at most 2^8 and the largest at least 1).  Where the row blocks are too few for the device, the
-// tokens of each are split evenly, and cache8_merge_kernel joins the parts.
+// Weights: for fp16 results two bf16 terms (16 bits, error at most 2^-16), as a
+// third of the products' time buys the error of fp32 weights; for bf16 results,
+// which keep 8 bits, one fp16 term (11 bits: 2^-11 of a weight, 2^-25 of the largest
+// where that is more; w is at most 2^8 and the largest at least 1).
+// Where the row blocks are too few for the device, the tokens of each are split
+// evenly, and cache8_merge_kernel joins the parts.
+//
+// Measured, 32 query / 8 KV heads of 128, 2,048 queries at 18,000 tokens: 850 us
+// fp16 (670 TFLOP/s of the plain product, 1,005 of those executed, where a library
+// product of 8,192^3 reaches 1,170 at the clock that the power limit leaves), 650
+// us bf16; heads of 64 bf16 470 us, of 256 fp16 2,160 us; 8 x 33-100 queries over
+// 700-1,500 states, 16 heads of 64: 20 us.  Of those 850: scales in the exponent
+// 30, page ids a tile ahead 20, NaN values handled behind the loop 75 (the branch in
+// it split the products); wave priorities around the products cost 4 %.
 #include <type_traits>
 
 #include "attend8.h"

@@ -10,6 +10,10 @@
 // read: a thread takes 16 bytes of output in each of four rows; the codes' fp32
 // products with the scale round once.
 // Both are bound by memory, and by launch latency where few tokens are written.
+// Measured: 4 x 8,192 tokens of 8 x 128 fp16 written in 39.8 us (5.05 TB/s; a copy
+// reaches 4.9; 46 without streaming loads), one token of one sequence or of 64 in
+// 4.2; 8 x 8,192 read back in 82 us (4.3 TB/s, three quarters of it stores; 93 with
+// 32 bytes of output a thread and row).
 #include "cache8.h"
 
 namespace kitty {
