@@ -37,7 +37,8 @@
 // 30, page ids a tile ahead 20, NaN values handled behind the loop 75 (the branch in
 // it split the products); wave priorities around the products cost 4 %, and two fp16
 // terms instead of bf16, a sixth fewer vector instructions, 2 % (their products draw
-// more power; at 64 channels they are worth 3 %).
+// more power; at 64 channels they are worth 3 %).  Eight waves a workgroup gain 1 to 5
+// % where their row blocks fill the device exactly, and lose up to 19 elsewhere.
 #include <type_traits>
 
 #include "attend8.h"
