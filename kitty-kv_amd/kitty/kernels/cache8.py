@@ -224,6 +224,7 @@ class Cache8:
                 for t in out:
                     _need(tuple(t.shape) == shape and t.dtype == k.dtype and t.dtype in _SRC and t.stride(3) == 1,
                           f"out must be two {shape} tensors of one type with contiguous channels")
+                    _need(torch._debug_has_internal_overlap(t) != 1, "out must not share memory between its rows")
                     self._here("out", t)
                 dtype = k.dtype
             if B == 0 or tokens == 0:
@@ -288,6 +289,7 @@ class Cache8:
             if out is not None:
                 _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(3) == 1,
                       "out must have q's shape and dtype and contiguous channels")
+                _need(torch._debug_has_internal_overlap(out) != 1, "out must not share memory between its rows")
                 self._here("out", out)
             if B == 0 or T == 0 or not self._on_device:
                 if out is None:
@@ -304,8 +306,9 @@ class Cache8:
                     _hip.KITTY_DTYPE_F16 if q.dtype == torch.float16 else _hip.KITTY_DTYPE_BF16, scale)
             bt_stride = block_table.stride(0) if B > 1 else 0
             size = ctypes.c_size_t(0)
-            _hip.check(self._lib.kitty_cache8_attention_workspace_size(
-                self._ref, _ATTENTION.pack(0, 0, 0, *[0] * 6, 0, bt_stride, 0, 0, *rest, 0, 0), ctypes.byref(size)))
+            with torch.cuda.device(self._index):      # the plan is the pools' device's
+                _hip.check(self._lib.kitty_cache8_attention_workspace_size(
+                    self._ref, _ATTENTION.pack(0, 0, 0, *[0] * 6, 0, bt_stride, 0, 0, *rest, 0, 0), ctypes.byref(size)))
             found = self._keep(sig, (in_place, q.is_contiguous(), head, bt_stride, rest, size.value))
         in_place, like_q, head, bt_stride, rest, need = found
         if not in_place or q.data_ptr() % 16 or (out is not None and out.data_ptr() % 16):

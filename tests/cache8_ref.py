@@ -137,12 +137,12 @@ def tolerance(dtype, ref, spread, mag, small, rows, D, n):
     sums add up the errors of the weights:
     * twice (weight and total) fp32's: scores of D products and sums and 6 factors, 2^-24
       of `mag` each, an exponent's absolute error being the weight's relative one; exp2 and
-      the logarithm of a scale, 2^-20 together (log2 of 2^-64 .. 2^120 to 2^-24 of it);
-      sums of n weights, n 2^-24;
+      the logarithm of a scale, 2^-20 together (log2 is exact for powers of two, and off by
+      2^-24 of 8 at most for the others here); sums of n weights, n 2^-24;
     * the weights' own: two bf16 terms, the first off by half a step, 2^-8 of the weight,
-      the second by 2^-8 of that rest: 2^-16; for bf16 and more than 64 rows of a KV head (32 at
-      more than 128 channels) one fp16 term, 2^-11, and where a weight lies below fp16's normal numbers 2^-25 of the largest
-      weight times its scale, on every code."""
+      the second by 2^-8 of that rest: 2^-16; for bf16 and more than 64 rows of a KV head
+      (32 at more than 128 channels) one fp16 term, 2^-11, and where a weight lies below
+      fp16's normal numbers 2^-25 of the largest weight times its scale, on every code."""
     half = torch.finfo(dtype).eps / 2
     one = dtype == torch.bfloat16 and rows > (64 if D <= 128 else 32)
     w = 2 * ((D + 6) * 2.0 ** -24 * mag + 2.0 ** -20 + n * 2.0 ** -24) + (2.0 ** -11 if one else 2.0 ** -16)

@@ -273,7 +273,9 @@ def test_attend_shared_by_lengths(dev, dtype, causal, B, Hq, H, T, D, G, lens):
     cache.scale[::3] *= 1.61
     wide = torch.full((B, max(8192 // G, W)), 1 << 30, dtype=torch.int32, device=dev)
     wide[:, :W] = tables(gen, B, W, B * W + 1, dev)
-    check_attend(cache, torch.randn(B, Hq, T, D, generator=gen).to(dtype), wide, lens, causal=causal)
+    q = torch.randn(B, Hq, T, D, generator=gen).to(dtype)
+    check_attend(cache, q, wide, lens, causal=causal)
+    check_attend(cache, q, wide, lens, causal=causal, max_tokens=1)      # a wrong hint changes no result
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -484,6 +486,10 @@ def test_refusals():
             c.attend(q, t, n, sm_scale=s)
     with pytest.raises(ValueError, match="out"):
         c.attend(q, t, n, out=q.float())
+    with pytest.raises(ValueError, match="share memory"):
+        c.attend(q, t, n, out=q[:, :1].expand(1, 4, 3, 64))
+    with pytest.raises(ValueError, match="share memory"):
+        c.read(t, n, 3, out=(x, x[:, :, :1].expand(1, 2, 3, 64)))
     with pytest.raises(ValueError, match="out"):
         c.read(t, n, 3, out=(x, x.half()))
     with pytest.raises(ValueError, match="dtype"):
