@@ -116,7 +116,7 @@ class KittyCache8:
         slots = [self.slot(i) for i in seq_ids]
         if len(set(slots)) != len(slots):
             raise ValueError("a sequence appears twice in one batch")
-        s0 = slots[0]
+        s0 = slots[0] if slots else 0
         if slots == list(range(s0, s0 + len(slots))):
             return slots, self.block_table[s0:s0 + len(slots)], self.lens[layer, s0:s0 + len(slots)], None
         key = tuple(slots)
@@ -146,13 +146,13 @@ class KittyCache8:
     def attend(self, layer: int, q: torch.Tensor, seq_ids: Sequence[int], sm_scale: Optional[float] = None) -> torch.Tensor:
         """Causal attention of the last T tokens of each sequence, q (B, Hq, T, D)."""
         slots, table, lens, _ = self._batch(layer, seq_ids)
-        longest = int(self._held[layer, slots].max())
+        longest = int(self._held[layer, slots].max(initial=0))
         return self.layers[layer].attend(q, table, lens, sm_scale=sm_scale, max_tokens=_bucket(longest))
 
     def read(self, layer: int, seq_ids: Sequence[int], dtype: Optional[torch.dtype] = None):
         """(keys, values) of the sequences, (B, H, longest, D), zeros behind the shorter ones."""
         slots, table, lens, _ = self._batch(layer, seq_ids)
-        return self.layers[layer].read(table, lens, int(self._held[layer, slots].max()), dtype=dtype or self.dtype)
+        return self.layers[layer].read(table, lens, int(self._held[layer, slots].max(initial=0)), dtype=dtype or self.dtype)
 
 
 def _bucket(tokens: int) -> int:
@@ -177,6 +177,8 @@ class KittyPagedAttention8(nn.Module):
                 seq_id: Union[int, Sequence[int]] = 0, attention_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q (B, Hq, T, D), k and v (B, Hkv, T, D): the tokens join the cache, and each
         attends over what its sequence holds up to itself; (B, Hq, T, D) in q's type.
+        attention_mask is not read, as in ``KittyPagedAttention``: sequences of unequal
+        lengths are told apart by their ids, and a padded prompt goes in without its padding.
         There is no backward: call under torch.no_grad()."""
         B, nqh, T, D = q.shape
         assert nqh == self.num_q_heads

@@ -114,6 +114,8 @@ def test_refusals_and_limits():
     assert cache.pages_free == 3
     mod(x(1, 1), x(1, 1), x(1, 1), seq_id=3)
     assert mod(x(0, 1), x(0, 1), x(0, 1)).shape == (0, 2, 1, 64)
+    assert cache.attend(0, x(0, 1), []).shape == (0, 2, 1, 64)
+    assert [t.shape for t in cache.read(0, [])] == [(0, 2, 0, 64)] * 2
     assert mod(x(1, 1).float(), x(1, 1).float(), x(1, 1).float(), seq_id=3).dtype == torch.float32
     with pytest.raises(RuntimeError, match="no backward"):
         mod(x(1, 1).requires_grad_(), x(1, 1), x(1, 1), seq_id=3)
