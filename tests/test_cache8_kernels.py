@@ -1,0 +1,48 @@
+"""Attention over the 8-bit cache, kernel by kernel: each case names the kernel that
+its sizes choose (on the CPU path the same numbers are asked of the torch code)."""
+import pytest
+import torch
+
+from cache8_plan import SPLIT, TILE, TILES, WHOLE, plan, planned, widened
+from test_cache8 import BF16, DEVICES, F16, check_attend, filled, tables
+
+
+# every head size the tile kernel has an instance for and between them, in parts and in
+# one; groups that begin and end inside a block of 128 rows, chunks longer than it
+TILE_SHAPES = [
+    (TILES, 1, 4, 1, 40, 128, 64, [700]), (TILES, 2, 3, 1, 43, 64, 16, [43, 300]), (TILES, 1, 4, 2, 70, 80, 32, [500]),
+    (TILES, 1, 1, 1, 97, 96, 128, [400]), (TILES, 2, 5, 1, 27, 16, 16, [90, 27]), (TILES, 1, 2, 1, 65, 32, 256, [1]),
+    (TILES, 1, 3, 1, 50, 192, 32, [200]), (TILES, 1, 2, 1, 66, 256, 16, [333]), (TILES, 2, 2, 2, 130, 128, 16, [0, 257]),
+    (TILE, 29, 3, 3, 65, 64, 16, None), (TILE, 29, 3, 3, 65, 128, 32, None), (TILE, 29, 3, 3, 65, 80, 16, None), (TILE, 1, 6, 1, 7, 240, 64, [90])]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kernel,B,Hq,H,T,D,G,lens", TILE_SHAPES)
+def test_tile_kernel_matches_float64(dev, dtype, causal, kernel, B, Hq, H, T, D, G, lens):
+    gen = torch.Generator().manual_seed(B * 100 + Hq * 10 + T + D)
+    if lens is None:
+        lens = [(37 * b) % 131 if b % 5 == 0 else b % 3 for b in range(B)]
+    W = max(1, (max(lens) + G - 1) // G)
+    cache = filled(gen, B * W + 1, H, D, G, dev)
+    cache.scale[::3] *= 1.61
+    table = tables(gen, B, W, B * W + 1, dev)
+    if kernel == TILES:
+        table = widened(table, 4096 // G)
+    q = torch.randn(B, Hq, T, D, generator=gen).to(dtype)
+    assert planned(cache, q, table) == kernel
+    check_attend(cache, q, table, lens, causal=causal)
+
+
+def test_plans_are_the_librarys():
+    """The restated rule at both sides of its borders."""
+    for args in ((1, 8, 8, 1, 128, 128, 8), (1, 8, 8, 1, 128, 128, 9), (1, 8, 8, 1, 64, 16, 128), (1, 8, 8, 1, 64, 16, 129),
+                 (600, 32, 8, 1, 128, 16, 64), (1, 8, 8, 1, 192, 128, 1), (4, 16, 8, 32, 64, 16, 100), (5, 16, 8, 32, 64, 16, 100),
+                 (1, 8, 1, 8, 128, 64, 999), (1, 8, 1, 9, 128, 64, 999), (1, 8, 1, 4, 256, 64, 999), (1, 11, 1, 3, 256, 64, 999),
+                 (8, 32, 8, 2048, 128, 128, 300), (33, 32, 8, 2048, 128, 128, 300), (1, 1, 1, 1, 16, 16, 0)):
+        plan(*args)
+        plan(*args, max_tokens=100)
+    assert plan(1, 8, 8, 1, 128, 128, 8) == WHOLE and plan(1, 8, 8, 1, 128, 128, 9) == SPLIT
+    assert plan(1, 8, 8, 1, 128, 128, 9, max_tokens=1024) == WHOLE
+    assert plan(1, 8, 1, 8, 128, 64, 999) == SPLIT and plan(1, 8, 1, 9, 128, 64, 999) == TILES
