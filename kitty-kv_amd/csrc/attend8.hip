@@ -478,6 +478,8 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
             const int t = (r0 + r) / p.gq, h = kh * p.gq + (r0 + r) - t * p.gq;
             const bool none = !sq.bad && visible8(p, sq, t) == 0;
             const float inv = sq.bad ? __builtin_nanf("") : none ? 0.0f : 1.0f / l;
+            if (none)   // steps that no row masks went into its sums too, NaN among them
+                acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (!CUT || ch < p.c.D)
                 *(uint2 *)(p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok + ch) =
                     make_uint2((uint32_t)f2x(acc.x * inv, BF16) | (uint32_t)f2x(acc.y * inv, BF16) << 16,
@@ -563,6 +565,8 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
     if (ch >= p.c.D)
         return;
     const bool none = !sq.bad && visible8(p, sq, t) == 0;
+    if (none)   // steps that no row masks went into its sums too, NaN among them
+        o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     const float inv = none ? 0.0f : 1.0f / l;
     *(uint2 *)(p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok + ch) =
         make_uint2((uint32_t)f2x(o.x * inv, BF16) | (uint32_t)f2x(o.y * inv, BF16) << 16,

@@ -397,6 +397,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
     }
     const bool none = !sq.bad && W.vis == 0;
     const float inv = sq.bad ? __builtin_nanf("") : none ? 0.0f : 1.0f / l;
+    auto result = [&](float x) -> uint32_t { return f2x(none ? 0.0f : x * inv, BF16); };   // none: tiles that no row masks went into x too
     uint16_t *o = p.out + b * p.o_s_seq + h * p.o_s_head + t * p.o_s_tok;
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt)
@@ -404,8 +405,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
         for (int j = 0; j < 4; ++j) {
             const int ch = 32 * dt + 8 * j + 4 * g;
             if (!CUT || ch < p.c.D)
-                *(uint2 *)(o + ch) = make_uint2((uint32_t)f2x(W.o[dt][4 * j] * inv, BF16) | (uint32_t)f2x(W.o[dt][4 * j + 1] * inv, BF16) << 16,
-                                                (uint32_t)f2x(W.o[dt][4 * j + 2] * inv, BF16) | (uint32_t)f2x(W.o[dt][4 * j + 3] * inv, BF16) << 16);
+                *(uint2 *)(o + ch) = make_uint2(result(W.o[dt][4 * j]) | result(W.o[dt][4 * j + 1]) << 16,
+                                                result(W.o[dt][4 * j + 2]) | result(W.o[dt][4 * j + 3]) << 16);
         }
     if (g == 0 && p.lse)
         p.lse[((int64_t)b * p.Hq + h) * p.T + t] =

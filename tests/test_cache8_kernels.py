@@ -35,6 +35,48 @@ def test_tile_kernel_matches_float64(dev, dtype, causal, kernel, B, Hq, H, T, D,
     check_attend(cache, q, table, lens, causal=causal)
 
 
+# (kernel, sequences, query heads, KV heads, queries, head size): a batch whose other
+# sequences make the sizes, and a first one that the test is about
+PADDED = [(WHOLE, 2, 2, 2, 5, 64), (WHOLE, 2, 6, 1, 9, 128), (SPLIT, 2, 2, 1, 5, 64), (SPLIT, 2, 4, 2, 16, 128), (SPLIT, 2, 2, 1, 10, 256),
+          (SPLIT, 130, 8, 1, 2, 64), (TILES, 2, 4, 2, 40, 64), (TILES, 2, 2, 1, 70, 96), (TILES, 2, 2, 1, 33, 256),
+          (TILE, 87, 1, 1, 66, 64), (TILE, 87, 1, 1, 66, 128)]
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("kernel,B,Hq,H,T,D", PADDED)
+def test_padded_rows_are_zero_whatever_real_rows_see(dev, dtype, causal, kernel, B, Hq, H, T, D):
+    """NaN keys, NaN values and a missing page in early tokens, which every real row of
+    the block sees: NaN rows where the row is real, zeros and -inf behind q_lens."""
+    gen = torch.Generator().manual_seed(B + T + D)
+    G, n = 16, 150
+    few = B > 2                                    # the others of a large batch hold a token or nothing
+    cache = filled(gen, 2 * 10 + 2, H, D, G, dev)
+    table = widened(tables(gen, 2, 10, 20, dev), 10 if kernel == TILE or kernel == WHOLE else 4096 // G)
+    if few:
+        table = torch.cat([table, table[1:].expand(B - 2, -1)])
+    q = torch.randn(B, Hq, T, D, generator=gen).to(dtype)
+    lens = [n, 140] + [b % 2 for b in range(B - 2)]
+    q_lens = [max(T - 3, T // 2), T // 2] + [b % 3 % (T + 1) for b in range(B - 2)]
+    assert planned(cache, q, table) == kernel
+
+    def check():
+        out = check_attend(cache, q, table, lens, q_lens=q_lens, causal=causal)
+        for b in range(2):
+            assert (out[b, :, q_lens[b]:] == 0).all()
+
+    check()
+    cache.value.view(torch.uint8)[int(table[0, 0]), 0, 3, 5] = 0x7F
+    check()
+    cache.key.view(torch.uint8)[int(table[1, 1]), H - 1, 7, D - 1] = 0xFF
+    check()
+    table[0, 1] = 22                               # outside the pool
+    if few:
+        table[2:, 0] = -1                          # of sequences whose one token no or one row sees
+    check()
+
+
 def test_plans_are_the_librarys():
     """The restated rule at both sides of its borders."""
     for args in ((1, 8, 8, 1, 128, 128, 8), (1, 8, 8, 1, 128, 128, 9), (1, 8, 8, 1, 64, 16, 128), (1, 8, 8, 1, 64, 16, 129),
