@@ -17,28 +17,32 @@
 //  8g + e of a 16-token step stand for tokens 4g + e (e < 4) and 8 + 4g + e - 4,
 //  and ds_read_b64_tr_b16 fetches the value rows in that order.
 //
-// Scales belong to 16-token steps (a page holds 16 tokens or more): the key's is
-// a factor of the scores, the logarithm of the value's is added to them, so that
-// the running maximum m is that of weight times scale, the exponential gives
-// w = p * scale in one step, and p's sum is that of w by 1 / scale.  It is raised
-// only when a tile passes it by 2^8.
-// Weights: for fp16 results two bf16 terms (16 bits, error at most 2^-16), as a
-// third of the products' time buys the error of fp32 weights; for bf16 results,
-// which keep 8 bits, one fp16 term (11 bits: 2^-11 of a weight, 2^-25 of the largest
-// where that is more; w is at most 2^8 and the largest at least 1).
+// Scales belong to 16-token steps (a page holds 16 tokens or more): the key's is a
+// factor of the scores, the value's of the weights.
+// Weights: for fp16 results two bf16 terms of weight times scale (16 bits, error at
+// most 2^-16, with fp32's range), as a third of the products' time buys the error of
+// fp32 weights.  For bf16 results, which keep 8 bits, one fp16 term (11 bits: 2^-11 of
+// a weight, 2^-25 of the largest where that is more), as long as the value scales met
+// lie close enough for its range; the logarithm of the scale is then added to the
+// scores, so that the running maximum m is that of weight times scale, the exponential
+// gives w = p * scale in one step (at most 2^8, the largest at least 1), and p's sum is
+// that of w by 1 / scale.  From the first tile with a scale beyond (a page of zeros has
+// 2^-64) the two terms.  The maximum is raised only when a tile passes it by 2^8.
 // Where the row blocks are too few for the device, the tokens of each are split
 // evenly, and cache8_merge_kernel joins the parts.
 //
-// Measured, 32 query / 8 KV heads of 128, 2,048 queries at 18,000 tokens: 850 us
-// fp16 (670 TFLOP/s of the plain product, 1,005 of those executed, where a library
-// product of 8,192^3 reaches 1,170 at the clock that the power limit leaves), 650
-// us bf16; heads of 64 bf16 470 us, of 256 fp16 2,160 us; 8 x 33-100 queries over
-// 700-1,500 states, 16 heads of 64: 20 us.  Of those 850: scales in the exponent
-// 30, page ids a tile ahead 20, NaN values handled behind the loop 75 (the branch in
-// it split the products); wave priorities around the products cost 4 %, and two fp16
-// terms instead of bf16, a sixth fewer vector instructions, 2 % (their products draw
-// more power; at 64 channels they are worth 3 %).  Eight waves a workgroup gain 1 to 5
-// % where their row blocks fill the device exactly, and lose up to 19 elsewhere.
+// Measured, 32 query / 8 KV heads of 128, 2,048 queries at 18,000 tokens (785 to 940 by
+// card and data; the same card for all of these): 848 us fp16 (670 TFLOP/s of the plain
+// product, 1,005 of those executed, where a library product of 8,192^3 reaches 1,170 at
+// the clock that the power limit leaves), 658 us bf16, 835 from a far value scale on;
+// heads of 64 fp16 581, bf16 466 us, of 256 2,090 and 1,925 us; 8 x 33-100 queries over
+// 1,500 states, 16 heads of 64, bf16: 25 us with the merge.  Of the bf16 figures the look
+// at the value scales is 1 to 5 % (64 channels 458 without, 256 1,838).  Of the 848: page
+// ids a tile ahead 20, NaN values handled behind the loop 75 (the branch in it split the
+// products); wave priorities around the products cost 4 %, and two fp16 terms instead of
+// bf16, a sixth fewer vector instructions, 2 % (their products draw more power; at 64
+// channels they are worth 3 %).  Eight waves a workgroup gain 1 to 5 % where their row
+// blocks fill the device exactly, and lose up to 19 elsewhere.
 #include <type_traits>
 
 #include "attend8.h"
@@ -101,20 +105,27 @@ template <int DP>
 struct TileState {
     u32x4 q[DP / 16];    // k-step s: channels 16s + 8g .. + 7
     f32x16 o[DP / 32];   // O^T: channels 32dt + 8 (i / 4) + 4g + i % 4
-    float m, l;          // running maximum of score + log2(value scale), this lane's half of the sum
+    float m, l;          // running maximum of score (one term: + log2(value scale)), this lane's half of the sum
     int vis;             // tokens the row sees
     int k_base, v_base[DP / 32];
 };
 
-// Scales of a 16-token step: the key's times sm_scale * log2(e), and of the value's
-// the logarithm and the reciprocal.
+// One fp16 term takes value scales (as bits of positive floats) within 2^12 of each
+// other, so that its 2^-25 of the largest product of weight and scale is at most 2^-13
+// of a weight near 1, and from 2^-64 to 2^32, so that neither the reciprocals nor the
+// sum of weights leave fp32's range.
+constexpr uint32_t kLeastScale = (127 - 64) << 23, kMostScale = (127 + 32) << 23, kSpan = 12 << 23;
+
+// Scales of a 16-token step: the key's times sm_scale * log2(e); of the value's the
+// scale itself (two terms) or the logarithm and the reciprocal (one term).
 struct StepScale {
-    float key, log_v, inv_v;
+    float key, value, inv_v;
 };
 
 // Tokens t0 .. t0 + 63 in a stage folded into the wave's rows.  mask: some row does
-// not see them all.
-template <int DP, bool BF16>
+// not see them all.  Sums and outputs are relative to 2^m, whatever m was taken from:
+// a wave may go over from one term to two at any tile.
+template <int DP, bool BF16, int TERMS>
 __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char *kst, const unsigned char *vst, int t0,
                                           const StepScale (&sc)[4], int lane, bool mask)
 {
@@ -147,7 +158,7 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
 #pragma unroll
         for (int i = 1; i < 8; ++i)
             a = fmaxf(a, S[st >> 1][8 * (st & 1) + i]);
-        mx = fmaxf(mx, __builtin_fmaf(a, sc[st].key, sc[st].log_v));
+        mx = fmaxf(mx, TERMS == 2 ? a * sc[st].key : __builtin_fmaf(a, sc[st].key, sc[st].value));
     }
     mx = other_max(mx);
     const bool raise = mx > W.m + 8.0f;
@@ -162,11 +173,10 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
             for (int i = 0; i < 16; ++i)
                 W.o[dt][i] *= alpha;
     }
-    constexpr int TERMS = BF16 ? 1 : 2;
     unsigned pt[TERMS][2][8];
 #pragma unroll
     for (int st = 0; st < 4; ++st) {
-        const float add = sc[st].log_v - W.m;
+        const float add = TERMS == 2 ? -W.m : sc[st].value - W.m;
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int i = 4 * (st & 1); i < 4 * (st & 1) + 4; ++i) {
@@ -174,12 +184,12 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
             const float b = __builtin_amdgcn_exp2f(__builtin_fmaf(S[st >> 1][2 * i + 1], sc[st].key, add));
             sum[0] += a;
             sum[1] += b;
-            if constexpr (BF16)
+            if constexpr (TERMS == 1)
                 pt[0][st >> 1][i] = pack_f16(a, b);
             else
-                split_bf16(a, b, pt[0][st >> 1][i], pt[1][st >> 1][i]);
+                split_bf16(a * sc[st].value, b * sc[st].value, pt[0][st >> 1][i], pt[1][st >> 1][i]);
         }
-        W.l = __builtin_fmaf(sum[0] + sum[1], sc[st].inv_v, W.l);
+        W.l = TERMS == 2 ? W.l + (sum[0] + sum[1]) : __builtin_fmaf(sum[0] + sum[1], sc[st].inv_v, W.l);
     }
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -199,7 +209,7 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
             const u32x4 w = {pt[k][mt][r], pt[k][mt][r + 1], pt[k][mt][r + 2], pt[k][mt][r + 3]};
 #pragma unroll
             for (int dt = 0; dt < DP / 32; ++dt)
-                W.o[dt] = mfma32<!BF16>(vf[dt], w, W.o[dt]);
+                W.o[dt] = mfma32<TERMS == 2>(vf[dt], w, W.o[dt]);
         }
     }
 }
@@ -268,6 +278,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
     uint64_t raw[4];         // the next tile's scales
     int ids[4];              // page ids of the tile that load() takes
     unsigned lost = 0;       // bits of the next tile's steps that have no page
+    uint32_t least = kMostScale, most = 0;   // value scales met, as bits
+    bool far = false;        // whether one fp16 term does not take them
     auto fetch_ids = [&](int tile) {
 #pragma unroll
         for (int st = 0; st < 4; ++st)
@@ -294,7 +306,16 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
         }
         fetch_ids(tile + 1);   // a step ahead: the loads above wait for no scalar load of their own
     };
-    auto store = [&](int tile, int stage) {
+    auto store = [&](int tile, int stage, auto terms) {
+        constexpr int TERMS = decltype(terms)::value;
+        if constexpr (TERMS == 1) {
+#pragma unroll
+            for (int st = 0; st < 4; ++st) {
+                least = min(least, (uint32_t)(raw[st] >> 32));
+                most = max(most, (uint32_t)(raw[st] >> 32));
+            }
+            far = least < kLeastScale || most > kMostScale || most > least + kSpan;
+        }
         bool odd = false;
         const bool ragged = (tile + 1) * kTile > vis_min;
 #pragma unroll
@@ -321,7 +342,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
             unsigned char *k = ks[stage] + rw * 2 * DP;
             *(u32x4 *)(k + 16 * key_slot<DP>(rw, 2 * lc)) = x[0];
             *(u32x4 *)(k + 16 * key_slot<DP>(rw, 2 * lc + 1)) = x[1];
-            widen16<!BF16>(vr[j], x);
+            widen16<TERMS == 2>(vr[j], x);
             unsigned char *v = vs[stage] + rw * 2 * DP;
             *(u32x4 *)(v + 16 * value_slot<DP>(rw, 2 * lc)) = x[0];
             *(u32x4 *)(v + 16 * value_slot<DP>(rw, 2 * lc + 1)) = x[1];
@@ -331,28 +352,42 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
             const float vs = fmaxf(__builtin_bit_cast(float, (uint32_t)(raw[st] >> 32)), 1.175494351e-38f);
-            sc[st] = StepScale{__builtin_bit_cast(float, (uint32_t)raw[st]) * p.cs, __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
+            sc[st] = StepScale{__builtin_bit_cast(float, (uint32_t)raw[st]) * p.cs, TERMS == 2 ? vs : __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
         }
     };
     if (threadIdx.x == 0)
         met_nan = 0;
     __syncthreads();
+    typedef std::integral_constant<int, BF16 ? 1 : 2> Terms;
+    int tile = first;
     if (first < end) {
         fetch_ids(first);
         load(first);
-        store(first, 0);
+        store(first, 0, Terms{});
     }
-    for (int tile = first; tile < end; ++tile) {
+    for (; tile < end && (!BF16 || !far); ++tile) {
         const int stage = (tile - first) & 1, t0 = tile * kTile;
         __syncthreads();   // the tile is in its stage; every wave is done with the other one
         const bool more = tile + 1 < end;
         if (more)
             load(tile + 1);
-        if (t0 < wave_max) {
-            tile_step<DP, BF16>(W, ks[stage], vs[stage], t0, sc, lane, t0 + kTile > wave_min);
-        }
+        if (t0 < wave_max)
+            tile_step<DP, BF16, Terms::value>(W, ks[stage], vs[stage], t0, sc, lane, t0 + kTile > wave_min);
         if (more)
-            store(tile + 1, stage ^ 1);
+            store(tile + 1, stage ^ 1, Terms{});
+    }
+    if constexpr (BF16) {
+        // from the first tile whose value scales one term does not take: nothing is fetched
+        // ahead, which keeps the loop above in its registers
+        for (; tile < end; ++tile) {
+            __syncthreads();
+            fetch_ids(tile);
+            load(tile);
+            store(tile, 0, std::integral_constant<int, 2>{});
+            __syncthreads();
+            if (tile * kTile < wave_max)
+                tile_step<DP, BF16, 2>(W, ks[0], vs[0], tile * kTile, sc, lane, (tile + 1) * kTile > wave_min);
+        }
     }
 
     __syncthreads();

@@ -1,9 +1,11 @@
 """Attention over the 8-bit cache, kernel by kernel: each case names the kernel that
 its sizes choose (on the CPU path the same numbers are asked of the torch code)."""
+import numpy as np
 import pytest
 import torch
 
 from cache8_plan import SPLIT, TILE, TILES, WHOLE, plan, planned, widened
+from cache8_ref import Ref, numpy, tolerance
 from test_cache8 import BF16, DEVICES, F16, check_attend, filled, tables
 
 
@@ -88,3 +90,63 @@ def test_plans_are_the_librarys():
     assert plan(1, 8, 8, 1, 128, 128, 8) == WHOLE and plan(1, 8, 8, 1, 128, 128, 9) == SPLIT
     assert plan(1, 8, 8, 1, 128, 128, 9, max_tokens=1024) == WHOLE
     assert plan(1, 8, 1, 8, 128, 64, 999) == SPLIT and plan(1, 8, 1, 9, 128, 64, 999) == TILES
+
+
+# (kernel, query heads, queries, head size) on one KV head
+FAR = [(WHOLE, 4, 5, 64), (SPLIT, 4, 5, 64), (SPLIT, 8, 7, 128), (TILES, 4, 40, 64), (TILES, 2, 70, 128), (TILES, 2, 20, 256),
+       (TILE, 2, 20, 192)]
+
+
+def far_cache(gen, D, exponents, dev):
+    """Pages of 16 tokens in order, the value scales 2^e; a page of 2^-64 is what a page of zeros leaves."""
+    cache = filled(gen, len(exponents), 1, D, 16, dev)
+    cache.scale[:, 0, 1] = torch.tensor([2.0 ** e for e in exponents], device=dev)
+    for p, e in enumerate(exponents):
+        if e == -64:
+            cache.value.view(torch.uint8)[p] = 0
+    table = torch.arange(len(exponents), dtype=torch.int32, device=dev)[None]
+    return cache, table
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("exponents", [
+    [-64, 90] * 5, [90] + [-64] * 9, [-64] * 9 + [90], [-8] * 6 + [-64, 100, -8, -8], [-100, 5] * 5, [100, -8] * 5,
+    [-8] * 8 + [-100, 110], [3, -30, -8] * 3 + [4]])
+@pytest.mark.parametrize("kernel,Hq,T,D", FAR)
+def test_value_scales_far_apart(dev, kernel, Hq, T, D, exponents):
+    """Pages of one sequence whose value scales lie up to 2^210 apart, as large values beside
+    a page of zeros leave them: each page keeps its share of the softmax."""
+    gen = torch.Generator().manual_seed(T + D)
+    cache, table = far_cache(gen, D, exponents, dev)
+    cache.scale[:, 0, 0] = 2.0 ** -8
+    if kernel in (SPLIT, TILES):
+        table = widened(table, 300)
+    q = torch.randn(1, Hq, T, D, generator=gen).to(BF16)
+    assert planned(cache, q, table) == kernel
+    for causal in (True, False):
+        check_attend(cache, q, table, [16 * len(exponents) - 3], causal=causal)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kernel,Hq,T,D", FAR)
+def test_small_pages_beside_a_large_one(dev, kernel, Hq, T, D, dtype):
+    """A page with one huge channel: in the others its codes are zeros, and what the small
+    pages hold there keeps its bits, however much larger the weight times scale of that page."""
+    gen = torch.Generator().manual_seed(T + D)
+    for small, large in ((-20, 0), (-14, 6), (-100, -8)) if dtype == BF16 else ((-20, -5), (-100, -8)):
+        cache, table = far_cache(gen, D, [small] * 4 + [large] + [small] * 5, dev)
+        cache.value.view(torch.uint8)[4, :, :, 1:] = 0
+        cache.scale[:, 0, 0] = 2.0 ** -9
+        if kernel in (SPLIT, TILES):
+            table = widened(table, 300)
+        q = torch.randn(1, Hq, T, D, generator=gen).to(dtype)
+        assert planned(cache, q, table) == kernel
+        out = numpy(cache.attend(q.to(dev), table, torch.tensor([157], dtype=torch.int32, device=dev), causal=False))
+        want, _, spread, mag, weak = Ref(cache).attend(numpy(q), table.cpu().numpy(), [157], causal=False)
+        tol = tolerance(dtype, want, spread, mag, weak, 1, D, 157)          # of one row: weights of two terms
+        if dtype == BF16 and kernel in (TILE, TILES):
+            # the first 64 tokens are of small pages alone: one fp16 term, off by 2^-11 of a weight, and
+            # by 2^-25 of the largest of them where that is more; weights here are within 2^6 of each other
+            tol = tol + (2.0 ** -11 + 2.0 ** -25 * 2.0 ** 6) * spread
+        assert (np.abs(out - want) <= tol).all()
