@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
                 }
                 const uint64_t sc = uniform_load((const uint64_t *)(sp + page * p.c.scale_s_page));
                 buf.sc[hf] = make_float2(bad ? __builtin_nanf("") : __builtin_bit_cast(float, (uint32_t)sc),
-                                         __builtin_bit_cast(float, (uint32_t)(sc >> 32)));
+                                         bad ? 1.0f : __builtin_bit_cast(float, (uint32_t)(sc >> 32)));   // page 0's may be no number
             }
         };
         // A ring of NB steps' codes, NB - 1 in flight while one is computed; the page

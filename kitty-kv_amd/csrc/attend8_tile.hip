@@ -32,12 +32,12 @@
 // evenly, and cache8_merge_kernel joins the parts.
 //
 // Measured, 32 query / 8 KV heads of 128, 2,048 queries at 18,000 tokens (785 to 940 by
-// card and data; the same card for all of these): 848 us fp16 (670 TFLOP/s of the plain
+// card and data; the same card for all of these): 847 us fp16 (670 TFLOP/s of the plain
 // product, 1,005 of those executed, where a library product of 8,192^3 reaches 1,170 at
-// the clock that the power limit leaves), 658 us bf16, 835 from a far value scale on;
-// heads of 64 fp16 581, bf16 466 us, of 256 2,090 and 1,925 us; 8 x 33-100 queries over
+// the clock that the power limit leaves), 660 us bf16, 831 from a far value scale on;
+// heads of 64 fp16 583, bf16 472 us, of 256 2,085 and 1,915 us; 8 x 33-100 queries over
 // 1,500 states, 16 heads of 64, bf16: 25 us with the merge.  Of the bf16 figures the look
-// at the value scales is 1 to 5 % (64 channels 458 without, 256 1,838).  Of the 848: page
+// at the value scales is 1 to 5 % (64 channels 459 without, 256 1,839).  Of the 847: page
 // ids a tile ahead 20, NaN values handled behind the loop 75 (the branch in it split the
 // products); wave priorities around the products cost 4 %, and two fp16 terms instead of
 // bf16, a sixth fewer vector instructions, 2 % (their products draw more power; at 64
@@ -308,6 +308,11 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
     };
     auto store = [&](int tile, int stage, auto terms) {
         constexpr int TERMS = decltype(terms)::value;
+        if (lost) {   // scales 1 for the steps without a page: page 0's may be no numbers
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+                raw[st] = lost >> st & 1 ? 0x3f8000003f800000ull : raw[st];
+        }
         if constexpr (TERMS == 1) {
 #pragma unroll
             for (int st = 0; st < 4; ++st) {
@@ -351,7 +356,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
             met_nan = 1;
 #pragma unroll
         for (int st = 0; st < 4; ++st) {
-            const float vs = fmaxf(__builtin_bit_cast(float, (uint32_t)(raw[st] >> 32)), 1.175494351e-38f);
+            const float vs = __builtin_bit_cast(float, (uint32_t)(raw[st] >> 32));
             sc[st] = StepScale{__builtin_bit_cast(float, (uint32_t)raw[st]) * p.cs, TERMS == 2 ? vs : __builtin_amdgcn_logf(vs), __builtin_amdgcn_rcpf(vs)};
         }
     };

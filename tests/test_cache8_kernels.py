@@ -150,3 +150,25 @@ def test_small_pages_beside_a_large_one(dev, kernel, Hq, T, D, dtype):
             # by 2^-25 of the largest of them where that is more; weights here are within 2^6 of each other
             tol = tol + (2.0 ** -11 + 2.0 ** -25 * 2.0 ** 6) * spread
         assert (np.abs(out - want) <= tol).all()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scales", [[float("nan")] * 2, [0.0] * 2, [float("inf")] * 2, [1.0, float("nan")]])
+@pytest.mark.parametrize("kernel,Hq,T,D", FAR)
+def test_missing_page_takes_nothing_from_page_0(dev, kernel, Hq, T, D, dtype, scales):
+    """Page 0 is nobody's and its scales are no numbers: a page id outside the pool reaches
+    the rows that see its tokens and no other."""
+    gen = torch.Generator().manual_seed(T + D)
+    cache = filled(gen, 12, 1, D, 16, dev)
+    table = torch.arange(1, 11, dtype=torch.int32, device=dev)[None]
+    if kernel in (SPLIT, TILES):
+        table = widened(table, 300)
+    q = torch.randn(1, Hq, T, D, generator=gen).to(dtype)
+    assert planned(cache, q, table) == kernel
+    want = cache.attend(q.to(dev), table, torch.tensor([147], dtype=torch.int32, device=dev))
+    table[0, 9] = 12
+    cache.scale[0, 0] = torch.tensor(scales, device=dev)
+    out = cache.attend(q.to(dev), table, torch.tensor([147], dtype=torch.int32, device=dev))
+    assert out[:, :, -3:].isnan().all()                    # tokens 144 .. 146 are behind the table's last page
+    assert torch.equal(out[:, :, :-3], want[:, :, :-3])
