@@ -32,12 +32,12 @@
 // evenly, and cache8_merge_kernel joins the parts.
 //
 // Measured, 32 query / 8 KV heads of 128, 2,048 queries at 18,000 tokens (785 to 940 by
-// card and data; the same card for all of these): 847 us fp16 (670 TFLOP/s of the plain
-// product, 1,005 of those executed, where a library product of 8,192^3 reaches 1,170 at
-// the clock that the power limit leaves), 660 us bf16, 831 from a far value scale on;
-// heads of 64 fp16 583, bf16 472 us, of 256 2,085 and 1,915 us; 8 x 33-100 queries over
+// card and data; the same card for all of these): 851 us fp16 (665 TFLOP/s of the plain
+// product, 995 of those executed, where a library product of 8,192^3 reaches 1,170 at
+// the clock that the power limit leaves), 665 us bf16, 830 from a far value scale on;
+// heads of 64 fp16 581, bf16 469 us, of 256 2,087 and 1,928 us; 8 x 33-100 queries over
 // 1,500 states, 16 heads of 64, bf16: 25 us with the merge.  Of the bf16 figures the look
-// at the value scales is 1 to 5 % (64 channels 459 without, 256 1,839).  Of the 847: page
+// at the value scales is 1 to 5 % (64 channels 460 without, 256 1,840).  Of the 851: page
 // ids a tile ahead 20, NaN values handled behind the loop 75 (the branch in it split the
 // products); wave priorities around the products cost 4 %, and two fp16 terms instead of
 // bf16, a sixth fewer vector instructions, 2 % (their products draw more power; at 64
@@ -127,7 +127,7 @@ struct StepScale {
 // a wave may go over from one term to two at any tile.
 template <int DP, bool BF16, int TERMS>
 __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char *kst, const unsigned char *vst, int t0,
-                                          const StepScale (&sc)[4], int lane, bool mask)
+                                          StepScale (&sc)[4], int lane, bool mask)
 {
     const int g = lane >> 5, n = lane & 31;
     f32x16 S[2];
@@ -150,6 +150,9 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 S[mt][i] = t0 + 32 * mt + 8 * (i >> 2) + 4 * g + (i & 3) < W.vis ? S[mt][i] : -__builtin_inff();
+#pragma unroll
+        for (int st = 0; st < 4; ++st)   // above 0 as a factor of -infinity; the scores are 0 either way
+            sc[st].key = sc[st].key < 1.175494351e-38f ? 1.175494351e-38f : sc[st].key;
     }
     float mx = -__builtin_inff();
 #pragma unroll

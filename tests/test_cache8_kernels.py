@@ -172,3 +172,19 @@ def test_missing_page_takes_nothing_from_page_0(dev, kernel, Hq, T, D, dtype, sc
     out = cache.attend(q.to(dev), table, torch.tensor([147], dtype=torch.int32, device=dev))
     assert out[:, :, -3:].isnan().all()                    # tokens 144 .. 146 are behind the table's last page
     assert torch.equal(out[:, :, :-3], want[:, :, :-3])
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("kernel,Hq,T,D", FAR)
+def test_scores_that_underflow(dev, kernel, Hq, T, D, dtype):
+    """Key scales and sm_scale whose product is below fp32's numbers: every visible token
+    weighs the same, masked ones nothing."""
+    gen = torch.Generator().manual_seed(T + D)
+    cache, table = far_cache(gen, D, [-8] * 10, dev)
+    cache.scale[:, 0, 0] = 2.0 ** -64
+    if kernel in (SPLIT, TILES):
+        table = widened(table, 300)
+    q = torch.randn(1, Hq, T, D, generator=gen).to(dtype)
+    assert planned(cache, q, table) == kernel
+    check_attend(cache, q, table, [150], sm_scale=2.0 ** -90)
