@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import heapq
 import math
-from typing import Dict, List, Optional, Sequence, Union
+from typing import Dict, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -41,9 +41,10 @@ class KittyCache8:
         self.layers: List[Cache8] = [Cache8.empty(P, H, D, G, device=config.device) for _ in range(L)]
         self.device = self.layers[0].device if L else torch.device(config.device)
         self.max_pages_per_seq = -(-config.max_seq_len // G)
-        self.block_table = torch.zeros(n, self.max_pages_per_seq, dtype=torch.int32, device=self.device)
-        self.lens = torch.zeros(L, n, dtype=torch.int32, device=self.device)     # tokens by layer and slot
-        self._held = np.zeros((L, n), np.int64)                                  # the same on the host
+        # a row per slot, and one of no tokens for sequences that hold none
+        self.block_table = torch.zeros(n + 1, self.max_pages_per_seq, dtype=torch.int32, device=self.device)
+        self.lens = torch.zeros(L, n + 1, dtype=torch.int32, device=self.device)     # tokens by layer and slot
+        self._held = np.zeros((L, n + 1), np.int64)                                  # the same on the host
         self._pages: List[List[int]] = [[] for _ in range(n)]
         self._fresh, self._freed, self._num_pages = 0, [], P
         self._slot_of: Dict[int, int] = {}
@@ -74,29 +75,46 @@ class KittyCache8:
             return torch.tensor(list(values), dtype=torch.int32)
         return stage_i32(np.asarray(values, np.int32), self.device)
 
-    def _room(self, layer: int, slots: Sequence[int], tokens: int) -> None:
-        """Pages for `tokens` more tokens of each slot, all or nothing."""
+    def _join(self, layer: int, seq_ids: Sequence[int], tokens: int) -> Tuple[List[int], List[int], List[int]]:
+        """Slots of the sequences, with pages for `tokens` more tokens of each, all or
+        nothing; also which sequences are new and how many pages each slot got."""
+        new = [i for i in seq_ids if i not in self._slot_of]
+        if len(new) > len(self._free_slots):
+            raise RuntimeError(f"all {len(self._pages)} sequence slots are in use; "
+                               "raise KittyConfig.max_batch_size or reset finished sequences")
+        taken = dict(zip(new, heapq.nsmallest(len(new), self._free_slots)))
+        slots = [self._slot_of.get(i, taken.get(i)) for i in seq_ids]
         G = self.config.q_buffer_size
-        need = [-(-(int(self._held[layer, s]) + tokens) // G) - len(self._pages[s]) for s in slots]
+        need = [max(0, -(-(int(self._held[layer, s]) + tokens) // G) - len(self._pages[s])) for s in slots]
         for s, n in zip(slots, need):
             if len(self._pages[s]) + n > self.max_pages_per_seq:
                 raise RuntimeError(f"a sequence exceeds max_seq_len={self.config.max_seq_len}")
-        if sum(max(n, 0) for n in need) > self.pages_free:
-            raise RuntimeError(f"KV Cache page pool exhausted! {self.pages_free} free pages, "
-                               f"{sum(max(n, 0) for n in need)} needed.")
+        if sum(need) > self.pages_free:
+            raise RuntimeError(f"KV Cache page pool exhausted! {self.pages_free} free pages, {sum(need)} needed.")
+        for i in new:
+            self.slot(i)
         for s, n in zip(slots, need):
-            if n <= 0:
+            if n == 0:
                 continue
-            new = []
+            ids = []
             for _ in range(n):
                 if self._freed:
-                    new.append(heapq.heappop(self._freed))
+                    ids.append(heapq.heappop(self._freed))
                 else:
-                    new.append(self._fresh)
+                    ids.append(self._fresh)
                     self._fresh += 1
             at = len(self._pages[s])
-            self._pages[s] += new
-            self.block_table[s, at:at + n].copy_(self._i32(new))
+            self._pages[s] += ids
+            self.block_table[s, at:at + n].copy_(self._i32(ids))
+        return slots, new, need
+
+    def _leave(self, slots: Sequence[int], new: Sequence[int], got: Sequence[int]) -> None:
+        """Takes a _join back."""
+        for s, n in zip(slots, got):
+            for _ in range(n):
+                heapq.heappush(self._freed, self._pages[s].pop())
+        for i in new:
+            heapq.heappush(self._free_slots, self._slot_of.pop(i))
 
     def reset_sequence(self, seq_id: int) -> None:
         """Drops a sequence: its pages and its slot are free again."""
@@ -111,32 +129,40 @@ class KittyCache8:
         heapq.heappush(self._free_slots, s)
 
     # -------------------------------------------------------------------- calls
-    def _batch(self, layer: int, seq_ids: Sequence[int]):
-        """(slots, block table and lengths of the batch, slots on the device where they are no run)."""
-        slots = [self.slot(i) for i in seq_ids]
-        if len(set(slots)) != len(slots):
+    def _slots(self, seq_ids: Sequence[int]) -> List[int]:
+        """Slots of a batch to read; sequences that hold nothing take none."""
+        if len(set(seq_ids)) != len(seq_ids):
             raise ValueError("a sequence appears twice in one batch")
+        return [self._slot_of.get(i, len(self._pages)) for i in seq_ids]
+
+    def _rows(self, layer: int, slots: Sequence[int]):
+        """Block table and lengths of the slots, and the slots on the device where they are no run."""
         s0 = slots[0] if slots else 0
         if slots == list(range(s0, s0 + len(slots))):
-            return slots, self.block_table[s0:s0 + len(slots)], self.lens[layer, s0:s0 + len(slots)], None
+            return self.block_table[s0:s0 + len(slots)], self.lens[layer, s0:s0 + len(slots)], None
         key = tuple(slots)
         idx = self._slots_dev.get(key)
         if idx is None:
             if len(self._slots_dev) >= 64:
                 self._slots_dev.clear()
             idx = self._slots_dev[key] = self._i32(slots).long()
-        return slots, self.block_table[idx], self.lens[layer][idx], idx
+        return self.block_table[idx], self.lens[layer][idx], idx
 
     def push(self, layer: int, keys: torch.Tensor, values: torch.Tensor, seq_ids: Sequence[int]) -> None:
-        """T tokens for each of B sequences: keys / values (B, H, T, D)."""
+        """T tokens for each of B sequences: keys / values (B, H, T, D).  A call that is
+        refused leaves slots, pages and tokens as they were."""
         if keys.shape[0] != len(seq_ids):
             raise ValueError(f"{len(seq_ids)} sequence ids for a batch of {keys.shape[0]}")
+        self._slots(seq_ids)
         if keys.shape[0] == 0 or keys.shape[2] == 0:
             return
-        slots = self._batch(layer, seq_ids)[0]
-        self._room(layer, slots, keys.shape[2])
-        _, table, lens, idx = self._batch(layer, seq_ids)
-        self.layers[layer].write(keys.to(self.device), values.to(self.device), table, lens)
+        slots, new, got = self._join(layer, seq_ids, keys.shape[2])
+        try:
+            table, lens, idx = self._rows(layer, slots)
+            self.layers[layer].write(keys.to(self.device), values.to(self.device), table, lens)
+        except Exception:
+            self._leave(slots, new, got)
+            raise
         if idx is None:
             lens.add_(keys.shape[2])
         else:
@@ -144,14 +170,18 @@ class KittyCache8:
         self._held[layer, slots] += keys.shape[2]
 
     def attend(self, layer: int, q: torch.Tensor, seq_ids: Sequence[int], sm_scale: Optional[float] = None) -> torch.Tensor:
-        """Causal attention of the last T tokens of each sequence, q (B, Hq, T, D)."""
-        slots, table, lens, _ = self._batch(layer, seq_ids)
+        """Causal attention of the last T tokens of each sequence, q (B, Hq, T, D); zeros
+        for a sequence that holds nothing."""
+        slots = self._slots(seq_ids)
+        table, lens, _ = self._rows(layer, slots)
         longest = int(self._held[layer, slots].max(initial=0))
         return self.layers[layer].attend(q, table, lens, sm_scale=sm_scale, max_tokens=_bucket(longest))
 
     def read(self, layer: int, seq_ids: Sequence[int], dtype: Optional[torch.dtype] = None):
-        """(keys, values) of the sequences, (B, H, longest, D), zeros behind the shorter ones."""
-        slots, table, lens, _ = self._batch(layer, seq_ids)
+        """(keys, values) of the sequences, (B, H, longest, D), zeros behind the shorter
+        ones; a sequence that was never pushed, or was reset, holds nothing."""
+        slots = self._slots(seq_ids)
+        table, lens, _ = self._rows(layer, slots)
         return self.layers[layer].read(table, lens, int(self._held[layer, slots].max(initial=0)), dtype=dtype or self.dtype)
 
 
@@ -165,6 +195,8 @@ class KittyPagedAttention8(nn.Module):
 
     def __init__(self, config: KittyConfig, num_q_heads: int, cache: KittyCache8, layer: int) -> None:
         super().__init__()
+        if num_q_heads <= 0 or num_q_heads % config.num_kv_heads:      # or its first call would push, and then raise
+            raise ValueError(f"num_q_heads must be a positive multiple of {config.num_kv_heads}")
         self.config = config
         self.num_q_heads = num_q_heads
         self.num_kv_heads = config.num_kv_heads
