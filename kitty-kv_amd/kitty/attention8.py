@@ -9,7 +9,8 @@ next to the 2-bit ones.  At head_dim 128 a token takes 256 bytes a KV head again
 
 A page holds ``q_buffer_size`` tokens (16, 32, 64, 128 or 256) of one sequence and
 stands at the same place in every layer's pools, so one block table serves all
-layers; ``max_pages`` (or ``pool_pages_override``) pages are allocated per layer.
+layers; a layer's pools hold ``max_seq_len`` tokens of every slot, or
+``pool_pages_override`` pages if that is less.
 Tokens are quantised as they are written (``kernels.cache8``), there are no 16-bit
 sinks or windows, and a chunk of any length attends over everything its sequence
 holds, itself included.  No step waits for the GPU: lengths live on the device and
@@ -36,11 +37,12 @@ class KittyCache8:
     def __init__(self, config: KittyConfig, num_layers: Optional[int] = None) -> None:
         self.config = config
         L = config.num_layers if num_layers is None else int(num_layers)
-        H, G, D, P, n = config.num_kv_heads, config.q_buffer_size, config.head_dim, config.pool_pages, config.max_batch_size
+        H, G, D, n = config.num_kv_heads, config.q_buffer_size, config.head_dim, config.max_batch_size
+        self.max_pages_per_seq = -(-config.max_seq_len // G)
+        P = _layer_pages(config, n * self.max_pages_per_seq)
         self.dtype = torch.float16 if config.dtype == "float16" else torch.bfloat16
         self.layers: List[Cache8] = [Cache8.empty(P, H, D, G, device=config.device) for _ in range(L)]
         self.device = self.layers[0].device if L else torch.device(config.device)
-        self.max_pages_per_seq = -(-config.max_seq_len // G)
         # a row per slot, and one of no tokens for sequences that hold none
         self.block_table = torch.zeros(n + 1, self.max_pages_per_seq, dtype=torch.int32, device=self.device)
         self.lens = torch.zeros(L, n + 1, dtype=torch.int32, device=self.device)     # tokens by layer and slot
@@ -183,6 +185,15 @@ class KittyCache8:
         slots = self._slots(seq_ids)
         table, lens, _ = self._rows(layer, slots)
         return self.layers[layer].read(table, lens, int(self._held[layer, slots].max(initial=0)), dtype=dtype or self.dtype)
+
+
+def _layer_pages(config: KittyConfig, most: int) -> int:
+    """Pages of an 8-bit layer whose slots can name `most`.  pool_pages_override sizes the
+    pool that the 2-bit layers share, often for all of them together: here it is a bound.
+    Without it, max_pages (it leaves room for the sinks, which are tokens like others here, out)."""
+    if config.pool_pages_override is None:
+        return max(config.pool_pages, most)
+    return min(config.pool_pages, most)
 
 
 def _bucket(tokens: int) -> int:

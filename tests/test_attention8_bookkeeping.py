@@ -68,3 +68,22 @@ def test_reading_takes_no_slot(dev):
     assert state(cache) == before
     cache.push(0, tokens(1, 1, dev=dev), tokens(1, 1, dev=dev), [9])      # the slot that reading 1, 2 and 3 left
     np.testing.assert_array_equal(cache.lens[0].cpu().numpy()[:2], [20, 1])
+
+
+def test_pages_of_a_layer():
+    """Each layer has the pages that the slots' tables can name: not a pool sized for all
+    layers together, and enough for every slot's max_seq_len whatever the sinks."""
+    from kitty import KittyAttentionFactory, KittyCache8
+    cfg = config("cpu", max_batch_size=2, num_layers=6)
+    cfg.pool_pages_override = cfg.max_pages * cfg.num_layers
+    bi = torch.full((6, 2, 64), cfg.sentinel, dtype=torch.uint8)
+    bi[:, :, :cfg.d_boost] = torch.arange(cfg.d_boost, dtype=torch.uint8)
+    cache = KittyAttentionFactory.from_config(cfg, bi, 4, eight_bit_layers=[0, 5])[2][0].cache
+    assert [c.num_pages for c in cache.layers] == [32, 32] and cache.pages_free == 32      # 2 x 256 tokens
+    for sinks in (4, 100):
+        cfg = config("cpu", max_batch_size=2, max_seq_len=250, sink_size=sinks)
+        cache = KittyCache8(cfg, 1)
+        cache.push(0, tokens(2, 250), tokens(2, 250), [1, 2])
+        assert cache.tokens(1) == cache.tokens(2) == 250
+    small = KittyCache8(config("cpu", max_batch_size=2, pool_pages_override=3), 1)
+    assert small.pages_free == small.layers[0].num_pages == 3
