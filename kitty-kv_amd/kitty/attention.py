@@ -146,8 +146,9 @@ class KittyAttentionFactory:
                                                                    List[nn.Module]]:
         """One module per layer.  Layers in eight_bit_layers (numbers, not in the
         reference) keep their keys and values in 8 bits: ``KittyPagedAttention8``
-        modules over one ``KittyCache8``, theirs to reset with the pipeline's
-        sequences."""
+        modules over one ``KittyCache8``, whose sequences the pipeline's
+        ``reset_sequence`` drops with its own.  (The pipeline's 16-bit buffers are
+        allocated for these layers too, and stay empty.)"""
         layout = PageCentricKVLayoutManager(config, boost_idx_uint8)
         pipeline = KittyInferencePipeline(config, layout, boost_idx_uint8)
         layers: List[nn.Module] = [KittyPagedAttention(config, num_q_heads, layout, pipeline, i)
@@ -156,6 +157,8 @@ class KittyAttentionFactory:
         if chosen and not (0 <= chosen[0] and chosen[-1] < config.num_layers):
             raise ValueError(f"eight_bit_layers must be in [0, {config.num_layers})")
         cache = KittyCache8(config, len(chosen)) if chosen else None
+        if cache is not None:
+            pipeline.also_reset.append(cache.reset_sequence)
         for n, i in enumerate(chosen):
             layers[i] = KittyPagedAttention8(config, num_q_heads, cache, n)
         return layout, pipeline, layers

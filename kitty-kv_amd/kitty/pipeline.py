@@ -54,7 +54,7 @@ complete G-token page of the chunk is quantised straight from it.
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import Callable, Dict, List, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -113,6 +113,7 @@ class KittyInferencePipeline:
         self._slots_dev: Dict[Tuple[int, ...], torch.Tensor] = {}
         # slot arrays of batches of sequence ids seen before (cleared when a slot is freed)
         self._slots_of_ids: Dict[Tuple[int, ...], np.ndarray] = {}
+        self.also_reset: List[Callable[[int], None]] = []   # what else holds the sequences: called by reset_sequence
         self._slot_epoch = 0        # advances whenever a slot is freed: slots cached by id are stale then
         # append arguments per (layer, slots): everything but the token pointers
         self._append_args: Dict[Tuple[int, Tuple[int, ...]], Tuple[_hip.AppendArgs, torch.Tensor]] = {}
@@ -851,7 +852,10 @@ class KittyInferencePipeline:
 
     # ------------------------------------------------------------- reset
     def reset_sequence(self, seq_id: int = 0) -> None:
-        """Free the sequence's pages and slot (pipeline.py:286-313)."""
+        """Free the sequence's pages and slot (pipeline.py:286-313), and those it has in a
+        factory's 8-bit layers."""
+        for reset in self.also_reset:
+            reset(seq_id)
         self.layout.free_sequence(seq_id)
         s = self._slot_of.pop(seq_id, None)
         if s is None:

@@ -87,3 +87,35 @@ def test_pages_of_a_layer():
         assert cache.tokens(1) == cache.tokens(2) == 250
     small = KittyCache8(config("cpu", max_batch_size=2, pool_pages_override=3), 1)
     assert small.pages_free == small.layers[0].num_pages == 3
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_reset_of_a_mixed_model(dev):
+    """pipeline.reset_sequence drops a sequence from the factory's 8-bit layers too: its id
+    begins anew in every layer, and the other sequences stay."""
+    from kitty import KittyAttentionFactory
+    cfg = config(dev, max_batch_size=2, num_layers=2)
+    cfg.pool_pages_override = cfg.max_pages * cfg.num_layers
+    bi = torch.full((2, 2, 64), cfg.sentinel, dtype=torch.uint8)
+    bi[:, :, :cfg.d_boost] = torch.arange(cfg.d_boost, dtype=torch.uint8)
+    _, pipeline, mods = KittyAttentionFactory.from_config(cfg, bi, 4, eight_bit_layers=[1])
+    cache = mods[1].cache
+
+    def run(ids, T):
+        x = [tokens(len(ids), T, h, dev=dev) for h in (4, 2, 2)]
+        with torch.no_grad():
+            return [m(*x, seq_id=ids) for m in mods]
+
+    first = run([3, 8], 30)
+    pipeline.reset_sequence(3)
+    assert cache.tokens(3) == 0 and cache.tokens(8) == 30 and cache.pages_free == cache.layers[0].num_pages - 2
+    cache.reset_sequence(3)                     # as programs that reset both do
+    pipeline.reset_sequence(3)
+    pipeline.reset_sequence(77)
+    again = run([3], 30)
+    assert cache.tokens(3) == 30
+    x = [tokens(2, 30, h, dev=dev)[:1] for h in (4, 2, 2)]
+    pipeline.reset_sequence(3)
+    with torch.no_grad():
+        assert torch.equal(mods[1](*x, seq_id=3), first[1][:1])
+    assert again[1].shape == (1, 4, 30, 64)
