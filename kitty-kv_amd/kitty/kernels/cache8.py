@@ -57,6 +57,15 @@ def _given(t: torch.Tensor, name: str) -> torch.Tensor:
     return t.resolve_neg() if t.is_neg() else t
 
 
+def _into(t: torch.Tensor) -> None:
+    """An output of the program's own: as torch's in-place writes."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("out needs a gradient and the 8-bit cache has no backward: call under torch.no_grad()")
+
+
+_written = torch.autograd.graph.increment_version      # what torch's own writes do
+
+
 class Cache8:
     """Pools of an 8-bit paged cache and the calls that work on them.
 
@@ -205,6 +214,9 @@ class Cache8:
         if calls_followed():
             raise NotImplementedError(_FOLLOWED)
         tokens = int(tokens)
+        if out is not None:
+            _into(out[0])
+            _into(out[1])
         sig = ("read", tokens, dtype, _sig(block_table), _sig(lens), _sig(start),
                None if out is None else (_sig(out[0]), _sig(out[1])))
         found = self._known.get(sig) if self._on_device else None
@@ -229,7 +241,7 @@ class Cache8:
                 dtype = k.dtype
             if B == 0 or tokens == 0:
                 return k, v
-            if not self._on_device:
+            if not self._on_device:      # its writes are torch's
                 cpu8.read(self.key, self.value, self.scale, block_table, lens, start, (k, v))
                 return k, v
             like = k.new_empty(1).expand(shape)      # what new outputs look like, of one element
@@ -241,10 +253,12 @@ class Cache8:
             v = torch.empty_like(k)
         else:
             k, v = out
-            if not aligned or k.data_ptr() % 16 or v.data_ptr() % 16:      # rows the kernel does not write in place
+            kp, vp = k.data_ptr(), v.data_ptr()
+            if not aligned or kp % 16 or vp % 16:      # rows the kernel does not write in place
                 for t, x in zip(out, self.read(block_table, lens, tokens, start, k.dtype)):
                     t.copy_(x)
                 return k, v
+            _written((k, v))
         self._launch(self._lib.kitty_cache8_read, _ROWS.pack(
             k.data_ptr(), v.data_ptr(), *strides, block_table.data_ptr(), bt_stride,
             0 if start is None else start.data_ptr(), lens.data_ptr(), *rest))
@@ -269,6 +283,8 @@ class Cache8:
             raise NotImplementedError(_FOLLOWED)
         if q.requires_grad or q.is_neg():
             q = _given(q, "q")
+        if out is not None:
+            _into(out)
         causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
         max_tokens = 0 if max_tokens is None else int(max_tokens)
         sig = (q.shape, q.stride(), q.dtype, q.device, _sig(block_table), _sig(lens), None if q_lens is None else _sig(q_lens),
@@ -311,7 +327,13 @@ class Cache8:
                     self._ref, _ATTENTION.pack(0, 0, 0, *[0] * 6, 0, bt_stride, 0, 0, *rest, 0, 0), ctypes.byref(size)))
             found = self._keep(sig, (in_place, q.is_contiguous(), head, bt_stride, rest, size.value))
         in_place, like_q, head, bt_stride, rest, need = found
-        if not in_place or q.data_ptr() % 16 or (out is not None and out.data_ptr() % 16):
+        qp = q.data_ptr()
+        if out is not None:
+            if out.data_ptr() % 16:
+                in_place = False
+            else:
+                _written(out)
+        if not in_place or qp % 16:
             # rows the kernel does not read or write in place
             got = self.attend(q.clone(memory_format=torch.contiguous_format), block_table, lens, q_lens, causal, sm_scale,
                               None, return_lse, max_tokens)
@@ -326,6 +348,6 @@ class Cache8:
         # on other streams and in captured graphs never share one
         ws = q.new_empty((need + 1) // 2) if need else None
         self._launch(self._lib.kitty_cache8_attention, _ATTENTION.pack(
-            q.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, block_table.data_ptr(), bt_stride,
+            qp, out.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, block_table.data_ptr(), bt_stride,
             lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), *rest, 0 if ws is None else ws.data_ptr(), need))
         return (out, lse) if return_lse else out
