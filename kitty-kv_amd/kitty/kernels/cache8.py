@@ -254,7 +254,7 @@ class Cache8:
         else:
             k, v = out
             kp, vp = k.data_ptr(), v.data_ptr()
-            if not aligned or kp % 16 or vp % 16:      # rows the kernel does not write in place
+            if not aligned or kp % 16 or vp % 16 or k.is_neg() or v.is_neg():      # rows the kernel does not write in place
                 for t, x in zip(out, self.read(block_table, lens, tokens, start, k.dtype)):
                     t.copy_(x)
                 return k, v
@@ -329,7 +329,7 @@ class Cache8:
         in_place, like_q, head, bt_stride, rest, need = found
         qp = q.data_ptr()
         if out is not None:
-            if out.data_ptr() % 16:
+            if out.data_ptr() % 16 or out.is_neg():
                 in_place = False
             else:
                 _written(out)

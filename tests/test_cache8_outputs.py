@@ -38,3 +38,17 @@ def test_outputs_and_gradients(dev):
             write(target)
             with pytest.raises(RuntimeError, match="modified by an inplace operation"):
                 y.backward()
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_negated_outputs(dev):
+    """A view whose elements are read negated gets the values, not their negatives."""
+    cache, table, lens, q = setup(dev)
+    want = cache.attend(q, table, lens)
+    pair = cache.read(table, lens, 8)
+    for _ in range(2):
+        out = torch._neg_view(torch.zeros_like(q))
+        assert cache.attend(q, table, lens, out=out) is out and torch.equal(out, want)
+        outs = torch.zeros_like(pair[0]), torch._neg_view(torch.zeros_like(pair[1]))
+        got = cache.read(table, lens, 8, out=outs)
+        assert torch.equal(got[0], pair[0]) and torch.equal(got[1], pair[1])
