@@ -66,6 +66,11 @@ def _into(t: torch.Tensor) -> None:
 _written = torch.autograd.graph.increment_version      # what torch's own writes do
 
 
+def _span(t: torch.Tensor) -> int:
+    """Bytes from a tensor's first element to behind its last."""
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
 class Cache8:
     """Pools of an 8-bit paged cache and the calls that work on them.
 
@@ -210,7 +215,7 @@ class Cache8:
         """(keys, values), each (B, H, tokens, D) of `dtype` (or the tensors of
         `out`): row t is token start[b] + t (start None: from 0) of sequence b,
         code * scale rounded once; 0 behind its lens[b] tokens, NaN where the
-        token has no page."""
+        token has no page.  The two tensors of `out` share no element."""
         if calls_followed():
             raise NotImplementedError(_FOLLOWED)
         tokens = int(tokens)
@@ -238,6 +243,7 @@ class Cache8:
                           f"out must be two {shape} tensors of one type with contiguous channels")
                     _need(torch._debug_has_internal_overlap(t) != 1, "out must not share memory between its rows")
                     self._here("out", t)
+                _need(tokens == 0 or B == 0 or k.data_ptr() != v.data_ptr(), "out must not be the same memory twice")
                 dtype = k.dtype
             if B == 0 or tokens == 0:
                 return k, v
@@ -254,6 +260,7 @@ class Cache8:
         else:
             k, v = out
             kp, vp = k.data_ptr(), v.data_ptr()
+            _need(kp != vp, "out must not be the same memory twice")
             if not aligned or kp % 16 or vp % 16 or k.is_neg() or v.is_neg():      # rows the kernel does not write in place
                 for t, x in zip(out, self.read(block_table, lens, tokens, start, k.dtype)):
                     t.copy_(x)
@@ -278,7 +285,8 @@ class Cache8:
         to D^-1/2.  Scores, softmax and sums are float32.  return_lse: also the
         rows' log of the sum of exp(score), float32 (B, Hq, T), -inf where a row
         sees nothing.  max_tokens: the largest lens[b] where the program knows it
-        (default: what the table can hold); it only chooses how the work is split."""
+        (default: what the table can hold); it only chooses how the work is split.
+        out may be q, or lie in its memory in any way (a copy of q is then read)."""
         if calls_followed():
             raise NotImplementedError(_FOLLOWED)
         if q.requires_grad or q.is_neg():
@@ -315,6 +323,8 @@ class Cache8:
                     cpu8.attend(self.key, self.value, self.scale, q, block_table, lens, q_lens, causal, scale, out, lse)
                 return (out, lse) if return_lse else out
             in_place = q.stride(3) == 1 and _aligned16(q) and (out is None or _aligned16(out))
+            # where the two lie in one piece of memory: their spans, and whether their rows are at the same places
+            spans = None if out is None else (_span(q), _span(out), _strides(q) == _strides(out))
             o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
             W = block_table.shape[1]
             head = (*_strides(q), *_strides(o))
@@ -325,12 +335,13 @@ class Cache8:
             with torch.cuda.device(self._index):      # the plan is the pools' device's
                 _hip.check(self._lib.kitty_cache8_attention_workspace_size(
                     self._ref, _ATTENTION.pack(0, 0, 0, *[0] * 6, 0, bt_stride, 0, 0, *rest, 0, 0), ctypes.byref(size)))
-            found = self._keep(sig, (in_place, q.is_contiguous(), head, bt_stride, rest, size.value))
-        in_place, like_q, head, bt_stride, rest, need = found
+            found = self._keep(sig, (in_place, q.is_contiguous(), head, bt_stride, rest, size.value, spans))
+        in_place, like_q, head, bt_stride, rest, need, spans = found
         qp = q.data_ptr()
         if out is not None:
-            if out.data_ptr() % 16 or out.is_neg():
-                in_place = False
+            op = out.data_ptr()
+            if op % 16 or out.is_neg() or (qp < op + spans[1] and op < qp + spans[0] and not (qp == op and spans[2])):
+                in_place = False    # also: rows of out over other rows of q, which may be read after they are written
             else:
                 _written(out)
         if not in_place or qp % 16:

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from test_cache8 import DEVICES, F16, filled, i32, tables
+from test_cache8 import BF16, DEVICES, F16, filled, i32, tables
 
 
 def setup(dev, T=3, D=64):
@@ -52,3 +52,42 @@ def test_negated_outputs(dev):
         outs = torch.zeros_like(pair[0]), torch._neg_view(torch.zeros_like(pair[1]))
         got = cache.read(table, lens, 8, out=outs)
         assert torch.equal(got[0], pair[0]) and torch.equal(got[1], pair[1])
+
+
+# a call of one launch, one that is split, a chunk in tiles
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T,wide", [(3, 0), (3, 300), (40, 300)])
+def test_output_over_other_queries(dev, T, wide):
+    """out in q's memory but in another place or order: the results of a tensor of its own."""
+    cache, table, lens, q = setup(dev, T)
+    table = torch.cat([table, torch.zeros(2, wide, dtype=torch.int32, device=dev)], 1)
+    want = cache.attend(q, table, lens)
+    n = q.numel()
+    for _ in range(2):
+        room = torch.zeros(n + 64 * T, dtype=F16, device=dev)
+        for a, b in ((0, 64 * T), (64 * T, 0), (8, 0)):            # one head or a few channels apart
+            room.zero_()
+            src = room[a:a + n].view(q.shape).copy_(q)
+            out = room[b:b + n].view(q.shape)
+            cache.attend(src, table, lens, out=out)
+            assert torch.equal(out, want)
+        src = room[:n].view(q.shape).copy_(q)
+        out = room[:n].view(2, T, 4, 64).transpose(1, 2)           # the same memory as (B, T, H, D)
+        cache.attend(src, table, lens, out=out)
+        assert torch.equal(out, want)
+        fused = torch.zeros(2, T, 3 * 256, dtype=F16, device=dev)  # beside the queries, row by row
+        src, out = (fused[..., i:i + 256].unflatten(2, (4, 64)).transpose(1, 2) for i in (0, 512))
+        src.copy_(q)
+        cache.attend(src, table, lens, out=out)
+        assert torch.equal(out, want) and torch.equal(src, q)
+
+
+def test_read_refuses_one_output_twice():
+    cache, table, lens, q = setup("cpu")
+    x = torch.zeros(2, 2, 8, 64, dtype=BF16)
+    with pytest.raises(ValueError, match="same memory"):
+        cache.read(table, lens, 8, out=(x, x))
+    both = torch.zeros(2, 2, 8, 2, 64, dtype=BF16)
+    got = cache.read(table, lens, 8, out=(both[..., 0, :], both[..., 1, :]))
+    want = cache.read(table, lens, 8, dtype=BF16)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
