@@ -96,23 +96,25 @@ def attend(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch
         if n == 0 or t == 0:
             continue
         ids, ok = _page_ids(table[b:b + 1], torch.arange(-(-n // G))[None], P)
-        kv = []
+        # codes and scales apart, as in the kernels: their products may pass fp32's range
+        kv, factors = [], []
         for i, pool in enumerate((key, value)):
-            x = torch.zeros(ids.shape[1], H, G, D)
+            x, f = torch.zeros(ids.shape[1], H, G, D), torch.ones(ids.shape[1], H)
             if P:
-                x = pool.view(torch.uint8)[ids[0]].view(E4M3).float() * scale[ids[0], :, i][..., None, None]
+                x, f = pool.view(torch.uint8)[ids[0]].view(E4M3).float(), torch.where(ok[0][:, None], scale[ids[0], :, i], f)
             x = torch.where(ok[0][:, None, None, None], x, torch.full_like(x, math.nan))
             kv.append(x.transpose(0, 1).flatten(1, 2)[:, :n])
+            factors.append(f.t().repeat_interleave(G, 1)[:, None, :n])       # (H, 1, n)
         sees = torch.ones(t, n, dtype=torch.bool)
         if causal:
             sees = torch.arange(n) <= torch.arange(n - t, n)[:, None]
-        s = (q[b, :, :t].reshape(H, gq * t, D) @ kv[0].transpose(1, 2)).view(H, gq, t, n) * sm_scale
+        s = (q[b, :, :t].reshape(H, gq * t, D) @ kv[0].transpose(1, 2) * (factors[0] * sm_scale)).view(H, gq, t, n)
         s = s.masked_fill(~sees, -math.inf)
         l = torch.logsumexp(s, -1)
         none = ~sees.any(-1)                                   # rows that see nothing
         w = torch.exp(s - torch.where(none, torch.zeros_like(l), l)[..., None])
         gone = kv[1].isnan()                                   # masked NaN values stay out of the product
-        o = w.view(H, gq * t, n) @ kv[1].masked_fill(gone, 0.0)
+        o = (w.view(H, gq * t, n) * factors[1]) @ kv[1].masked_fill(gone, 0.0)
         met = (sees.float().repeat(gq, 1) @ gone.float()) > 0
         o = o.masked_fill(met, math.nan).view(H, gq, t, D).masked_fill(none[:, None], 0.0)
         out[b, :, :t] = o.reshape(Hq, t, D).to(out.dtype)

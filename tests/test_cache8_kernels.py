@@ -188,3 +188,23 @@ def test_scores_that_underflow(dev, kernel, Hq, T, D, dtype):
     q = torch.randn(1, Hq, T, D, generator=gen).to(dtype)
     assert planned(cache, q, table) == kernel
     check_attend(cache, q, table, [150], sm_scale=2.0 ** -90)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("kernel,Hq,T,D", FAR)
+def test_masked_values_beyond_fp32(dev, kernel, Hq, T, D):
+    """A page written elsewhere whose codes times scale pass fp32's range, keys and values:
+    rows that do not see its tokens keep their numbers."""
+    gen = torch.Generator().manual_seed(T + D)
+    cache, table = far_cache(gen, D, [-8] * 10, dev)
+    cache.scale[:, 0, 0] = 2.0 ** -8
+    if kernel in (SPLIT, TILES):
+        table = widened(table, 300)
+    q = torch.randn(1, Hq, T, D, generator=gen).to(BF16).to(dev)
+    lens = torch.tensor([147], dtype=torch.int32, device=dev)
+    want = numpy(cache.attend(q, table, lens))[:, :, :-3]
+    cache.scale[9] = 2.0 ** 125
+    got = numpy(cache.attend(q, table, lens))[:, :, :-3]          # tokens 144 .. 146 are the last page's
+    assert np.isfinite(got).all()
+    # both within half a step of the same sums, and with one fp16 term within 2^-11 of the values' size
+    assert (np.abs(got - want) <= 2.0 ** -7 * np.abs(want) + 2.0 ** -10 * np.abs(want).max()).all()
