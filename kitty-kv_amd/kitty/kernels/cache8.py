@@ -100,6 +100,10 @@ class Cache8:
             raise NotImplementedError("the 8-bit cache is built for head_dim up to 256")
         _need(scale.dtype == torch.float32 and tuple(scale.shape) == (P, H, 2) and scale.stride(2) == 1,
               "scale must be float32 (P, H, 2) with the two streams next to each other")
+        for name, t in (("key", key), ("value", value), ("scale", scale)):
+            if t.requires_grad:
+                raise RuntimeError(f"{name} needs a gradient and the 8-bit cache has no backward: detach it")
+            _need(not t.is_neg(), f"{name} must not be a negated view")
         if value.device != key.device or scale.device != key.device:
             raise RuntimeError("key, value and scale must be on one device")
         self.key, self.value, self.scale = key, value, scale

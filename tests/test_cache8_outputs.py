@@ -91,3 +91,15 @@ def test_read_refuses_one_output_twice():
     got = cache.read(table, lens, 8, out=(both[..., 0, :], both[..., 1, :]))
     want = cache.read(table, lens, 8, dtype=BF16)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_pools_are_plain_tensors():
+    """Pools that need a gradient, which no call would give them, and negated views are refused."""
+    from kitty.kernels import Cache8
+    key, value = (torch.zeros(3, 2, 16, 32, dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2))
+    scale = torch.ones(3, 2, 2)
+    with pytest.raises(RuntimeError, match="gradient"):
+        Cache8(key, value, scale.clone().requires_grad_())
+    with pytest.raises(ValueError, match="negated"):
+        Cache8(key, value, torch._neg_view(scale))
+    Cache8(key, value, scale.clone().requires_grad_().detach())
