@@ -14,7 +14,8 @@ layers; a layer's pools hold ``max_seq_len`` tokens of every slot, or
 Tokens are quantised as they are written (``kernels.cache8``), there are no 16-bit
 sinks or windows, and a chunk of any length attends over everything its sequence
 holds, itself included.  No step waits for the GPU: lengths live on the device and
-in a host copy, and only new pages send their ids over.
+in a host copy, and only new pages send their ids over.  (For that host copy a step
+that adds tokens is not captured into a graph; the calls of ``Cache8`` are.)
 """
 from __future__ import annotations
 
@@ -158,6 +159,9 @@ class KittyCache8:
         self._slots(seq_ids)
         if keys.shape[0] == 0 or keys.shape[2] == 0:
             return
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("KittyCache8 counts its tokens on the host, so its steps cannot be captured: "
+                               "capture the calls of kitty.kernels.Cache8")
         slots, new, got = self._join(layer, seq_ids, keys.shape[2])
         try:
             table, lens, idx = self._rows(layer, slots)

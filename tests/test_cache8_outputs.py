@@ -103,3 +103,21 @@ def test_pools_are_plain_tensors():
     with pytest.raises(ValueError, match="negated"):
         Cache8(key, value, torch._neg_view(scale))
     Cache8(key, value, scale.clone().requires_grad_().detach())
+
+
+@pytest.mark.gpu
+def test_module_steps_are_not_captured(dev):
+    """KittyCache8 counts tokens on the host too, so a captured push is refused and leaves
+    nothing; Cache8's own calls are captured."""
+    from kitty import KittyCache8
+    from test_attention8 import config
+    cache = KittyCache8(config("cuda:0"), 1)
+    x = torch.randn(1, 2, 1, 64, device=dev).half()
+    cache.push(0, x, x, [4])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="captured"):
+            cache.push(0, x, x, [4])
+        out = cache.layers[0].attend(x, cache.block_table[:1], cache.lens[0, :1])
+    graph.replay()
+    assert torch.equal(out, cache.attend(0, x, [4])) and cache.tokens(4) == 1 and cache.lens[0, 0].item() == 1
