@@ -516,8 +516,8 @@ int kitty_channel_scores(const kitty_score_layer *layers, int32_t n, int32_t num
  * version 8; no counterpart in the reference, whose only cache is the 2-bit
  * one).  Code c (e4m3: 4 exponent and 3 mantissa bits, no infinities, 0x7f and
  * 0xff NaN) of page p, head h stands for c * scale[p, h, s], s = 0 for keys and
- * 1 for values; any finite positive float scale is read, kitty_cache8_write
- * makes powers of two.  Strides are in elements: bytes for the codes (multiples
+ * 1 for values; any finite scale from 2^-100 on is read, kitty_cache8_write makes
+ * powers of two (2^-64 to 2^120).  Strides are in elements: bytes for the codes (multiples
  * of 16, the channel stride 1, bases 16-byte aligned), floats for the scales
  * (even, the two streams next to each other, base 8-byte aligned). */
 typedef struct {
@@ -592,9 +592,14 @@ int kitty_cache8_read(const kitty_cache8 *cache, const kitty_cache8_read_args *a
  * gives NaN rows, and so does a page id outside the pool to the rows that see
  * one of its tokens; masked tokens, whatever they hold, reach no row.
  * Scores, softmax and sums are fp32, the 8-bit codes enter their products
- * exactly.  Weights enter theirs in two bf16 terms (16 bits); for bf16 results of
- * more than 64 rows a KV head (32 where head_dim is above 128; rows: heads of the
- * group times tokens) in one fp16 term (11 bits).  |q . code| must stay finite.
+ * exactly.  Weights times value scales enter theirs in two bf16 terms (16 bits, fp32's
+ * range).  Results in bf16 of more than 64 rows a KV head (32 where head_dim is above
+ * 128; rows: heads of the group times tokens) take one fp16 term instead (11 bits of a
+ * weight, and 2^-25 of the largest weight times scale where that is more), except where
+ * one launch does short contexts (as plan_tokens has it) and from a page on whose value
+ * scale is not within 2^12 of those before it, or not from 2^-64 to 2^32.  |q . code|, sm_scale times a key
+ * scale, and 2^8 times the sum of a row's weighted |values| before it is divided by that
+ * of its weights must stay finite in fp32.
  * block_table entries behind a sequence's last page are not read; a row of it may
  * name up to 2^30 tokens.
  * plan_tokens: what the caller knows of the largest lens[b] (0: table_pages *

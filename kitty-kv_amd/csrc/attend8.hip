@@ -593,6 +593,8 @@ static size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 // is at most kDirectBytes and there are at most kDirectItems of them, or a workgroup
 // a CU where a pair has several row blocks.  It saves the merge (on the host too) and
 // reads lengths less often, and loses where its few workgroups leave the device idle.
+// (The rule has no least number of items: one sequence near the bound would be up to 1.6
+// us faster split, as the first row and the 64 channels' have it.)
 // us, one launch / split and merge, 8 KV heads, one query, groups of 4, fp16:
 //   channels 128, tokens    128          512          1,024        2,048
 //   1 sequence              5.0 /  8.5   7.0 /  9.6    9.9 /  9.6  15.8 / 10.0

@@ -12,7 +12,9 @@
 // Both are bound by memory, and by launch latency where few tokens are written.
 // Measured: 4 x 8,192 tokens of 8 x 128 fp16 written in 39.8 us (5.05 TB/s; a copy
 // reaches 4.9; 46 without streaming loads), one token of one sequence or of 64 in
-// 4.2; 8 x 8,192 read back in 82 us (4.3 TB/s, three quarters of it stores; 93 with
+// 4.2; pages of more than 128 x 128 elements, whose later rows are read twice (the
+// second time mostly from the L2): 128 channels and 256 tokens 46.5 us (4.3 TB/s, 41.4 at
+// 128 tokens on the same card), 256 and 128 44 us, 256 and 256 55 us; 8 x 8,192 read back in 82 us (4.3 TB/s, three quarters of it stores; 93 with
 // 32 bytes of output a thread and row).
 #include "cache8.h"
 

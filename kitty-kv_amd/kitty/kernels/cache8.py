@@ -78,7 +78,7 @@ class Cache8:
     (P, H, 2) float32, of keys and of values.  G is 16, 32, 64, 128 or 256, D a
     multiple of 16 up to 256; pages and heads may lie at any 16-byte aligned
     strides.  Code c of a page stands for c * scale; pages written elsewhere may
-    hold any finite positive scale.  One pool serves any number of sequences:
+    hold any finite scale from 2^-100 on.  One pool serves any number of sequences:
     ``block_table`` (B, W) int32 names each sequence's pages in order, and a page
     may stand in several tables (a shared prefix) as long as one sequence of a
     call writes to it.
