@@ -208,3 +208,70 @@ def test_masked_values_beyond_fp32(dev, kernel, Hq, T, D):
     assert np.isfinite(got).all()
     # both within half a step of the same sums, and with one fp16 term within 2^-11 of the values' size
     assert (np.abs(got - want) <= 2.0 ** -7 * np.abs(want) + 2.0 ** -10 * np.abs(want).max()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_tile_kernel_beyond_4_gib(dev, dtype):
+    """Pages whose byte offsets pass 2^32 in either pool, chunks in tiles."""
+    from kitty.kernels import Cache8
+    gen = torch.Generator().manual_seed(4)
+    P, H, D, G = 70000, 4, 128, 128            # 4.6 GB a pool
+    near = filled(gen, 6, H, D, G, dev)
+    key, value = (torch.zeros(P, H, G, D, dtype=torch.uint8, device=dev).view(torch.float8_e4m3fn) for _ in range(2))
+    cache = Cache8(key, value, torch.ones(P, H, 2, device=dev))
+    pages = [P - 1, 3, P - 3, P - 2, 65537, 66000]
+    for a, b in ((cache.key, near.key), (cache.value, near.value)):
+        a.view(torch.uint8)[pages] = b.view(torch.uint8)
+    cache.scale[pages] = near.scale
+    table = widened(torch.tensor(pages, dtype=torch.int32, device=dev).view(2, 3), 40)
+    at = widened(torch.arange(6, dtype=torch.int32, device=dev).view(2, 3), 40)
+    q = torch.randn(2, 8, 100, D, generator=gen).to(dtype)
+    assert planned(cache, q, table) == TILES
+    lens = torch.tensor([300, 307], dtype=torch.int32, device=dev)
+    assert torch.equal(cache.attend(q.to(dev), table, lens), near.attend(q.to(dev), at, lens))
+    check_attend(near, q, at, [300, 307])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("T,D", [(80, 80), (90, 128), (30, 208)])
+def test_tile_kernel_on_pools_in_other_orders(dev, dtype, T, D):
+    """Pools with heads inside tokens, slices of larger ones: the same results."""
+    from kitty.kernels import Cache8
+    gen = torch.Generator().manual_seed(T)
+    P, H, G = 20, 2, 32
+    plain = filled(gen, P, H, D, G, dev)
+    other = []
+    for t in (plain.key, plain.value):
+        big = torch.full((P + 1, G, H + 1, D + 16), 0xFF, dtype=torch.uint8, device=dev)
+        view = big[1:, :, 1:, 16:].permute(0, 2, 1, 3)
+        view.copy_(t.view(torch.uint8))
+        other.append(view)
+    scale = torch.full((P, H, 6), float("nan"), device=dev)[..., 2:4]
+    scale.copy_(plain.scale)
+    cache = Cache8(*other, scale)
+    table = widened(tables(gen, 2, 9, P, dev), 300, -1)
+    q = torch.randn(2, 6, T, D, generator=gen).to(dtype)
+    assert planned(cache, q, table) == TILES
+    lens = torch.tensor([250, 77], dtype=torch.int32, device=dev)
+    assert torch.equal(cache.attend(q.to(dev), table, lens), plain.attend(q.to(dev), table, lens))
+    check_attend(cache, q, table, [250, 77])
+
+
+@pytest.mark.gpu
+def test_tile_kernel_repeats_itself(dev):
+    """Value scales near and far, in parts and in one: no order of arrival enters a result."""
+    gen = torch.Generator().manual_seed(1)
+    for far in (False, True):
+        cache = filled(gen, 300, 4, 128, 64, dev)
+        if far:
+            cache.scale[::7, :, 1] = 2.0 ** 40
+        table = tables(gen, 8, 32, 300, dev)
+        lens = torch.tensor([2000, 1, 700, 64, 2048, 1999, 1024, 300], dtype=torch.int32, device=dev)
+        for B, T, kernel in ((8, 130, TILES), (2, 500, TILES), (8, 2100, TILE)):
+            q = torch.randn(B, 8, T, 128, generator=gen).bfloat16().to(dev)
+            assert planned(cache, q, table) == kernel
+            first = cache.attend(q, table[:B], lens[:B])
+            for _ in range(4):
+                assert torch.equal(cache.attend(q, table[:B], lens[:B]), first)
