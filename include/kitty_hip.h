@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define KITTY_ABI_VERSION 8
+#define KITTY_ABI_VERSION 9
 
 /* Element type of 16-bit data (the *_dtype fields below). */
 #define KITTY_DTYPE_F16 0
@@ -626,6 +626,40 @@ typedef struct {
 int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
                                           size_t *bytes);
 int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, kitty_stream_t stream);
+
+/* Attention for sequences that share prefixes, whose pages are read once for all of
+ * them: sequence b is the prefix_lens[f] tokens of prefix f = b / (batch / prefixes),
+ * in the pages that row f of prefix_table names, followed by the lens[b] tokens of its
+ * own; everything else is kitty_cache8_attention over the two together (a prefix may
+ * end inside a page; its sequences' own tokens begin in pages of their own).  With
+ * causal, row i is token prefix_lens[f] + lens[b] - q_lens[b] + i: where lens[b] <
+ * q_lens[b] the first rows are tokens of the prefix.  A prefix whose length is negative
+ * or more than prefix_pages pages hold gives NaN rows to its sequences.  batch is a
+ * multiple of prefixes.  plan_prefix and plan_tokens: what the caller knows of the
+ * largest lengths (0: what the tables hold); they only choose how the work is split. */
+typedef struct {
+    const uint16_t *q; /* (B, Hq, T, D), 16-byte aligned rows */
+    uint16_t *out;     /* (B, Hq, T, D), 16-byte aligned rows, q's type; may be q */
+    float *lse;        /* (B, Hq, T) contiguous, or NULL */
+    int64_t q_s_seq, q_s_head, q_s_tok, o_s_seq, o_s_head, o_s_tok;
+    const int32_t *prefix_table; /* (prefixes, prefix_pages) page ids */
+    int64_t pt_stride;
+    const int32_t *prefix_lens;  /* (prefixes,) */
+    const int32_t *block_table;  /* (B, table_pages) page ids */
+    int64_t bt_stride;
+    const int32_t *lens;         /* (B,) own tokens in the cache, those of the queries included */
+    const int32_t *q_lens;       /* (B,) or NULL */
+    int32_t prefixes, batch, num_q_heads, tokens, prefix_pages, table_pages, plan_prefix, plan_tokens;
+    int32_t causal;
+    int32_t dtype;               /* KITTY_DTYPE_F16 or KITTY_DTYPE_BF16: q and out */
+    float sm_scale;
+    void *workspace;             /* kitty_cache8_shared_attention_workspace_size bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} kitty_cache8_shared_args;
+
+int kitty_cache8_shared_attention_workspace_size(const kitty_cache8 *cache, const kitty_cache8_shared_args *args,
+                                                 size_t *bytes);
+int kitty_cache8_shared_attention(const kitty_cache8 *cache, const kitty_cache8_shared_args *args, kitty_stream_t stream);
 
 #ifdef __cplusplus
 }

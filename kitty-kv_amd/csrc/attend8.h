@@ -1,5 +1,7 @@
 // Attention over the 8-bit paged cache: what its two kernels share.
 #pragma once
+#include <algorithm>
+
 #include "cache8.h"
 
 namespace kitty {
@@ -29,6 +31,12 @@ struct Attend8 {
     float *ws_o;        // partials: (slots, rows of a block, D padded)
     float2 *ws_ml;      // (slots, rows of a block): maximum (log2 units) and sum
     int2 *ws_tab;       // row kernel, (items): first slot (-1: written whole), last workgroup
+    // Sequences that share prefixes: a launch works on `entries` entries from entry e0 on.
+    // Entry f < F is prefix f with the query rows of its `per` sequences, F + b what is
+    // sequence b's own.
+    const int32_t *prefix_table, *prefix_lens;
+    int64_t pt_stride;
+    int F, per, prefix_pages, e0, entries;
 };
 
 constexpr int kTileRows = 128;   // query rows of the tile kernel's workgroup
@@ -49,6 +57,7 @@ __device__ __forceinline__ T uniform_load(const T *p)
 struct Seq8 {
     int n, tq;      // tokens in the cache, query rows
     bool bad;       // lengths that break the rules: NaN rows, no pages read
+    bool prefix;    // SHARED: a prefix; tq then is what its sequences have together, padding included
 };
 
 __device__ __forceinline__ Seq8 seq8(const Attend8 &p, int b)
@@ -57,7 +66,35 @@ __device__ __forceinline__ Seq8 seq8(const Attend8 &p, int b)
     s.n = p.lens[b];
     s.tq = p.q_lens ? p.q_lens[b] : p.T;
     s.bad = s.n < 0 || s.n > (int64_t)p.table_pages << p.c.lg || s.tq < 0 || s.tq > p.T || (s.n > 0 && p.c.num_pages == 0);
+    s.prefix = false;
     return s;
+}
+
+// Entry i of a launch: sequence i, or of SHARED launches a prefix or a sequence.
+template <bool SHARED>
+__device__ __forceinline__ Seq8 entry8(const Attend8 &p, int i)
+{
+    if constexpr (SHARED) {
+        const int e = p.e0 + i;
+        if (e < p.F) {
+            Seq8 s;
+            s.n = p.prefix_lens[e];
+            s.tq = p.per * p.T;
+            s.bad = s.n < 0 || s.n > (int64_t)p.prefix_pages << p.c.lg || (s.n > 0 && p.c.num_pages == 0);
+            s.prefix = true;
+            return s;
+        }
+        return seq8(p, e - p.F);
+    }
+    return seq8(p, i);
+}
+
+template <bool SHARED>
+__device__ __forceinline__ const int32_t *table8(const Attend8 &p, const Seq8 &s, int i)
+{
+    if constexpr (SHARED)
+        return s.prefix ? p.prefix_table + (p.e0 + i) * p.pt_stride : p.table + (p.e0 + i - p.F) * p.bt_stride;
+    return p.table + i * p.bt_stride;
 }
 
 // Tokens that query row t of a sequence sees: those below the result.
@@ -66,6 +103,42 @@ __device__ __forceinline__ int visible8(const Attend8 &p, const Seq8 &s, int t)
     if (t >= s.tq)
         return 0;
     return p.causal ? max(s.n - s.tq + t + 1, 0) : s.n;
+}
+
+// Query row r of an entry and KV head: sequence, head and token, whether there is such a
+// row, and the entry's tokens that it sees.
+struct Row8 {
+    int b, h, t, vis;
+    bool real;
+};
+
+template <bool SHARED>
+__device__ __forceinline__ Row8 row8(const Attend8 &p, const Seq8 &s, int i, int kh, int r)
+{
+    Row8 w;
+    w.t = r / p.gq;
+    w.h = kh * p.gq + r - w.t * p.gq;
+    w.b = i;
+    if constexpr (SHARED) {
+        w.b = p.e0 + i - p.F;
+        if (s.prefix) {
+            const int q = w.t / p.T;
+            w.t -= q * p.T;
+            w.b = (p.e0 + i) * p.per + q;
+            w.real = false, w.vis = 0;
+            if (!s.bad && q < p.per) {
+                // rows that are tokens of the prefix itself see it up to themselves
+                const Seq8 own = seq8(p, w.b);
+                w.real = !own.bad && w.t < own.tq;
+                if (w.real)
+                    w.vis = p.causal ? max(s.n + min(own.n - own.tq + w.t + 1, 0), 0) : s.n;
+            }
+            return w;
+        }
+    }
+    w.real = !s.bad && w.t < s.tq;
+    w.vis = visible8(p, s, w.t);
+    return w;
 }
 
 template <bool BF16>
@@ -104,5 +177,20 @@ __device__ __forceinline__ unsigned nan_codes(unsigned w)
 {
     return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
+
+// Rows from which the merge gives each a lane group instead of a workgroup (12,800
+// rows of four parts 5.6 us / 9.0 with a wave a row; 1,280 rows of nine 6.5 / 4.6).
+constexpr int64_t kMergeRows = 2048;
+
+inline int device_cus()
+{
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess ||
+        hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+        cus = 256;
+    return cus;
+}
+
+inline size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 } // namespace kitty

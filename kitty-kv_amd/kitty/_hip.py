@@ -19,7 +19,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # KITTY_HIP_LIBRARY selects another build of the same ABI (e.g. a tuning variant).
 LIB_PATH = os.environ.get("KITTY_HIP_LIBRARY") or os.path.join(_HERE, "libkitty_hip.so")
 
-KITTY_ABI_VERSION = 8
+KITTY_ABI_VERSION = 9
 KITTY_OK = 0
 KITTY_E_INVALID = -1
 KITTY_E_HIP = -2
@@ -191,6 +191,21 @@ class Cache8AttentionArgs(ctypes.Structure):
     ]
 
 
+class Cache8SharedArgs(ctypes.Structure):
+    """kitty_cache8_shared_args."""
+    _fields_ = [
+        ("q", _vp), ("out", _vp), ("lse", _vp),
+        ("q_s_seq", _i64), ("q_s_head", _i64), ("q_s_tok", _i64),
+        ("o_s_seq", _i64), ("o_s_head", _i64), ("o_s_tok", _i64),
+        ("prefix_table", _vp), ("pt_stride", _i64), ("prefix_lens", _vp),
+        ("block_table", _vp), ("bt_stride", _i64), ("lens", _vp), ("q_lens", _vp),
+        ("prefixes", _i32), ("batch", _i32), ("num_q_heads", _i32), ("tokens", _i32), ("prefix_pages", _i32),
+        ("table_pages", _i32), ("plan_prefix", _i32), ("plan_tokens", _i32),
+        ("causal", _i32), ("dtype", _i32), ("sm_scale", ctypes.c_float),
+        ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "kitty_abi_version", "kitty_last_error", "kitty_quantize_kv_blocks",
     "kitty_dequantize_key_page", "kitty_dequantize_value_page",
@@ -200,7 +215,7 @@ EXPORTED_SYMBOLS = (
     "kitty_channel_abs_sum_flush", "kitty_store_i32", "kitty_prefill_attention",
     "kitty_store_prompt", "kitty_zero_regions", "kitty_decode_step", "kitty_channel_abs_sum_first",
     "kitty_channel_scores", "kitty_cache8_write", "kitty_cache8_read", "kitty_cache8_attention_workspace_size",
-    "kitty_cache8_attention",
+    "kitty_cache8_attention", "kitty_cache8_shared_attention_workspace_size", "kitty_cache8_shared_attention",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -251,6 +266,8 @@ def load() -> ctypes.CDLL:
     L.kitty_cache8_read.argtypes = L.kitty_cache8_write.argtypes
     L.kitty_cache8_attention_workspace_size.argtypes = [ctypes.POINTER(Cache8), _vp, ctypes.POINTER(ctypes.c_size_t)]
     L.kitty_cache8_attention.argtypes = L.kitty_cache8_write.argtypes
+    L.kitty_cache8_shared_attention_workspace_size.argtypes = L.kitty_cache8_attention_workspace_size.argtypes
+    L.kitty_cache8_shared_attention.argtypes = L.kitty_cache8_write.argtypes
     if L.kitty_abi_version() != KITTY_ABI_VERSION:
         raise ImportError(f"libkitty_hip ABI {L.kitty_abi_version()} != {KITTY_ABI_VERSION}")
     _lib = L

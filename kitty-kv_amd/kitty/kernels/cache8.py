@@ -27,10 +27,11 @@ from .ops import _need, calls_followed
 
 _SRC = {torch.float16: _hip.KITTY_SRC_F16, torch.bfloat16: _hip.KITTY_SRC_BF16, torch.float32: _hip.KITTY_SRC_F32}
 _PAGE_TOKENS = (16, 32, 64, 128, 256)
-# kitty_cache8_write_args / _read_args and kitty_cache8_attention_args as the C
+# kitty_cache8_write_args / _read_args, kitty_cache8_attention_args and _shared_args as the C
 # compiler lays them out (packing one takes a quarter of a ctypes structure's time)
 _ROWS = struct.Struct("2P6qPq2P4i")
 _ATTENTION = struct.Struct("3P6qPq2P7ifPN")
+_SHARED = struct.Struct("3P6qPqPPq2P10ifPN")
 
 
 _FOLLOWED = "calls of the 8-bit cache cannot be traced, compiled or transformed"
@@ -145,10 +146,10 @@ class Cache8:
               f"{name} must be int32 ({B},)")
         self._here(name, t)
 
-    def _check_table(self, t: torch.Tensor, B: int) -> None:
+    def _check_table(self, t: torch.Tensor, B: int, name: str = "block_table") -> None:
         _need(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] == B and (t.shape[1] <= 1 or t.stride(1) == 1),
-              f"block_table must be int32 ({B}, W) with contiguous rows")
-        self._here("block_table", t)
+              f"{name} must be int32 ({B}, W) with contiguous rows")
+        self._here(name, t)
 
     def _keep(self, sig, found):
         if len(self._known) >= 512:
@@ -366,3 +367,103 @@ class Cache8:
             qp, out.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, block_table.data_ptr(), bt_stride,
             lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), *rest, 0 if ws is None else ws.data_ptr(), need))
         return (out, lse) if return_lse else out
+
+    def _check_queries(self, q: torch.Tensor, out: Optional[torch.Tensor], sm_scale: Optional[float]) -> float:
+        """Checks of an attention's queries and output; its scale."""
+        _need(q.dim() == 4 and q.shape[3] == self.head_dim, f"q must be (B, Hq, T, {self.head_dim})")
+        _need(q.dtype in (torch.float16, torch.bfloat16), "q must be float16 or bfloat16")
+        self._here("q", q)
+        _need(q.shape[1] > 0 and q.shape[1] % self.num_kv_heads == 0,
+              f"q heads must be a positive multiple of {self.num_kv_heads}")
+        scale = 1.0 / math.sqrt(self.head_dim) if sm_scale is None else sm_scale
+        _need(0.0 < scale <= 1e30, "sm_scale must be positive and finite")
+        if out is not None:
+            _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(3) == 1,
+                  "out must have q's shape and dtype and contiguous channels")
+            _need(torch._debug_has_internal_overlap(out) != 1, "out must not share memory between its rows")
+            self._here("out", out)
+        return scale
+
+    def attend_shared(self, q: torch.Tensor, prefix_table: torch.Tensor, prefix_lens: torch.Tensor, block_table: torch.Tensor,
+                      lens: torch.Tensor, q_lens: Optional[torch.Tensor] = None, causal: bool = True,
+                      sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                      max_prefix: Optional[int] = None, max_tokens: Optional[int] = None):
+        """``attend`` for sequences that share prefixes (a system prompt, the samples of
+        one prompt), which are read once for all of them.
+
+        prefix_table (F, Wp) and prefix_lens (F,) name the prefixes, of any length; B is
+        a multiple of F, and sequence b is prefix b // (B / F) followed by the lens[b]
+        tokens of its own in the pages of block_table's row b (lens[b] may be 0; the first
+        of them is row 0 of its first page).  causal: the q_lens[b] queries of sequence b
+        are the last tokens of the two together; otherwise every query sees all of both.
+        Results are ``attend``'s over the two in one table but for rounding.  max_prefix
+        and max_tokens: the largest prefix_lens[f] and lens[b] where the program knows
+        them; they only choose how the work is split.  out may be q or lie in its memory
+        in any way."""
+        if calls_followed():
+            raise NotImplementedError(_FOLLOWED)
+        if q.requires_grad or q.is_neg():
+            q = _given(q, "q")
+        if out is not None:
+            _into(out)
+        causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
+        max_prefix = 0 if max_prefix is None else int(max_prefix)
+        max_tokens = 0 if max_tokens is None else int(max_tokens)
+        sig = ("shared", q.shape, q.stride(), q.dtype, q.device, _sig(prefix_table), _sig(prefix_lens), _sig(block_table),
+               _sig(lens), _sig(q_lens), causal, sm_scale, _sig(out), max_prefix, max_tokens)
+        found = self._known.get(sig) if self._on_device else None
+        if found is None:
+            scale = self._check_queries(q, out, sm_scale)
+            B, Hq, T, _ = q.shape
+            _need(prefix_table.dim() == 2 and prefix_table.shape[0] > 0 and B % prefix_table.shape[0] == 0,
+                  "prefix_table must be int32 (F, Wp), and the batch a multiple of F")
+            F = prefix_table.shape[0]
+            self._check_table(prefix_table, F, "prefix_table")
+            self._i32("prefix_lens", prefix_lens, F)
+            self._check_table(block_table, B)
+            self._i32("lens", lens, B)
+            self._i32("q_lens", q_lens, B, optional=True)
+            for name, n in (("max_prefix", max_prefix), ("max_tokens", max_tokens)):
+                _need(0 <= n < 1 << 31, f"{name} must be in [0, 2^31)")
+            if B == 0 or T == 0 or not self._on_device:
+                o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+                lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
+                if B and T:
+                    cpu8.attend_shared(self.key, self.value, self.scale, q, prefix_table, prefix_lens, block_table, lens,
+                                       q_lens, causal, scale, o, lse)
+                return (o, lse) if return_lse else o
+            in_place = q.stride(3) == 1 and _aligned16(q), out is None or _aligned16(out)
+            o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+            # copies of rows that the kernel does not read or write in place are contiguous
+            Hs, Ts = Hq * T * self.head_dim, T * self.head_dim
+            packed = tuple(0 if n == 1 else s for n, s in zip((B, Hq, T), (Hs, Ts, self.head_dim)))
+            head = (*(_strides(q) if in_place[0] else packed), *(_strides(o) if in_place[1] else packed))
+            tables = prefix_table.stride(0) if F > 1 else 0, block_table.stride(0) if B > 1 else 0
+            rest = (F, B, Hq, T, prefix_table.shape[1], block_table.shape[1], max_prefix, max_tokens, causal,
+                    _hip.KITTY_DTYPE_F16 if q.dtype == torch.float16 else _hip.KITTY_DTYPE_BF16, scale)
+            size = ctypes.c_size_t(0)
+            with torch.cuda.device(self._index):      # the plan is the pools' device's
+                _hip.check(self._lib.kitty_cache8_shared_attention_workspace_size(
+                    self._ref, _SHARED.pack(0, 0, 0, *head, 0, tables[0], 0, 0, tables[1], 0, 0, *rest, 0, 0), ctypes.byref(size)))
+            found = self._keep(sig, (in_place, q.is_contiguous(), packed, head, tables, rest, size.value))
+        (q_ok, out_ok), like_q, packed, head, tables, rest, need = found
+        if not q_ok or q.data_ptr() % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            head = (*packed, *head[3:])
+        o = out
+        if out is None or not out_ok or out.data_ptr() % 16 or out.is_neg():
+            o = torch.empty_like(q) if like_q else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            if out is not None:
+                head = (*head[:3], *packed)
+        else:
+            _written(out)
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+        ws = q.new_empty((need + 1) // 2)      # of the call's own, as attend's
+        self._launch(self._lib.kitty_cache8_shared_attention, _SHARED.pack(
+            q.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, prefix_table.data_ptr(), tables[0],
+            prefix_lens.data_ptr(), block_table.data_ptr(), tables[1], lens.data_ptr(),
+            0 if q_lens is None else q_lens.data_ptr(), *rest, ws.data_ptr(), need))
+        if out is not None and o is not out:
+            out.copy_(o)
+            o = out
+        return (o, lse) if return_lse else o

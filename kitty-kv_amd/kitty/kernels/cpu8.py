@@ -78,12 +78,48 @@ def read(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: tor
         out[i].copy_(torch.where(here[..., None, None], x, torch.zeros_like(x)).transpose(1, 2))
 
 
+def _tokens(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: torch.Tensor, n: int):
+    """Codes (H, n, D) and scales (H, 1, n) of keys and values of the n tokens that a
+    table row names, apart, as in the kernels: their products may pass fp32's range."""
+    P, H, G, D = key.shape
+    ids, ok = _page_ids(table[None], torch.arange(-(-n // G))[None], P)
+    codes, scales = [], []
+    for i, pool in enumerate((key, value)):
+        x, f = torch.zeros(ids.shape[1], H, G, D), torch.ones(ids.shape[1], H)
+        if P:
+            x, f = pool.view(torch.uint8)[ids[0]].view(E4M3).float(), torch.where(ok[0][:, None], scale[ids[0], :, i], f)
+        x = torch.where(ok[0][:, None, None, None], x, torch.full_like(x, math.nan))
+        codes.append(x.transpose(0, 1).flatten(1, 2)[:, :n])
+        scales.append(f.t().repeat_interleave(G, 1)[:, None, :n])
+    return codes, scales
+
+
+def _rows(q: torch.Tensor, codes, scales, causal: bool, sm_scale: float):
+    """Attention of q (Hq, t, D) over tokens as _tokens has them, the queries their last:
+    (out, log-sum-exp, softmax weights (H, gq, t, n))."""
+    Hq, t, D = q.shape
+    H, n, _ = codes[0].shape
+    gq = Hq // H
+    sees = torch.ones(t, n, dtype=torch.bool)
+    if causal:
+        sees = torch.arange(n) <= torch.arange(n - t, n)[:, None]
+    s = (q.reshape(H, gq * t, D) @ codes[0].transpose(1, 2) * (scales[0] * sm_scale)).view(H, gq, t, n)
+    s = s.masked_fill(~sees, -math.inf)
+    l = torch.logsumexp(s, -1)
+    none = ~sees.any(-1)                                   # rows that see nothing
+    w = torch.exp(s - torch.where(none, torch.zeros_like(l), l)[..., None])
+    gone = codes[1].isnan()                                # masked NaN values stay out of the product
+    o = (w.view(H, gq * t, n) * scales[1]) @ codes[1].masked_fill(gone, 0.0)
+    met = (sees.float().repeat(gq, 1) @ gone.float()) > 0
+    o = o.masked_fill(met, math.nan).view(H, gq, t, D).masked_fill(none[:, None], 0.0)
+    return o.reshape(Hq, t, D), l.masked_fill(none, -math.inf).reshape(Hq, t), w
+
+
 def attend(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch.Tensor, table: torch.Tensor,
            lens: torch.Tensor, q_lens: Optional[torch.Tensor], causal: bool, sm_scale: float, out: torch.Tensor,
            lse: torch.Tensor) -> None:
     B, Hq, T, D = q.shape
-    P, H, G = key.shape[:3]
-    gq = Hq // H
+    G = key.shape[2]
     q = q.float()       # a copy: out may be q
     out.zero_()
     lse.fill_(-math.inf)
@@ -95,27 +131,33 @@ def attend(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch
             continue
         if n == 0 or t == 0:
             continue
-        ids, ok = _page_ids(table[b:b + 1], torch.arange(-(-n // G))[None], P)
-        # codes and scales apart, as in the kernels: their products may pass fp32's range
-        kv, factors = [], []
-        for i, pool in enumerate((key, value)):
-            x, f = torch.zeros(ids.shape[1], H, G, D), torch.ones(ids.shape[1], H)
-            if P:
-                x, f = pool.view(torch.uint8)[ids[0]].view(E4M3).float(), torch.where(ok[0][:, None], scale[ids[0], :, i], f)
-            x = torch.where(ok[0][:, None, None, None], x, torch.full_like(x, math.nan))
-            kv.append(x.transpose(0, 1).flatten(1, 2)[:, :n])
-            factors.append(f.t().repeat_interleave(G, 1)[:, None, :n])       # (H, 1, n)
-        sees = torch.ones(t, n, dtype=torch.bool)
-        if causal:
-            sees = torch.arange(n) <= torch.arange(n - t, n)[:, None]
-        s = (q[b, :, :t].reshape(H, gq * t, D) @ kv[0].transpose(1, 2) * (factors[0] * sm_scale)).view(H, gq, t, n)
-        s = s.masked_fill(~sees, -math.inf)
-        l = torch.logsumexp(s, -1)
-        none = ~sees.any(-1)                                   # rows that see nothing
-        w = torch.exp(s - torch.where(none, torch.zeros_like(l), l)[..., None])
-        gone = kv[1].isnan()                                   # masked NaN values stay out of the product
-        o = (w.view(H, gq * t, n) * factors[1]) @ kv[1].masked_fill(gone, 0.0)
-        met = (sees.float().repeat(gq, 1) @ gone.float()) > 0
-        o = o.masked_fill(met, math.nan).view(H, gq, t, D).masked_fill(none[:, None], 0.0)
-        out[b, :, :t] = o.reshape(Hq, t, D).to(out.dtype)
-        lse[b, :, :t] = l.masked_fill(none, -math.inf).reshape(Hq, t)
+        o, l, _ = _rows(q[b, :, :t], *_tokens(key, value, scale, table[b], n), causal, sm_scale)
+        out[b, :, :t] = o.to(out.dtype)
+        lse[b, :, :t] = l
+
+
+def attend_shared(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch.Tensor, prefix_table: torch.Tensor,
+                  prefix_lens: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, q_lens: Optional[torch.Tensor],
+                  causal: bool, sm_scale: float, out: torch.Tensor, lse: torch.Tensor) -> None:
+    B, Hq, T, D = q.shape
+    G, each = key.shape[2], B // prefix_table.shape[0]
+    q = q.float()       # a copy: out may be q
+    out.zero_()
+    lse.fill_(-math.inf)
+    rows = [T] * B if q_lens is None else q_lens.tolist()
+    prefix = prefix_lens.tolist()
+    for b, (n, t) in enumerate(zip(lens.tolist(), rows)):
+        f = b // each
+        before = prefix[f]
+        if n < 0 or n > table.shape[1] * G or not 0 <= t <= T or before < 0 or before > prefix_table.shape[1] * G:
+            out[b] = math.nan
+            lse[b] = math.nan
+            continue
+        if n + before == 0 or t == 0:
+            continue
+        parts = _tokens(key, value, scale, prefix_table[f], before), _tokens(key, value, scale, table[b], n)
+        codes = [torch.cat([p[0][i] for p in parts], 1) for i in range(2)]
+        scales = [torch.cat([p[1][i] for p in parts], 2) for i in range(2)]
+        o, l, _ = _rows(q[b, :, :t], codes, scales, causal, sm_scale)
+        out[b, :, :t] = o.to(out.dtype)
+        lse[b, :, :t] = l
