@@ -661,6 +661,59 @@ int kitty_cache8_shared_attention_workspace_size(const kitty_cache8 *cache, cons
                                                  size_t *bytes);
 int kitty_cache8_shared_attention(const kitty_cache8 *cache, const kitty_cache8_shared_args *args, kitty_stream_t stream);
 
+/* kitty_cache8_attention that also adds what the tokens got: with p the softmax of a
+ * row (exp(score - lse)), weights[b * s_seq + h * s_head + j] += the sum of p_j over the
+ * rows of KV head h's group, for tokens j < min(lens[b], tokens) that some row sees.
+ * Weights of other tokens stay as they are; a row whose softmax is NaN makes the
+ * weights of the tokens that it sees NaN, a sequence whose lengths break the rules
+ * changes none.  out must not lie in q's memory.  The same call gives the same bits. */
+typedef struct {
+    float *weights;          /* (B, H, tokens), stride 1 between tokens */
+    int64_t s_seq, s_head;
+    int32_t tokens;
+} kitty_cache8_weights;
+
+int kitty_cache8_weighed_attention_workspace_size(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
+                                                  const kitty_cache8_weights *weights, size_t *bytes);
+int kitty_cache8_weighed_attention(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
+                                   const kitty_cache8_weights *weights, kitty_stream_t stream);
+
+/* Eviction by weight.  Of sequence b's n = lens[b] tokens m = min(n, keep) stay, in each
+ * KV head its own: where n > keep the first `first`, the last `last`, and of those
+ * between the keep - first - last heaviest by weights[b, h, j] (of equal ones the
+ * earlier; both zeros are equal, NaN is heavier than all else, as torch.sort has it).
+ * They become tokens 0 .. m - 1, in their order, of the pages that row b of `into`
+ * names, or of block_table where into is NULL (pages of `into` must not be among those
+ * that the call reads; no page may be written for two sequences).  A page's scale
+ * becomes the largest of the pages that its tokens come from, and a code c of one with
+ * another scale s becomes e4m3(c * (s / scale)), both in fp32; others move as they are.
+ * Rows behind the last token keep their bytes.
+ * out_lens[b] = m; kept[b, h, i] = the position of token i, -1 for i >= m;
+ * out_weights[b, h, i] = its weight, 0 for i >= m.  A token whose page is outside the
+ * pool moves as NaN codes and takes no part in the scale (1 where a page has no other);
+ * tokens whose new page is outside the pool, or that `into` has no page for, are
+ * dropped.  A length that is negative, or more than table_pages pages or weight_tokens
+ * hold, gives out_lens -1, nothing kept and no page written. */
+typedef struct {
+    const float *weights;        /* (B, H, weight_tokens), stride 1 between tokens */
+    int64_t w_s_seq, w_s_head;
+    const int32_t *block_table;  /* (B, table_pages) page ids */
+    int64_t bt_stride;
+    const int32_t *lens;         /* (B,) */
+    const int32_t *into;         /* (B, into_pages) page ids, or NULL: in place */
+    int64_t into_stride;
+    int32_t *out_lens;           /* (B,), apart from lens */
+    int32_t *kept;               /* (B, H, min(keep, weight_tokens)) contiguous */
+    float *out_weights;          /* (B, H, weight_tokens) contiguous, apart from weights */
+    int32_t batch, table_pages, into_pages, weight_tokens;
+    int32_t keep, first, last;
+    void *workspace;             /* in place: kitty_cache8_evict_workspace_size bytes, 16-byte aligned */
+    size_t workspace_bytes;
+} kitty_cache8_evict_args;
+
+int kitty_cache8_evict_workspace_size(const kitty_cache8 *cache, const kitty_cache8_evict_args *args, size_t *bytes);
+int kitty_cache8_evict(const kitty_cache8 *cache, const kitty_cache8_evict_args *args, kitty_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -191,6 +191,4 @@ inline int device_cus()
     return cus;
 }
 
-inline size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
-
 } // namespace kitty

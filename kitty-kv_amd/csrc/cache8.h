@@ -20,6 +20,8 @@ int check_cache8(const kitty_cache8 *cache, Cache8 &c);
 // Workgroups of up to 256 threads that one launch takes (a grid has less than 2^32 threads).
 constexpr int64_t kMaxBlocks = 0xffffffffll / 256;
 
+inline size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
+
 inline bool aligned(const void *p, unsigned a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 __device__ __forceinline__ bool bad_page(const Cache8 &c, int id) { return id < 0 || id >= c.num_pages; }

@@ -1,0 +1,331 @@
+// Eviction from the 8-bit paged cache by weight, on gfx950: which tokens of a sequence
+// and KV head stay, and their move together.
+//
+// cache8_select_kernel, a workgroup per (sequence, KV head): the weights between the
+// first and last tokens, which stay, map to unsigned keys in the floats' order (both
+// zeros alike, NaN above all); four passes over 8 bits each, counted in LDS, find the
+// key of the lightest token that stays and how many of its equals do.  One more pass
+// writes positions and weights in order: a token's place is the count of heavier ones
+// before it plus that of its equals, as far as they stay.  Counts are integers: any
+// order of additions gives the same.
+// cache8_pack_kernel, a workgroup per (page, KV head, stream) of the result: the page's
+// scale is the largest of the pages that its tokens come from, and codes of smaller
+// scales are multiplied by the quotient and rounded again (exact but for subnormals
+// where scales are powers of two).  In place the codes go through the workspace, as a
+// page of the result may hold tokens that another page of the result needs.
+#include "cache8.h"
+
+namespace kitty {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+struct Evict8 {
+    Cache8 c;
+    const float *weights;
+    int64_t w_s_seq, w_s_head;
+    const int32_t *table, *lens, *into;
+    int64_t bt_stride, into_stride;
+    int32_t *out_lens, *kept;
+    float *out_weights;
+    uint8_t *ws_codes;    // in place: (sequence, KV head, stream, K, D)
+    float *ws_scale;      //           (sequence, KV head, stream, K)
+    int B, N, K, keep, first, last, table_pages, into_pages, tiles;
+};
+
+constexpr int kSelect = 1024;
+
+__device__ __forceinline__ uint32_t weight_key(float x)
+{
+    const uint32_t u = x == 0.0f ? 0u : __builtin_bit_cast(uint32_t, x);
+    return x != x ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
+}
+
+// Tokens of sequence b that stay, -1 where its length breaks the rules.
+__device__ __forceinline__ int kept8(const Evict8 &p, int n)
+{
+    return n < 0 || n > (int64_t)p.table_pages << p.c.lg || n > p.N ? -1 : min(n, p.keep);
+}
+
+__global__ __launch_bounds__(kSelect) void cache8_select_kernel(Evict8 p)
+{
+    __shared__ unsigned hist[256], sums[kSelect / 64];
+    __shared__ unsigned found[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b = blockIdx.x / p.c.H, h = blockIdx.x - b * p.c.H;
+    const int n = p.lens[b], m = kept8(p, n);
+    const float *w = p.weights + b * p.w_s_seq + h * p.w_s_head;
+    int32_t *kept = p.kept + (int64_t)blockIdx.x * p.K;
+    float *out = p.out_weights + (int64_t)blockIdx.x * p.N;
+    if (h == 0 && tid == 0)
+        p.out_lens[b] = m;
+    // tokens lo .. hi - 1 may go, `need` of them stay
+    int lo = 0, hi = 0, need = 0;
+    uint32_t key = 0;          // of the lightest that stays: all above it do, and `need` of its equals
+    if (m >= 0 && n > m) {
+        lo = p.first, hi = n - p.last, need = m - p.first - p.last;
+        if (need > 0) {
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                const uint32_t above = shift == 24 ? 0u : ~0u << (shift + 8);
+                if (tid < 256)
+                    hist[tid] = 0;
+                __syncthreads();
+                for (int i = lo + tid; i < hi; i += kSelect) {
+                    const uint32_t k = weight_key(w[i]);
+                    if (((k ^ key) & above) == 0)
+                        atomicAdd(&hist[k >> shift & 255], 1u);
+                }
+                __syncthreads();
+                if (wave == 0) {
+                    // from the heaviest: lane l has bins 255 - 4 l .. 252 - 4 l
+                    unsigned c[4], all = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        all += c[j] = hist[255 - 4 * lane - j];
+                    unsigned inc = all;
+#pragma unroll
+                    for (int off = 1; off < 64; off <<= 1) {
+                        const unsigned y = __shfl_up(inc, off);
+                        inc += lane >= off ? y : 0;
+                    }
+                    unsigned before = inc - all;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (before < (unsigned)need && before + c[j] >= (unsigned)need)
+                            found[0] = 255 - 4 * lane - j, found[1] = need - before;
+                        before += c[j];
+                    }
+                }
+                __syncthreads();
+                key |= found[0] << shift;
+                need = (int)found[1];
+            }
+        }
+    }
+    // positions in order: low halves count tokens that stay whatever the others are, high halves equals of `key`
+    const int end = max(m < 0 ? 0 : n, 0);
+    int sure = 0, equal = 0;
+    const bool some = need > 0;
+    for (int i0 = 0; i0 < end; i0 += kSelect) {
+        const int i = i0 + tid;
+        float x = 0.0f;
+        bool stays = false, same = false;
+        if (i < end) {
+            x = w[i];
+            const uint32_t k = weight_key(x);
+            const bool may_go = i >= lo && i < hi;
+            stays = !may_go || (some && k > key);
+            same = may_go && some && k == key;
+        }
+        const unsigned mine = (stays ? 1u : 0u) | (same ? 0x10000u : 0u);
+        unsigned inc = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const unsigned y = __shfl_up(inc, off);
+            inc += lane >= off ? y : 0;
+        }
+        if (lane == 63)
+            sums[wave] = inc;
+        __syncthreads();
+        unsigned before = inc - mine, total = 0;
+#pragma unroll
+        for (int k = 0; k < kSelect / 64; ++k) {
+            before += k < wave ? sums[k] : 0;
+            total += sums[k];
+        }
+        __syncthreads();
+        const int e = equal + (int)(before >> 16);
+        if (stays || (same && e < need)) {
+            const int at = sure + (int)(before & 0xffff) + min(e, need);
+            kept[at] = i;
+            out[at] = x;
+        }
+        sure += (int)(total & 0xffff), equal += (int)(total >> 16);
+    }
+    for (int i = max(m, 0) + tid; i < p.N; i += kSelect)
+        out[i] = 0.0f;
+    for (int i = max(m, 0) + tid; i < p.K; i += kSelect)
+        kept[i] = -1;
+}
+
+// Where a kept token's codes are.
+struct Source8 {
+    const uint8_t *codes;    // NULL: it has no page
+    float scale;
+};
+
+__device__ __forceinline__ Source8 source8(const Evict8 &p, int b, int h, int st, int pos)
+{
+    const int id = pos < 0 ? -1 : p.table[b * p.bt_stride + (pos >> p.c.lg)];
+    if (bad_page(p.c, id))
+        return Source8{nullptr, 0.0f};
+    const uint32_t row = (uint32_t)pos & ((1u << p.c.lg) - 1);
+    return Source8{st ? p.c.value + id * p.c.value_s_page + h * p.c.value_s_head + row * p.c.value_s_tok
+                      : p.c.key + id * p.c.key_s_page + h * p.c.key_s_head + row * p.c.key_s_tok,
+                   p.c.scale[id * p.c.scale_s_page + h * p.c.scale_s_head + st]};
+}
+
+// The kept tokens' codes and scales, in their new order, into the workspace.
+__global__ __launch_bounds__(256) void cache8_stage_kernel(Evict8 p)
+{
+    uint32_t i = blockIdx.x;
+    const int tile = (int)(i % (uint32_t)p.tiles);
+    i /= (uint32_t)p.tiles;
+    const int st = (int)(i & 1);
+    const int h = (int)((i >> 1) % (uint32_t)p.c.H), b = (int)((i >> 1) / (uint32_t)p.c.H);
+    const int cpr = p.c.D >> 4, rows = 256 / cpr, r = threadIdx.x / cpr, c = threadIdx.x - r * cpr;
+    const int64_t seq = (int64_t)(b * p.c.H + h), list = (2 * seq + st) * p.K;
+    const int at = tile * rows + r;
+    if (r >= rows || at >= kept8(p, p.lens[b]))
+        return;
+    const Source8 s = source8(p, b, h, st, p.kept[seq * p.K + at]);
+    *(u32x4 *)(p.ws_codes + (list + at) * p.c.D + 16 * c) =
+        s.codes ? *(const u32x4 *)(s.codes + 16 * c) : u32x4{0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f};
+    if (c == 0)
+        p.ws_scale[list + at] = s.codes ? s.scale : -1.0f;
+}
+
+__device__ __forceinline__ unsigned times(unsigned w, float f)
+{
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * f, lo[1] * f, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * f, hi[1] * f, r, true);
+}
+
+template <bool STAGED>
+__global__ __launch_bounds__(256) void cache8_pack_kernel(Evict8 p)
+{
+    __shared__ const uint8_t *src[256];
+    __shared__ float scale[256], part[4];
+    uint32_t i = blockIdx.x;
+    const int page = (int)(i % (uint32_t)p.tiles);
+    i /= (uint32_t)p.tiles;
+    const int st = (int)(i & 1);
+    const int h = (int)((i >> 1) % (uint32_t)p.c.H), b = (int)((i >> 1) / (uint32_t)p.c.H);
+    const int lg = p.c.lg, first = page << lg, m = kept8(p, p.lens[b]);
+    if (first >= m || page >= p.into_pages)
+        return;
+    const int id = p.into[b * p.into_stride + page];
+    if (bad_page(p.c, id))
+        return;
+    const int rows = min(1 << lg, m - first);
+    const int64_t seq = (int64_t)(b * p.c.H + h), list = (2 * seq + st) * p.K;
+    float mine = -1.0f;       // of a token without a page
+    if ((int)threadIdx.x < rows) {
+        const int at = first + threadIdx.x;
+        if constexpr (STAGED) {
+            mine = p.ws_scale[list + at];
+            src[threadIdx.x] = p.ws_codes + (list + at) * p.c.D;
+        } else {
+            const Source8 s = source8(p, b, h, st, p.kept[seq * p.K + at]);
+            mine = s.codes ? s.scale : -1.0f;
+            src[threadIdx.x] = s.codes;
+        }
+        scale[threadIdx.x] = mine;
+    }
+    float top = mine;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1)
+        top = fmaxf(top, __shfl_xor(top, off));
+    if ((threadIdx.x & 63) == 0)
+        part[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+    if (top < 0.0f)
+        top = 1.0f;           // none of its tokens has a page
+    uint8_t *dst = st ? p.c.value + id * p.c.value_s_page + h * p.c.value_s_head
+                      : p.c.key + id * p.c.key_s_page + h * p.c.key_s_head;
+    const uint32_t d_tok = st ? p.c.value_s_tok : p.c.key_s_tok;
+    const int cpr = p.c.D >> 4, rpp = 256 / cpr, r0 = threadIdx.x / cpr, c = threadIdx.x - r0 * cpr;
+    if (r0 < rpp)
+        for (int r = r0; r < rows; r += rpp) {
+            const uint8_t *s = src[r];
+            const float was = scale[r];
+            u32x4 x = {0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f, 0x7f7f7f7f};
+            if (STAGED || s)
+                x = *(const u32x4 *)(s + 16 * c);
+            if (was != top && was >= 0.0f) {
+                const float f = was / top;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[e] = times(x[e], f);
+            }
+            *(u32x4 *)(dst + (uint32_t)r * d_tok + 16 * c) = x;
+        }
+    if (threadIdx.x == 0)
+        p.c.scale[id * p.c.scale_s_page + h * p.c.scale_s_head + st] = top;
+}
+
+static int check_evict(const kitty_cache8 *cache, const kitty_cache8_evict_args *args, Evict8 &p, size_t &need)
+{
+    if (!args)
+        return fail(KITTY_E_INVALID, "args is NULL");
+    if (const int rc = check_cache8(cache, p.c))
+        return rc;
+    const kitty_cache8_evict_args &a = *args;
+    if (a.batch < 0 || a.table_pages < 0 || a.into_pages < 0 || a.weight_tokens < 0)
+        return fail(KITTY_E_INVALID, "batch, table_pages, into_pages and weight_tokens must not be negative");
+    if (a.keep < 0 || a.first < 0 || a.last < 0 || (int64_t)a.first + a.last > a.keep)
+        return fail(KITTY_E_INVALID, "first and last must not be negative, and keep at least both together");
+    if ((int64_t)a.table_pages << p.c.lg > 1 << 30 || a.weight_tokens > 1 << 30)
+        return fail(KITTY_E_UNSUPPORTED, "a sequence is limited to 2^30 tokens");
+    p.B = a.batch, p.N = a.weight_tokens, p.K = a.keep < a.weight_tokens ? a.keep : a.weight_tokens;
+    if ((int64_t)p.B * p.c.H > kMaxBlocks / 4 || (int64_t)p.B * p.c.H * 2 * (((int64_t)p.K >> 4) + 1) > kMaxBlocks)
+        return fail(KITTY_E_UNSUPPORTED, "too many tokens for one launch");
+    need = a.into ? 0 : up16((size_t)p.B * p.c.H * 2 * p.K * p.c.D) + up16((size_t)p.B * p.c.H * 2 * p.K * 4);
+    return KITTY_OK;
+}
+
+} // namespace kitty
+
+using namespace kitty;
+
+extern "C" int kitty_cache8_evict_workspace_size(const kitty_cache8 *cache, const kitty_cache8_evict_args *args, size_t *bytes)
+{
+    Evict8 p{};
+    if (!bytes)
+        return fail(KITTY_E_INVALID, "bytes is NULL");
+    return check_evict(cache, args, p, *bytes);
+}
+
+extern "C" int kitty_cache8_evict(const kitty_cache8 *cache, const kitty_cache8_evict_args *args, kitty_stream_t stream)
+{
+    Evict8 p{};
+    size_t need;
+    if (const int rc = check_evict(cache, args, p, need))
+        return rc;
+    const kitty_cache8_evict_args &a = *args;
+    if (a.batch == 0)
+        return KITTY_OK;
+    if (!a.lens || !a.out_lens || (!a.block_table && a.table_pages) || (a.weight_tokens && (!a.weights || !a.out_weights)) ||
+        (p.K && !a.kept))
+        return fail(KITTY_E_INVALID, "NULL lens, out_lens, block_table, weights, out_weights or kept");
+    if (!aligned(a.weights, 4) || !aligned(a.out_weights, 4))
+        return fail(KITTY_E_INVALID, "weights and out_weights must be 4-byte aligned");
+    if (need && (!a.workspace || !aligned(a.workspace, 16) || a.workspace_bytes < need))
+        return fail(KITTY_E_INVALID, "workspace is NULL, misaligned or smaller than kitty_cache8_evict_workspace_size");
+    p.weights = a.weights, p.w_s_seq = a.w_s_seq, p.w_s_head = a.w_s_head;
+    p.table = a.block_table, p.bt_stride = a.bt_stride, p.table_pages = a.table_pages, p.lens = a.lens;
+    p.into = a.into ? a.into : a.block_table, p.into_stride = a.into ? a.into_stride : a.bt_stride;
+    p.into_pages = a.into ? a.into_pages : a.table_pages;
+    p.out_lens = a.out_lens, p.kept = a.kept, p.out_weights = a.out_weights;
+    p.keep = a.keep, p.first = a.first, p.last = a.last;
+    p.ws_codes = (uint8_t *)a.workspace;
+    p.ws_scale = (float *)((char *)a.workspace + up16((size_t)p.B * p.c.H * 2 * p.K * p.c.D));
+    const hipStream_t st = (hipStream_t)stream;
+    const unsigned pairs = (unsigned)(p.B * p.c.H);
+    hipLaunchKernelGGL(cache8_select_kernel, dim3(pairs), dim3(kSelect), 0, st, p);
+    if (p.K > 0) {
+        if (!a.into) {
+            const int rows = 256 / (p.c.D >> 4);
+            p.tiles = (p.K + rows - 1) / rows;
+            hipLaunchKernelGGL(cache8_stage_kernel, dim3(pairs * 2 * (unsigned)p.tiles), dim3(256), 0, st, p);
+        }
+        p.tiles = ((p.K - 1) >> p.c.lg) + 1;
+        if (a.into)
+            hipLaunchKernelGGL(cache8_pack_kernel<false>, dim3(pairs * 2 * (unsigned)p.tiles), dim3(256), 0, st, p);
+        else
+            hipLaunchKernelGGL(cache8_pack_kernel<true>, dim3(pairs * 2 * (unsigned)p.tiles), dim3(256), 0, st, p);
+    }
+    return check_launch("8-bit cache eviction");
+}

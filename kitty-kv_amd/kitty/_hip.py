@@ -206,6 +206,21 @@ class Cache8SharedArgs(ctypes.Structure):
     ]
 
 
+class Cache8Weights(ctypes.Structure):
+    """kitty_cache8_weights."""
+    _fields_ = [("weights", _vp), ("s_seq", _i64), ("s_head", _i64), ("tokens", _i32)]
+
+
+class Cache8EvictArgs(ctypes.Structure):
+    """kitty_cache8_evict_args."""
+    _fields_ = [
+        ("weights", _vp), ("w_s_seq", _i64), ("w_s_head", _i64), ("block_table", _vp), ("bt_stride", _i64), ("lens", _vp),
+        ("into", _vp), ("into_stride", _i64), ("out_lens", _vp), ("kept", _vp), ("out_weights", _vp),
+        ("batch", _i32), ("table_pages", _i32), ("into_pages", _i32), ("weight_tokens", _i32),
+        ("keep", _i32), ("first", _i32), ("last", _i32), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "kitty_abi_version", "kitty_last_error", "kitty_quantize_kv_blocks",
     "kitty_dequantize_key_page", "kitty_dequantize_value_page",
@@ -216,6 +231,8 @@ EXPORTED_SYMBOLS = (
     "kitty_store_prompt", "kitty_zero_regions", "kitty_decode_step", "kitty_channel_abs_sum_first",
     "kitty_channel_scores", "kitty_cache8_write", "kitty_cache8_read", "kitty_cache8_attention_workspace_size",
     "kitty_cache8_attention", "kitty_cache8_shared_attention_workspace_size", "kitty_cache8_shared_attention",
+    "kitty_cache8_weighed_attention_workspace_size", "kitty_cache8_weighed_attention", "kitty_cache8_evict_workspace_size",
+    "kitty_cache8_evict",
 )
 
 _lib: Optional[ctypes.CDLL] = None
@@ -268,6 +285,11 @@ def load() -> ctypes.CDLL:
     L.kitty_cache8_attention.argtypes = L.kitty_cache8_write.argtypes
     L.kitty_cache8_shared_attention_workspace_size.argtypes = L.kitty_cache8_attention_workspace_size.argtypes
     L.kitty_cache8_shared_attention.argtypes = L.kitty_cache8_write.argtypes
+    L.kitty_cache8_weighed_attention_workspace_size.argtypes = [ctypes.POINTER(Cache8), _vp, _vp,
+                                                                ctypes.POINTER(ctypes.c_size_t)]
+    L.kitty_cache8_weighed_attention.argtypes = [ctypes.POINTER(Cache8), _vp, _vp, _vp]
+    L.kitty_cache8_evict_workspace_size.argtypes = L.kitty_cache8_attention_workspace_size.argtypes
+    L.kitty_cache8_evict.argtypes = L.kitty_cache8_write.argtypes
     if L.kitty_abi_version() != KITTY_ABI_VERSION:
         raise ImportError(f"libkitty_hip ABI {L.kitty_abi_version()} != {KITTY_ABI_VERSION}")
     _lib = L

@@ -32,6 +32,8 @@ _PAGE_TOKENS = (16, 32, 64, 128, 256)
 _ROWS = struct.Struct("2P6qPq2P4i")
 _ATTENTION = struct.Struct("3P6qPq2P7ifPN")
 _SHARED = struct.Struct("3P6qPqPPq2P10ifPN")
+_WEIGHTS = struct.Struct("P2qi")
+_EVICT = struct.Struct("P2qPqPPq3P7iPN")
 
 
 _FOLLOWED = "calls of the 8-bit cache cannot be traced, compiled or transformed"
@@ -429,7 +431,7 @@ class Cache8:
                 o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
                 lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
                 if B and T:
-                    cpu8.attend_shared(self.key, self.value, self.scale, q, prefix_table, prefix_lens, block_table, lens,
+                    cpu8.attend_shared(self.key, self.value, self.scale, q.contiguous(), prefix_table, prefix_lens, block_table, lens,
                                        q_lens, causal, scale, o, lse)
                 return (o, lse) if return_lse else o
             in_place = q.stride(3) == 1 and _aligned16(q), out is None or _aligned16(out)
@@ -467,3 +469,160 @@ class Cache8:
             out.copy_(o)
             o = out
         return (o, lse) if return_lse else o
+
+    def _check_weights(self, weights: torch.Tensor, B: int) -> None:
+        _need(weights.dtype == torch.float32 and weights.dim() == 3 and tuple(weights.shape[:2]) == (B, self.num_kv_heads)
+              and (weights.shape[2] <= 1 or weights.stride(2) == 1),
+              f"weights must be float32 ({B}, {self.num_kv_heads}, N) with contiguous tokens")
+        self._here("weights", weights)
+        _need(weights.shape[2] <= 1 << 30, "weights must be of at most 2^30 tokens")
+
+    def attend_weighed(self, q: torch.Tensor, block_table: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor,
+                       q_lens: Optional[torch.Tensor] = None, causal: bool = True, sm_scale: Optional[float] = None,
+                       out: Optional[torch.Tensor] = None, return_lse: bool = False, max_tokens: Optional[int] = None):
+        """``attend`` that also adds to weights[b, h, j] (B, H, N) float32, for the tokens
+        j < lens[b], what token j of KV head h got: the softmax weights of the rows of the
+        head's group, summed over the queries that see it.  ``evict`` goes by such sums.
+
+        Weights behind lens[b], or of tokens that no query sees, stay as they are, and
+        tokens from N on have none; a row whose softmax is NaN makes what it sees NaN.  To
+        weigh the tokens by a prompt's last queries alone, pass those (they are causal to
+        what the cache holds); the sums repeat bit for bit.  The other arguments are
+        ``attend``'s."""
+        if calls_followed():
+            raise NotImplementedError(_FOLLOWED)
+        if q.requires_grad or q.is_neg():
+            q = _given(q, "q")
+        if out is not None:
+            _into(out)
+        if weights.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("weights need a gradient and the 8-bit cache has no backward: call under torch.no_grad()")
+        causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
+        max_tokens = 0 if max_tokens is None else int(max_tokens)
+        sig = ("weighed", q.shape, q.stride(), q.dtype, q.device, _sig(block_table), _sig(lens), _sig(weights), _sig(q_lens),
+               causal, sm_scale, _sig(out), max_tokens, weights.is_neg())
+        found = self._known.get(sig) if self._on_device else None
+        if found is None:
+            scale = self._check_queries(q, out, sm_scale)
+            B, Hq, T, _ = q.shape
+            self._check_table(block_table, B)
+            self._i32("lens", lens, B)
+            self._i32("q_lens", q_lens, B, optional=True)
+            self._check_weights(weights, B)
+            _need(not weights.is_neg(), "weights must not be a negated view")
+            _need(torch._debug_has_internal_overlap(weights) != 1, "weights must not share memory between sequences or heads")
+            _need(0 <= max_tokens < 1 << 31, "max_tokens must be in [0, 2^31)")
+            if B == 0 or T == 0 or not self._on_device:
+                o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+                lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
+                if B and T:
+                    cpu8.attend(self.key, self.value, self.scale, q.contiguous(), block_table, lens, q_lens, causal, scale, o, lse,
+                                weights)
+                return (o, lse) if return_lse else o
+            in_place = q.stride(3) == 1 and _aligned16(q), out is None or _aligned16(out)
+            o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
+            # copies of rows that the kernel does not read or write in place are contiguous
+            packed = tuple(0 if n == 1 else s for n, s in zip((B, Hq, T), (Hq * T * self.head_dim, T * self.head_dim, self.head_dim)))
+            head = (*(_strides(q) if in_place[0] else packed), *(_strides(o) if in_place[1] else packed))
+            rest = (B, Hq, T, block_table.shape[1], max_tokens, causal,
+                    _hip.KITTY_DTYPE_F16 if q.dtype == torch.float16 else _hip.KITTY_DTYPE_BF16, scale)
+            bt_stride = block_table.stride(0) if B > 1 else 0
+            w = (*_strides(weights)[:2], weights.shape[2])
+            size = ctypes.c_size_t(0)
+            with torch.cuda.device(self._index):      # the plan is the pools' device's
+                _hip.check(self._lib.kitty_cache8_weighed_attention_workspace_size(
+                    self._ref, _ATTENTION.pack(0, 0, 0, *head, 0, bt_stride, 0, 0, *rest, 0, 0),
+                    _WEIGHTS.pack(weights.data_ptr(), *w), ctypes.byref(size)))
+            found = self._keep(sig, (in_place, q.is_contiguous(), packed, head, bt_stride, rest, w, size.value,
+                                     None if out is None else (_span(q), _span(out))))
+        (q_ok, out_ok), like_q, packed, head, bt_stride, rest, w, need, spans = found
+        qp = q.data_ptr()
+        o = out
+        if out is None or not out_ok or out.data_ptr() % 16 or out.is_neg():
+            o = torch.empty_like(q) if like_q else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+            if out is not None or not like_q:
+                head = (*head[:3], *packed)
+        else:
+            _written(out)
+            # the queries are read again after the output is written
+            q_ok = q_ok and not (qp < out.data_ptr() + spans[1] and out.data_ptr() < qp + spans[0])
+        if not q_ok or qp % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            qp = q.data_ptr()
+            head = (*packed, *head[3:])
+        lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
+        ws = q.new_empty((need + 1) // 2)      # of the call's own, as attend's
+        _written(weights)
+        args = _ATTENTION.pack(qp, o.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, block_table.data_ptr(), bt_stride,
+                               lens.data_ptr(), 0 if q_lens is None else q_lens.data_ptr(), *rest, ws.data_ptr(), need)
+        held = _WEIGHTS.pack(weights.data_ptr(), *w)
+        fn = self._lib.kitty_cache8_weighed_attention
+        self._launch(lambda ref, a, stream: fn(ref, a, held, stream), args)
+        if out is not None and o is not out:
+            out.copy_(o)
+            o = out
+        return (o, lse) if return_lse else o
+
+    def evict(self, block_table: torch.Tensor, lens: torch.Tensor, weights: torch.Tensor, keep: int, first: int = 0,
+              last: int = 0, into: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Cuts sequences of more than `keep` tokens down to that many by their weights
+        (B, H, N), N at least the longest; (lengths (B,) int32, positions kept (B, H,
+        min(keep, N)) int32, weights (B, H, N)), new tensors.
+
+        Each KV head keeps tokens of its own: the first `first` (which many models lean
+        on), the last `last`, and of those between the heaviest (of equal ones the
+        earlier; NaN counts as heaviest).  The kept ones become tokens 0 .. of the
+        sequence in their old order, in block_table's first pages, or in those of `into`
+        (B, W') where given, which leaves the old pages as they are; `into` must name
+        pages that no sequence of the call has.  Pages behind the new length are free to
+        be used again, and attention over the new lengths goes on as before (keys keep the
+        positions they were made with).  A page's scale is the largest of its tokens'
+        former pages'; codes that had a smaller one are rounded again.  Positions behind
+        the kept ones are -1, weights 0.  A length that is negative, or more than
+        block_table or weights hold, comes back as -1 and its sequence as it was."""
+        if calls_followed():
+            raise NotImplementedError(_FOLLOWED)
+        if weights.requires_grad or weights.is_neg():
+            weights = _given(weights, "weights")
+        keep, first, last = int(keep), int(first), int(last)
+        sig = ("evict", _sig(block_table), _sig(lens), _sig(weights), keep, first, last, _sig(into))
+        found = self._known.get(sig) if self._on_device else None
+        if found is None:
+            _need(first >= 0 and last >= 0 and first + last <= keep < 1 << 31,
+                  "first and last must not be negative, and keep at least both together and below 2^31")
+            _need(block_table.dim() == 2, "block_table must be int32 (B, W)")
+            B, W = block_table.shape
+            self._check_table(block_table, B)
+            self._i32("lens", lens, B)
+            self._check_weights(weights, B)
+            H, N = weights.shape[1:]
+            K = min(keep, N)
+            if into is not None:
+                self._check_table(into, B, "into")
+                _need(into.shape[1] * self.page_tokens >= min(K, W * self.page_tokens), f"into must have pages for {keep} tokens")
+            if B == 0 or not self._on_device:
+                out = (torch.empty(B, dtype=torch.int32, device=self.device),
+                       torch.empty(B, H, K, dtype=torch.int32, device=self.device),
+                       torch.empty(B, H, N, device=self.device))
+                if B:
+                    cpu8.evict(self.key, self.value, self.scale, block_table, lens, weights, keep, first, last,
+                               block_table if into is None else into, *out)
+                return out
+            strides = (*_strides(weights)[:2], block_table.stride(0) if B > 1 else 0,
+                       0 if into is None or B <= 1 else into.stride(0))
+            rest = (B, W, 0 if into is None else into.shape[1], N, keep, first, last)
+            size = ctypes.c_size_t(0)
+            _hip.check(self._lib.kitty_cache8_evict_workspace_size(
+                self._ref, _EVICT.pack(0, 0, 0, 0, 0, 0, 0 if into is None else 16, 0, 0, 0, 0, *rest, 0, 0), ctypes.byref(size)))
+            found = self._keep(sig, ((B, H, K), (B, H, N), strides, rest, size.value))
+        kept_shape, shape, strides, rest, need = found
+        if into is not None and into.data_ptr() == block_table.data_ptr() and strides[2] == strides[3]:
+            return self.evict(block_table, lens, weights, keep, first, last)       # the same pages: in place
+        out_lens = lens.new_empty(shape[0])
+        kept, out_weights = lens.new_empty(kept_shape), weights.new_empty(shape)
+        ws = lens.new_empty(need // 4) if need else None
+        self._launch(self._lib.kitty_cache8_evict, _EVICT.pack(
+            weights.data_ptr(), *strides[:2], block_table.data_ptr(), strides[2], lens.data_ptr(),
+            0 if into is None else into.data_ptr(), strides[3], out_lens.data_ptr(), kept.data_ptr(), out_weights.data_ptr(),
+            *rest, 0 if ws is None else ws.data_ptr(), need))
+        return out_lens, kept, out_weights

@@ -96,7 +96,7 @@ def _tokens(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: 
 
 def _rows(q: torch.Tensor, codes, scales, causal: bool, sm_scale: float):
     """Attention of q (Hq, t, D) over tokens as _tokens has them, the queries their last:
-    (out, log-sum-exp, softmax weights (H, gq, t, n))."""
+    (out, log-sum-exp, softmax weights (H, gq, t, n), 0 where a row does not see a token)."""
     Hq, t, D = q.shape
     H, n, _ = codes[0].shape
     gq = Hq // H
@@ -112,12 +112,12 @@ def _rows(q: torch.Tensor, codes, scales, causal: bool, sm_scale: float):
     o = (w.view(H, gq * t, n) * scales[1]) @ codes[1].masked_fill(gone, 0.0)
     met = (sees.float().repeat(gq, 1) @ gone.float()) > 0
     o = o.masked_fill(met, math.nan).view(H, gq, t, D).masked_fill(none[:, None], 0.0)
-    return o.reshape(Hq, t, D), l.masked_fill(none, -math.inf).reshape(Hq, t), w
+    return o.reshape(Hq, t, D), l.masked_fill(none, -math.inf).reshape(Hq, t), w.masked_fill(~sees, 0.0)
 
 
 def attend(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch.Tensor, table: torch.Tensor,
            lens: torch.Tensor, q_lens: Optional[torch.Tensor], causal: bool, sm_scale: float, out: torch.Tensor,
-           lse: torch.Tensor) -> None:
+           lse: torch.Tensor, weights: Optional[torch.Tensor] = None) -> None:
     B, Hq, T, D = q.shape
     G = key.shape[2]
     q = q.float()       # a copy: out may be q
@@ -131,9 +131,12 @@ def attend(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch
             continue
         if n == 0 or t == 0:
             continue
-        o, l, _ = _rows(q[b, :, :t], *_tokens(key, value, scale, table[b], n), causal, sm_scale)
+        o, l, w = _rows(q[b, :, :t], *_tokens(key, value, scale, table[b], n), causal, sm_scale)
         out[b, :, :t] = o.to(out.dtype)
         lse[b, :, :t] = l
+        if weights is not None:
+            n = min(n, weights.shape[2])
+            weights[b, :, :n] += w[..., :n].sum((1, 2))
 
 
 def attend_shared(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q: torch.Tensor, prefix_table: torch.Tensor,
@@ -161,3 +164,46 @@ def attend_shared(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q
         o, l, _ = _rows(q[b, :, :t], codes, scales, causal, sm_scale)
         out[b, :, :t] = o.to(out.dtype)
         lse[b, :, :t] = l
+
+
+def evict(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+          weights: torch.Tensor, keep: int, first: int, last: int, into: torch.Tensor, out_lens: torch.Tensor,
+          kept: torch.Tensor, out_weights: torch.Tensor) -> None:
+    P, H, G, D = key.shape
+    N, K = weights.shape[2], kept.shape[2]
+    heads = torch.arange(H)[:, None]
+    kept.fill_(-1)
+    out_weights.zero_()
+    for b, n in enumerate(lens.tolist()):
+        if n < 0 or n > table.shape[1] * G or n > N:
+            out_lens[b] = -1
+            continue
+        m = out_lens[b] = min(n, keep)
+        at = torch.arange(n).expand(H, n)
+        if n > m:
+            between = weights[b, :, first:n - last].sort(dim=-1, descending=True, stable=True).indices[:, :m - first - last]
+            at = torch.cat([at[:, :first], first + between.sort(-1).values, at[:, n - last:]], 1)
+        kept[b, :, :m] = at
+        out_weights[b, :, :m] = weights[b].gather(1, at)
+        if m == 0:
+            continue
+        ids, ok = _page_ids(table[b:b + 1].expand(H, -1), at // G, P)
+        new, there = _page_ids(into[b:b + 1], torch.arange(-(-m // G))[None], P)
+        if P == 0:
+            continue
+        # all that moves is read before any of it is written
+        moved = []
+        for i, pool in enumerate((key, value)):
+            was = torch.where(ok, scale[ids, heads, i], torch.full(ids.shape, -1.0))
+            codes = torch.where(ok[..., None], pool.view(torch.uint8)[ids, heads, at % G], torch.tensor(0x7F, dtype=torch.uint8))
+            moved.append((was, codes))
+        for page, (p, there_) in enumerate(zip(new[0].tolist(), there[0].tolist())):
+            if not there_:
+                continue
+            for i, pool in enumerate((key, value)):
+                was, codes = (x[:, page * G:(page + 1) * G] for x in moved[i])
+                top = was.amax(1, keepdim=True)
+                top = torch.where(top < 0, torch.ones_like(top), top)
+                again = (codes.contiguous().view(E4M3).float() * (was / top)[..., None]).to(E4M3).view(torch.uint8)
+                pool.view(torch.uint8)[p, :, :codes.shape[1]] = torch.where(((was == top) | (was < 0))[..., None], codes, again)
+                scale[p, :, i] = top[:, 0]
