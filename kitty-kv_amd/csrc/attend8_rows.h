@@ -461,12 +461,14 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
                         make_float4(W.o[rt][4 * d4][i], W.o[rt][4 * d4 + 1][i], W.o[rt][4 * d4 + 2][i], W.o[rt][4 * d4 + 3][i]);
         }
         __syncthreads();
-        const bool whole = !SHARED && first && last_part;
-        const int slot = 2 * wg + (u == u0 ? 0 : 1);
+        const bool whole = first && last_part;
+        // a run may hold the whole of any number of items, and has a part of at most two others
+        const int slot = SHARED && whole ? 2 * p.n_wg + b * per_seq + item : 2 * wg + (u == u0 ? 0 : 1);
         const int rows = min(RM, (SHARED && sq.prefix ? p.gq * p.per : p.gq) * p.T - r0);
         if (!DIRECT && first && threadIdx.x == 0)
             p.ws_tab[b * per_seq + item] =
-                whole ? make_int2(-1, 0) : make_int2(slot, run_of(R.total, R.N, pre + (item + 1) * units - 1));
+                whole ? make_int2(SHARED ? slot : -1, SHARED ? -1 : 0)
+                      : make_int2(slot, run_of(R.total, R.N, pre + (item + 1) * units - 1));
         for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
             const int r = i / (DP / 4), ch = 4 * (i - r * (DP / 4));
             float m = kLowest, l = 0.0f;
@@ -484,7 +486,7 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
                 l += f * ml[w].y;
                 acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
             }
-            if (!whole) {
+            if (SHARED || !whole) {
                 *(float4 *)(p.ws_o + ((int64_t)slot * RM + r) * DP + ch) = acc;
                 if (ch == 0)
                     p.ws_ml[slot * RM + r] = make_float2(m, l);

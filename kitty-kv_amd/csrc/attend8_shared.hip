@@ -20,7 +20,7 @@ namespace kitty {
 struct Part8 {
     const float *o;
     const float2 *ml;
-    const int2 *tab;    // row kernel: by (entry, KV head)
+    const int2 *tab;    // row kernel, by (entry, KV head): first slot, last workgroup (-1: all in one slot)
     int e0, nrb, RM;    // its first entry, row blocks of an entry, rows of a block
     int splits, n_wg;   // parts of a row block (tile kernel; 0: row kernel), workgroups (row kernel)
 };
@@ -58,8 +58,8 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
         if (s.splits == 0) {
             const int2 tab = s.tab[item];
             // (bounds for lengths that another stream changes under the call)
-            slot = min(max(tab.x, 0), 2 * s.n_wg - 1), first = slot >> 1;
-            count = min(tab.y, s.n_wg - 1) - first + 1;
+            slot = min(max(tab.x, 0), tab.y < 0 ? 2 * s.n_wg + item : 2 * s.n_wg - 1), first = slot >> 1;
+            count = tab.y < 0 ? 1 : min(tab.y, s.n_wg - 1) - first + 1;
         }
         for (int i = ALONE ? group : 0; i < count; i += 4 * STEP) {
             float2 ml[4];
@@ -158,7 +158,7 @@ static int plan_shared(const Cache8 &c, const kitty_cache8_shared_args &a, Share
             if (units > 0x7fffffff)
                 return fail(KITTY_E_UNSUPPORTED, "too many rows and pages for one launch");
             la.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>((two_per_cu(pl.DP, la.RT) ? 2 : 1) * cus, units));
-            slots = 2 * la.n_wg;
+            slots = 2 * la.n_wg + items;
         }
         la.o_at = pl.bytes;
         la.ml_at = la.o_at + up16((size_t)slots * RM * pl.DP * 4);

@@ -52,6 +52,8 @@ SHAPES = [
     (1, 1, 1, 1, 1, 16, 16, [1], [0]), (1, 4, 8, 8, 1, 128, 128, [1000], [1, 40, 13, 0]), (2, 3, 4, 1, 1, 64, 16, [130, 0], [5, 0, 300, 1, 2, 0]),
     (3, 2, 4, 2, 3, 80, 32, [33, 64, 500], [3, 70, 2, 1, 40, 3]), (1, 11, 4, 1, 1, 128, 64, [777], [9 * b for b in range(11)]),
     (1, 16, 4, 1, 1, 128, 16, [300], [b % 3 for b in range(16)]), (1, 2, 16, 1, 1, 256, 32, [200], [0, 37]), (70, 1, 2, 1, 1, 32, 16, [(7 * f) % 90 for f in range(70)], [f % 40 for f in range(70)]),
+    # more entries than workgroups: runs that hold several whole ones
+    (200, 1, 16, 8, 1, 16, 16, [(5 * f) % 23 for f in range(200)], [f % 19 for f in range(200)]), (2, 150, 16, 8, 1, 16, 16, [70, 3], [(3 * b) % 40 for b in range(300)]),
     # the prefix in tiles, the sequences' own by rows
     (1, 17, 4, 1, 1, 128, 64, [700], [(31 * b) % 150 for b in range(17)]), (2, 40, 3, 1, 1, 64, 16, [150, 401], [b % 50 for b in range(80)]),
     (1, 9, 4, 1, 1, 256, 128, [600], [10] * 9), (1, 13, 5, 1, 3, 96, 32, [257], [3 + b for b in range(13)]), (3, 20, 4, 1, 1, 16, 256, [300, 0, 63], [b for b in range(60)]),
