@@ -37,7 +37,21 @@ struct Attend8 {
     const int32_t *prefix_table, *prefix_lens;
     int64_t pt_stride;
     int F, per, prefix_pages, e0, entries;
+    // For a second pass over the tokens: each row's maximum (log2 units) and 1 / sum, like
+    // lse; of kScores launches also the scores (log2 units, -inf where masked) of a KV
+    // head's up to 16 rows and sc_cap (a multiple of 16) tokens, (16 tokens, row, token).
+    float2 *stat;
+    float *scores;
+    int64_t sc_cap;
 };
+
+// What a row kernel does beside plain attention: nothing, leave all parts of prefixes and
+// sequences, leave the scores.
+constexpr int kPlain = 0, kShared = 1, kScores = 2;
+
+// kitty_cache8_attention that also leaves stat and, where given, the scores.
+int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, float2 *stat,
+            float *scores, int64_t sc_cap);
 
 constexpr int kTileRows = 128;   // query rows of the tile kernel's workgroup
 

@@ -82,6 +82,8 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
                    (uint32_t)f2x(o.z * inv, BF16) | (uint32_t)f2x(o.w * inv, BF16) << 16);
     if (ch == 0 && p.lse)
         p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
+    if (ch == 0 && p.stat)
+        p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
 }
 
 // Which kernel takes a call, by its sizes alone (rows: of a KV head, its group's
@@ -178,29 +180,10 @@ static int check_attend8(const kitty_cache8 *cache, const kitty_cache8_attention
     return KITTY_OK;
 }
 
-} // namespace kitty
-
-using namespace kitty;
-
-extern "C" int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
-                                                     size_t *bytes)
+int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, float2 *stat,
+            float *scores, int64_t sc_cap)
 {
-    Cache8 c;
-    Plan8 pl;
-    if (!bytes)
-        return fail(KITTY_E_INVALID, "bytes is NULL");
-    if (const int rc = check_attend8(cache, args, c))
-        return rc;
-    if (const int rc = plan8(c, *args, pl))
-        return rc;
-    *bytes = pl.bytes;
-    return KITTY_OK;
-}
-
-extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
-                                      kitty_stream_t stream)
-{
-    Attend8 p;
+    Attend8 p{};
     Plan8 pl;
     if (const int rc = check_attend8(cache, args, p.c))
         return rc;
@@ -229,7 +212,8 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
     char *ws = (char *)a.workspace;
     p.ws_o = (float *)ws, p.ws_ml = (float2 *)(ws + pl.o_bytes), p.ws_tab = (int2 *)(ws + pl.o_bytes + pl.ml_bytes);
 
-    const hipStream_t st = (hipStream_t)stream;
+    p.stat = stat, p.scores = scores, p.sc_cap = sc_cap;
+    const hipStream_t st = stream;
     const bool bf16 = a.dtype == KITTY_DTYPE_BF16;
     const dim3 block(64 * kWaves);
     auto merge = [&](auto dp, auto bf, auto tiles) {
@@ -249,18 +233,35 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
         constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
         constexpr bool BF = decltype(bf)::value;
         const dim3 pairs((unsigned)(p.B * p.c.H * p.nrb)), runs((unsigned)p.n_wg), waves(64 * row_waves(RT, true));
+        if constexpr (RT == 1) {
+            if (scores) {
+                if constexpr (DP <= 128) {
+                    if (pl.direct && p.c.D == DP)
+                        hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true, kScores>), pairs, waves, 0, st, p);
+                    else if (pl.direct)
+                        hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true, kScores>), pairs, waves, 0, st, p);
+                    if (pl.direct)
+                        return;
+                }
+                if (p.c.D == DP)
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, false, kScores>), runs, block, 0, st, p);
+                else
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, false, kScores>), runs, block, 0, st, p);
+                return;
+            }
+        }
         if constexpr (DP <= 128 && RT <= 2) {
             if (pl.direct && p.c.D == DP)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true, false>), pairs, waves, 0, st, p);
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true, kPlain>), pairs, waves, 0, st, p);
             else if (pl.direct)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true, false>), pairs, waves, 0, st, p);
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true, kPlain>), pairs, waves, 0, st, p);
             if (pl.direct)
                 return;
         }
         if (p.c.D == DP)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, false, false>), runs, block, 0, st, p);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, false, kPlain>), runs, block, 0, st, p);
         else
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, false, false>), runs, block, 0, st, p);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, false, kPlain>), runs, block, 0, st, p);
     };
     auto go = [&](auto dp, auto bf) {
         constexpr int DP = decltype(dp)::value;
@@ -296,4 +297,29 @@ extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cac
     else
         by_type(std::integral_constant<int, 256>{});
     return check_launch("8-bit cache attention");
+}
+
+} // namespace kitty
+
+using namespace kitty;
+
+extern "C" int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
+                                                     size_t *bytes)
+{
+    Cache8 c;
+    Plan8 pl;
+    if (!bytes)
+        return fail(KITTY_E_INVALID, "bytes is NULL");
+    if (const int rc = check_attend8(cache, args, c))
+        return rc;
+    if (const int rc = plan8(c, *args, pl))
+        return rc;
+    *bytes = pl.bytes;
+    return KITTY_OK;
+}
+
+extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
+                                      kitty_stream_t stream)
+{
+    return attend8(cache, args, (hipStream_t)stream, nullptr, nullptr, 0);
 }

@@ -92,8 +92,12 @@ __device__ __forceinline__ u32x4 value_operand(const unsigned (&v)[8][DP / 64], 
 
 // 32 tokens from `tok` on, in `buf`, folded into the wave's rows.  mask: some
 // row may not see all of them.
-template <int DP, int RT, bool BF16>
-__device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &buf, int tok, int vis_max, float cs, int g, bool mask)
+// SCORES: they also go to `out`, at byte `at` plus `step` for every 16 tokens; beyond its
+// end (lanes without a row, tokens that have no weight) the store itself drops them: a
+// branch around it would make every wait one for all loads.
+template <int DP, int RT, bool BF16, bool SCORES>
+__device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &buf, int tok, int vis_max, float cs, int g, bool mask,
+                                         __amdgpu_buffer_rsrc_t out, uint32_t at, uint32_t step)
 {
     f32x4 S[RT][2];
 #pragma unroll
@@ -137,6 +141,14 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 s[e] = tok + 16 * (e >> 2) + 4 * g + (e & 3) < W.vis[rt] ? s[e] : -__builtin_inff();
+        if constexpr (SCORES) {
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+                __builtin_amdgcn_raw_buffer_store_b128(
+                    u32x4{__builtin_bit_cast(unsigned, s[4 * hf]), __builtin_bit_cast(unsigned, s[4 * hf + 1]),
+                          __builtin_bit_cast(unsigned, s[4 * hf + 2]), __builtin_bit_cast(unsigned, s[4 * hf + 3])},
+                    out, at + hf * step, 0, 0);
+        }
         float mx = s[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e)
@@ -296,11 +308,12 @@ constexpr bool two_per_cu(int DP, int RT) { return DP <= 128 && DP * RT <= 256; 
 
 // CUT: D is below DP, and the lanes beyond it read nothing.  DIRECT: a workgroup takes
 // the whole of one (pair, row block) and writes its rows, so that no merge follows.
-// SHARED: the entries are prefixes and sequences, of one row block each, and all parts
-// are left to cache8_join_kernel.
-template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, bool SHARED>
+// MODE kShared: the entries are prefixes and sequences, of one row block each, and all
+// parts are left to cache8_join_kernel.
+template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
 __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 : two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
 {
+    constexpr bool SHARED = MODE == kShared, SCORES = MODE == kScores;
     constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NW = row_waves(RT, DIRECT), NB = NW == 16 ? 1 : 2, STRIDE = 32 * NW;
     __shared__ __attribute__((aligned(16))) float lds_o[NW][RM][LD];
     __shared__ float2 lds_ml[NW][RM];
@@ -417,6 +430,11 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
                                          bad ? 1.0f : __builtin_bit_cast(float, (uint32_t)(sc >> 32)));   // page 0's may be no number
             }
         };
+        // a KV head's scores are at most 1 GiB
+        const int rows_all = p.gq * p.T;
+        const uint32_t sc_step = 64 * rows_all, sc_bytes = SCORES ? (uint32_t)(p.sc_cap * rows_all * 4) : 0;
+        const __amdgpu_buffer_rsrc_t scores = __builtin_amdgcn_make_buffer_rsrc(
+            SCORES ? (void *)(p.scores + (int64_t)(b * p.c.H + kh) * rows_all * p.sc_cap) : nullptr, 0, sc_bytes, 0x00027000);
         // A ring of NB steps' codes, NB - 1 in flight while one is computed; the page
         // ids of the next load are fetched a step before it.  Loads past the wave's
         // last step repeat that step's: a branch around them would make every wait
@@ -440,7 +458,9 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
                         break;
                     load(min(tok + (NB - 1) * STRIDE, final), id[NB - 1], ring[(j + NB - 1) % NB]);
                     ids(min(tok + NB * STRIDE, final), id[NB - 1]);
-                    row_step<DP, RT, BF16>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min);
+                    row_step<DP, RT, BF16, SCORES>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min, scores,
+                                                   SCORES && n < rows_all && tok < p.sc_cap ? (uint32_t)(tok >> 4) * sc_step + 64 * n + 16 * g : 1u << 31,
+                                                   sc_step);
                     tok += STRIDE;
                     more = tok < end;
                 }
@@ -504,6 +524,8 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
             if (ch == 0 && p.lse)
                 p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
                     sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
+            if (ch == 0 && p.stat)
+                p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
         }
         if constexpr (DIRECT)
             return;

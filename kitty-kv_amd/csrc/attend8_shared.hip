@@ -281,14 +281,14 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
         }
         const dim3 runs((unsigned)la.n_wg);
         if (la.RT == 1)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, 1, BF, CUT, false, true>), runs, block, 0, st, x);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, 1, BF, CUT, false, kShared>), runs, block, 0, st, x);
         else if (la.RT == 2)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, 2, BF, CUT, false, true>), runs, block, 0, st, x);
+            hipLaunchKernelGGL((cache8_rows_kernel<DP, 2, BF, CUT, false, kShared>), runs, block, 0, st, x);
         else if constexpr (DP <= 128) {
             if (la.RT == 3)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, 3, BF, CUT, false, true>), runs, block, 0, st, x);
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, 3, BF, CUT, false, kShared>), runs, block, 0, st, x);
             else
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, 4, BF, CUT, false, true>), runs, block, 0, st, x);
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, 4, BF, CUT, false, kShared>), runs, block, 0, st, x);
         }
     };
     auto go = [&](auto dp, auto bf, auto cut) {

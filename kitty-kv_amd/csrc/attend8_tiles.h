@@ -480,6 +480,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
     if (g == 0 && p.lse)
         p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
             sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (W.m + __builtin_log2f(l)) / kLog2e;
+    if (g == 0 && p.stat)
+        p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(W.m, inv);
 }
 
 } // namespace kitty

@@ -2,17 +2,19 @@
 // and KV head stay, and their move together.
 //
 // cache8_select_kernel, a workgroup per (sequence, KV head): the weights between the
-// first and last tokens, which stay, map to unsigned keys in the floats' order (both
-// zeros alike, NaN above all); four passes over 8 bits each, counted in LDS, find the
-// key of the lightest token that stays and how many of its equals do.  One more pass
-// writes positions and weights in order: a token's place is the count of heavier ones
-// before it plus that of its equals, as far as they stay.  Counts are integers: any
-// order of additions gives the same.
+// first and last tokens, which stay, map to unsigned keys in the floats' order; three passes over 11, 11 and 10 bits, counted in LDS, find
+// the key of the lightest token that stays and how many of its equals do.  Positions and
+// weights are written in order: a token's place is the count of heavier ones before it
+// plus that of its equals, as far as they stay, by ballots of a wave over its run of
+// tokens and the waves' counts.  Counts are integers: any order of additions gives the
+// same.
 // cache8_pack_kernel, a workgroup per (page, KV head, stream) of the result: the page's
 // scale is the largest of the pages that its tokens come from, and codes of smaller
 // scales are multiplied by the quotient and rounded again (exact but for subnormals
 // where scales are powers of two).  In place the codes go through the workspace, as a
 // page of the result may hold tokens that another page of the result needs.
+#include <algorithm>
+
 #include "cache8.h"
 
 namespace kitty {
@@ -33,12 +35,15 @@ struct Evict8 {
     int B, N, K, keep, first, last, table_pages, into_pages, tiles;
 };
 
-constexpr int kSelect = 1024;
+constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
+constexpr int kBins = 2048, kCopies = 4;   // counters of a pass; copies, so that fewer lanes meet at one
 
+// A weight as an unsigned key in the floats' order: both zeros alike, NaN above all.  0
+// and 0xffffffff are no weight's: of places behind the sequence and of tokens that stay.
 __device__ __forceinline__ uint32_t weight_key(float x)
 {
     const uint32_t u = x == 0.0f ? 0u : __builtin_bit_cast(uint32_t, x);
-    return x != x ? 0xffffffffu : u >> 31 ? ~u : u | 0x80000000u;
+    return x != x ? 0xfffffffeu : u >> 31 ? ~u : u | 0x80000000u;
 }
 
 // Tokens of sequence b that stay, -1 where its length breaks the rules.
@@ -47,11 +52,40 @@ __device__ __forceinline__ int kept8(const Evict8 &p, int n)
     return n < 0 || n > (int64_t)p.table_pages << p.c.lg || n > p.N ? -1 : min(n, p.keep);
 }
 
+// The sum of a value over the lanes up to this one.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned add_dpp(unsigned v)
+{
+    return v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ unsigned scan64(unsigned v)
+{
+    v = add_dpp<0x111, 0xf>(v);   // row_shr 1, 2, 4, 8
+    v = add_dpp<0x112, 0xf>(v);
+    v = add_dpp<0x114, 0xf>(v);
+    v = add_dpp<0x118, 0xf>(v);
+    v = add_dpp<0x142, 0xa>(v);   // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+    return add_dpp<0x143, 0xc>(v);
+}
+
+// The sum of the waves' values before this one's.
+__device__ __forceinline__ unsigned sum_before(const unsigned *v, int wave)
+{
+    unsigned s = 0;
+#pragma unroll
+    for (int k = 0; k < kSelectWaves; ++k)
+        s += k < wave ? v[k] : 0;
+    return s;
+}
+
+// A wave takes a run of 64 j tokens; EACH: j at most, the weights then stay in registers
+// (0: any j, they are read again in every pass).
+template <int EACH>
 __global__ __launch_bounds__(kSelect) void cache8_select_kernel(Evict8 p)
 {
-    __shared__ unsigned hist[256], sums[kSelect / 64];
+    __shared__ __attribute__((aligned(16))) unsigned hist[kCopies][kBins], sums[2][kSelectWaves];
     __shared__ unsigned found[2];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int b = blockIdx.x / p.c.H, h = blockIdx.x - b * p.c.H;
     const int n = p.lens[b], m = kept8(p, n);
     const float *w = p.weights + b * p.w_s_seq + h * p.w_s_head;
@@ -59,89 +93,94 @@ __global__ __launch_bounds__(kSelect) void cache8_select_kernel(Evict8 p)
     float *out = p.out_weights + (int64_t)blockIdx.x * p.N;
     if (h == 0 && tid == 0)
         p.out_lens[b] = m;
-    // tokens lo .. hi - 1 may go, `need` of them stay
-    int lo = 0, hi = 0, need = 0;
-    uint32_t key = 0;          // of the lightest that stays: all above it do, and `need` of its equals
-    if (m >= 0 && n > m) {
-        lo = p.first, hi = n - p.last, need = m - p.first - p.last;
-        if (need > 0) {
-            for (int shift = 24; shift >= 0; shift -= 8) {
-                const uint32_t above = shift == 24 ? 0u : ~0u << (shift + 8);
-                if (tid < 256)
-                    hist[tid] = 0;
-                __syncthreads();
-                for (int i = lo + tid; i < hi; i += kSelect) {
-                    const uint32_t k = weight_key(w[i]);
-                    if (((k ^ key) & above) == 0)
-                        atomicAdd(&hist[k >> shift & 255], 1u);
-                }
-                __syncthreads();
-                if (wave == 0) {
-                    // from the heaviest: lane l has bins 255 - 4 l .. 252 - 4 l
-                    unsigned c[4], all = 0;
+    const int end = m < 0 ? 0 : n, last = end - p.last;
+    const int steps = (end + kSelect - 1) / kSelect;           // of 64 tokens, a wave
+    const int pos0 = wave * steps * 64 + lane;
+    auto key_at = [&](int i, float v) { return i >= end ? 0u : i < p.first || i >= last ? 0xffffffffu : weight_key(v); };
+    float x[EACH > 0 ? EACH : 1];
+    uint32_t keys[EACH > 0 ? EACH : 1];
+    if constexpr (EACH > 0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        all += c[j] = hist[255 - 4 * lane - j];
-                    unsigned inc = all;
+        for (int j = 0; j < EACH; ++j)
+            x[j] = pos0 + 64 * j < end && j < steps ? w[pos0 + 64 * j] : 0.0f;
 #pragma unroll
-                    for (int off = 1; off < 64; off <<= 1) {
-                        const unsigned y = __shfl_up(inc, off);
-                        inc += lane >= off ? y : 0;
-                    }
-                    unsigned before = inc - all;
+        for (int j = 0; j < EACH; ++j)
+            keys[j] = j < steps ? key_at(pos0 + 64 * j, x[j]) : 0;
+    }
+    auto each = [&](auto body) {
+        if constexpr (EACH > 0) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        if (before < (unsigned)need && before + c[j] >= (unsigned)need)
-                            found[0] = 255 - 4 * lane - j, found[1] = need - before;
-                        before += c[j];
-                    }
-                }
-                __syncthreads();
-                key |= found[0] << shift;
-                need = (int)found[1];
+            for (int j = 0; j < EACH; ++j)
+                if (j < steps)
+                    body(pos0 + 64 * j, x[j], keys[j]);
+        } else {
+            for (int j = 0; j < steps; ++j) {
+                const int i = pos0 + 64 * j;
+                const float v = i < end ? w[i] : 0.0f;
+                body(i, v, key_at(i, v));
             }
         }
+    };
+    uint32_t key = 0;          // tokens above it stay, and `need` of its equals
+    int need = 0;
+    if (n > m && m > 0) {
+        need = m;
+        // 11, 11 and 10 bits: signs, exponents and two bits of the fraction first
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t above = pass == 0 ? 0u : ~0u << (pass == 1 ? 21 : 10), bins = pass == 2 ? 1023 : 2047;
+            for (int i = tid; i < kCopies * kBins / 4; i += kSelect)
+                ((u32x4 *)hist)[i] = u32x4{0, 0, 0, 0};
+            __syncthreads();
+            each([&](int, float, uint32_t k) {
+                if (((k ^ key) & above) == 0 && k != 0)
+                    atomicAdd(&hist[wave & (kCopies - 1)][k >> shift & bins], 1u);
+            });
+            __syncthreads();
+            // from the heaviest: thread t has bins 2047 - 2 t and 2046 - 2 t
+            unsigned c[2] = {0, 0};
+#pragma unroll
+            for (int k = 0; k < kCopies; ++k) {
+                const uint2 two = *(const uint2 *)&hist[k][kBins - 2 - 2 * tid];
+                c[0] += two.y, c[1] += two.x;
+            }
+            const unsigned inc = scan64(c[0] + c[1]);
+            if (lane == 63)
+                sums[0][wave] = inc;
+            __syncthreads();
+            unsigned before = inc - c[0] - c[1] + sum_before(sums[0], wave);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (before < (unsigned)need && before + c[e] >= (unsigned)need)
+                    found[0] = kBins - 1 - 2 * tid - e, found[1] = need - before;
+                before += c[e];
+            }
+            __syncthreads();
+            key |= found[0] << shift;
+            need = (int)found[1];
+        }
+    } else if (m == 0) {
+        key = 0xffffffffu;     // none stays (first and last are 0)
     }
-    // positions in order: low halves count tokens that stay whatever the others are, high halves equals of `key`
-    const int end = max(m < 0 ? 0 : n, 0);
-    int sure = 0, equal = 0;
-    const bool some = need > 0;
-    for (int i0 = 0; i0 < end; i0 += kSelect) {
-        const int i = i0 + tid;
-        float x = 0.0f;
-        bool stays = false, same = false;
-        if (i < end) {
-            x = w[i];
-            const uint32_t k = weight_key(x);
-            const bool may_go = i >= lo && i < hi;
-            stays = !may_go || (some && k > key);
-            same = may_go && some && k == key;
-        }
-        const unsigned mine = (stays ? 1u : 0u) | (same ? 0x10000u : 0u);
-        unsigned inc = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const unsigned y = __shfl_up(inc, off);
-            inc += lane >= off ? y : 0;
-        }
-        if (lane == 63)
-            sums[wave] = inc;
-        __syncthreads();
-        unsigned before = inc - mine, total = 0;
-#pragma unroll
-        for (int k = 0; k < kSelect / 64; ++k) {
-            before += k < wave ? sums[k] : 0;
-            total += sums[k];
-        }
-        __syncthreads();
-        const int e = equal + (int)(before >> 16);
-        if (stays || (same && e < need)) {
-            const int at = sure + (int)(before & 0xffff) + min(e, need);
+    int n_above = 0, n_same = 0;
+    each([&](int, float, uint32_t k) {
+        n_above += __popcll(__ballot(k > key));
+        n_same += __popcll(__ballot(k == key));
+    });
+    if (lane == 0)
+        sums[0][wave] = n_above, sums[1][wave] = n_same;
+    __syncthreads();
+    n_above = (int)sum_before(sums[0], wave), n_same = (int)sum_before(sums[1], wave);   // of the waves before this one
+    each([&](int i, float v, uint32_t k) {
+        const uint64_t a = __ballot(k > key), c = __ballot(k == key);
+        const int e = n_same + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(c >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)c, 0));
+        if (k > key || (k == key && e < need)) {
+            const int at = n_above + (int)__builtin_amdgcn_mbcnt_hi((unsigned)(a >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)a, 0)) + min(e, need);
             kept[at] = i;
-            out[at] = x;
+            out[at] = v;
         }
-        sure += (int)(total & 0xffff), equal += (int)(total >> 16);
-    }
+        n_above += __popcll(a), n_same += __popcll(c);
+    });
     for (int i = max(m, 0) + tid; i < p.N; i += kSelect)
         out[i] = 0.0f;
     for (int i = max(m, 0) + tid; i < p.K; i += kSelect)
@@ -314,7 +353,14 @@ extern "C" int kitty_cache8_evict(const kitty_cache8 *cache, const kitty_cache8_
     p.ws_scale = (float *)((char *)a.workspace + up16((size_t)p.B * p.c.H * 2 * p.K * p.c.D));
     const hipStream_t st = (hipStream_t)stream;
     const unsigned pairs = (unsigned)(p.B * p.c.H);
-    hipLaunchKernelGGL(cache8_select_kernel, dim3(pairs), dim3(kSelect), 0, st, p);
+    // by what a sequence can hold: 8 or 32 weights a lane in registers
+    const int64_t cap = std::min<int64_t>((int64_t)p.table_pages << p.c.lg, p.N);
+    if (cap <= 8 * kSelect)
+        hipLaunchKernelGGL(cache8_select_kernel<8>, dim3(pairs), dim3(kSelect), 0, st, p);
+    else if (cap <= 32 * kSelect)
+        hipLaunchKernelGGL(cache8_select_kernel<32>, dim3(pairs), dim3(kSelect), 0, st, p);
+    else
+        hipLaunchKernelGGL(cache8_select_kernel<0>, dim3(pairs), dim3(kSelect), 0, st, p);
     if (p.K > 0) {
         if (!a.into) {
             const int rows = 256 / (p.c.D >> 4);
