@@ -37,6 +37,11 @@ struct Attend8 {
     const int32_t *prefix_table, *prefix_lens;
     int64_t pt_stride;
     int F, per, prefix_pages, e0, entries;
+    int own_nrb, item0;   // row blocks of a sequence's own rows in tiles, the number of their first item
+    // Padded queries of SHARED launches, or NULL: a prefix's real queries by their number
+    // (sequence of the prefix times T plus query), how many each prefix has, and the
+    // number of each sequence's first.
+    int32_t *row_map, *row_count, *row_first;
     // For a second pass over the tokens: each row's maximum (log2 units) and 1 / sum, like
     // lse; of kScores launches also the scores (log2 units, -inf where masked) of a KV
     // head's up to 16 rows and sc_cap (a multiple of 16) tokens, (16 tokens, row, token).
@@ -119,6 +124,15 @@ __device__ __forceinline__ int visible8(const Attend8 &p, const Seq8 &s, int t)
     return p.causal ? max(s.n - s.tq + t + 1, 0) : s.n;
 }
 
+// Query rows of an entry and KV head.
+template <bool SHARED>
+__device__ __forceinline__ int rows8(const Attend8 &p, const Seq8 &s, int i)
+{
+    if (SHARED && s.prefix)
+        return p.gq * (p.row_map ? p.row_count[p.e0 + i] : p.per * p.T);
+    return p.gq * p.T;
+}
+
 // Query row r of an entry and KV head: sequence, head and token, whether there is such a
 // row, and the entry's tokens that it sees.
 struct Row8 {
@@ -136,9 +150,12 @@ __device__ __forceinline__ Row8 row8(const Attend8 &p, const Seq8 &s, int i, int
     if constexpr (SHARED) {
         w.b = p.e0 + i - p.F;
         if (s.prefix) {
+            const int f = p.e0 + i;
+            if (p.row_map)
+                w.t = w.t < p.row_count[f] ? p.row_map[(int64_t)f * p.per * p.T + w.t] : p.per * p.T;
             const int q = w.t / p.T;
             w.t -= q * p.T;
-            w.b = (p.e0 + i) * p.per + q;
+            w.b = f * p.per + q;
             w.real = false, w.vis = 0;
             if (!s.bad && q < p.per) {
                 // rows that are tokens of the prefix itself see it up to themselves

@@ -247,9 +247,9 @@ __device__ __forceinline__ int run_of(int total, int N, int u)
 }
 
 template <bool SHARED>
-__device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
+__device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R, int wg, int n_wg)
 {
-    const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb, wg = blockIdx.x;
+    const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb;
     const int B = SHARED ? p.entries : p.B;
     // 64 sequences at a time: tiles of each, units of each and the sum up to it
     auto tiles = [&](int b0) { return b0 + lane < B ? tiles8(entry8<SHARED>(p, b0 + lane)) : 0; };
@@ -266,7 +266,7 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
     // equal sequences whose pairs the workgroups divide evenly: no run begins a second one
     int t = tiles(0);
     const int each = __builtin_amdgcn_readlane(t, 0), items = B * per_seq;
-    const int N0 = (int)min((int64_t)p.n_wg, (int64_t)each * items);
+    const int N0 = (int)min((int64_t)n_wg, (int64_t)each * items);
     R.start = kStart;
     if (B <= 64 && N0 > 0 && N0 % items == 0 && !__ballot(lane < B && t != each))
         R.start = 0;
@@ -276,7 +276,7 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R)
         total += __builtin_amdgcn_readlane(sums(tiles(b0), y), 63);
     }
     R.total = total;
-    R.N = min(p.n_wg, total);
+    R.N = min(n_wg, total);
     if (wg >= R.N)
         return false;
     R.u = run_start(total, R.N, wg);
@@ -310,22 +310,30 @@ constexpr bool two_per_cu(int DP, int RT) { return DP <= 128 && DP * RT <= 256; 
 // the whole of one (pair, row block) and writes its rows, so that no merge follows.
 // MODE kShared: the entries are prefixes and sequences, of one row block each, and all
 // parts are left to cache8_join_kernel.
+//
+// Workgroup wg of the n_wg that share the work.
+template <int DP, int RT, bool DIRECT>
+struct RowLds {
+    float o[row_waves(RT, DIRECT)][16 * RT][DP + 4];
+    float2 ml[row_waves(RT, DIRECT)][16 * RT];
+};
+
 template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
-__global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 : two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
+__device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, RowLds<DP, RT, DIRECT> &lds)
 {
     constexpr bool SHARED = MODE == kShared, SCORES = MODE == kScores;
-    constexpr int RM = 16 * RT, CB = DP / 16, LD = DP + 4, NW = row_waves(RT, DIRECT), NB = NW == 16 ? 1 : 2, STRIDE = 32 * NW;
-    __shared__ __attribute__((aligned(16))) float lds_o[NW][RM][LD];
-    __shared__ float2 lds_ml[NW][RM];
+    constexpr int RM = 16 * RT, CB = DP / 16, NW = row_waves(RT, DIRECT), NB = NW == 16 ? 1 : 2, STRIDE = 32 * NW;
+    auto &lds_o = lds.o;
+    auto &lds_ml = lds.ml;
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int per_seq = p.c.H * p.nrb, wg = blockIdx.x;
+    const int per_seq = p.c.H * p.nrb;
     Run8 R;
     if constexpr (DIRECT) {
         R.b = wg / per_seq;
         R.pre = 0, R.start = 0, R.u = wg - R.b * per_seq, R.u1 = R.u + 1;
     } else {
-        if (!find_run<SHARED>(p, R))
+        if (!find_run<SHARED>(p, R, wg, n_wg))
             return;
     }
     const int u0 = R.u, u1 = R.u1;
@@ -484,7 +492,7 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
         const bool whole = first && last_part;
         // a run may hold the whole of any number of items, and has a part of at most two others
         const int slot = SHARED && whole ? 2 * p.n_wg + b * per_seq + item : 2 * wg + (u == u0 ? 0 : 1);
-        const int rows = min(RM, (SHARED && sq.prefix ? p.gq * p.per : p.gq) * p.T - r0);
+        const int rows = min(RM, rows8<SHARED>(p, sq, b) - r0);
         if (!DIRECT && first && threadIdx.x == 0)
             p.ws_tab[b * per_seq + item] =
                 whole ? make_int2(SHARED ? slot : -1, SHARED ? -1 : 0)
@@ -532,6 +540,13 @@ __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 :
         __syncthreads();
         u += seg;
     }
+}
+
+template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
+__global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 : two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
+{
+    __shared__ __attribute__((aligned(16))) RowLds<DP, RT, DIRECT> lds;
+    rows_run<DP, RT, BF16, CUT, DIRECT, MODE>(p, blockIdx.x, p.n_wg, lds);
 }
 
 } // namespace kitty

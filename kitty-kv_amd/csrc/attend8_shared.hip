@@ -7,10 +7,15 @@
 // with M the largest m, sum 2^(m - M) o / sum 2^(m - M) l.  cache8_join_kernel does that
 // for the parts of both entries at once.
 //
-// Up to 64 rows of a prefix (32 at more than 128 channels) its entries and the
-// sequences' go through the row kernel together (attend8_rows.h): one launch shares the
-// units of all entries evenly.  More rows go through the tile kernel (attend8_tiles.h),
-// and the sequences' own tokens through whichever takes their rows.
+// Few rows of a prefix: its entries and the sequences' go through the row kernel together
+// (attend8_rows.h), whose one launch shares the units of all entries evenly.
+// More: cache8_shared_kernel, one launch for both kinds of work.  Some workgroups share
+// the prefixes' tiles (attend8_tiles.h), bound by the matrix cores and the softmax, the
+// others the sequences' own tokens, by the row kernel's body and bound by HBM; each kind
+// is cut evenly by lengths read on the device, and so are the workgroups between them.
+// The first half of a launch fills every CU once and the second half again, so that in
+// the middle of the range a CU holds one of each.  Sequences with more rows than the row
+// kernel's body takes go through tiles as well.
 #include "attend8_rows.h"
 #include "attend8_tiles.h"
 
@@ -20,9 +25,9 @@ namespace kitty {
 struct Part8 {
     const float *o;
     const float2 *ml;
-    const int2 *tab;    // row kernel, by (entry, KV head): first slot, last workgroup (-1: all in one slot)
-    int e0, nrb, RM;    // its first entry, row blocks of an entry, rows of a block
-    int splits, n_wg;   // parts of a row block (tile kernel; 0: row kernel), workgroups (row kernel)
+    const int2 *tab;        // by item: first slot, last workgroup (-1: all in one slot)
+    int e0, nrb, RM, n_wg;  // its first entry, row blocks of an entry, rows of a block, workgroups
+    int item0;              // the first entry's first item
 };
 
 // Joins the parts of each row, of its prefix and of its own tokens.  DP / 4 lanes take a
@@ -52,23 +57,19 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
     };
     auto parts = [&](const Part8 &s, int e, int r, int tokens) {
         if (tokens <= 0)
-            return;   // the row kernel left nothing of it
-        const int rb = r / s.RM, rr = r - rb * s.RM, item = ((e - s.e0) * p.c.H + kh) * s.nrb + rb;
-        int slot = 0, first = 0, count = s.splits;
-        if (s.splits == 0) {
-            const int2 tab = s.tab[item];
-            // (bounds for lengths that another stream changes under the call)
-            slot = min(max(tab.x, 0), tab.y < 0 ? 2 * s.n_wg + item : 2 * s.n_wg - 1), first = slot >> 1;
-            count = tab.y < 0 ? 1 : min(tab.y, s.n_wg - 1) - first + 1;
-        }
+            return;   // nothing is left of it
+        const int rb = r / s.RM, rr = r - rb * s.RM, item = s.item0 + ((e - s.e0) * p.c.H + kh) * s.nrb + rb;
+        const int2 tab = s.tab[item];
+        // (bounds for lengths that another stream changes under the call)
+        const int slot = min(max(tab.x, 0), tab.y < 0 ? 2 * s.n_wg + item : 2 * s.n_wg - 1), first = slot >> 1;
+        const int count = tab.y < 0 ? 1 : min(tab.y, s.n_wg - 1) - first + 1;
         for (int i = ALONE ? group : 0; i < count; i += 4 * STEP) {
             float2 ml[4];
             float4 x[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int k = min(i + j * STEP, count - 1);
-                const int64_t at = s.splits ? ((int64_t)item * s.splits + k) * s.RM + rr
-                                            : (int64_t)(k == 0 ? slot : 2 * (first + k)) * s.RM + rr;
+                const int64_t at = (int64_t)(k == 0 ? slot : 2 * (first + k)) * s.RM + rr;
                 ml[j] = s.ml[at];
                 x[j] = *(const float4 *)(s.o + at * DP + ch);
             }
@@ -78,8 +79,9 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
                     fold(ml[j].x, ml[j].y, x[j]);
         }
     };
-    if (!bad) {
-        parts(of_prefix, f, (b - f * p.per) * rows + row, before);
+    if (!bad && t < own.tq) {
+        const int q = p.row_map ? p.row_first[b] + t : (b - f * p.per) * p.T + t;
+        parts(of_prefix, f, q * p.gq + h - kh * p.gq, before);
         parts(of_own, p.F + b, row, own.n);
     }
     if constexpr (ALONE) {
@@ -110,18 +112,178 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
             bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
 }
 
-// One launch over entries e0 .. e0 + entries - 1, and its part of the workspace.
-struct Launch8 {
-    bool tiles;
-    int RT, e0, entries, nrb, n_wg, splits;
-    size_t o_at, ml_at, tab_at;
+// The prefixes' real queries where they are padded, a wave per prefix.
+__global__ __launch_bounds__(64 * kWaves) void cache8_shared_queries_kernel(Attend8 p)
+{
+    const int lane = threadIdx.x & 63, f = blockIdx.x * kWaves + (threadIdx.x >> 6);
+    if (f >= p.F)
+        return;
+    int count = 0;
+    int32_t *map = p.row_map + (int64_t)f * p.per * p.T;
+    for (int q0 = 0; q0 < p.per; q0 += 64) {
+        int mine = 0;
+        if (q0 + lane < p.per) {
+            const Seq8 own = seq8(p, f * p.per + q0 + lane);
+            mine = own.bad ? 0 : own.tq;
+        }
+        int inc = mine;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int y = __shfl_up(inc, off);
+            inc += lane >= off ? y : 0;
+        }
+        if (q0 + lane < p.per)
+            p.row_first[f * p.per + q0 + lane] = count + inc - mine;
+        for (int q = 0; q < min(64, p.per - q0); ++q) {
+            const int n = __builtin_amdgcn_readlane(mine, q), first = count + __builtin_amdgcn_readlane(inc, q) - n;
+            for (int t = lane; t < n; t += 64)
+                map[first + t] = (q0 + q) * p.T + t;
+        }
+        count += __builtin_amdgcn_readlane(inc, 63);
+    }
+    if (lane == 0)
+        p.row_count[f] = count;
+}
+
+// Units of tiles: kTile tokens for kTileRows rows, and kTileStart for what beginning an
+// item costs.
+constexpr int kTileStart = 2;
+
+struct Entry8 {
+    Seq8 sq;
+    int nrb, tiles, units;   // row blocks, tiles and units of an item
 };
 
+__device__ __forceinline__ Entry8 tile_entry(const Attend8 &p, int i)
+{
+    Entry8 e;
+    e.sq = entry8<true>(p, i);
+    e.nrb = (rows8<true>(p, e.sq, i) + kTileRows - 1) / kTileRows;
+    e.tiles = e.sq.bad ? 0 : (e.sq.n + kTile - 1) / kTile;
+    e.units = e.tiles && e.nrb ? e.tiles + kTileStart : 0;
+    return e;
+}
+
+// The sum over the lanes up to this one.
+__device__ __forceinline__ int lanes_sum(int v, int lane)
+{
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const int y = __shfl_up(v, off);
+        v += lane >= off ? y : 0;
+    }
+    return v;
+}
+
+// All units of a launch's tile entries, and of its row entries.
+__device__ __forceinline__ int tile_units(const Attend8 &p)
+{
+    const int lane = threadIdx.x & 63;
+    int sum = 0;
+    for (int i = lane; i < p.entries; i += 64) {
+        const Entry8 e = tile_entry(p, i);
+        sum += e.units * e.nrb * p.c.H;
+    }
+    return __builtin_amdgcn_readlane(lanes_sum(sum, lane), 63);
+}
+
+__device__ __forceinline__ int row_units(const Attend8 &p)
+{
+    const int lane = threadIdx.x & 63;
+    int sum = 0;
+    for (int i = lane; i < p.entries; i += 64)
+        sum += units8(tiles8(entry8<true>(p, i)), kStart) * p.c.H;
+    return __builtin_amdgcn_readlane(lanes_sum(sum, lane), 63);
+}
+
+// Workgroup wg of n_wg's run of the `total` units of the tile entries, by item: KV head
+// slowest, then row block, then tiles.
+template <int DP, bool BF16, bool CUT>
+__device__ __forceinline__ void tiles_run(const Attend8 &p, int wg, int n_wg, int total, unsigned char *lds)
+{
+    const int lane = threadIdx.x & 63, N = min(n_wg, total);
+    if (wg >= N)
+        return;
+    const int u0 = run_start(total, N, wg), u1 = run_start(total, N, wg + 1);
+    int i = -1, pre = 0;
+    for (int i0 = 0, base = 0; i0 < p.entries; i0 += 64) {
+        int x = 0;
+        if (i0 + lane < p.entries) {
+            const Entry8 e = tile_entry(p, i0 + lane);
+            x = e.units * e.nrb * p.c.H;
+        }
+        const int inc = lanes_sum(x, lane);
+        const unsigned long long past = __ballot(base + inc > u0);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            i = i0 + l;
+            pre = base + __builtin_amdgcn_readlane(inc - x, l);
+            break;
+        }
+        base += __builtin_amdgcn_readlane(inc, 63);
+    }
+    // (the bounds are for lengths that another stream changes under the call)
+    for (int u = u0; u < u1 && i >= 0 && i < p.entries;) {
+        const Entry8 e = tile_entry(p, i);
+        if (e.units == 0 || u >= pre + e.units * e.nrb * p.c.H) {
+            pre += e.units * e.nrb * p.c.H;
+            ++i;
+            continue;
+        }
+        const int item = (u - pre) / e.units, off = (u - pre) - item * e.units, seg = min(e.units - off, u1 - u);
+        if (off + seg > kTileStart) {
+            const bool first = off <= kTileStart, whole = first && off + seg == e.units;
+            const int kh = item / e.nrb, rb = item - kh * e.nrb;
+            const int at = (p.e0 + i < p.F ? (p.e0 + i) * p.c.H * p.nrb : p.item0 + (p.e0 + i - p.F) * p.c.H * p.own_nrb) +
+                           kh * (p.e0 + i < p.F ? p.nrb : p.own_nrb) + rb;
+            const int slot = whole ? 2 * p.n_wg + at : 2 * wg + (u == u0 ? 0 : 1);
+            if (first && threadIdx.x == 0)
+                p.ws_tab[at] = make_int2(slot, whole ? -1 : run_of(total, N, pre + (item + 1) * e.units - 1));
+            tile_part<DP, BF16, CUT, true>(p, e.sq, i, kh, rb, 0, max(off - kTileStart, 0), off + seg - kTileStart,
+                                           (int64_t)slot * kTileRows, lds);
+            __syncthreads();
+        }
+        u += seg;
+    }
+}
+
+// What a unit of each kind costs, relative to each other (tile, row).
+constexpr int kTileCost = 5, kRowCost = 4;
+
+// RT: the row blocks of a sequence's own rows; 0: they go through tiles, and `a` has all entries.
+template <int DP, bool BF16, bool CUT, int RT>
+__global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_shared_kernel(Attend8 a, Attend8 own)
+{
+    static_assert(kWaves == kTileWaves, "both kinds of work are of one workgroup's size");
+    typedef RowLds<DP, RT ? RT : 1, false> Rows;
+    constexpr int LDS = (int)sizeof(Rows) > kTileLds<DP> ? (int)sizeof(Rows) : kTileLds<DP>;
+    __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
+    // workgroup i runs on XCD i % 8: neighbours of a run share one
+    const int W = gridDim.x, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const int tiles = tile_units(a);
+    if constexpr (RT == 0) {
+        tiles_run<DP, BF16, CUT>(a, xcd * (W >> 3) + j, W, tiles, lds);
+    } else {
+        const int rows = row_units(own);
+        int n = 0;   // of an XCD's workgroups, those that take tiles
+        if (tiles > 0) {
+            const int64_t x = (int64_t)tiles * kTileCost, y = (int64_t)rows * kRowCost;
+            n = rows == 0 ? W >> 3 : min(max((int)(((W >> 3) * x + (x + y) / 2) / (x + y)), 1), (W >> 3) - 1);
+        }
+        const int m = (W >> 3) - n;
+        if (j < n)
+            tiles_run<DP, BF16, CUT>(a, xcd * n + j, 8 * n, tiles, lds);
+        else
+            rows_run<DP, RT, BF16, CUT, false, kShared>(own, xcd * m + j - n, 8 * m, *(Rows *)lds);
+    }
+}
+
 struct SharedPlan8 {
-    int DP;
-    bool together;        // one launch of the row kernel for prefixes and sequences
-    Launch8 prefix, own;
-    size_t bytes;
+    int DP, RT;               // RT: own row blocks, 0 where they are tiles
+    bool together;            // one launch of the row kernel for prefixes and sequences, RT blocks
+    int W, nrb, own_nrb;      // workgroups; row blocks of a prefix and of a sequence
+    int64_t items, own_items; // of the prefixes, of the sequences
+    size_t o_at, ml_at, tab_at, own_o_at, own_ml_at, own_tab_at, map_at, bytes;
 };
 
 static int row_blocks(int64_t rows, int DP)
@@ -136,49 +298,45 @@ static int plan_shared(const Cache8 &c, const kitty_cache8_shared_args &a, Share
         return fail(KITTY_E_UNSUPPORTED, "too many rows for one launch");
     const int64_t prefix_rows = own_rows * (a.batch / a.prefixes);
     const int64_t prefix_cap = (int64_t)a.prefix_pages << c.lg, own_cap = (int64_t)a.table_pages << c.lg;
+    const int64_t F = a.prefixes, B = a.batch, H = c.H;
     const int cus = device_cus();
     pl.DP = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
-    pl.bytes = 0;
-    const int most = pl.DP == 256 ? 32 : 64;   // rows of an entry that the row kernel takes
-    // row launches share at most `units` units
-    auto plan = [&](Launch8 &la, bool tiles, int64_t n, int e0, int entries, int64_t tokens, int64_t units) {
-        la.tiles = tiles, la.e0 = e0, la.entries = entries;
-        la.RT = row_blocks(n, pl.DP);
-        const int RM = tiles ? kTileRows : 16 * la.RT;
-        const int64_t nrb = (n + RM - 1) / RM, items = entries * (int64_t)c.H * nrb;
-        int64_t slots;
-        la.nrb = (int)nrb, la.n_wg = la.splits = 0;
-        if (tiles) {
-            const int64_t want = (pl.DP == 256 ? 1 : 2) * (int64_t)cus / std::max<int64_t>(items, 1);
-            la.splits = (int)std::max<int64_t>(1, std::min<int64_t>(want, tokens / 256));
-            slots = items * la.splits;
-            if (slots > kMaxBlocks)
-                return fail(KITTY_E_UNSUPPORTED, "too many rows for one launch");
-        } else {
-            if (units > 0x7fffffff)
-                return fail(KITTY_E_UNSUPPORTED, "too many rows and pages for one launch");
-            la.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>((two_per_cu(pl.DP, la.RT) ? 2 : 1) * cus, units));
-            slots = 2 * la.n_wg + items;
-        }
-        la.o_at = pl.bytes;
-        la.ml_at = la.o_at + up16((size_t)slots * RM * pl.DP * 4);
-        la.tab_at = la.ml_at + up16((size_t)slots * RM * 8);
-        pl.bytes = la.tab_at + (tiles ? 0 : up16((size_t)items * 8));
-        return KITTY_OK;
+    pl.together = prefix_rows <= (pl.DP == 256 ? 32 : 64);
+    const bool by_rows = pl.together || own_rows <= 32;
+    pl.RT = pl.together ? row_blocks(prefix_rows, pl.DP) : by_rows ? row_blocks(own_rows, pl.DP) : 0;
+    const int RM = by_rows ? 16 * pl.RT : kTileRows;
+    pl.nrb = pl.together ? 1 : (int)((prefix_rows + kTileRows - 1) / kTileRows);
+    pl.own_nrb = by_rows ? 1 : (int)((own_rows + kTileRows - 1) / kTileRows);
+    pl.items = F * H * pl.nrb, pl.own_items = B * H * pl.own_nrb;
+    // units as the kernels count them
+    const int64_t tile = pl.items * (kTileStart + (prefix_cap + kTile - 1) / kTile);
+    const int64_t own = pl.own_items * (by_rows ? kStart + (own_cap + kUnit - 1) / kUnit : kTileStart + (own_cap + kTile - 1) / kTile);
+    const int64_t together = pl.items * (kStart + (prefix_cap + kUnit - 1) / kUnit) + own;
+    if (tile > 0x7fffffff || own > 0x7fffffff || together > 0x7fffffff || (!by_rows && tile + own > 0x7fffffff))
+        return fail(KITTY_E_UNSUPPORTED, "too many rows and pages for one launch");
+    // workgroups: what the device holds at once, a multiple of eight; no more than there are units
+    const int64_t fit = (pl.together ? two_per_cu(pl.DP, pl.RT) : pl.DP <= 128) ? 2 * cus : cus;
+    pl.W = (int)std::min<int64_t>(fit, pl.together ? std::max<int64_t>(together, 1) : tile + own + 16);
+    if (!pl.together)
+        pl.W = std::max(pl.W / 8 * 8, 16);
+    size_t at = 0;
+    auto area = [&](int64_t slots, int rm, int64_t items, size_t &o, size_t &ml, size_t &tab) {
+        o = at;
+        ml = o + up16((size_t)slots * rm * pl.DP * 4);
+        tab = ml + up16((size_t)slots * rm * 8);
+        at = tab + up16((size_t)items * 8);
     };
-    const int64_t prefix_tokens = a.plan_prefix > 0 ? std::min<int64_t>(a.plan_prefix, prefix_cap) : prefix_cap;
-    const int64_t own_tokens = a.plan_tokens > 0 ? std::min<int64_t>(a.plan_tokens, own_cap) : own_cap;
-    const int64_t prefix_units = (int64_t)a.prefixes * c.H * (kStart + (prefix_cap + kUnit - 1) / kUnit);
-    const int64_t own_units = (int64_t)a.batch * c.H * (kStart + (own_cap + kUnit - 1) / kUnit);
-    pl.together = prefix_rows <= most;
-    if (pl.together) {
-        const int rc = plan(pl.prefix, false, prefix_rows, 0, a.prefixes + a.batch, 0, prefix_units + own_units);
-        pl.own = pl.prefix;
-        return rc;
+    if (pl.together || pl.RT == 0) {
+        const int64_t all = pl.items + pl.own_items;
+        area(2 * pl.W + all, pl.together ? RM : kTileRows, all, pl.o_at, pl.ml_at, pl.tab_at);
+        pl.own_o_at = pl.o_at, pl.own_ml_at = pl.ml_at, pl.own_tab_at = pl.tab_at;
+    } else {
+        area(2 * pl.W + pl.items, kTileRows, pl.items, pl.o_at, pl.ml_at, pl.tab_at);
+        area(2 * pl.W + pl.own_items, RM, pl.own_items, pl.own_o_at, pl.own_ml_at, pl.own_tab_at);
     }
-    if (const int rc = plan(pl.prefix, true, prefix_rows, 0, a.prefixes, prefix_tokens, 0))
-        return rc;
-    return plan(pl.own, own_rows > most, own_rows, a.prefixes, a.batch, own_tokens, own_units);
+    pl.map_at = at;
+    pl.bytes = at + (pl.together ? 0 : up16((size_t)(B * a.tokens + B + F) * 4));   // (the size does not go by q_lens)
+    return KITTY_OK;
 }
 
 static int check_shared(const kitty_cache8 *cache, const kitty_cache8_shared_args *args, Cache8 &c)
@@ -260,49 +418,48 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
     const hipStream_t st = (hipStream_t)stream;
     const dim3 block(64 * kWaves);
     char *ws = (char *)a.workspace;
-    auto with = [&](const Launch8 &la) {
-        Attend8 x = p;
-        x.e0 = la.e0, x.entries = la.entries, x.nrb = la.nrb, x.n_wg = la.n_wg, x.splits = la.splits;
-        x.ws_o = (float *)(ws + la.o_at), x.ws_ml = (float2 *)(ws + la.ml_at), x.ws_tab = (int2 *)(ws + la.tab_at);
-        return x;
-    };
-    auto part = [&](const Launch8 &la) {
-        return Part8{(const float *)(ws + la.o_at), (const float2 *)(ws + la.ml_at), (const int2 *)(ws + la.tab_at), la.e0,
-                     la.nrb, la.tiles ? kTileRows : 16 * la.RT, la.splits, la.n_wg};
-    };
-    auto launch = [&](const Launch8 &la, auto dp, auto bf, auto cut) {
-        constexpr int DP = decltype(dp)::value;
-        constexpr bool BF = decltype(bf)::value, CUT = decltype(cut)::value;
-        const Attend8 x = with(la);
-        if (la.tiles) {
-            const dim3 grid((unsigned)(la.entries * p.c.H * la.nrb * la.splits));
-            hipLaunchKernelGGL((cache8_tile_kernel<DP, BF, CUT, true>), grid, dim3(64 * kTileWaves), 0, st, x);
-            return;
-        }
-        const dim3 runs((unsigned)la.n_wg);
-        if (la.RT == 1)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, 1, BF, CUT, false, kShared>), runs, block, 0, st, x);
-        else if (la.RT == 2)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, 2, BF, CUT, false, kShared>), runs, block, 0, st, x);
-        else if constexpr (DP <= 128) {
-            if (la.RT == 3)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, 3, BF, CUT, false, kShared>), runs, block, 0, st, x);
-            else
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, 4, BF, CUT, false, kShared>), runs, block, 0, st, x);
-        }
-    };
+    if (a.q_lens && !pl.together) {
+        p.row_map = (int32_t *)(ws + pl.map_at), p.row_first = p.row_map + (int64_t)p.B * p.T, p.row_count = p.row_first + p.B;
+        hipLaunchKernelGGL(cache8_shared_queries_kernel, dim3((unsigned)((p.F + kWaves - 1) / kWaves)), block, 0, st, p);
+    }
+    p.nrb = pl.nrb, p.own_nrb = pl.own_nrb, p.n_wg = pl.W, p.item0 = (int)pl.items;
+    Attend8 x = p, y = p;     // the launch's tile entries, or all of them; its row entries
+    x.e0 = 0, x.entries = pl.together || pl.RT == 0 ? p.F + p.B : p.F;
+    x.ws_o = (float *)(ws + pl.o_at), x.ws_ml = (float2 *)(ws + pl.ml_at), x.ws_tab = (int2 *)(ws + pl.tab_at);
+    y.e0 = p.F, y.entries = p.B, y.nrb = 1;
+    y.ws_o = (float *)(ws + pl.own_o_at), y.ws_ml = (float2 *)(ws + pl.own_ml_at), y.ws_tab = (int2 *)(ws + pl.own_tab_at);
+    const bool apart = !pl.together && pl.RT != 0;
+    const int tile_rows = pl.together ? 16 * pl.RT : kTileRows, own_rows = pl.RT ? 16 * pl.RT : kTileRows;
+    const Part8 of_prefix = {x.ws_o, x.ws_ml, x.ws_tab, 0, pl.nrb, tile_rows, pl.W, 0};
+    const Part8 of_own = {y.ws_o, y.ws_ml, y.ws_tab, p.F, pl.own_nrb, own_rows, pl.W, apart ? 0 : (int)pl.items};
+    const dim3 grid((unsigned)pl.W);
     auto go = [&](auto dp, auto bf, auto cut) {
         constexpr int DP = decltype(dp)::value;
-        constexpr bool BF = decltype(bf)::value;
-        launch(pl.prefix, dp, bf, cut);
-        if (!pl.together)
-            launch(pl.own, dp, bf, cut);
+        constexpr bool BF = decltype(bf)::value, CUT = decltype(cut)::value;
+        if (pl.together) {
+            if (pl.RT == 1)
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, 1, BF, CUT, false, kShared>), grid, block, 0, st, x);
+            else if (pl.RT == 2)
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, 2, BF, CUT, false, kShared>), grid, block, 0, st, x);
+            else if constexpr (DP <= 128) {
+                if (pl.RT == 3)
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, 3, BF, CUT, false, kShared>), grid, block, 0, st, x);
+                else
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, 4, BF, CUT, false, kShared>), grid, block, 0, st, x);
+            }
+        } else if (pl.RT == 0) {
+            hipLaunchKernelGGL((cache8_shared_kernel<DP, BF, CUT, 0>), grid, block, 0, st, x, y);
+        } else if (pl.RT == 1) {
+            hipLaunchKernelGGL((cache8_shared_kernel<DP, BF, CUT, 1>), grid, block, 0, st, x, y);
+        } else {
+            hipLaunchKernelGGL((cache8_shared_kernel<DP, BF, CUT, 2>), grid, block, 0, st, x, y);
+        }
         const int64_t rows = (int64_t)p.B * p.Hq * p.T, groups = 256 * kWaves / DP;
-        const Part8 x = part(pl.prefix), y = part(pl.own);
         if (rows < kMergeRows)
-            hipLaunchKernelGGL((cache8_join_kernel<DP, BF, true>), dim3((unsigned)rows), block, 0, st, p, x, y);
+            hipLaunchKernelGGL((cache8_join_kernel<DP, BF, true>), dim3((unsigned)rows), block, 0, st, p, of_prefix, of_own);
         else
-            hipLaunchKernelGGL((cache8_join_kernel<DP, BF, false>), dim3((unsigned)((rows + groups - 1) / groups)), block, 0, st, p, x, y);
+            hipLaunchKernelGGL((cache8_join_kernel<DP, BF, false>), dim3((unsigned)((rows + groups - 1) / groups)), block, 0, st, p,
+                               of_prefix, of_own);
     };
     auto by_type = [&](auto dp) {
         const bool cut = p.c.D != decltype(dp)::value, bf16 = a.dtype == KITTY_DTYPE_BF16;

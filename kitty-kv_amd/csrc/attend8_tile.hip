@@ -10,9 +10,9 @@ void launch_tiles(const Attend8 &p, int DP, bool bf16, hipStream_t stream)
         constexpr int N = decltype(dp)::value;
         constexpr bool BF = decltype(bf)::value;
         if (p.c.D == N)
-            hipLaunchKernelGGL((cache8_tile_kernel<N, BF, false, false>), grid, block, 0, stream, p);
+            hipLaunchKernelGGL((cache8_tile_kernel<N, BF, false>), grid, block, 0, stream, p);
         else
-            hipLaunchKernelGGL((cache8_tile_kernel<N, BF, true, false>), grid, block, 0, stream, p);
+            hipLaunchKernelGGL((cache8_tile_kernel<N, BF, true>), grid, block, 0, stream, p);
     };
     auto by_size = [&](auto bf) {
         if (DP == 64)

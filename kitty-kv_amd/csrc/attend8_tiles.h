@@ -226,22 +226,26 @@ __device__ __forceinline__ void tile_step(TileState<DP> &W, const unsigned char 
     }
 }
 
-// SHARED: the entries are prefixes or sequences, and all parts are left to cache8_join_kernel.
+// LDS of a workgroup: two stages of keys and of values, and a flag.
+template <int DP>
+constexpr int kTileLds = 4 * kTile * DP * 2 + 16;
+
+// Tiles [tile0, tile1) of row block rb of an entry and KV head, by the whole workgroup.
+// SHARED: the entries are prefixes and sequences, and the part goes to row `at` of the
+// workspace; otherwise the tiles are split `split` of all, which are written or left to
+// the merge.
 template <int DP, bool BF16, bool CUT, bool SHARED>
-__global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_tile_kernel(Attend8 p)
+__device__ __forceinline__ void tile_part(const Attend8 &p, const Seq8 &sq, int b, int kh, int rb, int split, int tile0, int tile1,
+                                          int64_t at, unsigned char *lds)
 {
     constexpr int RM = kTileRows, TPR = DP / 16, PASS = 64 * kTileWaves / TPR, NP = kTile / PASS;
-    __shared__ __attribute__((aligned(16))) unsigned char ks[2][kTile * DP * 2], vs[2][kTile * DP * 2];
-    __shared__ int met_nan;
+    unsigned char(&ks)[2][kTile * DP * 2] = *(unsigned char(*)[2][kTile * DP * 2])lds;
+    unsigned char(&vs)[2][kTile * DP * 2] = *(unsigned char(*)[2][kTile * DP * 2])(lds + 2 * kTile * DP * 2);
+    int &met_nan = *(int *)(lds + 4 * kTile * DP * 2);
     const int lane = threadIdx.x & 63, g = lane >> 5, n = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // pairs vary fastest, so with a multiple of eight pairs a pair's pages stay in
-    // one XCD's L2; the last row blocks, with the most tokens, start first
-    const int pairs = (SHARED ? p.entries : p.B) * p.c.H, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
-    const int split = rest % p.splits, rb = p.nrb - 1 - rest / p.splits;
-    const int b = pair / p.c.H, kh = pair - b * p.c.H, r0 = rb * RM;
-    const Seq8 sq = entry8<SHARED>(p, b);
-    const int rows_all = (SHARED && sq.prefix ? p.gq * p.per : p.gq) * p.T, rows = min(RM, rows_all - r0);
+    const int r0 = rb * RM;
+    const int rows_all = rows8<SHARED>(p, sq, b), rows = min(RM, rows_all - r0);
     const int t_lo = r0 / p.gq, t_hi = min((r0 + rows - 1) / p.gq, sq.tq - 1);
     int vis_max = sq.bad || t_hi < t_lo ? 0 : visible8(p, sq, t_hi), vis_min = visible8(p, sq, t_lo);
     if (SHARED && sq.prefix) {
@@ -255,7 +259,8 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
         vis_min = wave_min(vis_min);
     }
     const int nt = (vis_max + kTile - 1) / kTile;
-    const int first = (int)((int64_t)nt * split / p.splits), end = (int)((int64_t)nt * (split + 1) / p.splits);
+    const int first = SHARED ? min(tile0, nt) : (int)((int64_t)nt * split / p.splits);
+    const int end = SHARED ? min(tile1, nt) : (int)((int64_t)nt * (split + 1) / p.splits);
 
     TileState<DP> W;
     const int w0 = r0 + 32 * wave, r = w0 + n;
@@ -453,7 +458,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
     if (!row)
         return;
     if (SHARED || p.splits > 1) {
-        const int64_t at = ((int64_t)(pair * p.nrb + rb) * p.splits + split) * RM + 32 * wave + n;
+        at += 32 * wave + n;
         if (g == 0)
             p.ws_ml[at] = make_float2(W.m, l);
 #pragma unroll
@@ -482,6 +487,20 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_til
             sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (W.m + __builtin_log2f(l)) / kLog2e;
     if (g == 0 && p.stat)
         p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(W.m, inv);
+}
+
+template <int DP, bool BF16, bool CUT>
+__global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void cache8_tile_kernel(Attend8 p)
+{
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kTileLds<DP>];
+    // pairs vary fastest, so with a multiple of eight pairs a pair's pages stay in
+    // one XCD's L2; the last row blocks, with the most tokens, start first
+    const int pairs = p.B * p.c.H, pair = blockIdx.x % pairs, rest = blockIdx.x / pairs;
+    const int split = rest % p.splits, rb = p.nrb - 1 - rest / p.splits;
+    const int b = pair / p.c.H, kh = pair - b * p.c.H;
+    const Seq8 sq = seq8(p, b);
+    tile_part<DP, BF16, CUT, false>(p, sq, b, kh, rb, split, 0, 0,
+                                    ((int64_t)(pair * p.nrb + rb) * p.splits + split) * kTileRows, lds);
 }
 
 } // namespace kitty
