@@ -133,11 +133,12 @@ __device__ __forceinline__ int rows8(const Attend8 &p, const Seq8 &s, int i)
     return p.gq * p.T;
 }
 
-// Query row r of an entry and KV head: sequence, head and token, whether there is such a
-// row, and the entry's tokens that it sees.
+// Query row r of an entry and KV head: sequence, head and token, the entry's tokens that
+// it sees, whether it is a row of the call (no padding) and whether it may be loaded (of
+// SHARED prefixes padding too, whose sums no one reads: the loads wait for no length).
 struct Row8 {
     int b, h, t, vis;
-    bool real;
+    bool real, there;
 };
 
 template <bool SHARED>
@@ -157,7 +158,8 @@ __device__ __forceinline__ Row8 row8(const Attend8 &p, const Seq8 &s, int i, int
             w.t -= q * p.T;
             w.b = f * p.per + q;
             w.real = false, w.vis = 0;
-            if (!s.bad && q < p.per) {
+            w.there = !s.bad && q < p.per;
+            if (w.there) {
                 // rows that are tokens of the prefix itself see it up to themselves
                 const Seq8 own = seq8(p, w.b);
                 w.real = !own.bad && w.t < own.tq;
@@ -167,7 +169,7 @@ __device__ __forceinline__ Row8 row8(const Attend8 &p, const Seq8 &s, int i, int
             return w;
         }
     }
-    w.real = !s.bad && w.t < s.tq;
+    w.real = w.there = !s.bad && w.t < s.tq;
     w.vis = visible8(p, s, w.t);
     return w;
 }

@@ -246,15 +246,29 @@ __device__ __forceinline__ int run_of(int total, int N, int u)
     return u < cut ? u / (each + 1) : more + (u - cut) / each;
 }
 
+// (KV head, row block)s of an entry, and the number of its first among all.
+template <bool SHARED>
+__device__ __forceinline__ int items8(const Attend8 &p, int i)
+{
+    return p.c.H * (SHARED && p.e0 + i >= p.F ? 1 : p.nrb);
+}
+template <bool SHARED>
+__device__ __forceinline__ int first_item8(const Attend8 &p, int i)
+{
+    if (SHARED && p.e0 + i >= p.F)
+        return p.item0 + (p.e0 + i - p.F) * p.c.H;
+    return i * p.c.H * p.nrb;
+}
+
 template <bool SHARED>
 __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R, int wg, int n_wg)
 {
-    const int lane = threadIdx.x & 63, per_seq = p.c.H * p.nrb;
+    const int lane = threadIdx.x & 63;
     const int B = SHARED ? p.entries : p.B;
     // 64 sequences at a time: tiles of each, units of each and the sum up to it
     auto tiles = [&](int b0) { return b0 + lane < B ? tiles8(entry8<SHARED>(p, b0 + lane)) : 0; };
-    auto sums = [&](int t, int &x) {
-        x = units8(t, R.start) * per_seq;
+    auto sums = [&](int b0, int t, int &x) {
+        x = units8(t, R.start) * items8<SHARED>(p, b0 + lane);
         int inc = x;
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1) {
@@ -265,15 +279,15 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R, int wg, int 
     };
     // equal sequences whose pairs the workgroups divide evenly: no run begins a second one
     int t = tiles(0);
-    const int each = __builtin_amdgcn_readlane(t, 0), items = B * per_seq;
+    const int each = __builtin_amdgcn_readlane(t, 0), items = B * p.c.H * p.nrb;
     const int N0 = (int)min((int64_t)n_wg, (int64_t)each * items);
     R.start = kStart;
-    if (B <= 64 && N0 > 0 && N0 % items == 0 && !__ballot(lane < B && t != each))
+    if (!SHARED && B <= 64 && N0 > 0 && N0 % items == 0 && !__ballot(lane < B && t != each))
         R.start = 0;
-    int x, inc = sums(t, x), total = __builtin_amdgcn_readlane(inc, 63);
+    int x, inc = sums(0, t, x), total = __builtin_amdgcn_readlane(inc, 63);
     for (int b0 = 64; b0 < B; b0 += 64) {
         int y;
-        total += __builtin_amdgcn_readlane(sums(tiles(b0), y), 63);
+        total += __builtin_amdgcn_readlane(sums(b0, tiles(b0), y), 63);
     }
     R.total = total;
     R.N = min(n_wg, total);
@@ -292,7 +306,8 @@ __device__ __forceinline__ bool find_run(const Attend8 &p, Run8 &R, int wg, int 
             return true;
         }
         base += __builtin_amdgcn_readlane(inc, 63);
-        inc = sums(tiles(b0 += 64), x);
+        b0 += 64;
+        inc = sums(b0, tiles(b0), x);
     }
     return false;
 }
@@ -308,8 +323,8 @@ constexpr bool two_per_cu(int DP, int RT) { return DP <= 128 && DP * RT <= 256; 
 
 // CUT: D is below DP, and the lanes beyond it read nothing.  DIRECT: a workgroup takes
 // the whole of one (pair, row block) and writes its rows, so that no merge follows.
-// MODE kShared: the entries are prefixes and sequences, of one row block each, and all
-// parts are left to cache8_join_kernel.
+// MODE kShared: the entries are prefixes and sequences, the latter of one row block each,
+// and all parts are left to cache8_join_kernel.
 //
 // Workgroup wg of the n_wg that share the work.
 template <int DP, int RT, bool DIRECT>
@@ -327,9 +342,9 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
     auto &lds_ml = lds.ml;
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int per_seq = p.c.H * p.nrb;
     Run8 R;
     if constexpr (DIRECT) {
+        const int per_seq = p.c.H * p.nrb;
         R.b = wg / per_seq;
         R.pre = 0, R.start = 0, R.u = wg - R.b * per_seq, R.u1 = R.u + 1;
     } else {
@@ -345,6 +360,7 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         int item = u, seg = units, tile = 0, tile1 = tiles;                     // seg: units of this run's part
         bool first = true, last_part = true;                                    // whether it has the first and last tile
         if constexpr (!DIRECT) {
+            const int per_seq = items8<SHARED>(p, b);
             if (u >= pre + units * per_seq) {
                 pre += units * per_seq;
                 ++b;
@@ -360,7 +376,8 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
             first = off <= R.start, last_part = off + seg == units;
             tile = max(off - R.start, 0), tile1 = off + seg - R.start;
         }
-        const int kh = item / p.nrb, rb = item - kh * p.nrb, r0 = rb * RM;
+        const int nrb = SHARED && !sq.prefix ? 1 : p.nrb, kh = item / nrb, rb = item - kh * nrb, r0 = rb * RM;
+        const int at = DIRECT ? 0 : first_item8<SHARED>(p, b) + item;
         const int t_lo = r0 / p.gq, t_hi = min((r0 + RM - 1) / p.gq, sq.tq - 1);   // query tokens of the block
         int vis_min = visible8(p, sq, t_lo), vis_max = sq.bad || t_hi < t_lo ? 0 : visible8(p, sq, t_hi);
 
@@ -380,7 +397,7 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
             for (int c = 0; c < DP / 32; ++c) {
                 const int ch = 64 * (c >> 1) + 16 * g + 8 * (c & 1);
                 W.q[rt][c] = u32x4{0, 0, 0, 0};
-                if (row.real && (!CUT || ch < p.c.D))
+                if (row.there && (!CUT || ch < p.c.D))
                     W.q[rt][c] = *(const u32x4 *)(q + ch);
             }
 #pragma unroll
@@ -491,10 +508,10 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         __syncthreads();
         const bool whole = first && last_part;
         // a run may hold the whole of any number of items, and has a part of at most two others
-        const int slot = SHARED && whole ? 2 * p.n_wg + b * per_seq + item : 2 * wg + (u == u0 ? 0 : 1);
+        const int slot = SHARED && whole ? 2 * p.n_wg + at : 2 * wg + (u == u0 ? 0 : 1);
         const int rows = min(RM, rows8<SHARED>(p, sq, b) - r0);
         if (!DIRECT && first && threadIdx.x == 0)
-            p.ws_tab[b * per_seq + item] =
+            p.ws_tab[at] =
                 whole ? make_int2(SHARED ? slot : -1, SHARED ? -1 : 0)
                       : make_int2(slot, run_of(R.total, R.N, pre + (item + 1) * units - 1));
         for (int i = threadIdx.x; i < rows * (DP / 4); i += 64 * NW) {
@@ -546,7 +563,10 @@ template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
 __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 : two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
 {
     __shared__ __attribute__((aligned(16))) RowLds<DP, RT, DIRECT> lds;
-    rows_run<DP, RT, BF16, CUT, DIRECT, MODE>(p, blockIdx.x, p.n_wg, lds);
+    int wg = blockIdx.x;
+    if (MODE == kShared && gridDim.x % 8 == 0)   // neighbours of a run on one XCD: they read the same pages
+        wg = (wg & 7) * (gridDim.x >> 3) + (wg >> 3);
+    rows_run<DP, RT, BF16, CUT, DIRECT, MODE>(p, wg, p.n_wg, lds);
 }
 
 } // namespace kitty

@@ -175,25 +175,18 @@ __device__ __forceinline__ int lanes_sum(int v, int lane)
     return v;
 }
 
-// All units of a launch's tile entries, and of its row entries.
-__device__ __forceinline__ int tile_units(const Attend8 &p)
+// All units of a launch's tile entries and of its row entries: their loads go together.
+__device__ __forceinline__ int2 all_units(const Attend8 &a, const Attend8 &own, bool rows)
 {
-    const int lane = threadIdx.x & 63;
-    int sum = 0;
-    for (int i = lane; i < p.entries; i += 64) {
-        const Entry8 e = tile_entry(p, i);
-        sum += e.units * e.nrb * p.c.H;
+    const int lane = threadIdx.x & 63, most = rows ? max(a.entries, own.entries) : a.entries;
+    int x = 0, y = 0;
+    for (int i = lane; i - lane < most; i += 64) {
+        const Entry8 e = tile_entry(a, min(i, a.entries - 1));
+        const int n = rows ? units8(tiles8(seq8(own, min(i, own.entries - 1))), kStart) : 0;
+        x += i < a.entries ? e.units * e.nrb * a.c.H : 0;
+        y += i < own.entries ? n * own.c.H : 0;
     }
-    return __builtin_amdgcn_readlane(lanes_sum(sum, lane), 63);
-}
-
-__device__ __forceinline__ int row_units(const Attend8 &p)
-{
-    const int lane = threadIdx.x & 63;
-    int sum = 0;
-    for (int i = lane; i < p.entries; i += 64)
-        sum += units8(tiles8(entry8<true>(p, i)), kStart) * p.c.H;
-    return __builtin_amdgcn_readlane(lanes_sum(sum, lane), 63);
+    return make_int2(__builtin_amdgcn_readlane(lanes_sum(x, lane), 63), rows ? __builtin_amdgcn_readlane(lanes_sum(y, lane), 63) : 0);
 }
 
 // Workgroup wg of n_wg's run of the `total` units of the tile entries, by item: KV head
@@ -260,11 +253,11 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_shared_
     __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
     // workgroup i runs on XCD i % 8: neighbours of a run share one
     const int W = gridDim.x, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
-    const int tiles = tile_units(a);
+    const int2 units = all_units(a, own, RT != 0);
+    const int tiles = units.x, rows = units.y;
     if constexpr (RT == 0) {
         tiles_run<DP, BF16, CUT>(a, xcd * (W >> 3) + j, W, tiles, lds);
     } else {
-        const int rows = row_units(own);
         int n = 0;   // of an XCD's workgroups, those that take tiles
         if (tiles > 0) {
             const int64_t x = (int64_t)tiles * kTileCost, y = (int64_t)rows * kRowCost;
@@ -286,11 +279,6 @@ struct SharedPlan8 {
     size_t o_at, ml_at, tab_at, own_o_at, own_ml_at, own_tab_at, map_at, bytes;
 };
 
-static int row_blocks(int64_t rows, int DP)
-{
-    return rows <= 16 ? 1 : rows <= 32 || DP == 256 ? 2 : rows <= 48 ? 3 : 4;
-}
-
 static int plan_shared(const Cache8 &c, const kitty_cache8_shared_args &a, SharedPlan8 &pl)
 {
     const int64_t own_rows = (int64_t)a.num_q_heads / c.H * a.tokens, rows = (int64_t)a.batch * a.num_q_heads * a.tokens;
@@ -301,11 +289,11 @@ static int plan_shared(const Cache8 &c, const kitty_cache8_shared_args &a, Share
     const int64_t F = a.prefixes, B = a.batch, H = c.H;
     const int cus = device_cus();
     pl.DP = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
-    pl.together = prefix_rows <= (pl.DP == 256 ? 32 : 64);
-    const bool by_rows = pl.together || own_rows <= 32;
-    pl.RT = pl.together ? row_blocks(prefix_rows, pl.DP) : by_rows ? row_blocks(own_rows, pl.DP) : 0;
+    pl.together = prefix_rows <= 64 && own_rows <= 32;
+    const bool by_rows = own_rows <= 32;
+    pl.RT = by_rows ? (pl.together ? prefix_rows : own_rows) <= 16 ? 1 : 2 : 0;
     const int RM = by_rows ? 16 * pl.RT : kTileRows;
-    pl.nrb = pl.together ? 1 : (int)((prefix_rows + kTileRows - 1) / kTileRows);
+    pl.nrb = (int)((prefix_rows + (pl.together ? RM : kTileRows) - 1) / (pl.together ? RM : kTileRows));
     pl.own_nrb = by_rows ? 1 : (int)((own_rows + kTileRows - 1) / kTileRows);
     pl.items = F * H * pl.nrb, pl.own_items = B * H * pl.own_nrb;
     // units as the kernels count them
@@ -426,7 +414,7 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
     Attend8 x = p, y = p;     // the launch's tile entries, or all of them; its row entries
     x.e0 = 0, x.entries = pl.together || pl.RT == 0 ? p.F + p.B : p.F;
     x.ws_o = (float *)(ws + pl.o_at), x.ws_ml = (float2 *)(ws + pl.ml_at), x.ws_tab = (int2 *)(ws + pl.tab_at);
-    y.e0 = p.F, y.entries = p.B, y.nrb = 1;
+    y.e0 = p.F, y.entries = p.B, y.item0 = 0;
     y.ws_o = (float *)(ws + pl.own_o_at), y.ws_ml = (float2 *)(ws + pl.own_ml_at), y.ws_tab = (int2 *)(ws + pl.own_tab_at);
     const bool apart = !pl.together && pl.RT != 0;
     const int tile_rows = pl.together ? 16 * pl.RT : kTileRows, own_rows = pl.RT ? 16 * pl.RT : kTileRows;
@@ -439,14 +427,8 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
         if (pl.together) {
             if (pl.RT == 1)
                 hipLaunchKernelGGL((cache8_rows_kernel<DP, 1, BF, CUT, false, kShared>), grid, block, 0, st, x);
-            else if (pl.RT == 2)
+            else
                 hipLaunchKernelGGL((cache8_rows_kernel<DP, 2, BF, CUT, false, kShared>), grid, block, 0, st, x);
-            else if constexpr (DP <= 128) {
-                if (pl.RT == 3)
-                    hipLaunchKernelGGL((cache8_rows_kernel<DP, 3, BF, CUT, false, kShared>), grid, block, 0, st, x);
-                else
-                    hipLaunchKernelGGL((cache8_rows_kernel<DP, 4, BF, CUT, false, kShared>), grid, block, 0, st, x);
-            }
         } else if (pl.RT == 0) {
             hipLaunchKernelGGL((cache8_shared_kernel<DP, BF, CUT, 0>), grid, block, 0, st, x, y);
         } else if (pl.RT == 1) {

@@ -279,7 +279,7 @@ __device__ __forceinline__ void tile_part(const Attend8 &p, const Seq8 &sq, int 
 #pragma unroll
         for (int s = 0; s < DP / 16; ++s) {
             W.q[s] = u32x4{0, 0, 0, 0};
-            if (qr.real && (!CUT || 16 * s < p.c.D))
+            if (qr.there && (!CUT || 16 * s < p.c.D))
                 W.q[s] = *(const u32x4 *)(q + 16 * s + 8 * g);
         }
     }
