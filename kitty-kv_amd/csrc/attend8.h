@@ -48,15 +48,29 @@ struct Attend8 {
     float2 *stat;
     float *scores;
     int64_t sc_cap;
+    // Where a launch has the whole of a KV head's rows and tokens, it adds to the weights
+    // (of the first w_tokens tokens) itself.
+    float *weights;
+    int64_t w_s_seq, w_s_head;
+    int w_tokens;
 };
 
 // What a row kernel does beside plain attention: nothing, leave all parts of prefixes and
 // sequences, leave the scores.
 constexpr int kPlain = 0, kShared = 1, kScores = 2;
 
-// kitty_cache8_attention that also leaves stat and, where given, the scores.
-int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, float2 *stat,
-            float *scores, int64_t sc_cap);
+// kitty_cache8_attention that also leaves stat and, where given, the scores; weighed: the
+// weights are done as well.
+struct Leave8 {
+    float2 *stat;
+    float *scores;
+    int64_t sc_cap;
+    float *weights;
+    int64_t w_s_seq, w_s_head;
+    int w_tokens;
+    bool weighed;
+};
+int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, Leave8 &leave);
 
 constexpr int kTileRows = 128;   // query rows of the tile kernel's workgroup
 

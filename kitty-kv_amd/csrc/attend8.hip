@@ -180,8 +180,7 @@ static int check_attend8(const kitty_cache8 *cache, const kitty_cache8_attention
     return KITTY_OK;
 }
 
-int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, float2 *stat,
-            float *scores, int64_t sc_cap)
+int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, Leave8 &leave)
 {
     Attend8 p{};
     Plan8 pl;
@@ -212,7 +211,9 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
     char *ws = (char *)a.workspace;
     p.ws_o = (float *)ws, p.ws_ml = (float2 *)(ws + pl.o_bytes), p.ws_tab = (int2 *)(ws + pl.o_bytes + pl.ml_bytes);
 
-    p.stat = stat, p.scores = scores, p.sc_cap = sc_cap;
+    p.stat = leave.stat, p.scores = leave.scores, p.sc_cap = leave.sc_cap;
+    p.weights = leave.weights, p.w_s_seq = leave.w_s_seq, p.w_s_head = leave.w_s_head, p.w_tokens = leave.w_tokens;
+    leave.weighed = leave.scores && pl.direct;
     const hipStream_t st = stream;
     const bool bf16 = a.dtype == KITTY_DTYPE_BF16;
     const dim3 block(64 * kWaves);
@@ -234,7 +235,7 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
         constexpr bool BF = decltype(bf)::value;
         const dim3 pairs((unsigned)(p.B * p.c.H * p.nrb)), runs((unsigned)p.n_wg), waves(64 * row_waves(RT, true));
         if constexpr (RT == 1) {
-            if (scores) {
+            if (p.scores) {
                 if constexpr (DP <= 128) {
                     if (pl.direct && p.c.D == DP)
                         hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true, kScores>), pairs, waves, 0, st, p);
@@ -321,5 +322,6 @@ extern "C" int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, 
 extern "C" int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attention_args *args,
                                       kitty_stream_t stream)
 {
-    return attend8(cache, args, (hipStream_t)stream, nullptr, nullptr, 0);
+    Leave8 none{};
+    return attend8(cache, args, (hipStream_t)stream, none);
 }

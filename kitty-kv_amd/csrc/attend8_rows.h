@@ -331,6 +331,7 @@ template <int DP, int RT, bool DIRECT>
 struct RowLds {
     float o[row_waves(RT, DIRECT)][16 * RT][DP + 4];
     float2 ml[row_waves(RT, DIRECT)][16 * RT];
+    float2 stat[DIRECT && RT == 1 ? 16 : 1];
 };
 
 template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
@@ -551,6 +552,24 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                     sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
             if (ch == 0 && p.stat)
                 p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
+            if (SCORES && DIRECT && ch == 0)
+                lds.stat[r] = make_float2(m, inv);
+        }
+        if constexpr (SCORES && DIRECT) {
+            // the weights, from the scores that the waves left
+            __syncthreads();
+            float *weights = p.weights + b * p.w_s_seq + kh * p.w_s_head;
+            const float *left = p.scores + (int64_t)(b * p.c.H + kh) * rows_all * p.sc_cap;
+            const int tokens = sq.bad ? 0 : min(sq.n, p.w_tokens);
+            for (int tok = threadIdx.x; tok < tokens; tok += 64 * NW) {
+                const float was = weights[tok];
+                float sum = 0.0f;
+                for (int r = 0; r < rows_all; ++r)
+                    if (tok < visible8(p, sq, r / p.gq))
+                        sum = __builtin_fmaf(__builtin_amdgcn_exp2f(left[(int64_t)(tok >> 4) * 16 * rows_all + 16 * r + (tok & 15)] - lds.stat[r].x),
+                                             lds.stat[r].y, sum);
+                weights[tok] = was + sum;
+            }
         }
         if constexpr (DIRECT)
             return;

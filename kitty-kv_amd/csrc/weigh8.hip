@@ -58,26 +58,6 @@ __global__ __launch_bounds__(64 * kWeighWaves, DP <= 128 ? 3 : 1) void cache8_we
         const int tiles = (rows + kWeighRows - 1) / kWeighRows;
         const int begin = (int)((int64_t)tiles * part / w.parts), end = (int)((int64_t)tiles * (part + 1) / w.parts);
         const int tok0 = (int)first + 64 * wave;
-        u32x4 k[2][DP / 16];
-        float ks[2], sum[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int tok = tok0 + 32 * h + n, id = table[min(tok, sq.n - 1) >> lg];
-            const bool bad = bad_page(p.c, id);
-            const int64_t page = bad ? 0 : id;
-            const uint8_t *key = p.c.key + page * p.c.key_s_page + kh * p.c.key_s_head + ((uint32_t)tok & ((1u << lg) - 1)) * p.c.key_s_tok + 16 * g;
-            ks[h] = bad ? __builtin_nanf("") : p.c.scale[page * p.c.scale_s_page + kh * p.c.scale_s_head] * p.cs;
-            u32x4 raw[DP / 32];
-#pragma unroll
-            for (int c = 0; c < DP / 32; ++c)
-                raw[c] = CUT && 32 * c + 16 * g >= p.c.D ? u32x4{0, 0, 0, 0} : *(const u32x4 *)(key + 32 * c);
-#pragma unroll
-            for (int c = 0; c < DP / 32; ++c) {
-                u32x4 y[2];
-                widen16<BF16>(raw[c], y);
-                k[h][2 * c] = y[0], k[h][2 * c + 1] = y[1];
-            }
-        }
         // the thread's rows of the next tile to load, as (head, query); each tile is 32 rows on
         const int step_h = each ? kWeighRows / each : 0, step_t = kWeighRows - step_h * each;
         int lr = begin * kWeighRows, lh[NP], lt[NP], nh, nt;
@@ -123,11 +103,32 @@ __global__ __launch_bounds__(64 * kWeighWaves, DP <= 128 ? 3 : 1) void cache8_we
             if (threadIdx.x < kWeighRows)
                 lds_top[stage][n] = buf_stat.x, lds_inv[stage][n] = buf_stat.y, lds_vis[stage][n] = buf_vis;
         };
-        __syncthreads();   // of the block before
-        if (begin < end) {
+        if (begin < end)
             load();
-            store(0);
+        // the block's keys, behind the first rows' loads
+        u32x4 k[2][DP / 16];
+        float ks[2], sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int tok = tok0 + 32 * h + n, id = table[min(tok, sq.n - 1) >> lg];
+            const bool bad = bad_page(p.c, id);
+            const int64_t page = bad ? 0 : id;
+            const uint8_t *key = p.c.key + page * p.c.key_s_page + kh * p.c.key_s_head + ((uint32_t)tok & ((1u << lg) - 1)) * p.c.key_s_tok + 16 * g;
+            ks[h] = bad ? __builtin_nanf("") : p.c.scale[page * p.c.scale_s_page + kh * p.c.scale_s_head] * p.cs;
+            u32x4 raw[DP / 32];
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c)
+                raw[c] = CUT && 32 * c + 16 * g >= p.c.D ? u32x4{0, 0, 0, 0} : *(const u32x4 *)(key + 32 * c);
+#pragma unroll
+            for (int c = 0; c < DP / 32; ++c) {
+                u32x4 y[2];
+                widen16<BF16>(raw[c], y);
+                k[h][2 * c] = y[0], k[h][2 * c + 1] = y[1];
+            }
         }
+        __syncthreads();   // of the block before
+        if (begin < end)
+            store(0);
         for (int i = begin; i < end; ++i) {
             const int stage = (i - begin) & 1;
             __syncthreads();
@@ -343,9 +344,11 @@ extern "C" int kitty_cache8_weighed_attention(const kitty_cache8 *cache, const k
     a.workspace = ws + rows + pl.bytes;
     a.workspace_bytes -= rows + pl.bytes;
     const hipStream_t st = (hipStream_t)stream;
-    if (const int rc = attend8(cache, &a, st, p.stat, pl.scores && pl.cap ? p.scores : nullptr, p.sc_cap))
+    Leave8 leave = {p.stat, pl.scores && pl.cap ? p.scores : nullptr, p.sc_cap,
+                    weights->weights, weights->s_seq, weights->s_head, weights->tokens, false};
+    if (const int rc = attend8(cache, &a, st, leave))
         return rc;
-    if (pl.cap == 0)
+    if (pl.cap == 0 || leave.weighed)
         return KITTY_OK;
     p.q = a.q;
     p.q_s_seq = a.q_s_seq, p.q_s_head = a.q_s_head, p.q_s_tok = a.q_s_tok;
