@@ -71,6 +71,12 @@ struct Leave8 {
     bool weighed;
 };
 int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, Leave8 &leave);
+int attend8_bytes(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, size_t &bytes);
+
+// The tile kernel's work on sequences of unequal lengths, cut evenly by what they hold
+// (attend8_shared.hip): p with its queries, tables and outputs, in `bytes` of workspace.
+size_t tile_runs_bytes(const Cache8 &c, const kitty_cache8_attention_args &args);
+void launch_tile_runs(const Attend8 &p, bool bf16, void *workspace, hipStream_t stream);
 
 constexpr int kTileRows = 128;   // query rows of the tile kernel's workgroup
 

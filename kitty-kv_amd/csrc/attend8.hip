@@ -116,16 +116,18 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
 //   256 channels, 20 rows 281 in two blocks / 331 in one at a time
 // 8 sequences: 49 / 62, 62 / 61, 39 / 48.
 //
-// 3. The tile kernel beyond.
+// 3. The tile kernel beyond.  Where a weighed call (kitty_cache8_weighed_attention) would split the
+// tokens of each row block, cache8_shared_kernel's runs take them (32 queries of 8 sequences of
+// 4,000 to 16,000 tokens: @@ against 97 us in equal parts of each).
 constexpr int64_t kDirectBytes = 1024 * 128, kDirectItems = 4096;
 
 struct Plan8 {
-    bool tiles, direct;
+    bool tiles, direct, runs;
     int DP, RT, nrb, n_wg, splits;
     size_t o_bytes, ml_bytes, bytes;
 };
 
-static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &pl)
+static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, bool weighed, Plan8 &pl)
 {
     const int64_t rows = (int64_t)a.num_q_heads / c.H * a.tokens, pairs = (int64_t)a.batch * c.H;
     const int64_t cap = (int64_t)a.table_pages << c.lg, units = kStart + (cap + kUnit - 1) / kUnit;
@@ -154,6 +156,11 @@ static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, Plan8 &p
         pl.n_wg = (int)std::max<int64_t>(1, std::min<int64_t>((two_per_cu(pl.DP, pl.RT) ? 2 : 1) * cus, items * units));
         slots = 2 * pl.n_wg;
     }
+    pl.runs = weighed && pl.tiles && pl.splits > 1 && items * (cap / 64 + 4) <= 0x7fffffff;   // its units of 64 tokens
+    if (pl.runs) {
+        pl.bytes = tile_runs_bytes(c, a);
+        return KITTY_OK;
+    }
     pl.o_bytes = up16((size_t)slots * RM * pl.DP * 4);
     pl.ml_bytes = up16((size_t)slots * RM * 8);
     pl.bytes = pl.o_bytes + pl.ml_bytes + (pl.tiles || pl.direct ? 0 : up16((size_t)items * 8));
@@ -180,6 +187,18 @@ static int check_attend8(const kitty_cache8 *cache, const kitty_cache8_attention
     return KITTY_OK;
 }
 
+int attend8_bytes(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, size_t &bytes)
+{
+    Cache8 c;
+    Plan8 pl;
+    if (const int rc = check_attend8(cache, args, c))
+        return rc;
+    if (const int rc = plan8(c, *args, true, pl))
+        return rc;
+    bytes = pl.bytes;
+    return KITTY_OK;
+}
+
 int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, Leave8 &leave)
 {
     Attend8 p{};
@@ -196,7 +215,7 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
     for (int64_t s : {a.q_s_seq, a.q_s_head, a.q_s_tok, a.o_s_seq, a.o_s_head, a.o_s_tok})
         if (s % 8)
             return fail(KITTY_E_INVALID, "strides of q and out must be multiples of 8 elements (16-byte rows)");
-    if (const int rc = plan8(p.c, a, pl))
+    if (const int rc = plan8(p.c, a, leave.stat != nullptr, pl))
         return rc;
     if ((!a.workspace && pl.bytes) || !aligned(a.workspace, 16) || a.workspace_bytes < pl.bytes)
         return fail(KITTY_E_INVALID, "workspace is NULL, misaligned or smaller than kitty_cache8_attention_workspace_size");
@@ -267,6 +286,10 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
     auto go = [&](auto dp, auto bf) {
         constexpr int DP = decltype(dp)::value;
         if (pl.tiles) {
+            if (pl.runs) {
+                launch_tile_runs(p, bf16, ws, st);
+                return;
+            }
             launch_tiles(p, DP, bf16, st);
             if (p.splits > 1)
                 merge(dp, bf, std::true_type{});
@@ -313,7 +336,7 @@ extern "C" int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, 
         return fail(KITTY_E_INVALID, "bytes is NULL");
     if (const int rc = check_attend8(cache, args, c))
         return rc;
-    if (const int rc = plan8(c, *args, pl))
+    if (const int rc = plan8(c, *args, false, pl))
         return rc;
     *bytes = pl.bytes;
     return KITTY_OK;

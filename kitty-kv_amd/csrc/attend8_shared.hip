@@ -41,10 +41,20 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
     const int pair = all / rows, row = all - pair * rows;
     if (!ALONE && pair >= p.B * p.c.H)
         return;
-    const int b = pair / p.c.H, kh = pair - b * p.c.H, f = b / p.per;
+    const int b = pair / p.c.H, kh = pair - b * p.c.H, f = p.F ? b / p.per : 0;
     const int t = row / p.gq, h = kh * p.gq + row - t * p.gq;
+    // an item's table entry is loaded before its lengths are known; where nothing is left it holds anything
+    auto place = [&](const Part8 &s, int e, int r, int &rr) {
+        const int rb = r / s.RM;
+        rr = r - rb * s.RM;
+        return s.item0 + ((e - s.e0) * p.c.H + kh) * s.nrb + rb;
+    };
+    int rr_p, rr_o;
+    const int q = p.row_map ? min(p.row_first[b] + t, p.per * p.T - 1) : (b - f * p.per) * p.T + t;
+    const int item_p = place(of_prefix, f, q * p.gq + h - kh * p.gq, rr_p), item_o = place(of_own, p.F + b, row, rr_o);
+    const int2 tab_p = of_prefix.tab[p.F ? item_p : 0], tab_o = of_own.tab[item_o];
     const Seq8 own = seq8(p, b);
-    const int before = p.prefix_lens[f];
+    const int before = p.F ? p.prefix_lens[f] : 0;   // F: 0 for launch_tile_runs
     const bool bad = own.bad || before < 0 || before > (int64_t)p.prefix_pages << p.c.lg || (before > 0 && p.c.num_pages == 0);
     float m = kLowest, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -55,11 +65,9 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
         l = f0 * l + f1 * l1;
         o.x = f0 * o.x + f1 * x.x, o.y = f0 * o.y + f1 * x.y, o.z = f0 * o.z + f1 * x.z, o.w = f0 * o.w + f1 * x.w;
     };
-    auto parts = [&](const Part8 &s, int e, int r, int tokens) {
+    auto parts = [&](const Part8 &s, int item, int rr, int2 tab, int tokens) {
         if (tokens <= 0)
-            return;   // nothing is left of it
-        const int rb = r / s.RM, rr = r - rb * s.RM, item = s.item0 + ((e - s.e0) * p.c.H + kh) * s.nrb + rb;
-        const int2 tab = s.tab[item];
+            return;
         // (bounds for lengths that another stream changes under the call)
         const int slot = min(max(tab.x, 0), tab.y < 0 ? 2 * s.n_wg + item : 2 * s.n_wg - 1), first = slot >> 1;
         const int count = tab.y < 0 ? 1 : min(tab.y, s.n_wg - 1) - first + 1;
@@ -80,9 +88,8 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
         }
     };
     if (!bad && t < own.tq) {
-        const int q = p.row_map ? p.row_first[b] + t : (b - f * p.per) * p.T + t;
-        parts(of_prefix, f, q * p.gq + h - kh * p.gq, before);
-        parts(of_own, p.F + b, row, own.n);
+        parts(of_prefix, item_p, rr_p, tab_p, before);
+        parts(of_own, item_o, rr_o, tab_o, own.n);
     }
     if constexpr (ALONE) {
         __shared__ __attribute__((aligned(16))) float lds_o[GROUPS][DP];
@@ -110,6 +117,8 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Par
     if (ch == 0 && p.lse)
         p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
             bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
+    if (ch == 0 && p.stat)
+        p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
 }
 
 // The prefixes' real queries where they are padded, a wave per prefix.
@@ -327,6 +336,73 @@ static int plan_shared(const Cache8 &c, const kitty_cache8_shared_args &a, Share
     return KITTY_OK;
 }
 
+// Sizes of launch_tile_runs: slots of 128 rows for two parts a workgroup and one an item.
+struct TileRuns8 {
+    int DP, W, nrb;
+    int64_t items;
+    size_t ml_at, tab_at, bytes;
+};
+
+static TileRuns8 plan_tile_runs(int D, int H, int64_t batch, int64_t rows)
+{
+    TileRuns8 r;
+    r.DP = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    r.W = std::max((r.DP <= 128 ? 2 : 1) * device_cus() / 8 * 8, 16);
+    r.nrb = (int)((rows + kTileRows - 1) / kTileRows);
+    r.items = batch * H * r.nrb;
+    const size_t slots = 2 * r.W + (size_t)r.items;
+    r.ml_at = up16(slots * kTileRows * r.DP * 4);
+    r.tab_at = r.ml_at + up16(slots * kTileRows * 8);
+    r.bytes = r.tab_at + up16((size_t)r.items * 8);
+    return r;
+}
+
+size_t tile_runs_bytes(const Cache8 &c, const kitty_cache8_attention_args &a)
+{
+    return plan_tile_runs(c.D, c.H, a.batch, (int64_t)a.num_q_heads / c.H * a.tokens).bytes;
+}
+
+template <int DP, bool BF16>
+static void join(const Attend8 &p, const Part8 &of_prefix, const Part8 &of_own, hipStream_t st)
+{
+    const int64_t rows = (int64_t)p.B * p.Hq * p.T, groups = 256 * kWaves / DP;
+    if (rows < kMergeRows)
+        hipLaunchKernelGGL((cache8_join_kernel<DP, BF16, true>), dim3((unsigned)rows), dim3(64 * kWaves), 0, st, p, of_prefix, of_own);
+    else
+        hipLaunchKernelGGL((cache8_join_kernel<DP, BF16, false>), dim3((unsigned)((rows + groups - 1) / groups)), dim3(64 * kWaves), 0,
+                           st, p, of_prefix, of_own);
+}
+
+void launch_tile_runs(const Attend8 &args, bool bf16, void *workspace, hipStream_t st)
+{
+    Attend8 p = args;
+    const TileRuns8 r = plan_tile_runs(p.c.D, p.c.H, p.B, (int64_t)p.gq * p.T);
+    p.F = 0, p.per = 1, p.e0 = 0, p.entries = p.B, p.item0 = 0, p.nrb = p.own_nrb = r.nrb, p.n_wg = r.W;
+    p.ws_o = (float *)workspace, p.ws_ml = (float2 *)((char *)workspace + r.ml_at), p.ws_tab = (int2 *)((char *)workspace + r.tab_at);
+    const Part8 part = {p.ws_o, p.ws_ml, p.ws_tab, 0, r.nrb, kTileRows, r.W, 0};
+    auto go = [&](auto dp, auto bf) {
+        constexpr int DP = decltype(dp)::value;
+        constexpr bool BF = decltype(bf)::value;
+        if (p.c.D == DP)
+            hipLaunchKernelGGL((cache8_shared_kernel<DP, BF, false, 0>), dim3(r.W), dim3(64 * kWaves), 0, st, p, p);
+        else
+            hipLaunchKernelGGL((cache8_shared_kernel<DP, BF, true, 0>), dim3(r.W), dim3(64 * kWaves), 0, st, p, p);
+        join<DP, BF>(p, part, part, st);
+    };
+    auto by_size = [&](auto bf) {
+        if (r.DP == 64)
+            go(std::integral_constant<int, 64>{}, bf);
+        else if (r.DP == 128)
+            go(std::integral_constant<int, 128>{}, bf);
+        else
+            go(std::integral_constant<int, 256>{}, bf);
+    };
+    if (bf16)
+        by_size(std::true_type{});
+    else
+        by_size(std::false_type{});
+}
+
 static int check_shared(const kitty_cache8 *cache, const kitty_cache8_shared_args *args, Cache8 &c)
 {
     if (!args)
@@ -436,12 +512,7 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
         } else {
             hipLaunchKernelGGL((cache8_shared_kernel<DP, BF, CUT, 2>), grid, block, 0, st, x, y);
         }
-        const int64_t rows = (int64_t)p.B * p.Hq * p.T, groups = 256 * kWaves / DP;
-        if (rows < kMergeRows)
-            hipLaunchKernelGGL((cache8_join_kernel<DP, BF, true>), dim3((unsigned)rows), block, 0, st, p, of_prefix, of_own);
-        else
-            hipLaunchKernelGGL((cache8_join_kernel<DP, BF, false>), dim3((unsigned)((rows + groups - 1) / groups)), block, 0, st, p,
-                               of_prefix, of_own);
+        join<DP, BF>(p, of_prefix, of_own, st);
     };
     auto by_type = [&](auto dp) {
         const bool cut = p.c.D != decltype(dp)::value, bf16 = a.dtype == KITTY_DTYPE_BF16;

@@ -310,7 +310,9 @@ extern "C" int kitty_cache8_weighed_attention_workspace_size(const kitty_cache8 
     if (const int rc = check_weights(args, weights))
         return rc;
     Cache8 c;
-    if (const int rc = kitty_cache8_attention_workspace_size(cache, args, bytes))
+    if (!bytes)
+        return fail(KITTY_E_INVALID, "bytes is NULL");
+    if (const int rc = attend8_bytes(cache, args, *bytes))
         return rc;
     if (const int rc = check_cache8(cache, c))
         return rc;

@@ -56,7 +56,7 @@ SHAPES = [
     (200, 1, 16, 8, 1, 16, 16, [(5 * f) % 23 for f in range(200)], [f % 19 for f in range(200)]), (2, 150, 16, 8, 1, 16, 16, [70, 3], [(3 * b) % 40 for b in range(300)]),
     # the prefix in tiles, the sequences' own by rows
     (1, 17, 4, 1, 1, 128, 64, [700], [(31 * b) % 150 for b in range(17)]), (2, 40, 3, 1, 1, 64, 16, [150, 401], [b % 50 for b in range(80)]),
-    (1, 9, 4, 1, 1, 256, 128, [600], [10] * 9), (1, 13, 5, 1, 3, 96, 32, [257], [3 + b for b in range(13)]), (3, 20, 4, 1, 1, 16, 256, [300, 0, 63], [b for b in range(60)]),
+    (1, 9, 4, 1, 1, 256, 128, [600], [10] * 9), (1, 17, 4, 1, 1, 256, 128, [600], [10 + b for b in range(17)]), (1, 13, 5, 1, 3, 96, 32, [257], [3 + b for b in range(13)]), (3, 20, 4, 1, 1, 16, 256, [300, 0, 63], [b for b in range(60)]),
     (1, 3, 60, 1, 1, 128, 64, [1], [0, 0, 1]),
     # both in tiles
     (1, 2, 4, 2, 40, 64, 16, [300], [40, 55]), (2, 2, 3, 1, 43, 128, 32, [65, 500], [43, 43, 100, 50]), (1, 3, 2, 1, 33, 256, 16, [129], [33, 40, 200]),

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from cache8_plan import widened
-from cache8_ref import Ref, numpy
+from cache8_ref import Ref, numpy, tolerance
 from test_cache8 import BF16, DEVICES, F16, filled, i32, tables
 
 
@@ -50,7 +50,7 @@ def want_weights(cache, q, table, lens, q_lens, causal, sm_scale, weights):
 
 
 def check_weighed(cache, q, table, lens, N=None, q_lens=None, causal=True, sm_scale=None, weights=None, **kw):
-    """attend's output and log-sum-exp to the bit, and the weights."""
+    """Output and log-sum-exp as check_attend has them of attend, and the weights."""
     dev = cache.device
     gen = torch.Generator().manual_seed(len(lens))
     if weights is None:
@@ -65,10 +65,17 @@ def check_weighed(cache, q, table, lens, N=None, q_lens=None, causal=True, sm_sc
     bad = np.abs(got - want) > off
     assert not bad.any(), (float(np.nanmax(np.abs(got - want) - off)), np.argwhere(bad)[:4])
     assert (got[want == before] == before[want == before]).all()             # what no row sees stays as it is
-    plain, plain_lse = cache.attend(q.to(dev), *args, **more)
-    assert torch.equal(out.view(torch.int16), plain.view(torch.int16)) or torch.equal(out.isnan(), plain.isnan())
-    np.testing.assert_array_equal(numpy(out), numpy(plain))
-    np.testing.assert_array_equal(numpy(lse), numpy(plain_lse))
+    ref, rlse, spread, mag, small = Ref(cache).attend(numpy(q), table.cpu().numpy(), lens, q_lens, causal, sm_scale)
+    n, D = max(max(lens), 1), q.shape[3]
+    tol = tolerance(q.dtype, ref, spread, mag, small, q.shape[1] // cache.num_kv_heads * q.shape[2], D, n)
+    out, lse = numpy(out), numpy(lse)
+    np.testing.assert_array_equal(np.isnan(out), np.isnan(ref))
+    assert not (np.abs(out - ref) > tol).any()
+    np.testing.assert_array_equal(np.isnan(lse), np.isnan(rlse))
+    seen = np.isfinite(rlse)
+    assert (lse[np.isneginf(rlse)] == -np.inf).all()
+    room = (D + 8) * 2.0 ** -24 * mag[seen] + 2.0 ** -21 * (1 + np.abs(rlse[seen])) + n * 2.0 ** -24
+    assert (np.abs(lse[seen] - rlse[seen]) <= room).all()
     return weights
 
 
