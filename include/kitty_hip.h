@@ -635,8 +635,10 @@ int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attenti
  * causal, row i is token prefix_lens[f] + lens[b] - q_lens[b] + i: where lens[b] <
  * q_lens[b] the first rows are tokens of the prefix.  A prefix whose length is negative
  * or more than prefix_pages pages hold gives NaN rows to its sequences.  batch is a
- * multiple of prefixes.  plan_prefix and plan_tokens: what the caller knows of the
- * largest lengths (0: what the tables hold); they only choose how the work is split. */
+ * multiple of prefixes.  The work is split by the lengths alone.  Weights of bf16 calls
+ * have the 16 bits of two terms where the rows of a prefix (its sequences' queries times
+ * the group's heads) are at most 64 and a sequence's at most 32, and over a sequence's own
+ * tokens where its rows are at most 32; elsewhere one fp16 term, as above. */
 typedef struct {
     const uint16_t *q; /* (B, Hq, T, D), 16-byte aligned rows */
     uint16_t *out;     /* (B, Hq, T, D), 16-byte aligned rows, q's type; may be q */
@@ -649,7 +651,7 @@ typedef struct {
     int64_t bt_stride;
     const int32_t *lens;         /* (B,) own tokens in the cache, those of the queries included */
     const int32_t *q_lens;       /* (B,) or NULL */
-    int32_t prefixes, batch, num_q_heads, tokens, prefix_pages, table_pages, plan_prefix, plan_tokens;
+    int32_t prefixes, batch, num_q_heads, tokens, prefix_pages, table_pages;
     int32_t causal;
     int32_t dtype;               /* KITTY_DTYPE_F16 or KITTY_DTYPE_BF16: q and out */
     float sm_scale;

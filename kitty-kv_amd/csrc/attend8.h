@@ -71,7 +71,8 @@ struct Leave8 {
     bool weighed;
 };
 int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, hipStream_t stream, Leave8 &leave);
-int attend8_bytes(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, size_t &bytes);
+// Its workspace, with scores or without.
+int attend8_bytes(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, bool scores, size_t &bytes);
 
 // The tile kernel's work on sequences of unequal lengths, cut evenly by what they hold
 // (attend8_shared.hip): p with its queries, tables and outputs, in `bytes` of workspace.

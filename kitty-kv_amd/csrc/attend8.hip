@@ -118,7 +118,7 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
 //
 // 3. The tile kernel beyond.  Where a weighed call (kitty_cache8_weighed_attention) would split the
 // tokens of each row block, cache8_shared_kernel's runs take them (32 queries of 8 sequences of
-// 4,000 to 16,000 tokens: @@ against 97 us in equal parts of each).
+// 4,000 to 16,000 tokens: 79 and 10 for the join, against 97 and 8.5 us in equal parts of each).
 constexpr int64_t kDirectBytes = 1024 * 128, kDirectItems = 4096;
 
 struct Plan8 {
@@ -127,7 +127,8 @@ struct Plan8 {
     size_t o_bytes, ml_bytes, bytes;
 };
 
-static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, bool weighed, Plan8 &pl)
+// weighed: a call that leaves its rows' maxima and sums, and scores, the scores as well.
+static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, bool weighed, bool scores, Plan8 &pl)
 {
     const int64_t rows = (int64_t)a.num_q_heads / c.H * a.tokens, pairs = (int64_t)a.batch * c.H;
     const int64_t cap = (int64_t)a.table_pages << c.lg, units = kStart + (cap + kUnit - 1) / kUnit;
@@ -137,7 +138,7 @@ static int plan8(const Cache8 &c, const kitty_cache8_attention_args &a, bool wei
     const int cus = device_cus();
     pl.DP = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
     pl.direct = pl.DP <= 128 && tokens * pl.DP <= kDirectBytes &&
-                (rows <= 32 ? pairs <= kDirectItems : pairs * ((rows + 31) / 32) <= cus);
+                (rows <= 32 ? pairs <= kDirectItems : pairs * ((rows + 31) / 32) <= cus) && !(weighed && !scores && rows <= 16);
     pl.tiles = !pl.direct && rows > (pl.DP == 256 ? 32 : 64);
     pl.RT = rows <= 16 ? 1 : rows <= 32 || pl.direct || pl.DP == 256 ? 2 : rows <= 48 ? 3 : 4;
     const int RM = pl.tiles ? kTileRows : 16 * pl.RT;
@@ -187,13 +188,13 @@ static int check_attend8(const kitty_cache8 *cache, const kitty_cache8_attention
     return KITTY_OK;
 }
 
-int attend8_bytes(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, size_t &bytes)
+int attend8_bytes(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, bool scores, size_t &bytes)
 {
     Cache8 c;
     Plan8 pl;
     if (const int rc = check_attend8(cache, args, c))
         return rc;
-    if (const int rc = plan8(c, *args, true, pl))
+    if (const int rc = plan8(c, *args, true, scores, pl))
         return rc;
     bytes = pl.bytes;
     return KITTY_OK;
@@ -215,7 +216,7 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
     for (int64_t s : {a.q_s_seq, a.q_s_head, a.q_s_tok, a.o_s_seq, a.o_s_head, a.o_s_tok})
         if (s % 8)
             return fail(KITTY_E_INVALID, "strides of q and out must be multiples of 8 elements (16-byte rows)");
-    if (const int rc = plan8(p.c, a, leave.stat != nullptr, pl))
+    if (const int rc = plan8(p.c, a, leave.stat != nullptr, leave.scores != nullptr, pl))
         return rc;
     if ((!a.workspace && pl.bytes) || !aligned(a.workspace, 16) || a.workspace_bytes < pl.bytes)
         return fail(KITTY_E_INVALID, "workspace is NULL, misaligned or smaller than kitty_cache8_attention_workspace_size");
@@ -336,7 +337,7 @@ extern "C" int kitty_cache8_attention_workspace_size(const kitty_cache8 *cache, 
         return fail(KITTY_E_INVALID, "bytes is NULL");
     if (const int rc = check_attend8(cache, args, c))
         return rc;
-    if (const int rc = plan8(c, *args, false, pl))
+    if (const int rc = plan8(c, *args, false, false, pl))
         return rc;
     *bytes = pl.bytes;
     return KITTY_OK;

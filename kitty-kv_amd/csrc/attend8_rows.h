@@ -338,6 +338,7 @@ template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
 __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, RowLds<DP, RT, DIRECT> &lds)
 {
     constexpr bool SHARED = MODE == kShared, SCORES = MODE == kScores;
+    constexpr bool STAT = !(DIRECT && RT == 1 && MODE == kPlain);   // calls that want it take another instance (plan8)
     constexpr int RM = 16 * RT, CB = DP / 16, NW = row_waves(RT, DIRECT), NB = NW == 16 ? 1 : 2, STRIDE = 32 * NW;
     auto &lds_o = lds.o;
     auto &lds_ml = lds.ml;
@@ -550,7 +551,7 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
             if (ch == 0 && p.lse)
                 p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
                     sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
-            if (ch == 0 && p.stat)
+            if (STAT && ch == 0 && p.stat)
                 p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
             if (SCORES && DIRECT && ch == 0)
                 lds.stat[r] = make_float2(m, inv);

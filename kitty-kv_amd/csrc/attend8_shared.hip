@@ -410,8 +410,8 @@ static int check_shared(const kitty_cache8 *cache, const kitty_cache8_shared_arg
     if (const int rc = check_cache8(cache, c))
         return rc;
     const kitty_cache8_shared_args &a = *args;
-    if (a.batch < 0 || a.tokens < 0 || a.table_pages < 0 || a.prefix_pages < 0 || a.plan_tokens < 0 || a.plan_prefix < 0)
-        return fail(KITTY_E_INVALID, "batch, tokens, table_pages, prefix_pages, plan_tokens and plan_prefix must not be negative");
+    if (a.batch < 0 || a.tokens < 0 || a.table_pages < 0 || a.prefix_pages < 0)
+        return fail(KITTY_E_INVALID, "batch, tokens, table_pages and prefix_pages must not be negative");
     if (a.prefixes <= 0 || a.batch % a.prefixes)
         return fail(KITTY_E_INVALID, "batch must be a multiple of a positive number of prefixes");
     if (a.num_q_heads <= 0 || a.num_q_heads % c.H)

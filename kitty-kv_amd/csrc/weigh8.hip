@@ -312,12 +312,17 @@ extern "C" int kitty_cache8_weighed_attention_workspace_size(const kitty_cache8 
     Cache8 c;
     if (!bytes)
         return fail(KITTY_E_INVALID, "bytes is NULL");
-    if (const int rc = attend8_bytes(cache, args, *bytes))
-        return rc;
     if (const int rc = check_cache8(cache, c))
         return rc;
-    const size_t rows = up16((size_t)args->batch * args->num_q_heads * args->tokens * 8);
-    *bytes = up16(*bytes) + rows + (args->batch && args->tokens ? plan_weigh(c, *args, weights->tokens).bytes : 0);
+    if (const int rc = attend8_bytes(cache, args, false, *bytes))   // the checks
+        return rc;
+    *bytes = 0;
+    if (args->batch == 0 || args->tokens == 0)
+        return KITTY_OK;
+    const WeighPlan8 pl = plan_weigh(c, *args, weights->tokens);
+    if (const int rc = attend8_bytes(cache, args, pl.scores && pl.cap, *bytes))
+        return rc;
+    *bytes = up16(*bytes) + up16((size_t)args->batch * args->num_q_heads * args->tokens * 8) + pl.bytes;
     return KITTY_OK;
 }
 

@@ -200,8 +200,7 @@ class Cache8SharedArgs(ctypes.Structure):
         ("prefix_table", _vp), ("pt_stride", _i64), ("prefix_lens", _vp),
         ("block_table", _vp), ("bt_stride", _i64), ("lens", _vp), ("q_lens", _vp),
         ("prefixes", _i32), ("batch", _i32), ("num_q_heads", _i32), ("tokens", _i32), ("prefix_pages", _i32),
-        ("table_pages", _i32), ("plan_prefix", _i32), ("plan_tokens", _i32),
-        ("causal", _i32), ("dtype", _i32), ("sm_scale", ctypes.c_float),
+        ("table_pages", _i32), ("causal", _i32), ("dtype", _i32), ("sm_scale", ctypes.c_float),
         ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
     ]
 

@@ -31,7 +31,7 @@ _PAGE_TOKENS = (16, 32, 64, 128, 256)
 # compiler lays them out (packing one takes a quarter of a ctypes structure's time)
 _ROWS = struct.Struct("2P6qPq2P4i")
 _ATTENTION = struct.Struct("3P6qPq2P7ifPN")
-_SHARED = struct.Struct("3P6qPqPPq2P10ifPN")
+_SHARED = struct.Struct("3P6qPqPPq2P8ifPN")
 _WEIGHTS = struct.Struct("P2qi")
 _EVICT = struct.Struct("P2qPqPPq3P7iPN")
 
@@ -388,8 +388,7 @@ class Cache8:
 
     def attend_shared(self, q: torch.Tensor, prefix_table: torch.Tensor, prefix_lens: torch.Tensor, block_table: torch.Tensor,
                       lens: torch.Tensor, q_lens: Optional[torch.Tensor] = None, causal: bool = True,
-                      sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False,
-                      max_prefix: Optional[int] = None, max_tokens: Optional[int] = None):
+                      sm_scale: Optional[float] = None, out: Optional[torch.Tensor] = None, return_lse: bool = False):
         """``attend`` for sequences that share prefixes (a system prompt, the samples of
         one prompt), which are read once for all of them.
 
@@ -398,10 +397,8 @@ class Cache8:
         tokens of its own in the pages of block_table's row b (lens[b] may be 0; the first
         of them is row 0 of its first page).  causal: the q_lens[b] queries of sequence b
         are the last tokens of the two together; otherwise every query sees all of both.
-        Results are ``attend``'s over the two in one table but for rounding.  max_prefix
-        and max_tokens: the largest prefix_lens[f] and lens[b] where the program knows
-        them; they only choose how the work is split.  out may be q or lie in its memory
-        in any way."""
+        Results are ``attend``'s over the two in one table but for rounding.  out may be q
+        or lie in its memory in any way."""
         if calls_followed():
             raise NotImplementedError(_FOLLOWED)
         if q.requires_grad or q.is_neg():
@@ -409,10 +406,8 @@ class Cache8:
         if out is not None:
             _into(out)
         causal, sm_scale = bool(causal), None if sm_scale is None else float(sm_scale)
-        max_prefix = 0 if max_prefix is None else int(max_prefix)
-        max_tokens = 0 if max_tokens is None else int(max_tokens)
         sig = ("shared", q.shape, q.stride(), q.dtype, q.device, _sig(prefix_table), _sig(prefix_lens), _sig(block_table),
-               _sig(lens), _sig(q_lens), causal, sm_scale, _sig(out), max_prefix, max_tokens)
+               _sig(lens), _sig(q_lens), causal, sm_scale, _sig(out))
         found = self._known.get(sig) if self._on_device else None
         if found is None:
             scale = self._check_queries(q, out, sm_scale)
@@ -425,8 +420,6 @@ class Cache8:
             self._check_table(block_table, B)
             self._i32("lens", lens, B)
             self._i32("q_lens", q_lens, B, optional=True)
-            for name, n in (("max_prefix", max_prefix), ("max_tokens", max_tokens)):
-                _need(0 <= n < 1 << 31, f"{name} must be in [0, 2^31)")
             if B == 0 or T == 0 or not self._on_device:
                 o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
                 lse = torch.empty((B, Hq, T), dtype=torch.float32, device=q.device)
@@ -441,7 +434,7 @@ class Cache8:
             packed = tuple(0 if n == 1 else s for n, s in zip((B, Hq, T), (Hs, Ts, self.head_dim)))
             head = (*(_strides(q) if in_place[0] else packed), *(_strides(o) if in_place[1] else packed))
             tables = prefix_table.stride(0) if F > 1 else 0, block_table.stride(0) if B > 1 else 0
-            rest = (F, B, Hq, T, prefix_table.shape[1], block_table.shape[1], max_prefix, max_tokens, causal,
+            rest = (F, B, Hq, T, prefix_table.shape[1], block_table.shape[1], causal,
                     _hip.KITTY_DTYPE_F16 if q.dtype == torch.float16 else _hip.KITTY_DTYPE_BF16, scale)
             size = ctypes.c_size_t(0)
             with torch.cuda.device(self._index):      # the plan is the pools' device's

@@ -112,6 +112,7 @@ def _rows(q: torch.Tensor, codes, scales, causal: bool, sm_scale: float):
     o = (w.view(H, gq * t, n) * scales[1]) @ codes[1].masked_fill(gone, 0.0)
     met = (sees.float().repeat(gq, 1) @ gone.float()) > 0
     o = o.masked_fill(met, math.nan).view(H, gq, t, D).masked_fill(none[:, None], 0.0)
+    w = w.masked_fill((l == math.inf)[..., None], math.nan)     # inf / inf, as the kernels have every weight of such a row
     return o.reshape(Hq, t, D), l.masked_fill(none, -math.inf).reshape(Hq, t), w.masked_fill(~sees, 0.0)
 
 

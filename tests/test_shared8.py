@@ -12,7 +12,8 @@ from cache8_ref import numpy, tolerance
 from test_cache8 import BF16, DEVICES, F16, filled, i32
 
 
-def check_shared(cache, q, ptable, plens, table, lens, q_lens=None, causal=True, sm_scale=None, **kw):
+def check_shared(cache, q, ptable, plens, table, lens, q_lens=None, causal=True, sm_scale=None, infinite=False, **kw):
+    """infinite: of rows with infinite scores the log-sum-exp (-inf of no finite one, and +inf or NaN) is not looked at."""
     dev, F = cache.device, len(plens)
     out, lse = cache.attend_shared(q.to(dev), ptable, i32(plens, dev), table, i32(lens, dev),
                                    q_lens=None if q_lens is None else i32(q_lens, dev), causal=causal, sm_scale=sm_scale,
@@ -29,7 +30,8 @@ def check_shared(cache, q, ptable, plens, table, lens, q_lens=None, causal=True,
     np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
     bad = np.abs(got - want) > tol
     assert not bad.any(), (float(np.nanmax(np.abs(got - want) - tol)), np.argwhere(bad)[:4])
-    np.testing.assert_array_equal(np.isnan(glse), np.isnan(wlse))
+    if not infinite:
+        np.testing.assert_array_equal(np.isnan(glse), np.isnan(wlse))
     seen = np.isfinite(wlse)
     assert (glse[np.isneginf(wlse)] == -np.inf).all()
     room = (q.shape[3] + 8) * 2.0 ** -24 * mag[seen] + 2.0 ** -21 * (1 + np.abs(wlse[seen])) + n * 2.0 ** -24
@@ -73,10 +75,9 @@ def test_matches_float64(dev, dtype, causal, F, each, Hq, H, T, D, G, plens, len
     cache, ptable, table = pools(gen, F, F * each, Wp, W, H, D, G, dev)
     q = torch.randn(F * each, Hq, T, D, generator=gen).to(dtype)
     check_shared(cache, q, ptable, plens, table, lens, causal=causal)
-    # tables that could hold far more, and hints that are wrong: other ways to share the work
+    # tables that could hold far more
     wide = [torch.cat([t, torch.full((t.shape[0], 4096 // G), 1 << 30, dtype=torch.int32, device=dev)], 1) for t in (ptable, table)]
     check_shared(cache, q, wide[0], plens, wide[1], lens, causal=causal)
-    check_shared(cache, q, wide[0], plens, wide[1], lens, causal=causal, max_prefix=1, max_tokens=100)
 
 
 # (sequences of each, query heads, KV heads, queries): one launch, tiles and rows, tiles
@@ -95,10 +96,12 @@ def test_padded_rows_and_rows_in_the_prefix(dev, dtype, causal, each, Hq, H, T):
     q = torch.randn(3 * each, Hq, T, 64, generator=gen).to(dtype)
     lens = [(0, 130, 2, T, 1, 140)[b % 6] for b in range(3 * each)]
     q_lens = [(T, 1, T // 2, 0, T, T - 1, 3)[b % 7] for b in range(3 * each)]
+    for b, n in enumerate(q_lens):               # padding may hold anything
+        q[b, :, n:] = (math.nan, math.inf, 0.0)[b % 3]
     out = check_shared(cache, q, ptable, [77, 3, 0], table, lens, q_lens=q_lens, causal=causal)
     for b, n in enumerate(q_lens):
         assert (out[b, :, n:] == 0).all()
-    check_shared(cache, q, ptable, [80, 3, 1], table, lens, causal=causal)
+    check_shared(cache, q.nan_to_num(0.5, 0.5), ptable, [80, 3, 1], table, lens, causal=causal)
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -152,6 +155,27 @@ def test_broken_lengths(dev, each, Hq, H, T):
     q_lens = [T] * (3 * each)
     q_lens[0], q_lens[-1] = T + 1, -1
     check_shared(cache, q, ptable, [40, 0, 20], table, lens, q_lens=q_lens)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("each,Hq,H,T", WAYS)
+def test_infinite_queries(dev, each, Hq, H, T):
+    """Infinite scores as the softmax has them, in the prefix's tokens and a sequence's own: NaN
+    rows where one is +inf or none is finite, the others keep their numbers."""
+    gen = torch.Generator().manual_seed(T + 5)
+    B = 2 * each
+    cache, ptable, table = pools(gen, 2, B, 6, 9, H, 64, 16, dev)
+    cache.key.view(torch.uint8)[..., 7] = 0x38                               # 1.0
+    cache.key.view(torch.uint8)[int(ptable[0, 1]), :, 3, 9] = 0x38           # and one token's -1.0 elsewhere
+    cache.key.view(torch.uint8)[..., 9] = 0xB8
+    cache.key.view(torch.uint8)[int(ptable[0, 1]), :, 3, 9] = 0x38
+    q = torch.randn(B, Hq, T, 64, generator=gen).half()
+    q[0, 0, :, 7] = math.inf                                                 # every score +inf
+    q[1, 1, :, 7] = -math.inf                                                # every score -inf
+    q[1, 0, 0, 9] = -math.inf                                                # all +inf but one
+    q[0, 1, T // 2, 9] = math.inf                                            # one +inf in prefix 0, -inf elsewhere
+    q[-1, 1, T // 2, 9] = math.inf                                           # -inf alone
+    check_shared(cache, q, ptable, [90, 30], table, [T + b for b in range(B)], infinite=True)
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -240,9 +264,7 @@ def test_refusals():
                 lambda: cache.attend_shared(q, ptable, plens, table, lens, sm_scale=0.0),
                 lambda: cache.attend_shared(q, ptable, plens, table, lens, sm_scale=math.inf),
                 lambda: cache.attend_shared(q, ptable, plens, table, lens, out=q.float()),
-                lambda: cache.attend_shared(q, ptable, plens, table, lens, out=q[:, :1].expand(4, 4, 1, 64)),
-                lambda: cache.attend_shared(q, ptable, plens, table, lens, max_tokens=-1),
-                lambda: cache.attend_shared(q, ptable, plens, table, lens, max_prefix=1 << 31)):
+                lambda: cache.attend_shared(q, ptable, plens, table, lens, out=q[:, :1].expand(4, 4, 1, 64))):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(RuntimeError):
@@ -267,7 +289,7 @@ def test_abi_refusals():
     assert L.kitty_cache8_shared_attention(ctypes.byref(c), None, None) == _hip.KITTY_E_INVALID
     assert L.kitty_cache8_shared_attention(None, None, None) == _hip.KITTY_E_INVALID
     for kw in (dict(prefixes=0), dict(prefixes=-1), dict(prefixes=3), dict(batch=-1), dict(tokens=-1), dict(prefix_pages=-1),
-               dict(table_pages=-1), dict(plan_prefix=-1), dict(plan_tokens=-1), dict(num_q_heads=0), dict(dtype=2),
+               dict(table_pages=-1), dict(num_q_heads=0), dict(dtype=2),
                dict(sm_scale=0.0), dict(sm_scale=math.inf), dict(sm_scale=math.nan), dict(q=None), dict(out=None),
                dict(lens=None), dict(prefix_lens=None), dict(block_table=None), dict(prefix_table=None), dict(q=4098),
                dict(out=4104), dict(q_s_tok=4), dict(o_s_head=12), dict(workspace=None), dict(workspace=4100),

@@ -49,8 +49,9 @@ def want_weights(cache, q, table, lens, q_lens, causal, sm_scale, weights):
     return out, off + np.abs(out) * 2.0 ** -24
 
 
-def check_weighed(cache, q, table, lens, N=None, q_lens=None, causal=True, sm_scale=None, weights=None, **kw):
-    """Output and log-sum-exp as check_attend has them of attend, and the weights."""
+def check_weighed(cache, q, table, lens, N=None, q_lens=None, causal=True, sm_scale=None, weights=None, infinite=False, **kw):
+    """Output and log-sum-exp as check_attend has them of attend, and the weights; infinite: of rows
+    with infinite scores the log-sum-exp (-inf of no finite one, and +inf or NaN) is not looked at."""
     dev = cache.device
     gen = torch.Generator().manual_seed(len(lens))
     if weights is None:
@@ -71,7 +72,8 @@ def check_weighed(cache, q, table, lens, N=None, q_lens=None, causal=True, sm_sc
     out, lse = numpy(out), numpy(lse)
     np.testing.assert_array_equal(np.isnan(out), np.isnan(ref))
     assert not (np.abs(out - ref) > tol).any()
-    np.testing.assert_array_equal(np.isnan(lse), np.isnan(rlse))
+    if not infinite:
+        np.testing.assert_array_equal(np.isnan(lse), np.isnan(rlse))
     seen = np.isfinite(rlse)
     assert (lse[np.isneginf(rlse)] == -np.inf).all()
     room = (D + 8) * 2.0 ** -24 * mag[seen] + 2.0 ** -21 * (1 + np.abs(rlse[seen])) + n * 2.0 ** -24
@@ -88,7 +90,9 @@ SHAPES = [
     (2, 4, 1, 3, 128, 16, [2, 50]), (1, 8, 2, 4, 128, 128, [300]), (3, 4, 2, 8, 64, 32, [8, 100, 9]), (2, 6, 2, 9, 256, 16, [3, 90]),
     # chunks: heads that begin and end inside a block of rows, tokens that later queries alone see
     (1, 4, 2, 40, 128, 64, [40]), (2, 8, 2, 33, 64, 16, [33, 200]), (1, 3, 1, 130, 128, 128, [131]), (1, 4, 4, 70, 80, 32, [500]),
-    (2, 2, 1, 65, 256, 128, [64, 300]), (1, 4, 1, 100, 48, 16, [170])]
+    (2, 2, 1, 65, 256, 128, [64, 300]), (1, 4, 1, 100, 48, 16, [170]),
+    # rows in several parts, whose sums are added
+    (1, 4, 1, 150, 64, 16, [200]), (1, 3, 1, 200, 112, 32, [333]), (2, 2, 1, 300, 256, 16, [300, 31])]
 
 
 @pytest.mark.parametrize("dev", DEVICES)
@@ -150,6 +154,41 @@ def test_masked_and_missing_places(dev, Hq, T):
     check_weighed(cache, q, table, [n])
     cache.scale[0] = math.nan                    # page 0's scales stand for no missing page
     check_weighed(cache, q, table, [n], causal=False)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("T,wide", [(1, 0), (1, 500), (5, 0), (40, 500), (100, 0)])
+def test_infinite_queries(dev, T, wide):
+    """Infinite scores: the weights of what a row of NaN weights sees are NaN, a score of -inf
+    beside finite ones weighs nothing."""
+    gen = torch.Generator().manual_seed(T)
+    cache = filled(gen, 12, 2, 64, 16, dev)
+    cache.key.view(torch.uint8)[..., 7] = 0x38                               # 1.0
+    cache.key.view(torch.uint8)[..., 9] = 0x00
+    table = torch.cat([tables(gen, 1, 12, 12, dev), torch.zeros(1, wide, dtype=torch.int32, device=dev)], 1)
+    cache.key.view(torch.uint8)[int(table[0, 2]), 1, 5, 9] = 0xB8            # -1.0 in one token
+    q = torch.randn(1, 4, T, 64, generator=gen).half()
+    q[..., 9] = 1.0
+    q[0, 2, T // 2, 9] = 60000.0                                             # far below all others
+    check_weighed(cache, q, table, [180], N=192)
+    for row, value in (((0, 1, 0, 7), math.inf), ((0, 1, 0, 7), -math.inf)):
+        x = q.clone()
+        x[row] = value
+        w = check_weighed(cache, x, table, [180], N=192, infinite=True)
+        assert w[0, 0, :180 - T + 1].isnan().all() and w[0, 0, 180:].isfinite().all() and w[0, 1].isfinite().all()
+
+
+@pytest.mark.gpu
+def test_scores_beyond_a_gibibyte(dev):
+    """Weights for so many tokens that the scores of 16 rows are not kept: a second pass over the keys instead."""
+    gen = torch.Generator().manual_seed(3)
+    cache = filled(gen, 4, 1, 64, 256, dev)
+    q = torch.randn(1, 16, 1, 64, generator=gen).half()
+    for columns in (1 << 16, (1 << 16) + 1):
+        table = widened(tables(torch.Generator().manual_seed(9), 1, 4, 4, dev), columns)
+        weights = torch.zeros(1, 1, columns * 256, device=dev)
+        check_weighed(cache, q, table, [700], weights=weights, max_tokens=700)
+        assert (weights[..., 700:] == 0).all()
 
 
 @pytest.mark.parametrize("dev", DEVICES)
