@@ -58,23 +58,24 @@ __global__ __launch_bounds__(64 * kWeighWaves, DP <= 128 ? 3 : 1) void cache8_we
         const int tiles = (rows + kWeighRows - 1) / kWeighRows;
         const int begin = (int)((int64_t)tiles * part / w.parts), end = (int)((int64_t)tiles * (part + 1) / w.parts);
         const int tok0 = (int)first + 64 * wave;
-        // the thread's rows of the next tile to load, as (head, query); each tile is 32 rows on
+        // the thread's rows of the next tile to load: each tile is 32 rows on, by additions
         const int step_h = each ? kWeighRows / each : 0, step_t = kWeighRows - step_h * each;
-        int lr = begin * kWeighRows, lh[NP], lt[NP], nh, nt;
-        auto row_of = [&](int r, int &h, int &t) {
-            h = each ? r / each : 0;
-            t = r - h * each;
-        };
-        auto next_row = [&](int &h, int &t) {
-            h += step_h, t += step_t;
-            if (t >= each)
-                t -= each, ++h;
-        };
-#pragma unroll
-        for (int j = 0; j < NP; ++j)
-            row_of(lr + (int)threadIdx.x / CPR + PASS * j, lh[j], lt[j]);
-        row_of(lr + n, nh, nt);
+        const int64_t q_step = step_h * p.q_s_head + step_t * p.q_s_tok, q_wrap = p.q_s_head - each * p.q_s_tok;
         const int ch = 8 * (threadIdx.x % CPR);
+        int lr = begin * kWeighRows, lt[NP], nt = 0;
+        const uint16_t *src[NP];
+        const float2 *from = stat;
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int r = lr + (int)threadIdx.x / CPR + PASS * j, h = each ? r / each : 0;
+            lt[j] = r - h * each;
+            src[j] = qb + h * p.q_s_head + (t0 + lt[j]) * p.q_s_tok + ch;
+        }
+        if (wave == 0) {
+            const int h = each ? (lr + n) / each : 0;
+            nt = lr + n - h * each;
+            from = stat + (int64_t)h * p.T + t0 + nt;
+        }
         u32x4 buf[NP];
         float2 buf_stat = make_float2(0.0f, 0.0f);
         int buf_vis = 0;
@@ -83,15 +84,21 @@ __global__ __launch_bounds__(64 * kWeighWaves, DP <= 128 ? 3 : 1) void cache8_we
             for (int j = 0; j < NP; ++j) {
                 buf[j] = u32x4{0, 0, 0, 0};
                 if (lr + (int)threadIdx.x / CPR + PASS * j < rows && (!CUT || ch < p.c.D))
-                    buf[j] = *(const u32x4 *)(qb + lh[j] * p.q_s_head + (t0 + lt[j]) * p.q_s_tok + ch);
-                next_row(lh[j], lt[j]);
+                    buf[j] = *(const u32x4 *)src[j];
+                lt[j] += step_t;
+                src[j] += q_step;
+                if (lt[j] >= each)
+                    lt[j] -= each, src[j] += q_wrap;
             }
             if (wave == 0) {
                 const bool in = lr + n < rows;
-                buf_stat = in ? stat[(int64_t)nh * p.T + t0 + nt] : make_float2(0.0f, 0.0f);
+                buf_stat = in ? *from : make_float2(0.0f, 0.0f);
                 buf_vis = in ? visible8(p, sq, t0 + nt) : 0;
+                nt += step_t;
+                from += step_h * p.T + step_t;
+                if (nt >= each)
+                    nt -= each, from += p.T - each;
             }
-            next_row(nh, nt);
             lr += kWeighRows;
         };
         auto store = [&](int stage) {
