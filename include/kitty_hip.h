@@ -635,13 +635,13 @@ int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attenti
  * causal, row i is token prefix_lens[f] + lens[b] - q_lens[b] + i: where lens[b] <
  * q_lens[b] the first rows are tokens of the prefix.  A prefix whose length is negative
  * or more than prefix_pages pages hold gives NaN rows to its sequences.  batch is a
- * multiple of prefixes.  The work is split by the lengths alone.  Weights of bf16 calls
- * have the 16 bits of two terms where the rows of a prefix (its sequences' queries times
- * the group's heads) are at most 64 and a sequence's at most 32, and over a sequence's own
- * tokens where its rows are at most 32; elsewhere one fp16 term, as above. */
+ * multiple of prefixes.  Weights of bf16 calls have the 16 bits of two terms where the
+ * rows of a prefix (its sequences' queries times the group's heads) are at most 64 and a
+ * sequence's at most 32, and over a sequence's own tokens where its rows are at most 32;
+ * elsewhere one fp16 term, as above.  A workspace size of 0 needs none. */
 typedef struct {
     const uint16_t *q; /* (B, Hq, T, D), 16-byte aligned rows */
-    uint16_t *out;     /* (B, Hq, T, D), 16-byte aligned rows, q's type; may be q */
+    uint16_t *out;     /* (B, Hq, T, D), 16-byte aligned rows, q's type; may be q, row for row */
     float *lse;        /* (B, Hq, T) contiguous, or NULL */
     int64_t q_s_seq, q_s_head, q_s_tok, o_s_seq, o_s_head, o_s_tok;
     const int32_t *prefix_table; /* (prefixes, prefix_pages) page ids */

@@ -324,7 +324,8 @@ constexpr bool two_per_cu(int DP, int RT) { return DP <= 128 && DP * RT <= 256; 
 // CUT: D is below DP, and the lanes beyond it read nothing.  DIRECT: a workgroup takes
 // the whole of one (pair, row block) and writes its rows, so that no merge follows.
 // MODE kShared: the entries are prefixes and sequences, the latter of one row block each,
-// and all parts are left to cache8_join_kernel.
+// and all parts are left to cache8_join_kernel; with DIRECT the entries are sequences, and
+// each reads its prefix itself.
 //
 // Workgroup wg of the n_wg that share the work.
 template <int DP, int RT, bool DIRECT>
@@ -413,20 +414,12 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                 vis_min = min(vis_min, __shfl_xor(vis_min, off));
             vis_min = __builtin_amdgcn_readfirstlane(vis_min);
         }
-        const int end = min(tile1 * kUnit, vis_max);
-
-        const int32_t *table = table8<SHARED>(p, sq, b);
-        const int last = (sq.n - 1) >> p.c.lg, lg = p.c.lg;
+        const int lg = p.c.lg;
         const uint8_t *kp = p.c.key + kh * p.c.key_s_head, *vp = p.c.value + kh * p.c.value_s_head;
         const float *sp = p.c.scale + kh * p.c.scale_s_head;
         const uint32_t k_lane = (uint32_t)n * p.c.key_s_tok + 16 * g;
         const uint32_t v_ch = CUT && CB * n >= p.c.D ? 0 : CB * n;
         const uint32_t v_lane = (uint32_t)(4 * g) * p.c.value_s_tok + v_ch;
-        auto ids = [&](int tok, int (&id)[2]) {
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-                id[hf] = uniform_load(table + min((tok + 16 * hf) >> lg, last));
-        };
         auto load = [&](int tok, const int (&id)[2], RowBuf<DP, RT> &buf) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
@@ -462,12 +455,19 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         const uint32_t sc_step = 64 * rows_all, sc_bytes = SCORES ? (uint32_t)(p.sc_cap * rows_all * 4) : 0;
         const __amdgpu_buffer_rsrc_t scores = __builtin_amdgcn_make_buffer_rsrc(
             SCORES ? (void *)(p.scores + (int64_t)(b * p.c.H + kh) * rows_all * p.sc_cap) : nullptr, 0, sc_bytes, 0x00027000);
+        // The wave's steps from token `tok` to `end`, of pages table[0 .. last].
         // A ring of NB steps' codes, NB - 1 in flight while one is computed; the page
         // ids of the next load are fetched a step before it.  Loads past the wave's
         // last step repeat that step's: a branch around them would make every wait
         // one for all loads.
-        int tok = tile * kUnit + 32 * wave;
-        if (tok < end) {
+        auto stream = [&](const int32_t *table, int last, int vis_min, int vis_max, int tok, int end) {
+            if (tok >= end)
+                return;
+            auto ids = [&](int tok, int (&id)[2]) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+                    id[hf] = uniform_load(table + min((tok + 16 * hf) >> lg, last));
+            };
             const int final = tok + (end - 1 - tok) / STRIDE * STRIDE;
             RowBuf<DP, RT> ring[NB];
             int id[NB][2];
@@ -492,7 +492,36 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                     more = tok < end;
                 }
             }
+        };
+        // DIRECT and SHARED: the prefix's tokens first, then the sequence's own
+        Seq8 before{};
+        auto in_prefix = [&](int t) {   // tokens of the prefix that row t sees
+            if (before.bad || sq.bad || t >= sq.tq)
+                return 0;
+            return p.causal ? max(before.n + min(sq.n - sq.tq + t + 1, 0), 0) : before.n;
+        };
+        if constexpr (DIRECT && SHARED) {
+            const int f = b / p.per;
+            before.n = p.prefix_lens[f];
+            before.bad = before.n < 0 || before.n > (int64_t)p.prefix_pages << lg || (before.n > 0 && p.c.num_pages == 0);
+            int own[RT], least = max(before.n, 0);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const int t = (16 * rt + n) / p.gq;
+                own[rt] = W.vis[rt];
+                W.vis[rt] = in_prefix(t);
+                least = t < sq.tq ? min(least, W.vis[rt]) : least;
+            }
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1)
+                least = min(least, __shfl_xor(least, off));
+            const int most = before.bad || sq.bad || sq.tq <= 0 ? 0 : before.n;
+            stream(p.prefix_table + f * p.pt_stride, (before.n - 1) >> lg, __builtin_amdgcn_readfirstlane(least), most, 32 * wave, most);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                W.vis[rt] = own[rt];
         }
+        stream(table8<SHARED>(p, sq, b), (sq.n - 1) >> lg, vis_min, vis_max, tile * kUnit + 32 * wave, min(tile1 * kUnit, vis_max));
 
         // the waves' rows joined
 #pragma unroll
@@ -533,15 +562,16 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                 l += f * ml[w].y;
                 acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
             }
-            if (SHARED || !whole) {
+            if ((SHARED && !DIRECT) || !whole) {
                 *(float4 *)(p.ws_o + ((int64_t)slot * RM + r) * DP + ch) = acc;
                 if (ch == 0)
                     p.ws_ml[slot * RM + r] = make_float2(m, l);
                 continue;
             }
             const int t = (r0 + r) / p.gq, h = kh * p.gq + (r0 + r) - t * p.gq;
-            const bool none = !sq.bad && visible8(p, sq, t) == 0;
-            const float inv = sq.bad ? __builtin_nanf("") : none ? 0.0f : 1.0f / l;
+            const bool bad = sq.bad || (DIRECT && SHARED && before.bad);
+            const bool none = !bad && visible8(p, sq, t) == 0 && !(DIRECT && SHARED && in_prefix(t) > 0);
+            const float inv = bad ? __builtin_nanf("") : none ? 0.0f : 1.0f / l;
             if (none)   // steps that no row masks went into its sums too, NaN among them
                 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (!CUT || ch < p.c.D)
@@ -550,7 +580,7 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                                (uint32_t)f2x(acc.z * inv, BF16) | (uint32_t)f2x(acc.w * inv, BF16) << 16);
             if (ch == 0 && p.lse)
                 p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
-                    sq.bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
+                    bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
             if (STAT && ch == 0 && p.stat)
                 p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
             if (SCORES && DIRECT && ch == 0)

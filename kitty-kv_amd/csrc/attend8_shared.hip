@@ -280,8 +280,17 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_shared_
     }
 }
 
+// What takes a call, by its sizes.
+// 1. Whole sequences, prefix and all, a workgroup for each and KV head, where a stream of
+//    both is at most kSharedDirectBytes and the workgroups at most the CUs: one launch.
+// 2. The row kernel for prefixes and sequences together: up to 64 rows of a prefix, in
+//    blocks of 32, and 32 of a sequence.
+// 3. cache8_shared_kernel.
+constexpr int64_t kSharedDirectBytes = 1280 * 128;
+
 struct SharedPlan8 {
     int DP, RT;               // RT: own row blocks, 0 where they are tiles
+    bool direct;              // one launch of the row kernel on whole sequences
     bool together;            // one launch of the row kernel for prefixes and sequences, RT blocks
     int W, nrb, own_nrb;      // workgroups; row blocks of a prefix and of a sequence
     int64_t items, own_items; // of the prefixes, of the sequences
@@ -298,8 +307,13 @@ static int plan_shared(const Cache8 &c, const kitty_cache8_shared_args &a, Share
     const int64_t F = a.prefixes, B = a.batch, H = c.H;
     const int cus = device_cus();
     pl.DP = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
-    pl.together = prefix_rows <= 64 && own_rows <= 32;
     const bool by_rows = own_rows <= 32;
+    pl.direct = by_rows && pl.DP <= 128 && (prefix_cap + own_cap) * pl.DP <= kSharedDirectBytes && B * H <= cus;
+    if (pl.direct) {
+        pl.RT = own_rows <= 16 ? 1 : 2;
+        return KITTY_OK;
+    }
+    pl.together = prefix_rows <= 64 && by_rows;
     pl.RT = by_rows ? (pl.together ? prefix_rows : own_rows) <= 16 ? 1 : 2 : 0;
     const int RM = by_rows ? 16 * pl.RT : kTileRows;
     pl.nrb = (int)((prefix_rows + (pl.together ? RM : kTileRows) - 1) / (pl.together ? RM : kTileRows));
@@ -433,7 +447,7 @@ extern "C" int kitty_cache8_shared_attention_workspace_size(const kitty_cache8 *
                                                             size_t *bytes)
 {
     Cache8 c;
-    SharedPlan8 pl;
+    SharedPlan8 pl{};
     if (!bytes)
         return fail(KITTY_E_INVALID, "bytes is NULL");
     if (const int rc = check_shared(cache, args, c))
@@ -451,7 +465,7 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
                                              kitty_stream_t stream)
 {
     Attend8 p{};
-    SharedPlan8 pl;
+    SharedPlan8 pl{};
     if (const int rc = check_shared(cache, args, p.c))
         return rc;
     const kitty_cache8_shared_args &a = *args;
@@ -466,7 +480,7 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
             return fail(KITTY_E_INVALID, "strides of q and out must be multiples of 8 elements (16-byte rows)");
     if (const int rc = plan_shared(p.c, a, pl))
         return rc;
-    if (!a.workspace || !aligned(a.workspace, 16) || a.workspace_bytes < pl.bytes)
+    if ((!a.workspace && pl.bytes) || !aligned(a.workspace, 16) || a.workspace_bytes < pl.bytes)
         return fail(KITTY_E_INVALID,
                     "workspace is NULL, misaligned or smaller than kitty_cache8_shared_attention_workspace_size");
     p.q = a.q, p.out = a.out, p.lse = a.lse;
@@ -482,7 +496,7 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
     const hipStream_t st = (hipStream_t)stream;
     const dim3 block(64 * kWaves);
     char *ws = (char *)a.workspace;
-    if (a.q_lens && !pl.together) {
+    if (a.q_lens && !pl.together && !pl.direct) {
         p.row_map = (int32_t *)(ws + pl.map_at), p.row_first = p.row_map + (int64_t)p.B * p.T, p.row_count = p.row_first + p.B;
         hipLaunchKernelGGL(cache8_shared_queries_kernel, dim3((unsigned)((p.F + kWaves - 1) / kWaves)), block, 0, st, p);
     }
@@ -490,7 +504,7 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
     Attend8 x = p, y = p;     // the launch's tile entries, or all of them; its row entries
     x.e0 = 0, x.entries = pl.together || pl.RT == 0 ? p.F + p.B : p.F;
     x.ws_o = (float *)(ws + pl.o_at), x.ws_ml = (float2 *)(ws + pl.ml_at), x.ws_tab = (int2 *)(ws + pl.tab_at);
-    y.e0 = p.F, y.entries = p.B, y.item0 = 0;
+    y.e0 = p.F, y.entries = p.B, y.item0 = 0, y.nrb = pl.direct ? 1 : y.nrb;
     y.ws_o = (float *)(ws + pl.own_o_at), y.ws_ml = (float2 *)(ws + pl.own_ml_at), y.ws_tab = (int2 *)(ws + pl.own_tab_at);
     const bool apart = !pl.together && pl.RT != 0;
     const int tile_rows = pl.together ? 16 * pl.RT : kTileRows, own_rows = pl.RT ? 16 * pl.RT : kTileRows;
@@ -500,6 +514,16 @@ extern "C" int kitty_cache8_shared_attention(const kitty_cache8 *cache, const ki
     auto go = [&](auto dp, auto bf, auto cut) {
         constexpr int DP = decltype(dp)::value;
         constexpr bool BF = decltype(bf)::value, CUT = decltype(cut)::value;
+        if constexpr (DP <= 128) {
+            if (pl.direct) {
+                const dim3 pairs((unsigned)(p.B * p.c.H));
+                if (pl.RT == 1)
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, 1, BF, CUT, true, kShared>), pairs, dim3(64 * row_waves(1, true)), 0, st, y);
+                else
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, 2, BF, CUT, true, kShared>), pairs, dim3(64 * row_waves(2, true)), 0, st, y);
+                return;
+            }
+        }
         if (pl.together) {
             if (pl.RT == 1)
                 hipLaunchKernelGGL((cache8_rows_kernel<DP, 1, BF, CUT, false, kShared>), grid, block, 0, st, x);

@@ -84,7 +84,7 @@ template <int EACH>
 __global__ __launch_bounds__(kSelect) void cache8_select_kernel(Evict8 p)
 {
     __shared__ __attribute__((aligned(16))) unsigned hist[kCopies][kBins], sums[2][kSelectWaves];
-    __shared__ unsigned found[2];
+    __shared__ unsigned found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int b = blockIdx.x / p.c.H, h = blockIdx.x - b * p.c.H;
     const int n = p.lens[b], m = kept8(p, n);
@@ -152,12 +152,17 @@ __global__ __launch_bounds__(kSelect) void cache8_select_kernel(Evict8 p)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 if (before < (unsigned)need && before + c[e] >= (unsigned)need)
-                    found[0] = kBins - 1 - 2 * tid - e, found[1] = need - before;
+                    found[0] = kBins - 1 - 2 * tid - e, found[1] = need - before, found[2] = c[e];
                 before += c[e];
             }
             __syncthreads();
             key |= found[0] << shift;
             need = (int)found[1];
+            if (found[2] == found[1]) {   // all of the bin stay: often but one token is left in it
+                key -= key ? 1 : 0;
+                need = 0;
+                break;
+            }
         }
     } else if (m == 0) {
         key = 0xffffffffu;     // none stays (first and last are 0)

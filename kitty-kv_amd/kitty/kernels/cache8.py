@@ -440,24 +440,28 @@ class Cache8:
             with torch.cuda.device(self._index):      # the plan is the pools' device's
                 _hip.check(self._lib.kitty_cache8_shared_attention_workspace_size(
                     self._ref, _SHARED.pack(0, 0, 0, *head, 0, tables[0], 0, 0, tables[1], 0, 0, *rest, 0, 0), ctypes.byref(size)))
-            found = self._keep(sig, (in_place, q.is_contiguous(), packed, head, tables, rest, size.value))
-        (q_ok, out_ok), like_q, packed, head, tables, rest, need = found
-        if not q_ok or q.data_ptr() % 16:
-            q = q.clone(memory_format=torch.contiguous_format)
-            head = (*packed, *head[3:])
-        o = out
+            found = self._keep(sig, (in_place, q.is_contiguous(), packed, head, tables, rest, size.value,
+                                     None if out is None else (_span(q), _span(out), _strides(q) == _strides(out))))
+        (q_ok, out_ok), like_q, packed, head, tables, rest, need, spans = found
+        qp, o = q.data_ptr(), out
         if out is None or not out_ok or out.data_ptr() % 16 or out.is_neg():
             o = torch.empty_like(q) if like_q else torch.empty(q.shape, dtype=q.dtype, device=q.device)
             if out is not None:
                 head = (*head[:3], *packed)
         else:
             _written(out)
+            op = out.data_ptr()
+            # rows of out over other rows of q, which may be read after they are written
+            q_ok = q_ok and not (qp < op + spans[1] and op < qp + spans[0] and not (qp == op and spans[2]))
+        if not q_ok or qp % 16:
+            q = q.clone(memory_format=torch.contiguous_format)
+            head = (*packed, *head[3:])
         lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device) if return_lse else None
-        ws = q.new_empty((need + 1) // 2)      # of the call's own, as attend's
+        ws = q.new_empty((need + 1) // 2) if need else None      # of the call's own, as attend's
         self._launch(self._lib.kitty_cache8_shared_attention, _SHARED.pack(
             q.data_ptr(), o.data_ptr(), 0 if lse is None else lse.data_ptr(), *head, prefix_table.data_ptr(), tables[0],
             prefix_lens.data_ptr(), block_table.data_ptr(), tables[1], lens.data_ptr(),
-            0 if q_lens is None else q_lens.data_ptr(), *rest, ws.data_ptr(), need))
+            0 if q_lens is None else q_lens.data_ptr(), *rest, 0 if ws is None else ws.data_ptr(), need))
         if out is not None and o is not out:
             out.copy_(o)
             o = out

@@ -107,7 +107,7 @@ def copy_pools(a, b):
 # queries of attend_shared and attend_weighed: each of the shared ways, weights from scores (whole contexts in
 # one launch, split), from tiles in one part and several
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,T2,Hq,W", [(1, 1, 4, 20), (40, 30, 4, 20), (8, 8, 4, 20), (5, 1, 16, 140), (12, 200, 4, 60), (1, 700, 2, 20)])
+@pytest.mark.parametrize("T,T2,Hq,W", [(1, 1, 4, 20), (40, 30, 4, 20), (8, 8, 4, 20), (3, 2, 4, 100), (5, 1, 16, 140), (12, 200, 4, 60), (1, 700, 2, 20)])
 def test_captured(dev, T, T2, Hq, W):
     """In a graph, replayed with other lengths, pages, queries and weights in the same tensors,
     other work and synchronisations between: every replay is the eager call."""
@@ -317,6 +317,7 @@ def shared_way(B, F, Hq, H, T, D, G, Wp, W, plan=256):
     own, DP = Hq // H * T, 64 if D <= 64 else 128 if D <= 128 else 256
     prefix = own * (B // F)
     rows, both = own <= 32, prefix <= 64 and own <= 32
+    whole = rows and D <= 128 and (Wp + W) * G * DP <= 1280 * 128 and B * H <= plan
     RT = 0 if not rows else 1 if (prefix if both else own) <= 16 else 2
     RM = 16 * RT if rows else 128
     nrb = -(-prefix // (RM if both else 128))
@@ -334,6 +335,8 @@ def shared_way(B, F, Hq, H, T, D, G, Wp, W, plan=256):
         size = area(2 * WG + items, 128, items) + area(2 * WG + own_items, RM, own_items)
     if not both:
         size += up((B * T + B + F) * 4)
+    if whole:
+        size = 0
     c = _hip.Cache8(4096, 8192, 16384, H * G * D, G * D, D, H * G * D, G * D, D, 2 * H, 2, 4, H, D, G)
     a = _hip.Cache8SharedArgs()
     a.prefixes, a.batch, a.num_q_heads, a.tokens, a.prefix_pages, a.table_pages, a.sm_scale = F, B, Hq, T, Wp, W, 1.0
@@ -341,7 +344,7 @@ def shared_way(B, F, Hq, H, T, D, G, Wp, W, plan=256):
     L = _hip.load()
     assert L.kitty_cache8_shared_attention_workspace_size(ctypes.byref(c), ctypes.byref(a), ctypes.byref(got)) == _hip.KITTY_OK
     assert got.value == size, (got.value, size)
-    return "rows" if both else "tiles and rows" if rows else "tiles"
+    return "whole" if whole else "rows" if both else "tiles and rows" if rows else "tiles"
 
 
 def test_every_way_is_tested():
@@ -350,12 +353,15 @@ def test_every_way_is_tested():
     met = set()
     for F, each, Hq, H, T, D, G, plens, lens in SHAPES:
         W = [max(1, -(-max(n) // G)) for n in (plens, lens)]
-        met.add((shared_way(F * each, F, Hq, H, T, D, G, *W), 64 if D <= 64 else 128 if D <= 128 else 256))
-    assert met == {(w, d) for w in ("rows", "tiles and rows", "tiles") for d in (64, 128, 256)}
-    assert [shared_way(2 * e, 2, Hq, H, T, 64, 16, 8, 9) for e, Hq, H, T in WAYS] == ["rows", "tiles and rows", "tiles"]
-    assert shared_way(16, 1, 4, 1, 1, 128, 16, 8, 8) == "rows" and shared_way(17, 1, 4, 1, 1, 128, 16, 8, 8) == "tiles and rows"
-    assert shared_way(1, 1, 33, 1, 1, 128, 16, 8, 8) == "tiles" and shared_way(1, 1, 32, 1, 1, 128, 16, 8, 8) == "rows"
-    assert shared_way(600, 300, 4, 2, 2, 256, 16, 99, 99) == "rows"
+        for wide in (0, 4096 // G):
+            met.add((shared_way(F * each, F, Hq, H, T, D, G, W[0] + wide, W[1] + wide), 64 if D <= 64 else 128 if D <= 128 else 256))
+    assert met == {(w, d) for w in ("whole", "rows", "tiles and rows", "tiles") for d in (64, 128, 256)} - {("whole", 256)}
+    ways = ["whole", "whole", "rows", "tiles and rows", "tiles"]
+    assert [shared_way(2 * e, 2, Hq, H, T, 64, 16, 8, 9 + wide) for e, Hq, H, T, wide in WAYS] == ways
+    assert shared_way(16, 1, 4, 1, 1, 128, 16, 40, 41) == "rows" and shared_way(17, 1, 4, 1, 1, 128, 16, 40, 41) == "tiles and rows"
+    assert shared_way(16, 1, 4, 1, 1, 128, 16, 40, 40) == "whole" and shared_way(1, 1, 32, 1, 1, 128, 16, 40, 40) == "whole"
+    assert shared_way(1, 1, 33, 1, 1, 128, 16, 8, 8) == "tiles" and shared_way(1, 1, 32, 1, 1, 128, 16, 40, 41) == "rows"
+    assert shared_way(600, 300, 4, 2, 2, 256, 16, 99, 99) == "rows" and shared_way(129, 1, 2, 2, 1, 64, 16, 8, 8) == "tiles and rows"
 
 
 def test_references_agree():

@@ -39,13 +39,15 @@ def check_shared(cache, q, ptable, plens, table, lens, q_lens=None, causal=True,
     return out
 
 
-def pools(gen, F, B, Wp, W, H, D, G, dev, spare=1):
-    """A filled cache, tables of prefixes and sequences with pages of their own; page 0 is no one's."""
+def pools(gen, F, B, Wp, W, H, D, G, dev, spare=1, wide=0):
+    """A filled cache, tables of prefixes and sequences with pages of their own; page 0 is no one's.  wide: columns of
+    the sequences' table that name no pages (its width says whether a call is one launch)."""
     P = F * Wp + B * W + spare
     cache = filled(gen, P, H, D, G, dev)
     cache.scale[::3] *= 1.61                     # not only powers of two
     ids = (1 + torch.randperm(P - 1, generator=gen)).to(torch.int32)
-    return cache, ids[:F * Wp].view(F, Wp).to(dev), ids[F * Wp:F * Wp + B * W].view(B, W).to(dev)
+    own = torch.cat([ids[F * Wp:F * Wp + B * W].view(B, W), torch.full((B, wide), 1 << 30, dtype=torch.int32)], 1)
+    return cache, ids[:F * Wp].view(F, Wp).to(dev), own.to(dev)
 
 
 # prefixes and sequences: (prefixes, sequences of each, query heads, KV heads, queries, head size, page, prefix lengths, own lengths)
@@ -75,24 +77,25 @@ def test_matches_float64(dev, dtype, causal, F, each, Hq, H, T, D, G, plens, len
     cache, ptable, table = pools(gen, F, F * each, Wp, W, H, D, G, dev)
     q = torch.randn(F * each, Hq, T, D, generator=gen).to(dtype)
     check_shared(cache, q, ptable, plens, table, lens, causal=causal)
-    # tables that could hold far more
+    # tables that could hold far more: never whole sequences in one launch
     wide = [torch.cat([t, torch.full((t.shape[0], 4096 // G), 1 << 30, dtype=torch.int32, device=dev)], 1) for t in (ptable, table)]
     check_shared(cache, q, wide[0], plens, wide[1], lens, causal=causal)
 
 
-# (sequences of each, query heads, KV heads, queries): one launch, tiles and rows, tiles
-WAYS = [(2, 4, 2, 6), (5, 4, 2, 16), (2, 4, 2, 70)]
+# (sequences of each, query heads, KV heads, queries, wide): whole sequences of 16 rows and of 32, rows, tiles and
+# rows, tiles
+WAYS = [(2, 4, 2, 6, 0), (5, 4, 2, 16, 0), (2, 4, 2, 6, 300), (5, 4, 2, 16, 300), (2, 4, 2, 70, 0)]
 
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("causal", [True, False])
-@pytest.mark.parametrize("each,Hq,H,T", WAYS)
-def test_padded_rows_and_rows_in_the_prefix(dev, dtype, causal, each, Hq, H, T):
+@pytest.mark.parametrize("each,Hq,H,T,wide", WAYS)
+def test_padded_rows_and_rows_in_the_prefix(dev, dtype, causal, each, Hq, H, T, wide):
     """Padded queries, sequences without queries or without tokens, queries that are tokens
     of the prefix themselves, and more of them than both hold."""
     gen = torch.Generator().manual_seed(T)
-    cache, ptable, table = pools(gen, 3, 3 * each, 5, 9, H, 64, 16, dev)
+    cache, ptable, table = pools(gen, 3, 3 * each, 5, 9, H, 64, 16, dev, wide=wide)
     q = torch.randn(3 * each, Hq, T, 64, generator=gen).to(dtype)
     lens = [(0, 130, 2, T, 1, 140)[b % 6] for b in range(3 * each)]
     q_lens = [(T, 1, T // 2, 0, T, T - 1, 3)[b % 7] for b in range(3 * each)]
@@ -106,13 +109,13 @@ def test_padded_rows_and_rows_in_the_prefix(dev, dtype, causal, each, Hq, H, T):
 
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", [F16, BF16])
-@pytest.mark.parametrize("each,Hq,H,T", WAYS)
-def test_masked_and_missing_places(dev, dtype, each, Hq, H, T):
+@pytest.mark.parametrize("each,Hq,H,T,wide", WAYS)
+def test_masked_and_missing_places(dev, dtype, each, Hq, H, T, wide):
     """NaN codes behind the last tokens, NaN keys and values that some rows see, missing
     pages of the prefix and of one sequence: they reach the rows that see them alone."""
     gen = torch.Generator().manual_seed(T + 1)
     B, G = 2 * each, 16
-    cache, ptable, table = pools(gen, 2, B, 8, 9, H, 128, G, dev)
+    cache, ptable, table = pools(gen, 2, B, 8, 9, H, 128, G, dev, wide=wide)
     q = torch.randn(B, Hq, T, 128, generator=gen).to(dtype)
     plens, lens = [100, 97], [(75, 0, 3, 130, 16, 1)[b % 6] for b in range(B)]
     q_lens = [(T, 2, T - 1)[b % 3] for b in range(B)]
@@ -142,14 +145,14 @@ def test_masked_and_missing_places(dev, dtype, each, Hq, H, T):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("each,Hq,H,T", WAYS)
-def test_broken_lengths(dev, each, Hq, H, T):
+@pytest.mark.parametrize("each,Hq,H,T,wide", WAYS)
+def test_broken_lengths(dev, each, Hq, H, T, wide):
     """Lengths that break the rules give NaN rows to their sequences alone: to all of a prefix, or to one."""
     gen = torch.Generator().manual_seed(T + 2)
-    cache, ptable, table = pools(gen, 3, 3 * each, 3, 9, H, 64, 16, dev)
+    cache, ptable, table = pools(gen, 3, 3 * each, 3, 9, H, 64, 16, dev, wide=wide)
     q = torch.randn(3 * each, Hq, T, 64, generator=gen).half()
     lens = [100] * (3 * each)
-    lens[1], lens[-1] = -1, 9 * 16 + 1
+    lens[1], lens[-1] = -1, (9 + wide) * 16 + 1
     check_shared(cache, q, ptable, [48, 49, 20], table, lens)
     check_shared(cache, q, ptable, [-1, 0, 1 << 30], table, lens)
     q_lens = [T] * (3 * each)
@@ -158,13 +161,13 @@ def test_broken_lengths(dev, each, Hq, H, T):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("each,Hq,H,T", WAYS)
-def test_infinite_queries(dev, each, Hq, H, T):
+@pytest.mark.parametrize("each,Hq,H,T,wide", WAYS)
+def test_infinite_queries(dev, each, Hq, H, T, wide):
     """Infinite scores as the softmax has them, in the prefix's tokens and a sequence's own: NaN
     rows where one is +inf or none is finite, the others keep their numbers."""
     gen = torch.Generator().manual_seed(T + 5)
     B = 2 * each
-    cache, ptable, table = pools(gen, 2, B, 6, 9, H, 64, 16, dev)
+    cache, ptable, table = pools(gen, 2, B, 6, 9, H, 64, 16, dev, wide=wide)
     cache.key.view(torch.uint8)[..., 7] = 0x38                               # 1.0
     cache.key.view(torch.uint8)[int(ptable[0, 1]), :, 3, 9] = 0x38           # and one token's -1.0 elsewhere
     cache.key.view(torch.uint8)[..., 9] = 0xB8
@@ -179,13 +182,13 @@ def test_infinite_queries(dev, each, Hq, H, T):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("each,Hq,H,T", WAYS)
-def test_layouts(dev, each, Hq, H, T):
+@pytest.mark.parametrize("each,Hq,H,T,wide", WAYS)
+def test_layouts(dev, each, Hq, H, T, wide):
     """Queries and outputs in other memory orders, unaligned, negated, one memory for both;
     pools of other strides; prefix and own pages the same; a scale of the program's own."""
     gen = torch.Generator().manual_seed(T + 3)
     D, B = 64, 2 * each
-    cache, ptable, table = pools(gen, 2, B, 8, 9, H, D, 16, dev)
+    cache, ptable, table = pools(gen, 2, B, 8, 9, H, D, 16, dev, wide=wide)
     q = torch.randn(B, Hq, T, D, generator=gen).half()
     lens = [T + b for b in range(B)]
     args = [ptable, i32([100, 128], dev), table, i32(lens, dev)]
@@ -214,7 +217,7 @@ def test_layouts(dev, each, Hq, H, T):
     turned = [t.view(torch.uint8).permute(2, 1, 0, 3).contiguous().permute(2, 1, 0, 3) for t in (cache.key, cache.value)]
     other = Cache8(*(t.view(torch.float8_e4m3fn) for t in turned), cache.scale.transpose(0, 1).contiguous().transpose(0, 1))
     assert torch.equal(other.attend_shared(q, *args, sm_scale=0.2), want)
-    check_shared(cache, q.cpu(), ptable, [100, 128], ptable[:1].expand(B, -1), [T] * B)
+    check_shared(cache, q.cpu(), ptable, [100, 128], ptable[:1].expand(B, -1), [min(T, 128)] * B)
     # one prefix of no pages at all, and a batch of none
     none = torch.zeros(1, 0, dtype=torch.int32, device=dev)
     check_shared(cache, q.cpu(), none, [0], table, lens)
@@ -280,7 +283,7 @@ def test_abi_refusals():
     def call(fn=L.kitty_cache8_shared_attention, **kw):
         a = _hip.Cache8SharedArgs()
         a.q = a.out = a.prefix_table = a.prefix_lens = a.block_table = a.lens = a.workspace = 4096
-        a.prefixes, a.batch, a.num_q_heads, a.tokens, a.prefix_pages, a.table_pages = 2, 4, 2, 1, 4, 4
+        a.prefixes, a.batch, a.num_q_heads, a.tokens, a.prefix_pages, a.table_pages = 2, 4, 2, 1, 4, 400
         a.sm_scale, a.workspace_bytes = 1.0, 1 << 40
         for k, v in kw.items():
             setattr(a, k, v)
@@ -303,6 +306,7 @@ def test_abi_refusals():
     assert call(get, batch=0) == _hip.KITTY_OK and size.value == 0
     assert call(get) == _hip.KITTY_OK and size.value > 0
     assert call(workspace_bytes=size.value - 1) == _hip.KITTY_E_INVALID
+    assert call(get, table_pages=4) == _hip.KITTY_OK and size.value == 0       # one launch
     assert call(lambda cache, args, _: L.kitty_cache8_shared_attention_workspace_size(cache, args, None)) == _hip.KITTY_E_INVALID
 
 
