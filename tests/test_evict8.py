@@ -83,7 +83,7 @@ SHAPES = [
     (1, 1, 16, 16, [1], 1, 0, 0), (1, 1, 16, 16, [2], 1, 0, 0), (2, 2, 64, 16, [40, 17], 16, 1, 4), (1, 8, 128, 128, [300], 200, 4, 64),
     (3, 2, 80, 32, [0, 100, 500], 77, 3, 0), (1, 3, 128, 64, [700], 699, 0, 0), (2, 1, 256, 256, [511, 256], 256, 10, 10),
     (1, 2, 48, 16, [333], 64, 32, 32), (1, 1, 64, 32, [1030], 1, 0, 1), (2, 2, 32, 16, [1024, 1025], 1000, 0, 0),
-    (1, 1, 16, 16, [5000], 2100, 1024, 1000), (4, 1, 192, 64, [64, 65, 0, 128], 64, 0, 63), (1, 2, 144, 128, [90], 0, 0, 0), (70, 1, 16, 16, list(range(70)), 33, 2, 5)]
+    (1, 1, 16, 16, [5000], 2100, 1024, 1000), (1, 1, 16, 256, [2100], 2048, 0, 9), (2, 1, 112, 32, [1300, 1171], 1170, 7, 0), (2, 1, 48, 64, [2700, 10], 2049, 7, 0), (4, 1, 192, 64, [64, 65, 0, 128], 64, 0, 63), (1, 2, 144, 128, [90], 0, 0, 0), (70, 1, 16, 16, list(range(70)), 33, 2, 5)]
 
 
 @pytest.mark.parametrize("dev", DEVICES)
