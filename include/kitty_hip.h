@@ -635,9 +635,10 @@ int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attenti
  * causal, row i is token prefix_lens[f] + lens[b] - q_lens[b] + i: where lens[b] <
  * q_lens[b] the first rows are tokens of the prefix.  A prefix whose length is negative
  * or more than prefix_pages pages hold gives NaN rows to its sequences.  batch is a
- * multiple of prefixes.  Weights of bf16 calls have the 16 bits of two terms where the
- * rows of a prefix (its sequences' queries times the group's heads) are at most 64 and a
- * sequence's at most 32, and over a sequence's own tokens where its rows are at most 32;
+ * multiple of prefixes; a row of each table together name 2^30 tokens at most.  Weights
+ * of bf16 calls have the 16 bits of two terms where the rows of a prefix (its sequences'
+ * queries times the group's heads) are at most 64 and a sequence's at most 32, and over
+ * a sequence's own tokens where its rows are at most 32;
  * elsewhere one fp16 term, as above.  A workspace size of 0 needs none. */
 typedef struct {
     const uint16_t *q; /* (B, Hq, T, D), 16-byte aligned rows */
@@ -686,7 +687,7 @@ int kitty_cache8_weighed_attention(const kitty_cache8 *cache, const kitty_cache8
  * earlier; both zeros are equal, NaN is heavier than all else, as torch.sort has it).
  * They become tokens 0 .. m - 1, in their order, of the pages that row b of `into`
  * names, or of block_table where into is NULL (pages of `into` must not be among those
- * that the call reads; no page may be written for two sequences).  A page's scale
+ * that the call reads; no page may be written twice, for two sequences or for one).  A page's scale
  * becomes the largest of the pages that its tokens come from, and a code c of one with
  * another scale s becomes e4m3(c * (s / scale)), both in fp32; others move as they are.
  * Rows behind the last token keep their bytes.

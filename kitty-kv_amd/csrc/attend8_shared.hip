@@ -434,8 +434,8 @@ static int check_shared(const kitty_cache8 *cache, const kitty_cache8_shared_arg
         return fail(KITTY_E_INVALID, "dtype must be KITTY_DTYPE_F16 or KITTY_DTYPE_BF16");
     if (!(a.sm_scale > 0.0f) || a.sm_scale > 1e30f)
         return fail(KITTY_E_INVALID, "sm_scale must be positive and finite");
-    if ((int64_t)a.table_pages << c.lg > 1 << 30 || (int64_t)a.prefix_pages << c.lg > 1 << 30)
-        return fail(KITTY_E_UNSUPPORTED, "a block table is limited to 2^30 tokens a sequence");
+    if (((int64_t)a.table_pages + a.prefix_pages) << c.lg > 1 << 30)   // a row's place is an int
+        return fail(KITTY_E_UNSUPPORTED, "a sequence and its prefix are limited to 2^30 tokens together");
     return KITTY_OK;
 }
 

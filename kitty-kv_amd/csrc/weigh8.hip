@@ -266,7 +266,7 @@ __global__ __launch_bounds__(256) void cache8_weigh_sum_kernel(Weigh8 w)
 //
 // Up to 16 rows the scores are kept instead: reading and writing them is 8 bytes a row and
 // token where reading the keys again is head_dim, and costs products as well.  A gigabyte
-// of them at most.
+// of them at most, or of the parts' sums.
 struct WeighPlan8 {
     bool scores;
     int64_t cap;
@@ -290,7 +290,7 @@ static WeighPlan8 plan_weigh(const Cache8 &c, const kitty_cache8_attention_args 
     }
     const int64_t known = a.plan_tokens > 0 ? std::min<int64_t>(a.plan_tokens, pl.cap) : pl.cap;
     const int64_t blocks = (known + kWeighTokens - 1) / kWeighTokens, want = 12 * (int64_t)device_cus() / std::max<int64_t>(1, pairs * blocks);
-    pl.parts = (int)std::max<int64_t>(1, std::min<int64_t>({want, rows / (8 * kWeighRows), 64}));
+    pl.parts = (int)std::max<int64_t>(1, std::min<int64_t>({want, rows / (8 * kWeighRows), 64, kMostScores / (pairs * std::max<int64_t>(pl.cap, 1) * 4)}));
     pl.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((pl.cap + kWeighTokens - 1) / kWeighTokens, 65536 / (pairs * pl.parts)));
     pl.bytes = pl.parts > 1 ? up16((size_t)pairs * pl.parts * pl.cap * 4) : 0;
     return pl;

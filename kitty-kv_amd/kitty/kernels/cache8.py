@@ -571,7 +571,8 @@ class Cache8:
         earlier; NaN counts as heaviest).  The kept ones become tokens 0 .. of the
         sequence in their old order, in block_table's first pages, or in those of `into`
         (B, W') where given, which leaves the old pages as they are; `into` must name
-        pages that no sequence of the call has.  Pages behind the new length are free to
+        pages that no sequence of the call has.  No page may be written twice: sequences
+        that share pages are cut into pages of their own.  Pages behind the new length are free to
         be used again, and attention over the new lengths goes on as before (keys keep the
         positions they were made with).  A page's scale is the largest of its tokens'
         former pages'; codes that had a smaller one are rounded again.  Positions behind

@@ -15,6 +15,15 @@ from test_shared8 import check_shared, pools
 from test_weighed8 import check_weighed
 
 
+def _hip_lib():
+    from kitty import _hip
+    return _hip
+
+
+def _hip_cache(H, D, G):
+    return _hip_lib().Cache8(4096, 8192, 16384, H * G * D, G * D, D, H * G * D, G * D, D, 2 * H, 2, 4, H, D, G)
+
+
 @pytest.mark.parametrize("dev", DEVICES)
 @pytest.mark.parametrize("dtype", [F16, BF16])
 def test_samples_of_one_prompt(dev, dtype):
@@ -362,6 +371,34 @@ def test_every_way_is_tested():
     assert shared_way(16, 1, 4, 1, 1, 128, 16, 40, 40) == "whole" and shared_way(1, 1, 32, 1, 1, 128, 16, 40, 40) == "whole"
     assert shared_way(1, 1, 33, 1, 1, 128, 16, 8, 8) == "tiles" and shared_way(1, 1, 32, 1, 1, 128, 16, 40, 41) == "rows"
     assert shared_way(600, 300, 4, 2, 2, 256, 16, 99, 99) == "rows" and shared_way(129, 1, 2, 2, 1, 64, 16, 8, 8) == "tiles and rows"
+
+
+def test_a_sequence_and_its_prefix_are_limited_together():
+    """Tables of 2^30 tokens between them pass, a page more is refused: places of rows are ints."""
+    L = _hip_lib()
+    c = _hip_cache(1, 16, 16)
+    for pages, rc in (((1 << 26, 0), 0), ((1 << 25, 1 << 25), 0), ((0, 1 << 26), 0), ((1 << 25, (1 << 25) + 1), 2), ((1 << 26, 1), 2)):
+        a = L.Cache8SharedArgs()
+        a.prefixes = a.batch = a.num_q_heads = a.tokens = 1
+        a.prefix_pages, a.table_pages, a.sm_scale = *pages, 1.0
+        got = L.load().kitty_cache8_shared_attention_workspace_size(ctypes.byref(c), ctypes.byref(a), ctypes.byref(ctypes.c_size_t(0)))
+        assert got == (L.KITTY_E_UNSUPPORTED if rc else L.KITTY_OK), pages
+
+
+def test_sums_of_parts_stay_within_a_gibibyte():
+    """Many rows over a long table whose sequences are said to be short: parts, but not at any size."""
+    L = _hip_lib()
+    c = _hip_cache(8, 128, 128)
+    sizes = []
+    for plan, N in ((1, 1 << 30), (1, 1 << 20), (0, 1 << 30)):
+        a = L.Cache8AttentionArgs()
+        a.batch, a.num_q_heads, a.tokens, a.table_pages, a.sm_scale, a.plan_tokens = 1, 32, 8192, 1 << 17, 1.0, plan
+        w = L.Cache8Weights(4096, 8 * N, N, N)
+        size, plain = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        assert L.load().kitty_cache8_weighed_attention_workspace_size(ctypes.byref(c), ctypes.byref(a), ctypes.byref(w), ctypes.byref(size)) == 0
+        assert L.load().kitty_cache8_attention_workspace_size(ctypes.byref(c), ctypes.byref(a), ctypes.byref(plain)) == 0
+        sizes.append(size.value - plain.value)
+    assert all(0 < s < 1.25 * 2 ** 30 for s in sizes) and sizes[1] > 2 ** 29, sizes
 
 
 def test_references_agree():
