@@ -16,6 +16,18 @@
 // The first half of a launch fills every CU once and the second half again, so that in
 // the middle of the range a CU holds one of each.  Sequences with more rows than the row
 // kernel's body takes go through tiles as well.
+//
+// Measured, fp16 and 8 KV heads of 128 unless said: 64 sequences of 100-2,000 tokens
+// behind 16,384 shared ones, 32 query heads, bf16: 69 us, of them 8 for the join (the
+// tiles alone 51 of the kernel's 64, the rows alone 50, its beginning 5); eight samples of
+// each of 8 prompts of 2,000-9,000, 64 query heads: 61, of them 7; five draft tokens of 16
+// sequences behind 30,000, bf16: 97; six padded questions of up to 300 tokens about two
+// documents of 5,000-8,000, 16 / 4 heads of 64: 97; four samples of a prompt of 1,000,
+// 8 query heads: 11, one launch.  attend over the first in joined tables, whose pages it
+// reads for every sequence, takes 4.1 times as long, over the second and third 1.7.
+// The matrix cores' and the vector instructions' phases of a tile's waves stand one after
+// the other: three workgroups a CU at 64 channels, a third tile in flight and wave
+// priorities gained nothing.
 #include "attend8_rows.h"
 #include "attend8_tiles.h"
 
@@ -155,7 +167,7 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_shared_queries_kernel(Atte
 }
 
 // Units of tiles: kTile tokens for kTileRows rows, and kTileStart for what beginning an
-// item costs.
+// item costs (its queries' loads and the leaving of its part).
 constexpr int kTileStart = 2;
 
 struct Entry8 {
@@ -249,7 +261,9 @@ __device__ __forceinline__ void tiles_run(const Attend8 &p, int wg, int n_wg, in
     }
 }
 
-// What a unit of each kind costs, relative to each other (tile, row).
+// What a unit of each kind costs, relative to each other (tile, row): a CU's workgroups of
+// either kind slow the other's.  64 sequences behind one prefix / 16 drafts, us, at 5 : 4
+// 66 / 101, 4 : 3 66 / 100, 2 : 1 71 / 122, 3 : 1 76 / 159, 3 : 4 76.
 constexpr int kTileCost = 5, kRowCost = 4;
 
 // RT: the row blocks of a sequence's own rows; 0: they go through tiles, and `a` has all entries.
@@ -283,8 +297,12 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_shared_
 // What takes a call, by its sizes.
 // 1. Whole sequences, prefix and all, a workgroup for each and KV head, where a stream of
 //    both is at most kSharedDirectBytes and the workgroups at most the CUs: one launch.
+//    It reads a prefix once for each sequence, from L2 mostly, and saves the join: 4
+//    samples of 1,000 tokens and 40 of their own 11.1 us, 13.0 by way 2.
 // 2. The row kernel for prefixes and sequences together: up to 64 rows of a prefix, in
-//    blocks of 32, and 32 of a sequence.
+//    blocks of 32, and 32 of a sequence.  64 rows of each of 8 prefixes of 2,000-9,000
+//    tokens: 57.6 us in two blocks of 32, 64 by way 3, 74 in one block of 64 (its registers leave
+//    one wave a SIMD), 78 in four of 16.  Beyond, codes would be read a third time.
 // 3. cache8_shared_kernel.
 constexpr int64_t kSharedDirectBytes = 1280 * 128;
 

@@ -2,17 +2,27 @@
 // and KV head stay, and their move together.
 //
 // cache8_select_kernel, a workgroup per (sequence, KV head): the weights between the
-// first and last tokens, which stay, map to unsigned keys in the floats' order; three passes over 11, 11 and 10 bits, counted in LDS, find
-// the key of the lightest token that stays and how many of its equals do.  Positions and
-// weights are written in order: a token's place is the count of heavier ones before it
-// plus that of its equals, as far as they stay, by ballots of a wave over its run of
-// tokens and the waves' counts.  Counts are integers: any order of additions gives the
-// same.
+// first and last tokens, which stay, map to unsigned keys in the floats' order; three
+// passes over 11, 11 and 10 bits, counted in LDS, find the key of the lightest token that
+// stays and how many of its equals do (it ends where all of a bin stay, for weights
+// without equals mostly after two).  Positions and weights are written in order: a token's
+// place is the count of heavier ones before it plus that of its equals, as far as they
+// stay, by ballots of a wave over its run of tokens and the waves' counts.  Counts are
+// integers: any order of additions gives the same.
 // cache8_pack_kernel, a workgroup per (page, KV head, stream) of the result: the page's
 // scale is the largest of the pages that its tokens come from, and codes of smaller
 // scales are multiplied by the quotient and rounded again (exact but for subnormals
 // where scales are powers of two).  In place the codes go through the workspace, as a
 // page of the result may hold tokens that another page of the result needs.
+//
+// The selection is bound by latency: passes, each of counting, a scan and three barriers,
+// and a workgroup a CU at most where there are few sequences; the move by HBM.  Measured,
+// 8 heads of 128: 16 sequences of 32,768 tokens cut to 16,384 into other pages 254 us: 31
+// for the selection and 223 for 1,077 MB read and written (4.83 TB/s, where a copy reaches
+// 5.13); one sequence of 1,100 cut to 1,024 14.0, of which the kernels are 8.1 and 4.6
+// and the host's call, alongside, 14.6.  Small evictions in one launch, each selecting
+// workgroup moving its tokens: 21 to 24 where these are 12.7 (a CU alone moves 0.5 MB in
+// 12 us).
 #include <algorithm>
 
 #include "cache8.h"
@@ -79,7 +89,8 @@ __device__ __forceinline__ unsigned sum_before(const unsigned *v, int wave)
 }
 
 // A wave takes a run of 64 j tokens; EACH: j at most, the weights then stay in registers
-// (0: any j, they are read again in every pass).
+// (0: any j, they are read again in every pass).  Kept in registers rather than read again:
+// 16 x 32,768 tokens, 8 heads 31 us, 73 read again.
 template <int EACH>
 __global__ __launch_bounds__(kSelect) void cache8_select_kernel(Evict8 p)
 {
@@ -358,7 +369,8 @@ extern "C" int kitty_cache8_evict(const kitty_cache8 *cache, const kitty_cache8_
     p.ws_scale = (float *)((char *)a.workspace + up16((size_t)p.B * p.c.H * 2 * p.K * p.c.D));
     const hipStream_t st = (hipStream_t)stream;
     const unsigned pairs = (unsigned)(p.B * p.c.H);
-    // by what a sequence can hold: 8 or 32 weights a lane in registers
+    // by what a sequence can hold: 8 or 32 weights a lane in registers (1,100 tokens 8.2 us
+    // with room for 8, 12.1 with room for 32, 8.6 read again; 31 and 73 for 32,768 tokens)
     const int64_t cap = std::min<int64_t>((int64_t)p.table_pages << p.c.lg, p.N);
     if (cap <= 8 * kSelect)
         hipLaunchKernelGGL(cache8_select_kernel<8>, dim3(pairs), dim3(kSelect), 0, st, p);

@@ -1,5 +1,6 @@
-"""The 8-bit paged cache: written token by token or in chunks, read back, and
-attended over by one or many queries.
+"""The 8-bit paged cache: written token by token or in chunks, read back, attended
+over by one or many queries, by sequences that share prefixes, and cut down to the
+tokens that got the most attention.
 
 A layer that 2 bits cost too much (and that has no room for 16) keeps its keys
 and values in e4m3 with one float32 scale per page, head and stream.  Unlike the
@@ -7,10 +8,10 @@ and values in e4m3 with one float32 scale per page, head and stream.  Unlike the
 into their page as they come: the page's scale is a power of two that rises when
 a larger token arrives, and its older codes are rounded again to the new scale.
 
-Device tensors run the HIP kernels of csrc/cache8.hip and csrc/attend8*.hip, CPU
-tensors the torch code of ``kernels.cpu8``.  No call waits for the GPU, reads a
-length on the host or keeps state of its own, so calls may be captured into a
-graph and replayed with other lengths and tables in the same tensors.
+Device tensors run the HIP kernels of csrc/cache8.hip, attend8*.hip, weigh8.hip and
+evict8.hip, CPU tensors the torch code of ``kernels.cpu8``.  No call waits for the
+GPU, reads a length on the host or keeps state of its own, so calls may be captured
+into a graph and replayed with other lengths and tables in the same tensors.
 """
 from __future__ import annotations
 
@@ -27,8 +28,8 @@ from .ops import _need, calls_followed
 
 _SRC = {torch.float16: _hip.KITTY_SRC_F16, torch.bfloat16: _hip.KITTY_SRC_BF16, torch.float32: _hip.KITTY_SRC_F32}
 _PAGE_TOKENS = (16, 32, 64, 128, 256)
-# kitty_cache8_write_args / _read_args, kitty_cache8_attention_args and _shared_args as the C
-# compiler lays them out (packing one takes a quarter of a ctypes structure's time)
+# kitty_cache8_write_args / _read_args, kitty_cache8_attention_args, _shared_args, kitty_cache8_weights and
+# kitty_cache8_evict_args as the C compiler lays them out (packing one takes a quarter of a ctypes structure's time)
 _ROWS = struct.Struct("2P6qPq2P4i")
 _ATTENTION = struct.Struct("3P6qPq2P7ifPN")
 _SHARED = struct.Struct("3P6qPqPPq2P8ifPN")

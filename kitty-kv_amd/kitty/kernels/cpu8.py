@@ -1,5 +1,5 @@
-"""The 8-bit paged cache on CPU tensors: :class:`kitty.kernels.Cache8`'s three
-calls in torch code, with the rules of include/kitty_hip.h (kitty_cache8_*).
+"""The 8-bit paged cache on CPU tensors: :class:`kitty.kernels.Cache8`'s calls
+in torch code, with the rules of include/kitty_hip.h (kitty_cache8_*).
 Codes and scales are bit-identical to the HIP kernels'."""
 from __future__ import annotations
 
