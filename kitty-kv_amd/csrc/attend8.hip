@@ -11,7 +11,7 @@ namespace kitty {
 // otherwise a row per lane group.  TILES: the partials are the tile kernel's
 // p.splits parts.
 template <int DP, bool BF16, bool TILES, bool ALONE>
-__global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, int RM)
+__device__ __forceinline__ void merge_rows(const Attend8 &p, int RM)
 {
     constexpr int LPR = DP / 4, GROUPS = 64 * kWaves / LPR, STEP = ALONE ? GROUPS : 1;
     const int group = threadIdx.x / LPR, ch = 4 * (threadIdx.x % LPR);
@@ -84,6 +84,71 @@ __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, in
         p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
     if (ch == 0 && p.stat)
         p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
+}
+
+template <int DP, bool BF16, bool TILES, bool ALONE>
+__global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, int RM)
+{
+    merge_rows<DP, BF16, TILES, ALONE>(p, RM);
+}
+
+// The weights of a launch of the row kernel that left its scores.  The rows' tops and sums
+// are joined here again, a wave a row, so that merge and weights are one launch (4 rows of
+// one sequence of 4,096 tokens, 8 KV heads 13.6 us, 16.2 with a launch of their own).  Bound
+// by HBM where the scores are many: 67 MB of them for 16 x 32,768 tokens.
+__device__ __forceinline__ void weigh_scores(const Attend8 &p, int index, int blocks)
+{
+    __shared__ float2 stats[16];
+    __shared__ int vis[16];
+    const int pairs = p.B * p.c.H, pair = index % pairs, block = index / pairs;
+    const int b = pair / p.c.H, kh = pair - b * p.c.H, rows = p.gq * p.T;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int2 tab = p.ws_tab[pair];   // of a sequence without tokens it holds anything and is not used
+    const Seq8 sq = seq8(p, b);
+    const int tokens = sq.bad ? 0 : min(sq.n, p.w_tokens);
+    if ((int64_t)block * 1024 >= tokens)
+        return;
+    const int slot = min(tab.x, 2 * p.n_wg - 1), begin = slot >> 1, count = min(tab.y, p.n_wg - 1) - begin + 1;
+    if (threadIdx.x < 16)
+        vis[threadIdx.x] = (int)threadIdx.x < rows ? min(visible8(p, sq, threadIdx.x / p.gq), tokens) : 0;
+    for (int r = wave; r < rows; r += kWaves) {
+        if (slot < 0) {
+            const int t = r / p.gq, h = r - t * p.gq;
+            if (lane == 0)
+                stats[r] = p.stat[((int64_t)b * p.Hq + kh * p.gq + h) * p.T + t];
+            continue;
+        }
+        float m = kLowest, l = 0.0f;
+        for (int k = lane; k < count; k += 64) {
+            const float2 ml = p.ws_ml[(int64_t)(k == 0 ? slot : 2 * (begin + k)) * 16 + r];
+            const float mn = fmaxf(m, ml.x);
+            l = __builtin_amdgcn_exp2f(m - mn) * l + __builtin_amdgcn_exp2f(ml.x - mn) * ml.y;
+            m = mn;
+        }
+        float top = m;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1)
+            top = fmaxf(top, __shfl_xor(top, off));
+        l *= __builtin_amdgcn_exp2f(m - top);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1)
+            l += __shfl_xor(l, off);
+        if (lane == 0)
+            stats[r] = make_float2(top, 1.0f / l);
+    }
+    __syncthreads();
+    for (int64_t tok = (int64_t)block * 1024 + 4 * threadIdx.x; tok < tokens; tok += (int64_t)blocks * 1024)
+        weigh_scores4(p.scores + (int64_t)pair * rows * p.sc_cap, rows, stats, vis, (int)tok, tokens, p.weights + b * p.w_s_seq + kh * p.w_s_head);
+}
+
+// Both, `merges` workgroups of the first and `blocks` for each pair of the second.
+template <int DP, bool BF16, bool ALONE>
+__global__ __launch_bounds__(64 * kWaves) void cache8_merge_weigh_kernel(Attend8 p, int merges, int blocks)
+{
+    if ((int)blockIdx.x < merges)
+        merge_rows<DP, BF16, false, ALONE>(p, 16);
+    else
+        weigh_scores(p, (int)blockIdx.x - merges, blocks);
 }
 
 // Which kernel takes a call, by its sizes alone (rows: of a KV head, its group's
@@ -233,7 +298,7 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
 
     p.stat = leave.stat, p.scores = leave.scores, p.sc_cap = leave.sc_cap;
     p.weights = leave.weights, p.w_s_seq = leave.w_s_seq, p.w_s_head = leave.w_s_head, p.w_tokens = leave.w_tokens;
-    leave.weighed = leave.scores && pl.direct;
+    leave.weighed = leave.scores != nullptr;
     const hipStream_t st = stream;
     const bool bf16 = a.dtype == KITTY_DTYPE_BF16;
     const dim3 block(64 * kWaves);
@@ -242,6 +307,19 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
         constexpr bool BF = decltype(bf)::value, TILES = decltype(tiles)::value;
         const int64_t rows = (int64_t)p.B * p.Hq * p.T;
         const int RM = TILES ? kTileRows : 16 * pl.RT;
+        if constexpr (!TILES) {
+            if (p.scores) {
+                const int64_t pairs = (int64_t)p.B * p.c.H, groups = 256 * kWaves / DP;
+                const int64_t blocks = std::max<int64_t>(1, std::min<int64_t>((p.sc_cap + 1023) / 1024, 65536 / pairs));
+                const int64_t merges = rows < kMergeRows ? rows : (rows + groups - 1) / groups;
+                const dim3 grid((unsigned)(merges + pairs * blocks));
+                if (rows < kMergeRows)
+                    hipLaunchKernelGGL((cache8_merge_weigh_kernel<DP, BF, true>), grid, block, 0, st, p, (int)merges, (int)blocks);
+                else
+                    hipLaunchKernelGGL((cache8_merge_weigh_kernel<DP, BF, false>), grid, block, 0, st, p, (int)merges, (int)blocks);
+                return;
+            }
+        }
         if (rows < kMergeRows) {
             hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, true>), dim3((unsigned)rows), block, 0, st, p, RM);
         } else {

@@ -324,6 +324,42 @@ constexpr int row_waves(int RT, bool direct) { return !direct ? kWaves : RT == 1
 // Whether two workgroups' registers and LDS fit a CU.
 constexpr bool two_per_cu(int DP, int RT) { return DP <= 128 && DP * RT <= 256; }
 
+// Adds to the weights of tokens tok .. tok + 3 (tok a multiple of four) the sum over up to
+// 16 rows of 2^(score - top) / sum, from the scores that a kScores launch left.  vis: how
+// many tokens each row sees, 0 behind the last row.  Four rows' scores at a time: read one
+// by one the loads' latency was half of a short call (16 rows of 1,024 tokens 15.8 us / 13.0
+// in one launch, 27.7 / 14.7 split; four rows of 16 x 32,768 250.7 / 245.6).
+__device__ __forceinline__ void weigh_scores4(const float *scores, int rows, const float2 *stat, const int *vis, int tok, int tokens,
+                                              float *weights)
+{
+    const float *s = scores + (int64_t)(tok >> 4) * 16 * rows + (tok & 15);
+    float was[4], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        was[e] = tok + e < tokens ? weights[tok + e] : 0.0f;
+    for (int r0 = 0; r0 < rows; r0 += 4) {
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            x[i] = *(const float4 *)(s + 16 * min(r0 + i, rows - 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 st = stat[r0 + i];
+            const int v = vis[r0 + i];
+            const float xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float with = __builtin_fmaf(__builtin_amdgcn_exp2f(xs[e] - st.x), st.y, sum[e]);
+                sum[e] = tok + e < v ? with : sum[e];
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (tok + e < tokens)
+            weights[tok + e] = was[e] + sum[e];
+}
+
 // CUT: D is below DP, and the lanes beyond it read nothing.  DIRECT: a workgroup takes
 // the whole of one (pair, row block) and writes its rows, so that no merge follows.
 // MODE kShared: the entries are prefixes and sequences, the latter of one row block each,
@@ -336,6 +372,7 @@ struct RowLds {
     float o[row_waves(RT, DIRECT)][16 * RT][DP + 4];
     float2 ml[row_waves(RT, DIRECT)][16 * RT];
     float2 stat[DIRECT && RT == 1 ? 16 : 1];
+    int vis[DIRECT && RT == 1 ? 16 : 1];
 };
 
 template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
@@ -591,19 +628,13 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         }
         if constexpr (SCORES && DIRECT) {
             // the weights, from the scores that the waves left
-            __syncthreads();
-            float *weights = p.weights + b * p.w_s_seq + kh * p.w_s_head;
-            const float *left = p.scores + (int64_t)(b * p.c.H + kh) * rows_all * p.sc_cap;
             const int tokens = sq.bad ? 0 : min(sq.n, p.w_tokens);
-            for (int tok = threadIdx.x; tok < tokens; tok += 64 * NW) {
-                const float was = weights[tok];
-                float sum = 0.0f;
-                for (int r = 0; r < rows_all; ++r)
-                    if (tok < visible8(p, sq, r / p.gq))
-                        sum = __builtin_fmaf(__builtin_amdgcn_exp2f(left[(int64_t)(tok >> 4) * 16 * rows_all + 16 * r + (tok & 15)] - lds.stat[r].x),
-                                             lds.stat[r].y, sum);
-                weights[tok] = was + sum;
-            }
+            if (threadIdx.x < 16)
+                lds.vis[threadIdx.x] = (int)threadIdx.x < rows_all ? min(visible8(p, sq, threadIdx.x / p.gq), tokens) : 0;
+            __syncthreads();
+            for (int tok = 4 * threadIdx.x; tok < tokens; tok += 4 * 64 * NW)
+                weigh_scores4(p.scores + (int64_t)(b * p.c.H + kh) * rows_all * p.sc_cap, rows_all, lds.stat, lds.vis, tok, tokens,
+                              p.weights + b * p.w_s_seq + kh * p.w_s_head);
         }
         if constexpr (DIRECT)
             return;

@@ -3,7 +3,7 @@
 //
 // The attention leaves each row's maximum and 1 / sum (rather than their log-sum-exp,
 // whose rounding would be the weights' largest error).  Up to 16 rows of a KV head it
-// leaves the scores as well, and cache8_weigh_scores_kernel makes the weights from them.
+// leaves the scores as well, and makes the weights from them (attend8.hip).
 // Of more rows a second pass over the keys makes p = 2^(score - top) / sum again and sums
 // it over the rows of the KV head's group: S = Q K^T with
 // 32x32x16 MFMAs: A row = query, column = token, so a lane (n = token l & 31, g = l / 32)
@@ -220,40 +220,6 @@ __global__ __launch_bounds__(64 * kWeighWaves, DP <= 128 ? 3 : 1) void cache8_we
     }
 }
 
-// The weights of a launch of the row kernel that left its scores: each a sum over up to
-// 16 rows of 2^(score - top) / sum.  A thread has four tokens, 256 apart.  Bound by HBM:
-// 16 x 32,768 tokens, four rows: 23 us for 67 MB of scores and 17 MB of weights, read and
-// written (4.4 TB/s).
-__global__ __launch_bounds__(256) void cache8_weigh_scores_kernel(Weigh8 w)
-{
-    const Attend8 &p = w.a;
-    const int pairs = p.B * p.c.H, pair = blockIdx.x % pairs, block = blockIdx.x / pairs;
-    const int b = pair / p.c.H, kh = pair - b * p.c.H, rows = p.gq * p.T;
-    const Seq8 sq = seq8(p, b);
-    const int tokens = sq.bad ? 0 : min(sq.n, w.N);
-    float *weights = w.weights + b * w.w_s_seq + kh * w.w_s_head;
-    for (int64_t first = (int64_t)block * 1024; first < tokens; first += (int64_t)w.blocks * 1024) {
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int r = 0; r < rows; ++r) {
-            const int t = r / p.gq, h = r - t * p.gq, vis = min(visible8(p, sq, t), tokens);
-            const float2 stat = p.stat[((int64_t)b * p.Hq + kh * p.gq + h) * p.T + t];
-            const float *s = p.scores + (int64_t)pair * rows * p.sc_cap + 16 * r;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int tok = (int)first + (int)threadIdx.x + 256 * j;
-                if (tok < vis)
-                    sum[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(s[(int64_t)(tok >> 4) * 16 * rows + (tok & 15)] - stat.x), stat.y, sum[j]);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int tok = (int)first + (int)threadIdx.x + 256 * j;
-            if (tok < tokens)
-                weights[tok] += sum[j];
-        }
-    }
-}
-
 // The parts' sums into the weights, in their order.
 __global__ __launch_bounds__(256) void cache8_weigh_sum_kernel(Weigh8 w)
 {
@@ -278,7 +244,8 @@ __global__ __launch_bounds__(256) void cache8_weigh_sum_kernel(Weigh8 w)
 // Up to 16 rows the scores are kept instead: reading and writing them is 8 bytes a row and
 // token where reading the keys again is head_dim, and costs products as well.  A gibibyte
 // of them at most, or of the parts' sums.  Where one launch of the row kernel has all of a
-// head's rows and tokens, it adds to the weights itself (1,024 tokens 11.4 us, 13.4 in two).
+// head's rows and tokens, it adds to the weights itself (4 rows of 512 tokens of 16 sequences
+// 8.1 us, 14.5 split; one sequence of 1,024 11.1 / 10.6).
 struct WeighPlan8 {
     bool scores;
     int64_t cap;
@@ -290,14 +257,13 @@ constexpr int64_t kMostScores = 1ll << 30;
 
 static WeighPlan8 plan_weigh(const Cache8 &c, const kitty_cache8_attention_args &a, int weight_tokens)
 {
-    WeighPlan8 pl;
+    WeighPlan8 pl{};
     pl.cap = std::min<int64_t>((int64_t)a.table_pages << c.lg, weight_tokens);
     const int64_t pairs = (int64_t)a.batch * c.H, rows = (int64_t)a.num_q_heads / c.H * a.tokens;
     const int64_t sc_bytes = pairs * rows * ((pl.cap + 15) & ~15ll) * 4;
     pl.scores = rows <= 16 && sc_bytes <= kMostScores;
     if (pl.scores) {
-        pl.parts = 1, pl.bytes = up16((size_t)sc_bytes);
-        pl.blocks = (int)std::max<int64_t>(1, std::min<int64_t>((pl.cap + 1023) / 1024, 65536 / pairs));
+        pl.bytes = up16((size_t)sc_bytes);
         return pl;
     }
     const int64_t known = a.plan_tokens > 0 ? std::min<int64_t>(a.plan_tokens, pl.cap) : pl.cap;
@@ -386,10 +352,6 @@ extern "C" int kitty_cache8_weighed_attention(const kitty_cache8 *cache, const k
     w.blocks = pl.blocks, w.parts = pl.parts, w.cap = pl.cap;
     const unsigned pairs = (unsigned)(p.B * p.c.H);
     const dim3 grid(pairs * (unsigned)(pl.blocks * pl.parts)), block(64 * kWeighWaves);
-    if (pl.scores) {
-        hipLaunchKernelGGL(cache8_weigh_scores_kernel, grid, dim3(256), 0, st, w);
-        return check_launch("cache8_weigh_scores_kernel");
-    }
     auto go = [&](auto dp, auto bf) {
         constexpr int DP = decltype(dp)::value;
         constexpr bool BF = decltype(bf)::value;
