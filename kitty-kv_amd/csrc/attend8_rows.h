@@ -92,12 +92,13 @@ __device__ __forceinline__ u32x4 value_operand(const unsigned (&v)[8][DP / 64], 
 
 // 32 tokens from `tok` on, in `buf`, folded into the wave's rows.  mask: some
 // row may not see all of them.
-// SCORES: they also go to `out`, at byte `at` plus `step` for every 16 tokens; beyond its
-// end (lanes without a row, tokens that have no weight) the store itself drops them: a
-// branch around it would make every wait one for all loads.
-template <int DP, int RT, bool BF16, bool SCORES>
+// LEAVE: the scores go as well, at byte `at` plus `step` for every 16 tokens, to `out` (1),
+// where the store itself drops what is beyond its end (lanes without a row, tokens that
+// have no weight): a branch around it would make every wait one for all loads; or to
+// `stage` (2).
+template <int DP, int RT, bool BF16, int LEAVE>
 __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &buf, int tok, int vis_max, float cs, int g, bool mask,
-                                         __amdgpu_buffer_rsrc_t out, uint32_t at, uint32_t step)
+                                         __amdgpu_buffer_rsrc_t out, unsigned char *stage, uint32_t at, uint32_t step)
 {
     f32x4 S[RT][2];
 #pragma unroll
@@ -141,10 +142,13 @@ __device__ __forceinline__ void row_step(RowState<DP, RT> &W, RowBuf<DP, RT> &bu
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 s[e] = tok + 16 * (e >> 2) + 4 * g + (e & 3) < W.vis[rt] ? s[e] : -__builtin_inff();
-        // A sixteenth of the bytes that the stream reads, but a stream with writes in it runs
-        // at a copy's rate: 16 x 32,768 tokens 231 us, 174 with the stores dropped, 179 with
-        // all of a pair's to the same 4 KB; cache hints on them change nothing.
-        if constexpr (SCORES) {
+        if constexpr (LEAVE == 2) {
+            if (at < 1u << 31)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+                    *(float4 *)(stage + at + hf * step) = make_float4(s[4 * hf], s[4 * hf + 1], s[4 * hf + 2], s[4 * hf + 3]);
+        }
+        if constexpr (LEAVE == 1) {
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
                 __builtin_amdgcn_raw_buffer_store_b128(
@@ -367,16 +371,31 @@ __device__ __forceinline__ void weigh_scores4(const float *scores, int rows, con
 // each reads its prefix itself.
 //
 // Workgroup wg of the n_wg that share the work.
-template <int DP, int RT, bool DIRECT>
+// kScores: a stream of reads with writes in it runs at a copy's rate, though the scores of
+// four rows are a sixteenth of its bytes: 16 x 32,768 tokens 231 us, 174 with the stores
+// dropped, 179 with all of a pair's to the same 4 KB; cache hints change nothing.  So a
+// wave's scores wait in LDS, in what is its part of o afterwards, and leave in bursts, which
+// workgroups with equal runs have at about the same time: 210 us.  Bytes that wait: the
+// whole call 217 us at 20,064 (what two workgroups a CU allow), 218 at 16,896, 228 at
+// 12,288, 234 at 8,448 and 246 unless they wait.
+constexpr int kStage = 16896;
+
+// Rows of a wave's part of o.
+constexpr int row_lines(int DP, int RT, bool direct, int mode)
+{
+    return mode == kScores && !direct && kStage > 64 * RT * (DP + 4) ? (kStage + 4 * (DP + 4) - 1) / (4 * (DP + 4)) : 16 * RT;
+}
+
+template <int DP, int RT, bool DIRECT, int MODE>
 struct RowLds {
-    float o[row_waves(RT, DIRECT)][16 * RT][DP + 4];
+    float o[row_waves(RT, DIRECT)][row_lines(DP, RT, DIRECT, MODE)][DP + 4];
     float2 ml[row_waves(RT, DIRECT)][16 * RT];
     float2 stat[DIRECT && RT == 1 ? 16 : 1];
     int vis[DIRECT && RT == 1 ? 16 : 1];
 };
 
 template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
-__device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, RowLds<DP, RT, DIRECT> &lds)
+__device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, RowLds<DP, RT, DIRECT, MODE> &lds)
 {
     constexpr bool SHARED = MODE == kShared, SCORES = MODE == kScores;
     constexpr bool STAT = !(DIRECT && RT == 1 && MODE == kPlain);   // calls that want it take another instance (plan8)
@@ -518,6 +537,23 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
             for (int j = 0; j < NB - 1; ++j)
                 load(min(tok + j * STRIDE, final), id[j], ring[j]);
             bool more = true;
+            // LEAVE: scores go to memory as they come (1) or in bursts (2); `held` steps wait
+            constexpr int LEAVE = !SCORES ? 0 : DIRECT ? 1 : 2;
+            unsigned char *stage = (unsigned char *)&lds_o[wave][0][0];
+            const int each = 2 * sc_step, most = (int)sizeof(lds_o[0]) / each;
+            int held = 0;
+            auto burst = [&](int tok) {    // tok: where the step behind them begins
+                __builtin_amdgcn_wave_barrier();
+                const int per = each / 16, first = tok - held * STRIDE;
+                for (int c = lane; c < held * per; c += 64) {
+                    const int s = c / per, from = first + s * STRIDE;
+                    __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4 *)(stage + 16 * c), scores,
+                                                           from < p.sc_cap ? (uint32_t)(from >> 4) * sc_step + 16 * (c - s * per) : 1u << 31,
+                                                           0, 0);
+                }
+                __builtin_amdgcn_wave_barrier();
+                held = 0;
+            };
             while (more) {
 #pragma unroll
                 for (int j = 0; j < NB; ++j) {
@@ -525,11 +561,18 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                         break;
                     load(min(tok + (NB - 1) * STRIDE, final), id[NB - 1], ring[(j + NB - 1) % NB]);
                     ids(min(tok + NB * STRIDE, final), id[NB - 1]);
-                    row_step<DP, RT, BF16, SCORES>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min, scores,
-                                                   SCORES && n < rows_all && tok < p.sc_cap ? (uint32_t)(tok >> 4) * sc_step + 64 * n + 16 * g : 1u << 31,
-                                                   sc_step);
+                    uint32_t at = 0;
+                    if constexpr (LEAVE == 1)
+                        at = n < rows_all && tok < p.sc_cap ? (uint32_t)(tok >> 4) * sc_step + 64 * n + 16 * g : 1u << 31;
+                    else if constexpr (LEAVE == 2)
+                        at = n < rows_all ? held * each + 64 * n + 16 * g : 1u << 31;
+                    row_step<DP, RT, BF16, LEAVE>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min, scores, stage, at, sc_step);
                     tok += STRIDE;
                     more = tok < end;
+                    if constexpr (LEAVE == 2) {
+                        if (++held == most || !more)
+                            burst(tok);
+                    }
                 }
             }
         };
@@ -646,7 +689,7 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
 template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
 __global__ __launch_bounds__(64 * row_waves(RT, DIRECT), DIRECT && RT == 1 ? 4 : two_per_cu(DP, RT) ? 2 : 1) void cache8_rows_kernel(Attend8 p)
 {
-    __shared__ __attribute__((aligned(16))) RowLds<DP, RT, DIRECT> lds;
+    __shared__ __attribute__((aligned(16))) RowLds<DP, RT, DIRECT, MODE> lds;
     int wg = blockIdx.x;
     if (MODE == kShared && gridDim.x % 8 == 0)   // neighbours of a run on one XCD: they read the same pages
         wg = (wg & 7) * (gridDim.x >> 3) + (wg >> 3);

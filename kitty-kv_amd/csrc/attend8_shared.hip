@@ -271,7 +271,7 @@ template <int DP, bool BF16, bool CUT, int RT>
 __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_shared_kernel(Attend8 a, Attend8 own)
 {
     static_assert(kWaves == kTileWaves, "both kinds of work are of one workgroup's size");
-    typedef RowLds<DP, RT ? RT : 1, false> Rows;
+    typedef RowLds<DP, RT ? RT : 1, false, kShared> Rows;
     constexpr int LDS = (int)sizeof(Rows) > kTileLds<DP> ? (int)sizeof(Rows) : kTileLds<DP>;
     __shared__ __attribute__((aligned(16))) unsigned char lds[LDS];
     // workgroup i runs on XCD i % 8: neighbours of a run share one

@@ -179,6 +179,20 @@ def test_infinite_queries(dev, T, wide):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Hq,T,cut", [(128, 1, 0), (64, 1, 5000), (8, 13, 0), (40, 3, 16369)])
+def test_scores_in_bursts(dev, Hq, T, cut):
+    """Runs of more steps than a wave keeps scores of: several bursts, of whole pairs and of parts; weights
+    that end inside a burst."""
+    gen = torch.Generator().manual_seed(Hq)
+    B, H, D, G, W = 12, 8, 16, 256, 64
+    cache = filled(gen, 1 + B * W, H, D, G, dev)
+    table = (1 + torch.randperm(B * W, generator=gen)).view(B, W).int().to(dev)
+    lens = [16384, 16383, 1, 9000, 16370, 12345, 16384, 40, 16129, 16384, 15000, 16384]
+    q = torch.randn(B, Hq, T, D, generator=gen).half()
+    check_weighed(cache, q, table, lens, N=cut or 16384)
+
+
+@pytest.mark.gpu
 def test_scores_beyond_a_gibibyte(dev):
     """Weights for so many tokens that the scores of 16 rows are not kept: a second pass over the keys instead."""
     gen = torch.Generator().manual_seed(3)
