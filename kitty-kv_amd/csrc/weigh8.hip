@@ -261,7 +261,8 @@ static WeighPlan8 plan_weigh(const Cache8 &c, const kitty_cache8_attention_args 
     pl.cap = std::min<int64_t>((int64_t)a.table_pages << c.lg, weight_tokens);
     const int64_t pairs = (int64_t)a.batch * c.H, rows = (int64_t)a.num_q_heads / c.H * a.tokens;
     const int64_t sc_bytes = pairs * rows * ((pl.cap + 15) & ~15ll) * 4;
-    pl.scores = rows <= 16 && sc_bytes <= kMostScores;
+    // (merge and weights are one grid)
+    pl.scores = rows <= 16 && sc_bytes <= kMostScores && pairs <= kMaxBlocks / 2;
     if (pl.scores) {
         pl.bytes = up16((size_t)sc_bytes);
         return pl;

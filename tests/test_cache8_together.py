@@ -401,6 +401,21 @@ def test_sums_of_parts_stay_within_a_gibibyte():
     assert all(0 < s < 1.25 * 2 ** 30 for s in sizes) and sizes[1] > 2 ** 29, sizes
 
 
+def test_merge_and_weights_are_one_grid():
+    """Of more than half of a grid's pairs the scores are not kept: their launch would hold the merge as well."""
+    L = _hip_lib()
+    c = _hip_cache(1, 16, 16)
+    kept = []
+    for B in (0xffffffff // 512, 0xffffffff // 512 + 1):
+        a = L.Cache8AttentionArgs()
+        a.batch, a.num_q_heads, a.tokens, a.table_pages, a.sm_scale = B, 1, 1, 1, 1.0
+        size = ctypes.c_size_t(0)
+        w = L.Cache8Weights(4096, 16, 16, 16)
+        assert L.load().kitty_cache8_weighed_attention_workspace_size(ctypes.byref(c), ctypes.byref(a), ctypes.byref(w), ctypes.byref(size)) == 0
+        kept.append(size.value > B * 16 * 4)
+    assert kept == [True, False]
+
+
 def test_references_agree():
     """shared8_ref on an aligned prefix is cache8_ref on the joined table; evict_ref's zeros and NaN are torch.sort's."""
     gen = torch.Generator().manual_seed(1)
