@@ -48,8 +48,8 @@ struct Attend8 {
     float2 *stat;
     float *scores;
     int64_t sc_cap;
-    // Where a launch has the whole of a KV head's rows and tokens, it adds to the weights
-    // (of the first w_tokens tokens) itself.
+    // Weights (of the first w_tokens tokens), added to by the launch that leaves the scores
+    // where it has the whole of a KV head's rows and tokens, else by the merge's.
     float *weights;
     int64_t w_s_seq, w_s_head;
     int w_tokens;

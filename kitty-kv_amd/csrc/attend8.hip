@@ -1,5 +1,6 @@
 // Attention over the 8-bit paged cache, on gfx950: which kernel takes a call, its
-// launches, and the kernel that joins the parts of rows whose tokens were split.
+// launches, and the kernel that joins the parts of rows whose tokens were split and, for
+// calls that weigh tokens by the scores of a few rows, makes the weights.
 #include "attend8_rows.h"
 
 namespace kitty {
