@@ -44,9 +44,9 @@ struct Part8 {
 
 // Joins the parts of each row, of its prefix and of its own tokens.  DP / 4 lanes take a
 // row, four channels each; ALONE: a workgroup per row, whose lane groups share its parts.
-// Bound by the parts' bytes (33 MB in 8.4 us for 2,048 rows of a prefix in 17 parts): 8 or
-// 16 parts in flight take 8.4 and 10.1, a workgroup per row 8.7 there, 13.0 for 6.6 of
-// 4,096 rows in few parts.
+// 19 MB of parts in 8.4 us for 2,048 rows of a prefix in 18 parts: 8 or 16 parts in flight
+// take 8.4 and 10.1, a workgroup per row 8.7 there, and 13.0 where it is 6.6 for 4,096 rows
+// of few parts.
 template <int DP, bool BF16, bool ALONE>
 __global__ __launch_bounds__(64 * kWaves) void cache8_join_kernel(Attend8 p, Part8 of_prefix, Part8 of_own)
 {
