@@ -687,7 +687,8 @@ int kitty_cache8_weighed_attention(const kitty_cache8 *cache, const kitty_cache8
  * earlier; both zeros are equal, NaN is heavier than all else, as torch.sort has it).
  * They become tokens 0 .. m - 1, in their order, of the pages that row b of `into`
  * names, or of block_table where into is NULL (pages of `into` must not be among those
- * that the call reads; no page may be written twice, for two sequences or for one).  A page's scale
+ * that the call reads; no page may be written twice, for two sequences or for one; in
+ * place the pages of sequences with n <= keep are not written).  A page's scale
  * becomes the largest of the pages that its tokens come from, and a code c of one with
  * another scale s becomes e4m3(c * (s / scale)), both in fp32; others move as they are.
  * Rows behind the last token keep their bytes.

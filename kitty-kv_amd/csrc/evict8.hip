@@ -13,7 +13,8 @@
 // scale is the largest of the pages that its tokens come from, and codes of smaller
 // scales are multiplied by the quotient and rounded again (exact but for subnormals
 // where scales are powers of two).  In place the codes go through the workspace, as a
-// page of the result may hold tokens that another page of the result needs.
+// page of the result may hold tokens that another page of the result needs; sequences
+// within the budget are left alone.
 //
 // The selection is bound by latency: passes, each of counting, a scan and three barriers,
 // and a workgroup a CU at most where there are few sequences; the move by HBM.  Measured,
@@ -60,6 +61,14 @@ __device__ __forceinline__ uint32_t weight_key(float x)
 __device__ __forceinline__ int kept8(const Evict8 &p, int n)
 {
     return n < 0 || n > (int64_t)p.table_pages << p.c.lg || n > p.N ? -1 : min(n, p.keep);
+}
+
+// Of them, those that are written: in place none of a sequence that is not cut, whose pages
+// stay as they are.
+template <bool STAGED>
+__device__ __forceinline__ int written8(const Evict8 &p, int n)
+{
+    return STAGED && n <= p.keep ? 0 : kept8(p, n);
 }
 
 // The sum of a value over the lanes up to this one.
@@ -231,7 +240,7 @@ __global__ __launch_bounds__(256) void cache8_stage_kernel(Evict8 p)
     const int cpr = p.c.D >> 4, rows = 256 / cpr, r = threadIdx.x / cpr, c = threadIdx.x - r * cpr;
     const int64_t seq = (int64_t)(b * p.c.H + h), list = (2 * seq + st) * p.K;
     const int at = tile * rows + r;
-    if (r >= rows || at >= kept8(p, p.lens[b]))
+    if (r >= rows || at >= written8<true>(p, p.lens[b]))
         return;
     const Source8 s = source8(p, b, h, st, p.kept[seq * p.K + at]);
     *(u32x4 *)(p.ws_codes + (list + at) * p.c.D + 16 * c) =
@@ -257,7 +266,7 @@ __global__ __launch_bounds__(256) void cache8_pack_kernel(Evict8 p)
     i /= (uint32_t)p.tiles;
     const int st = (int)(i & 1);
     const int h = (int)((i >> 1) % (uint32_t)p.c.H), b = (int)((i >> 1) / (uint32_t)p.c.H);
-    const int lg = p.c.lg, first = page << lg, m = kept8(p, p.lens[b]);
+    const int lg = p.c.lg, first = page << lg, m = written8<STAGED>(p, p.lens[b]);
     if (first >= m || page >= p.into_pages)
         return;
     const int id = p.into[b * p.into_stride + page];

@@ -572,7 +572,8 @@ class Cache8:
         earlier; NaN counts as heaviest).  The kept ones become tokens 0 .. of the
         sequence in their old order, in block_table's first pages, or in those of `into`
         (B, W') where given, which leaves the old pages as they are; `into` must name
-        pages that no sequence of the call has.  No page may be written twice: sequences
+        pages that no sequence of the call has.  In place, sequences that are not cut keep
+        their pages as they are.  No page may be written twice: sequences
         that share pages are cut into pages of their own.  Pages behind the new length are free to
         be used again, and attention over the new lengths goes on as before (keys keep the
         positions they were made with).  A page's scale is the largest of its tokens'
@@ -599,16 +600,17 @@ class Cache8:
             if into is not None:
                 self._check_table(into, B, "into")
                 _need(into.shape[1] * self.page_tokens >= min(K, W * self.page_tokens), f"into must have pages for {keep} tokens")
+            strides = (*_strides(weights)[:2], block_table.stride(0) if B > 1 else 0,
+                       0 if into is None or B <= 1 else into.stride(0))
             if B == 0 or not self._on_device:
                 out = (torch.empty(B, dtype=torch.int32, device=self.device),
                        torch.empty(B, H, K, dtype=torch.int32, device=self.device),
                        torch.empty(B, H, N, device=self.device))
+                if into is not None and into.data_ptr() == block_table.data_ptr() and strides[2] == strides[3]:
+                    into = None
                 if B:
-                    cpu8.evict(self.key, self.value, self.scale, block_table, lens, weights, keep, first, last,
-                               block_table if into is None else into, *out)
+                    cpu8.evict(self.key, self.value, self.scale, block_table, lens, weights, keep, first, last, into, *out)
                 return out
-            strides = (*_strides(weights)[:2], block_table.stride(0) if B > 1 else 0,
-                       0 if into is None or B <= 1 else into.stride(0))
             rest = (B, W, 0 if into is None else into.shape[1], N, keep, first, last)
             size = ctypes.c_size_t(0)
             _hip.check(self._lib.kitty_cache8_evict_workspace_size(

@@ -168,7 +168,7 @@ def attend_shared(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q
 
 
 def evict(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
-          weights: torch.Tensor, keep: int, first: int, last: int, into: torch.Tensor, out_lens: torch.Tensor,
+          weights: torch.Tensor, keep: int, first: int, last: int, into: Optional[torch.Tensor], out_lens: torch.Tensor,
           kept: torch.Tensor, out_weights: torch.Tensor) -> None:
     P, H, G, D = key.shape
     N, K = weights.shape[2], kept.shape[2]
@@ -186,10 +186,10 @@ def evict(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: to
             at = torch.cat([at[:, :first], first + between.sort(-1).values, at[:, n - last:]], 1)
         kept[b, :, :m] = at
         out_weights[b, :, :m] = weights[b].gather(1, at)
-        if m == 0:
+        if m == 0 or (into is None and m == n):     # in place only what is cut is written
             continue
         ids, ok = _page_ids(table[b:b + 1].expand(H, -1), at // G, P)
-        new, there = _page_ids(into[b:b + 1], torch.arange(-(-m // G))[None], P)
+        new, there = _page_ids((table if into is None else into)[b:b + 1], torch.arange(-(-m // G))[None], P)
         if P == 0:
             continue
         # all that moves is read before any of it is written
