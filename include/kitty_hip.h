@@ -686,18 +686,19 @@ int kitty_cache8_weighed_attention(const kitty_cache8 *cache, const kitty_cache8
  * between the keep - first - last heaviest by weights[b, h, j] (of equal ones the
  * earlier; both zeros are equal, NaN is heavier than all else, as torch.sort has it).
  * They become tokens 0 .. m - 1, in their order, of the pages that row b of `into`
- * names, or of block_table where into is NULL (pages of `into` must not be among those
- * that the call reads; no page may be written twice, for two sequences or for one; in
- * place the pages of sequences with n <= keep are not written).  A page's scale
- * becomes the largest of the pages that its tokens come from, and a code c of one with
- * another scale s becomes e4m3(c * (s / scale)), both in fp32; others move as they are.
+ * names, or of block_table where into is NULL; in place the pages of sequences with
+ * n <= keep are not written.  A page's scale becomes the largest of the pages that its
+ * tokens come from, and a code c of one with another scale s becomes e4m3(c * (s /
+ * scale)), both in fp32; others move as they are.
  * Rows behind the last token keep their bytes.
  * out_lens[b] = m; kept[b, h, i] = the position of token i, -1 for i >= m;
  * out_weights[b, h, i] = its weight, 0 for i >= m.  A token whose page is outside the
  * pool moves as NaN codes and takes no part in the scale (1 where a page has no other);
  * tokens whose new page is outside the pool, or that `into` has no page for, are
  * dropped.  A length that is negative, or more than table_pages pages or weight_tokens
- * hold, gives out_lens -1, nothing kept and no page written. */
+ * hold, gives out_lens -1, nothing kept and no page written; so does a page that the
+ * sequence would write (the first ceil(m / page tokens) of its row) and that the call
+ * names once more, among the pages of any sequence's tokens or those that one writes. */
 typedef struct {
     const float *weights;        /* (B, H, weight_tokens), stride 1 between tokens */
     int64_t w_s_seq, w_s_head;

@@ -8,7 +8,8 @@
 // without equals mostly after two).  Positions and weights are written in order: a token's
 // place is the count of heavier ones before it plus that of its equals, as far as they
 // stay, by ballots of a wave over its run of tokens and the waves' counts.  Counts are
-// integers: any order of additions gives the same.
+// integers: any order of additions gives the same.  Further workgroups of the launch find
+// the sequences that name a page twice (new_lengths).
 // cache8_pack_kernel, a workgroup per (page, KV head, stream) of the result: the page's
 // scale is the largest of the pages that its tokens come from, and codes of smaller
 // scales are multiplied by the quotient and rounded again (exact but for subnormals
@@ -44,6 +45,9 @@ struct Evict8 {
     uint8_t *ws_codes;    // in place: (sequence, KV head, stream, K, D)
     float *ws_scale;      //           (sequence, KV head, stream, K)
     int B, N, K, keep, first, last, table_pages, into_pages, tiles;
+    int in_place, most_pages;   // pages that a sequence may write
+    int group, lanes;           // new_lengths
+    unsigned slots;             // cache8_named_kernel's, 0: new_lengths
 };
 
 constexpr int kSelect = 1024, kSelectWaves = kSelect / 64;
@@ -65,11 +69,13 @@ __device__ __forceinline__ int kept8(const Evict8 &p, int n)
 
 // Of them, those that are written: in place none of a sequence that is not cut, whose pages
 // stay as they are.
-template <bool STAGED>
 __device__ __forceinline__ int written8(const Evict8 &p, int n)
 {
-    return STAGED && n <= p.keep ? 0 : kept8(p, n);
+    return p.in_place && n <= p.keep ? 0 : kept8(p, n);
 }
+
+// Pages of n tokens, 0 of a length that breaks the rules.
+__device__ __forceinline__ int pages8(const Evict8 &p, int n) { return n <= 0 ? 0 : ((n - 1) >> p.c.lg) + 1; }
 
 // The sum of a value over the lanes up to this one.
 template <int CTRL, int ROWS>
@@ -97,6 +103,157 @@ __device__ __forceinline__ unsigned sum_before(const unsigned *v, int wave)
     return s;
 }
 
+// Lengths after the call: -1 also where a page that a sequence writes is named once more, as
+// one that the call reads or writes, as it would be lost or written by two workgroups at
+// once.  (A page that is read alone may be named often.)  The written pages' ids go into a
+// table of open addressing with the number of their entry; then every page that the call
+// names is looked up.
+//
+// Up to kNamed written pages in all, and kLooks in the tables: a workgroup of the selection's
+// launch does it, its table in LDS, half full, `lanes` threads for each sequence's pages;
+// beside the selection its time is not seen (1 x 1,100 tokens 14 us, 16 x 32,768 in pages of
+// 128 254, with and without).  More: three launches of 5 to 10 us before the selection, the
+// table in the memory of the weights that come out (cache8_named_kernel): 48 x 65,536 tokens
+// of one head of 64 in pages of 16 to half 397 us, where workgroups of the selection with
+// several tables take 753; 2,000 x 100 tokens, 2 heads of 64, 107 and 129; 16 x 65,536
+// tokens, 8 heads of 128 in pages of 128 602 and 581.  Where the memory is too small
+// (thousands of sequences of a few tokens) LDS again, for `group` sequences at a time.
+constexpr int kNamed = 2048, kSlots = 2 * kNamed;
+constexpr unsigned kFree = 0xffffffffu;   // no page's id
+constexpr int64_t kLooks = 1 << 17;       // pages of the tables, beyond which one workgroup would look too long
+
+// In the counters' LDS (with 16 KB more of it a select of 2,000 short sequences took 74 us, 52 without).
+struct Named8 {
+    unsigned ids[kSlots];
+    unsigned short entry[kSlots];
+    unsigned twice[kNamed / 32];   // a bit for each sequence of the group
+};
+static_assert(sizeof(Named8) <= kCopies * kBins * 4, "they share LDS");
+
+__device__ __forceinline__ unsigned slot_of(int id, unsigned slots)   // a power of two
+{
+    return (unsigned)id * 2654435769u >> (__builtin_clz(slots) + 1);
+}
+
+// Pages that a sequence of n tokens writes.
+__device__ __forceinline__ int written_pages8(const Evict8 &p, int n) { return min(pages8(p, written8(p, n)), p.into_pages); }
+
+__device__ __forceinline__ void new_lengths(const Evict8 &p, int number, Named8 &named)
+{
+    unsigned *slots = named.ids;
+    const int tid = threadIdx.x, b0 = number * p.group, b1 = min(b0 + p.group, p.B), span = p.most_pages;
+    auto flag = [&](int seq) { atomicOr(&named.twice[seq >> 5], 1u << (seq & 31)); };
+    if (tid < kNamed / 32)
+        named.twice[tid] = 0;
+    for (int i = tid; i < kSlots; i += kSelect)
+        slots[i] = kFree;
+    __syncthreads();
+    for (int e = tid; e < (b1 - b0) * span; e += kSelect) {   // kNamed at most
+        const int seq = e / span, i = e - seq * span;
+        const int id = i < written_pages8(p, p.lens[b0 + seq]) ? p.into[(b0 + seq) * p.into_stride + i] : -1;
+        if (bad_page(p.c, id))
+            continue;
+        for (unsigned s = slot_of(id, kSlots);; s = (s + 1) & (kSlots - 1)) {   // ends: half the slots are free
+            const unsigned was = atomicCAS(&slots[s], kFree, (unsigned)id);
+            if (was == kFree)
+                named.entry[s] = (unsigned short)e;
+            if (was == kFree || was == (unsigned)id)
+                break;
+        }
+    }
+    __syncthreads();
+    // a row's first `count` pages, of which the first `own` are entries from `base` on
+    auto look = [&](const int32_t *row, int count, int own, int base) {
+        for (int i0 = tid % p.lanes; i0 < count; i0 += 4 * p.lanes) {
+            int id[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                id[j] = i0 + j * p.lanes < count ? row[i0 + j * p.lanes] : -1;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (bad_page(p.c, id[j]))
+                    continue;
+                unsigned s = slot_of(id[j], kSlots);
+                while (slots[s] != kFree && slots[s] != (unsigned)id[j])
+                    s = (s + 1) & (kSlots - 1);
+                if (slots[s] == kFree)
+                    continue;
+                const int i = i0 + j * p.lanes, mine = i < own ? base + i : -1, e = named.entry[s];
+                if (e != mine) {
+                    flag(e / span);
+                    if (mine >= 0)
+                        flag(mine / span);
+                }
+            }
+        }
+    };
+    for (int b = span ? tid / p.lanes : p.B; b < p.B; b += kSelect / p.lanes) {
+        const int n = p.lens[b], w = min(written_pages8(p, n), span);
+        const int own = b >= b0 && b < b1 ? w : 0, base = (b - b0) * span;
+        look(p.table + b * p.bt_stride, kept8(p, n) < 0 ? 0 : pages8(p, n), p.in_place ? own : 0, base);
+        if (!p.in_place)
+            look(p.into + b * p.into_stride, w, own, base);
+    }
+    __syncthreads();
+    for (int b = b0 + tid; b < b1; b += kSelect)
+        p.out_lens[b] = named.twice[(b - b0) >> 5] >> ((b - b0) & 31) & 1 ? -1 : kept8(p, p.lens[b]);
+}
+
+// The same in three launches: 0 empties the table, 1 enters the written pages, 2 looks.  A
+// wave for 256 pages of a sequence, or more where it has many.
+template <int STEP>
+__global__ __launch_bounds__(64) void cache8_named_kernel(Evict8 p, int parts)
+{
+    unsigned *ids = (unsigned *)p.out_weights;
+    int *entries = (int *)p.out_weights + p.slots;
+    if constexpr (STEP == 0) {
+        for (int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x; i < p.slots; i += (int64_t)gridDim.x * 64)
+            ids[i] = kFree;
+        for (int b = blockIdx.x * 64 + threadIdx.x; b < p.B; b += gridDim.x * 64)
+            p.out_lens[b] = kept8(p, p.lens[b]);
+        return;
+    }
+    const int b = blockIdx.x / parts, part = blockIdx.x - b * parts;
+    const int n = p.lens[b], written = min(written_pages8(p, n), p.most_pages);
+    const int32_t *to = p.into + b * p.into_stride;
+    if constexpr (STEP == 1) {
+        for (int i = part * 64 + threadIdx.x; i < written; i += parts * 64) {
+            const int id = to[i];
+            if (bad_page(p.c, id))
+                continue;
+            for (unsigned s = slot_of(id, p.slots);; s = (s + 1) & (p.slots - 1)) {   // ends: at most half the slots are taken
+                const unsigned was = atomicCAS(&ids[s], kFree, (unsigned)id);
+                if (was == kFree)
+                    entries[s] = b * p.most_pages + i;
+                if (was == kFree || was == (unsigned)id)
+                    break;
+            }
+        }
+        return;
+    }
+    auto look = [&](const int32_t *row, int count, int own) {
+        for (int i = part * 64 + threadIdx.x; i < count; i += parts * 64) {
+            const int id = row[i];
+            if (bad_page(p.c, id))
+                continue;
+            unsigned s = slot_of(id, p.slots);
+            while (ids[s] != kFree && ids[s] != (unsigned)id)
+                s = (s + 1) & (p.slots - 1);
+            if (ids[s] == kFree)
+                continue;
+            const int mine = i < own ? b * p.most_pages + i : -1, e = entries[s];
+            if (e != mine) {
+                p.out_lens[e / p.most_pages] = -1;
+                if (mine >= 0)
+                    p.out_lens[b] = -1;
+            }
+        }
+    };
+    look(p.table + b * p.bt_stride, kept8(p, n) < 0 ? 0 : pages8(p, n), p.in_place ? written : 0);
+    if (!p.in_place)
+        look(to, written, written);
+}
+
 // A wave takes a run of 64 j tokens; EACH: j at most, the weights then stay in registers
 // (0: any j, they are read again in every pass).  Kept in registers rather than read again:
 // 16 x 32,768 tokens, 8 heads 31 us, 73 read again.
@@ -106,13 +263,16 @@ __global__ __launch_bounds__(kSelect) void cache8_select_kernel(Evict8 p)
     __shared__ __attribute__((aligned(16))) unsigned hist[kCopies][kBins], sums[2][kSelectWaves];
     __shared__ unsigned found[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int pairs = p.B * p.c.H;
+    if ((int)blockIdx.x >= pairs) {
+        new_lengths(p, blockIdx.x - pairs, *(Named8 *)hist);
+        return;
+    }
     const int b = blockIdx.x / p.c.H, h = blockIdx.x - b * p.c.H;
     const int n = p.lens[b], m = kept8(p, n);
     const float *w = p.weights + b * p.w_s_seq + h * p.w_s_head;
     int32_t *kept = p.kept + (int64_t)blockIdx.x * p.K;
     float *out = p.out_weights + (int64_t)blockIdx.x * p.N;
-    if (h == 0 && tid == 0)
-        p.out_lens[b] = m;
     const int end = m < 0 ? 0 : n, last = end - p.last;
     const int steps = (end + kSelect - 1) / kSelect;           // of 64 tokens, a wave
     const int pos0 = wave * steps * 64 + lane;
@@ -240,7 +400,7 @@ __global__ __launch_bounds__(256) void cache8_stage_kernel(Evict8 p)
     const int cpr = p.c.D >> 4, rows = 256 / cpr, r = threadIdx.x / cpr, c = threadIdx.x - r * cpr;
     const int64_t seq = (int64_t)(b * p.c.H + h), list = (2 * seq + st) * p.K;
     const int at = tile * rows + r;
-    if (r >= rows || at >= written8<true>(p, p.lens[b]))
+    if (r >= rows || at >= written8(p, p.lens[b]))
         return;
     const Source8 s = source8(p, b, h, st, p.kept[seq * p.K + at]);
     *(u32x4 *)(p.ws_codes + (list + at) * p.c.D + 16 * c) =
@@ -266,14 +426,24 @@ __global__ __launch_bounds__(256) void cache8_pack_kernel(Evict8 p)
     i /= (uint32_t)p.tiles;
     const int st = (int)(i & 1);
     const int h = (int)((i >> 1) % (uint32_t)p.c.H), b = (int)((i >> 1) / (uint32_t)p.c.H);
-    const int lg = p.c.lg, first = page << lg, m = written8<STAGED>(p, p.lens[b]);
+    const int64_t seq = (int64_t)(b * p.c.H + h), list = (2 * seq + st) * p.K;
+    const int lg = p.c.lg, first = page << lg, m = written8(p, p.lens[b]);
+    if (p.out_lens[b] < 0) {
+        // it stays as it was: what the selection said of it goes
+        if (i == 2 * (unsigned)seq && page == 0) {
+            for (int j = threadIdx.x; j < p.K; j += 256)
+                p.kept[seq * p.K + j] = -1;
+            for (int j = threadIdx.x; j < p.N; j += 256)
+                p.out_weights[seq * p.N + j] = 0.0f;
+        }
+        return;
+    }
     if (first >= m || page >= p.into_pages)
         return;
     const int id = p.into[b * p.into_stride + page];
     if (bad_page(p.c, id))
         return;
     const int rows = min(1 << lg, m - first);
-    const int64_t seq = (int64_t)(b * p.c.H + h), list = (2 * seq + st) * p.K;
     float mine = -1.0f;       // of a token without a page
     if ((int)threadIdx.x < rows) {
         const int at = first + threadIdx.x;
@@ -334,8 +504,21 @@ static int check_evict(const kitty_cache8 *cache, const kitty_cache8_evict_args 
     if ((int64_t)a.table_pages << p.c.lg > 1 << 30 || a.weight_tokens > 1 << 30)
         return fail(KITTY_E_UNSUPPORTED, "a sequence is limited to 2^30 tokens");
     p.B = a.batch, p.N = a.weight_tokens, p.K = a.keep < a.weight_tokens ? a.keep : a.weight_tokens;
-    if ((int64_t)p.B * p.c.H > kMaxBlocks / 4 || (int64_t)p.B * p.c.H * 2 * (((int64_t)p.K >> 4) + 1) > kMaxBlocks)
+    p.into_pages = a.into ? a.into_pages : a.table_pages;
+    p.most_pages = std::min(p.into_pages, p.K ? ((p.K - 1) >> p.c.lg) + 1 : 0);
+    // (the selection's launch has workgroups of 1,024 threads, up to 2,049 of them new_lengths')
+    if ((int64_t)p.B * p.c.H > kMaxBlocks / 4 - 2049 || (int64_t)p.B * p.c.H * 2 * (((int64_t)p.K >> 4) + 1) > kMaxBlocks)
         return fail(KITTY_E_UNSUPPORTED, "too many tokens for one launch");
+    const int64_t pages = (int64_t)p.B * p.most_pages, room = (int64_t)p.B * p.c.H * p.N / 2;
+    p.slots = 1;
+    while (p.slots < 2 * pages)
+        p.slots *= 2;
+    if ((pages <= kNamed && (int64_t)p.B * std::min(p.table_pages, (p.N >> p.c.lg) + 1) <= kLooks) || p.slots > room)
+        p.slots = 0;
+    p.group = std::max(1, kNamed / std::max(p.most_pages, 1));
+    p.lanes = 1;
+    while (p.lanes < kSelect && (int64_t)2 * p.lanes * p.B <= kSelect)
+        p.lanes *= 2;
     need = a.into ? 0 : up16((size_t)p.B * p.c.H * 2 * p.K * p.c.D) + up16((size_t)p.B * p.c.H * 2 * p.K * 4);
     return KITTY_OK;
 }
@@ -371,22 +554,28 @@ extern "C" int kitty_cache8_evict(const kitty_cache8 *cache, const kitty_cache8_
     p.weights = a.weights, p.w_s_seq = a.w_s_seq, p.w_s_head = a.w_s_head;
     p.table = a.block_table, p.bt_stride = a.bt_stride, p.table_pages = a.table_pages, p.lens = a.lens;
     p.into = a.into ? a.into : a.block_table, p.into_stride = a.into ? a.into_stride : a.bt_stride;
-    p.into_pages = a.into ? a.into_pages : a.table_pages;
     p.out_lens = a.out_lens, p.kept = a.kept, p.out_weights = a.out_weights;
-    p.keep = a.keep, p.first = a.first, p.last = a.last;
+    p.keep = a.keep, p.first = a.first, p.last = a.last, p.in_place = !a.into;
     p.ws_codes = (uint8_t *)a.workspace;
     p.ws_scale = (float *)((char *)a.workspace + up16((size_t)p.B * p.c.H * 2 * p.K * p.c.D));
     const hipStream_t st = (hipStream_t)stream;
-    const unsigned pairs = (unsigned)(p.B * p.c.H);
+    const unsigned pairs = (unsigned)(p.B * p.c.H), grid = pairs + (p.slots ? 0 : (unsigned)((p.B - 1) / p.group + 1));
+    if (p.slots) {
+        const int parts = std::min((std::max(std::min(p.table_pages, (p.N >> p.c.lg) + 1), p.most_pages) + 255) / 256, 64);
+        const dim3 waves((unsigned)p.B * (unsigned)parts), block(64);
+        hipLaunchKernelGGL(cache8_named_kernel<0>, dim3(std::min(p.slots / 256 + 1, 2048u)), block, 0, st, p, parts);
+        hipLaunchKernelGGL(cache8_named_kernel<1>, waves, block, 0, st, p, parts);
+        hipLaunchKernelGGL(cache8_named_kernel<2>, waves, block, 0, st, p, parts);
+    }
     // by what a sequence can hold: 8 or 32 weights a lane in registers (1,100 tokens 8.2 us
     // with room for 8, 12.1 with room for 32, 8.6 read again; 31 and 73 for 32,768 tokens)
     const int64_t cap = std::min<int64_t>((int64_t)p.table_pages << p.c.lg, p.N);
     if (cap <= 8 * kSelect)
-        hipLaunchKernelGGL(cache8_select_kernel<8>, dim3(pairs), dim3(kSelect), 0, st, p);
+        hipLaunchKernelGGL(cache8_select_kernel<8>, dim3(grid), dim3(kSelect), 0, st, p);
     else if (cap <= 32 * kSelect)
-        hipLaunchKernelGGL(cache8_select_kernel<32>, dim3(pairs), dim3(kSelect), 0, st, p);
+        hipLaunchKernelGGL(cache8_select_kernel<32>, dim3(grid), dim3(kSelect), 0, st, p);
     else
-        hipLaunchKernelGGL(cache8_select_kernel<0>, dim3(pairs), dim3(kSelect), 0, st, p);
+        hipLaunchKernelGGL(cache8_select_kernel<0>, dim3(grid), dim3(kSelect), 0, st, p);
     if (p.K > 0) {
         if (!a.into) {
             const int rows = 256 / (p.c.D >> 4);

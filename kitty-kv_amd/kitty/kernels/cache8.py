@@ -571,15 +571,17 @@ class Cache8:
         on), the last `last`, and of those between the heaviest (of equal ones the
         earlier; NaN counts as heaviest).  The kept ones become tokens 0 .. of the
         sequence in their old order, in block_table's first pages, or in those of `into`
-        (B, W') where given, which leaves the old pages as they are; `into` must name
-        pages that no sequence of the call has.  In place, sequences that are not cut keep
-        their pages as they are.  No page may be written twice: sequences
-        that share pages are cut into pages of their own.  Pages behind the new length are free to
-        be used again, and attention over the new lengths goes on as before (keys keep the
-        positions they were made with).  A page's scale is the largest of its tokens'
-        former pages'; codes that had a smaller one are rounded again.  Positions behind
-        the kept ones are -1, weights 0.  A length that is negative, or more than
-        block_table or weights hold, comes back as -1 and its sequence as it was."""
+        (B, W') where given, which leaves the old pages as they are.  In place, sequences
+        that are not cut keep their pages as they are.  Pages behind the new length are
+        free to be used again, and attention over the new lengths goes on as before (keys
+        keep the positions they were made with).  A page's scale is the largest of its
+        tokens' former pages'; codes that had a smaller one are rounded again.  Positions
+        behind the kept ones are -1, weights 0.
+
+        A sequence comes back as -1 and as it was if its length is negative, or more than
+        block_table or weights hold, or if a page that it would write is named once more by
+        the call: `into` names pages that none of its sequences has, each once, and
+        sequences that share pages are cut into pages of their own."""
         if calls_followed():
             raise NotImplementedError(_FOLLOWED)
         if weights.requires_grad or weights.is_neg():

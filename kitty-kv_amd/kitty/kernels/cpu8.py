@@ -4,7 +4,8 @@ Codes and scales are bit-identical to the HIP kernels'."""
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple
+from collections import Counter
+from typing import List, Optional, Tuple
 
 import torch
 
@@ -167,6 +168,11 @@ def attend_shared(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, q
         lse[b, :, :t] = l
 
 
+def _named(row: torch.Tensor, pages: int, num_pages: int) -> List[int]:
+    """Ids of the first `pages` pages that a table's row names, without those outside the pool."""
+    return [p for p in row[:max(pages, 0)].tolist() if 0 <= p < num_pages]
+
+
 def evict(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
           weights: torch.Tensor, keep: int, first: int, last: int, into: Optional[torch.Tensor], out_lens: torch.Tensor,
           kept: torch.Tensor, out_weights: torch.Tensor) -> None:
@@ -175,8 +181,17 @@ def evict(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: to
     heads = torch.arange(H)[:, None]
     kept.fill_(-1)
     out_weights.zero_()
-    for b, n in enumerate(lens.tolist()):
-        if n < 0 or n > table.shape[1] * G or n > N:
+    # pages that each sequence reads and writes, and how often the call names each: written ones once
+    lens = [n if 0 <= n <= min(table.shape[1] * G, N) else -1 for n in lens.tolist()]
+    named = [_named(table[b], -(-n // G), P) for b, n in enumerate(lens)]
+    if into is None:
+        written = [_named(table[b], -(-keep // G) if n > keep else 0, P) for b, n in enumerate(lens)]
+    else:
+        written = [_named(into[b], -(-min(n, keep) // G), P) for b, n in enumerate(lens)]
+        named += written
+    count = Counter(p for pages in named for p in pages)
+    for b, n in enumerate(lens):
+        if n < 0 or any(count[p] > 1 for p in written[b]):
             out_lens[b] = -1
             continue
         m = out_lens[b] = min(n, keep)
