@@ -698,7 +698,8 @@ int kitty_cache8_weighed_attention(const kitty_cache8 *cache, const kitty_cache8
  * dropped.  A length that is negative, or more than table_pages pages or weight_tokens
  * hold, gives out_lens -1, nothing kept and no page written; so does a page that the
  * sequence would write (the first ceil(m / page tokens) of its row) and that the call
- * names once more, among the pages of any sequence's tokens or those that one writes. */
+ * names once more, among the pages of any sequence's tokens (in place: of those that stay)
+ * or those that one writes. */
 typedef struct {
     const float *weights;        /* (B, H, weight_tokens), stride 1 between tokens */
     int64_t w_s_seq, w_s_head;

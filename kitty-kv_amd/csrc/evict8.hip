@@ -104,7 +104,7 @@ __device__ __forceinline__ unsigned sum_before(const unsigned *v, int wave)
 }
 
 // Lengths after the call: -1 also where a page that a sequence writes is named once more, as
-// one that the call reads or writes, as it would be lost or written by two workgroups at
+// one that another needs or writes, as it would be lost or written by two workgroups at
 // once.  (A page that is read alone may be named often.)  The written pages' ids go into a
 // table of open addressing with the number of their entry; then every page that the call
 // names is looked up.
@@ -137,6 +137,14 @@ __device__ __forceinline__ unsigned slot_of(int id, unsigned slots)   // a power
 
 // Pages that a sequence of n tokens writes.
 __device__ __forceinline__ int written_pages8(const Evict8 &p, int n) { return min(pages8(p, written8(p, n)), p.into_pages); }
+
+// Pages of its table that a sequence of n tokens needs while others are written: in place
+// those that it keeps, as all that moves is read before.
+__device__ __forceinline__ int needed8(const Evict8 &p, int n)
+{
+    const int m = kept8(p, n);
+    return m < 0 ? 0 : pages8(p, p.in_place ? m : n);
+}
 
 __device__ __forceinline__ void new_lengths(const Evict8 &p, int number, Named8 &named)
 {
@@ -190,7 +198,7 @@ __device__ __forceinline__ void new_lengths(const Evict8 &p, int number, Named8 
     for (int b = span ? tid / p.lanes : p.B; b < p.B; b += kSelect / p.lanes) {
         const int n = p.lens[b], w = min(written_pages8(p, n), span);
         const int own = b >= b0 && b < b1 ? w : 0, base = (b - b0) * span;
-        look(p.table + b * p.bt_stride, kept8(p, n) < 0 ? 0 : pages8(p, n), p.in_place ? own : 0, base);
+        look(p.table + b * p.bt_stride, needed8(p, n), p.in_place ? own : 0, base);
         if (!p.in_place)
             look(p.into + b * p.into_stride, w, own, base);
     }
@@ -249,7 +257,7 @@ __global__ __launch_bounds__(64) void cache8_named_kernel(Evict8 p, int parts)
             }
         }
     };
-    look(p.table + b * p.bt_stride, kept8(p, n) < 0 ? 0 : pages8(p, n), p.in_place ? written : 0);
+    look(p.table + b * p.bt_stride, needed8(p, n), p.in_place ? written : 0);
     if (!p.in_place)
         look(to, written, written);
 }

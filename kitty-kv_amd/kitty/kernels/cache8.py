@@ -581,7 +581,7 @@ class Cache8:
         A sequence comes back as -1 and as it was if its length is negative, or more than
         block_table or weights hold, or if a page that it would write is named once more by
         the call: `into` names pages that none of its sequences has, each once, and
-        sequences that share pages are cut into pages of their own."""
+        sequences that share pages they keep are cut into pages of their own."""
         if calls_followed():
             raise NotImplementedError(_FOLLOWED)
         if weights.requires_grad or weights.is_neg():

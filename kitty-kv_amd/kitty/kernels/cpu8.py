@@ -181,15 +181,16 @@ def evict(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: to
     heads = torch.arange(H)[:, None]
     kept.fill_(-1)
     out_weights.zero_()
-    # pages that each sequence reads and writes, and how often the call names each: written ones once
     lens = [n if 0 <= n <= min(table.shape[1] * G, N) else -1 for n in lens.tolist()]
-    named = [_named(table[b], -(-n // G), P) for b, n in enumerate(lens)]
+    # pages that each sequence needs and writes, and how often the call names each: written ones once
     if into is None:
-        written = [_named(table[b], -(-keep // G) if n > keep else 0, P) for b, n in enumerate(lens)]
+        needed = [_named(table[b], -(-min(n, keep) // G), P) for b, n in enumerate(lens)]
+        written = [pages if n > keep else [] for pages, n in zip(needed, lens)]
+        count = Counter(p for pages in needed for p in pages)
     else:
         written = [_named(into[b], -(-min(n, keep) // G), P) for b, n in enumerate(lens)]
-        named += written
-    count = Counter(p for pages in named for p in pages)
+        count = Counter(p for b, n in enumerate(lens) for p in _named(table[b], -(-n // G), P) + written[b])
+    moves = []          # all that moves is read before any of it is written
     for b, n in enumerate(lens):
         if n < 0 or any(count[p] > 1 for p in written[b]):
             out_lens[b] = -1
@@ -201,19 +202,18 @@ def evict(key: torch.Tensor, value: torch.Tensor, scale: torch.Tensor, table: to
             at = torch.cat([at[:, :first], first + between.sort(-1).values, at[:, n - last:]], 1)
         kept[b, :, :m] = at
         out_weights[b, :, :m] = weights[b].gather(1, at)
-        if m == 0 or (into is None and m == n):     # in place only what is cut is written
+        if m == 0 or P == 0 or (into is None and m == n):     # in place only what is cut is written
             continue
         ids, ok = _page_ids(table[b:b + 1].expand(H, -1), at // G, P)
         new, there = _page_ids((table if into is None else into)[b:b + 1], torch.arange(-(-m // G))[None], P)
-        if P == 0:
-            continue
-        # all that moves is read before any of it is written
         moved = []
         for i, pool in enumerate((key, value)):
             was = torch.where(ok, scale[ids, heads, i], torch.full(ids.shape, -1.0))
             codes = torch.where(ok[..., None], pool.view(torch.uint8)[ids, heads, at % G], torch.tensor(0x7F, dtype=torch.uint8))
             moved.append((was, codes))
-        for page, (p, there_) in enumerate(zip(new[0].tolist(), there[0].tolist())):
+        moves.append((new[0].tolist(), there[0].tolist(), moved))
+    for new, there, moved in moves:
+        for page, (p, there_) in enumerate(zip(new, there)):
             if not there_:
                 continue
             for i, pool in enumerate((key, value)):

@@ -50,11 +50,12 @@ def test_sequences_within_the_budget_keep_their_pages(dev):
 
 
 def refused(table, lens, keep, into, N, G, P):
-    """Sequences of which a page that they write is named once more, as one that the call reads or writes."""
+    """Sequences of which a page that they write is named once more, as one that another needs or writes."""
     B = len(lens)
     ok = [0 <= n <= min(N, table.shape[1] * G) for n in lens]
     used = [-(-n // G) if o else 0 for n, o in zip(lens, ok)]
-    if into is None:
+    if into is None:          # all that moves is read before: pages that stay count
+        used = [-(-min(n, keep) // G) if o else 0 for n, o in zip(lens, ok)]
         written = [-(-keep // G) if o and n > keep else 0 for n, o in zip(lens, ok)]
         read, rows = used, table
     else:
@@ -132,11 +133,13 @@ def test_shared_pages_are_not_cut_in_place(dev):
     for kw in ([((1, 0), (0, 0))], [((1, 2), (0, 1))]):
         check([80, 80, 10, 66], [True, True, False, False], *kw)      # two cut ones share a page
         check([80, 40, 10, 66], [True, False, False, False], *kw)     # one within the budget holds it
-    check([80, 80, 10, 66], [True, False, False, False], ((1, 4), (0, 0)))       # read by one, written by the other
+    check([80, 40, 10, 66], [True, False, False, False], ((1, 1), (0, 2)))
+    check([80, 80, 10, 66], [False] * 4, ((1, 4), (0, 0)))                       # read by one, written by the other
     check([80, 80, 10, 66], [False] * 4, ((1, 4), (0, 4)))                       # read by both
     check([80, 60, 10, 66], [False] * 4, ((1, 4), (0, 0)))                       # behind its tokens
     check([80, 80, 10, 66], [False, False, False, True], ((3, 2), (3, 0)))       # twice in one
-    check([80, 80, 10, 66], [False, False, False, True], ((3, 4), (3, 0)))
+    check([80, 80, 10, 66], [False] * 4, ((3, 4), (3, 0)))                       # and read once more
+    check([80, 80, 10, 66], [False] * 4, ((0, 4), (3, 0)), ((1, 3), (2, 0)), ((2, 4), (1, 1)), ((3, 4), (0, 2)))
     check([80, -1, 10, 66], [False] * 4, ((1, 0), (0, 0)))
 
 
