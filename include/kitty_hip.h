@@ -639,7 +639,9 @@ int kitty_cache8_attention(const kitty_cache8 *cache, const kitty_cache8_attenti
  * of bf16 calls have the 16 bits of two terms where the rows of a prefix (its sequences'
  * queries times the group's heads) are at most 64 and a sequence's at most 32, and over
  * a sequence's own tokens where its rows are at most 32;
- * elsewhere one fp16 term, as above.  A workspace size of 0 needs none. */
+ * elsewhere one fp16 term, as above.  A workspace size of 0 needs none; it is a gibibyte
+ * at most, or what one sequence's rows of one KV head need (twice 4 bytes a channel, heads
+ * padded to 64, 128 or 256): calls of more run in pieces, one behind the other. */
 typedef struct {
     const uint16_t *q; /* (B, Hq, T, D), 16-byte aligned rows */
     uint16_t *out;     /* (B, Hq, T, D), 16-byte aligned rows, q's type; may be q, row for row */

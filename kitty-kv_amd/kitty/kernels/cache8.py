@@ -399,7 +399,8 @@ class Cache8:
         of them is row 0 of its first page).  causal: the q_lens[b] queries of sequence b
         are the last tokens of the two together; otherwise every query sees all of both.
         Results are ``attend``'s over the two in one table but for rounding.  out may be q
-        or lie in its memory in any way."""
+        or lie in its memory in any way.  Parts of the rows take up to a gibibyte beside
+        it; calls of more run in pieces."""
         if calls_followed():
             raise NotImplementedError(_FOLLOWED)
         if q.requires_grad or q.is_neg():
