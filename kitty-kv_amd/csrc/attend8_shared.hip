@@ -265,9 +265,18 @@ __device__ __forceinline__ void tiles_run(const Attend8 &p, int wg, int n_wg, in
 }
 
 // What a unit of each kind costs, relative to each other (tile, row): a CU's workgroups of
-// either kind slow the other's.  64 sequences behind one prefix / 16 drafts, us, at 5 : 4
-// 66 / 101, 4 : 3 66 / 100, 2 : 1 71 / 122, 3 : 1 76 / 159, 3 : 4 76.
-constexpr int kTileCost = 5, kRowCost = 4;
+// either kind slow the other's.  us of calls at tile : row, 32 / 8 heads, fp16 / bf16:
+//   channels, sequences x queries, tokens shared, own   3:4        1:1        5:4        3:2        2:1
+//    64   64 x 1  16,384  1,000                        59 / 54    53 / 49    52 / 47    59 / 50    56 / 51
+//    64   32 x 5  16,384  1,000                        85 / 76    82 / 74    80 / 72    77 / 74    87 / 85
+//   128   64 x 1   4,000  1,000                        64 / 61    53 / 51    49 / 49    49 / 50    52 / 53
+//   128   32 x 5  16,384  1,000                       118 / 99   113 / 97   112 / 93   108 / 96   119 / 109
+//   128   64 x 4 (two prefixes)  8,000  3,000         157 / 148  140 / 133  131 / 129  135 / 138  132 / 119
+//   256   64 x 1   4,000  1,000                       161 / 136  129 / 112  115 / 100  102 / 91    87 / 86
+//   256   64 x 4 (two prefixes)  8,000  3,000         461 / 374  381 / 311  340 / 279  318 / 263  272 / 267
+//   256   32 x 5  16,384  1,000 (1:2 281 / 237)       266 / 267  359 / 361  416 / 417  417 / 417  499 / 498
+template <int DP, int RT>
+constexpr int2 unit_cost() { return DP <= 128 ? int2{5, 4} : RT == 1 ? int2{2, 1} : int2{2, 3}; }
 
 // RT: the row blocks of a sequence's own rows; 0: they go through tiles, and `a` has all entries.
 template <int DP, bool BF16, bool CUT, int RT>
@@ -286,7 +295,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_shared_
     } else {
         int n = 0;   // of an XCD's workgroups, those that take tiles
         if (tiles > 0) {
-            const int64_t x = (int64_t)tiles * kTileCost, y = (int64_t)rows * kRowCost;
+            const int64_t x = (int64_t)tiles * unit_cost<DP, RT>().x, y = (int64_t)rows * unit_cost<DP, RT>().y;
             n = rows == 0 ? W >> 3 : min(max((int)(((W >> 3) * x + (x + y) / 2) / (x + y)), 1), (W >> 3) - 1);
         }
         const int m = (W >> 3) - n;
@@ -300,8 +309,18 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void cache8_shared_
 // What takes a call, by its sizes.
 // 1. Whole sequences, prefix and all, a workgroup for each and KV head, where a stream of
 //    both is at most kSharedDirectBytes and the workgroups at most the CUs: one launch.
-//    It reads a prefix once for each sequence, from L2 mostly, and saves the join: 4
-//    samples of 1,000 tokens and 40 of their own 11.1 us, 13.0 by way 2.
+//    It reads a prefix once for each sequence, from L2 mostly, and saves the join.  The
+//    bound is where it begins to lose for few sequences (up to 1 us within it, 4 samples
+//    with 8 query heads); more of them or more rows would gain up to twice as far.  us, one
+//    launch / the other ways, fp16, 8 KV heads, one prefix, tokens of both together (64 own):
+//      channels, sequences x queries, heads  512          1,024        1,280        2,048        4,096
+//      128   4 x 1   8                       8.9 / 11.7  12.2 / 11.7  13.0 / 12.0  18.1 / 12.0  35.4 / 13.9
+//      128   8 x 1  32                       8.4 / 13.8  12.5 / 16.2  14.1 / 16.6  21.8 / 17.0  39.6 / 18.3
+//      128  32 x 1  32                       9.2 / 20.9  13.0 / 22.0  14.8 / 22.4  21.8 / 25.2  39.5 / 29.3
+//      128   8 x 8  32                      12.8 / 23.5  18.1 / 30.6  19.4 / 32.4  25.7 / 35.7  44.2 / 38.5
+//       64   4 x 1   8                       7.3 / 11.5   9.0 / 11.5   9.6 / 11.5  11.9 / 11.5  19.8 / 12.9
+//       64   8 x 1  32                       7.9 / 12.9  10.0 / 14.2  10.0 / 14.3  14.4 / 14.8  22.4 / 15.3
+//       64   8 x 8  32                       9.4 / 18.3  12.3 / 24.0  13.4 / 26.2  17.9 / 29.7  28.6 / 33.2
 // 2. The row kernel for prefixes and sequences together: up to 64 rows of a prefix, in
 //    blocks of 32, and 32 of a sequence.  64 rows of each of 8 prefixes of 2,000-9,000
 //    tokens: 57.6 us in two blocks of 32, 64 by way 3, 74 in one block of 64 (its registers leave
