@@ -56,8 +56,8 @@ struct Attend8 {
 };
 
 // What a row kernel does beside plain attention: nothing, leave all parts of prefixes and
-// sequences, leave the scores.
-constexpr int kPlain = 0, kShared = 1, kScores = 2;
+// sequences, leave the rows' maxima and sums and the scores, or those without the scores.
+constexpr int kPlain = 0, kShared = 1, kScores = 2, kStat = 3;
 
 // kitty_cache8_attention that also leaves stat and, where given, the scores; weighed: the
 // weights are done as well.

@@ -11,7 +11,7 @@ namespace kitty {
 // lane groups share its partials and join in LDS (few rows, many partials);
 // otherwise a row per lane group.  TILES: the partials are the tile kernel's
 // p.splits parts.
-template <int DP, bool BF16, bool TILES, bool ALONE>
+template <int DP, bool BF16, bool TILES, bool ALONE, bool STAT>
 __device__ __forceinline__ void merge_rows(const Attend8 &p, int RM)
 {
     constexpr int LPR = DP / 4, GROUPS = 64 * kWaves / LPR, STEP = ALONE ? GROUPS : 1;
@@ -83,14 +83,14 @@ __device__ __forceinline__ void merge_rows(const Attend8 &p, int RM)
                    (uint32_t)f2x(o.z * inv, BF16) | (uint32_t)f2x(o.w * inv, BF16) << 16);
     if (ch == 0 && p.lse)
         p.lse[((int64_t)b * p.Hq + h) * p.T + t] = none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
-    if (ch == 0 && p.stat)
+    if (STAT && ch == 0 && p.stat)
         p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
 }
 
-template <int DP, bool BF16, bool TILES, bool ALONE>
+template <int DP, bool BF16, bool TILES, bool ALONE, bool STAT>
 __global__ __launch_bounds__(64 * kWaves) void cache8_merge_kernel(Attend8 p, int RM)
 {
-    merge_rows<DP, BF16, TILES, ALONE>(p, RM);
+    merge_rows<DP, BF16, TILES, ALONE, STAT>(p, RM);
 }
 
 // The weights of a launch of the row kernel that left its scores.  The rows' tops and sums
@@ -147,7 +147,7 @@ template <int DP, bool BF16, bool ALONE>
 __global__ __launch_bounds__(64 * kWaves) void cache8_merge_weigh_kernel(Attend8 p, int merges, int blocks)
 {
     if ((int)blockIdx.x < merges)
-        merge_rows<DP, BF16, false, ALONE>(p, 16);
+        merge_rows<DP, BF16, false, ALONE, true>(p, 16);
     else
         weigh_scores(p, (int)blockIdx.x - merges, blocks);
 }
@@ -321,13 +321,19 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
                 return;
             }
         }
-        if (rows < kMergeRows) {
-            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, true>), dim3((unsigned)rows), block, 0, st, p, RM);
-        } else {
+        auto launch = [&](auto stat) {
+            constexpr bool STAT = decltype(stat)::value;
             const int64_t groups = 256 * kWaves / DP;
-            hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, false>), dim3((unsigned)((rows + groups - 1) / groups)), block,
-                               0, st, p, RM);
-        }
+            if (rows < kMergeRows)
+                hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, true, STAT>), dim3((unsigned)rows), block, 0, st, p, RM);
+            else
+                hipLaunchKernelGGL((cache8_merge_kernel<DP, BF, TILES, false, STAT>), dim3((unsigned)((rows + groups - 1) / groups)), block,
+                                   0, st, p, RM);
+        };
+        if (p.stat)
+            launch(std::true_type{});
+        else
+            launch(std::false_type{});
     };
     auto rows = [&](auto dp, auto rt, auto bf) {
         constexpr int DP = decltype(dp)::value, RT = decltype(rt)::value;
@@ -350,18 +356,25 @@ int attend8(const kitty_cache8 *cache, const kitty_cache8_attention_args *args, 
                 return;
             }
         }
-        if constexpr (DP <= 128 && RT <= 2) {
-            if (pl.direct && p.c.D == DP)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true, kPlain>), pairs, waves, 0, st, p);
-            else if (pl.direct)
-                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true, kPlain>), pairs, waves, 0, st, p);
-            if (pl.direct)
-                return;
-        }
-        if (p.c.D == DP)
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, false, kPlain>), runs, block, 0, st, p);
+        auto launch = [&](auto mode) {
+            constexpr int MODE = decltype(mode)::value;
+            if constexpr (DP <= 128 && RT <= 2 && !(RT == 1 && MODE == kStat)) {   // (plan8: those are split)
+                if (pl.direct && p.c.D == DP)
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, true, MODE>), pairs, waves, 0, st, p);
+                else if (pl.direct)
+                    hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, true, MODE>), pairs, waves, 0, st, p);
+                if (pl.direct)
+                    return;
+            }
+            if (p.c.D == DP)
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, false, false, MODE>), runs, block, 0, st, p);
+            else
+                hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, false, MODE>), runs, block, 0, st, p);
+        };
+        if (p.stat)
+            launch(std::integral_constant<int, kStat>{});
         else
-            hipLaunchKernelGGL((cache8_rows_kernel<DP, RT, BF, true, false, kPlain>), runs, block, 0, st, p);
+            launch(std::integral_constant<int, kPlain>{});
     };
     auto go = [&](auto dp, auto bf) {
         constexpr int DP = decltype(dp)::value;

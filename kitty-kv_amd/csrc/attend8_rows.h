@@ -372,12 +372,12 @@ __device__ __forceinline__ void weigh_scores4(const float *scores, int rows, con
 //
 // Workgroup wg of the n_wg that share the work.
 // kScores: a stream of reads with writes in it runs at a copy's rate, though the scores of
-// four rows are a sixteenth of its bytes: 16 x 32,768 tokens 231 us, 174 with the stores
-// dropped, 179 with all of a pair's to the same 4 KB; cache hints change nothing.  So a
+// four rows are a sixteenth of its bytes: 16 x 32,768 tokens 229 us, 168 with the stores
+// dropped (all of a pair's to the same 4 KB: 5 more; cache hints change nothing).  So a
 // wave's scores wait in LDS, in what is its part of o afterwards, and leave in bursts, which
-// workgroups with equal runs have at about the same time: 210 us.  Bytes that wait: the
+// workgroups with equal runs have at about the same time: 203 us.  Bytes that wait: the
 // whole call 217 us at 20,064 (what two workgroups a CU allow), 218 at 16,896, 228 at
-// 12,288, 234 at 8,448 and 246 unless they wait.
+// 12,288, 234 at 8,448 and 246 unless they wait (another card: 222 and 249).
 constexpr int kStage = 16896;
 
 // Rows of a wave's part of o.
@@ -398,15 +398,14 @@ template <int DP, int RT, bool BF16, bool CUT, bool DIRECT, int MODE>
 __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, RowLds<DP, RT, DIRECT, MODE> &lds)
 {
     constexpr bool SHARED = MODE == kShared, SCORES = MODE == kScores;
-    constexpr bool STAT = !(DIRECT && RT == 1 && MODE == kPlain);   // calls that want it take another instance (plan8)
     constexpr int RM = 16 * RT, CB = DP / 16, NW = row_waves(RT, DIRECT), NB = NW == 16 ? 1 : 2, STRIDE = 32 * NW;
     auto &lds_o = lds.o;
     auto &lds_ml = lds.ml;
     const int lane = threadIdx.x & 63, g = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int per_seq = p.c.H * p.nrb;   // SHARED: of a prefix
     Run8 R;
     if constexpr (DIRECT) {
-        const int per_seq = p.c.H * p.nrb;
         R.b = wg / per_seq;
         R.pre = 0, R.start = 0, R.u = wg - R.b * per_seq, R.u1 = R.u + 1;
     } else {
@@ -422,8 +421,14 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         int item = u, seg = units, tile = 0, tile1 = tiles;                     // seg: units of this run's part
         bool first = true, last_part = true;                                    // whether it has the first and last tile
         if constexpr (!DIRECT) {
-            const int per_seq = items8<SHARED>(p, b);
-            if (u >= pre + units * per_seq) {
+            if constexpr (SHARED) {
+                const int items = items8<true>(p, b);
+                if (u >= pre + units * items) {
+                    pre += units * items;
+                    ++b;
+                    continue;
+                }
+            } else if (u >= pre + units * per_seq) {
                 pre += units * per_seq;
                 ++b;
                 continue;
@@ -438,8 +443,10 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
             first = off <= R.start, last_part = off + seg == units;
             tile = max(off - R.start, 0), tile1 = off + seg - R.start;
         }
-        const int nrb = SHARED && !sq.prefix ? 1 : p.nrb, kh = item / nrb, rb = item - kh * nrb, r0 = rb * RM;
-        const int at = DIRECT ? 0 : first_item8<SHARED>(p, b) + item;
+        int nrb = p.nrb;
+        if constexpr (SHARED)
+            nrb = sq.prefix ? nrb : 1;
+        const int kh = item / nrb, rb = item - kh * nrb, r0 = rb * RM;
         const int t_lo = r0 / p.gq, t_hi = min((r0 + RM - 1) / p.gq, sq.tq - 1);   // query tokens of the block
         int vis_min = visible8(p, sq, t_lo), vis_max = sq.bad || t_hi < t_lo ? 0 : visible8(p, sq, t_hi);
 
@@ -448,9 +455,11 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         for (int rt = 0; rt < RT; ++rt) {
             const Row8 row = row8<SHARED>(p, sq, b, kh, r0 + 16 * rt + n);
             W.vis[rt] = row.vis;
-            if (SHARED && sq.prefix) {
-                vis_min = rt == 0 ? sq.n : vis_min;
-                vis_min = row.real ? min(vis_min, row.vis) : vis_min;
+            if constexpr (SHARED) {
+                if (sq.prefix) {
+                    vis_min = rt == 0 ? sq.n : vis_min;
+                    vis_min = row.real ? min(vis_min, row.vis) : vis_min;
+                }
             }
             W.m[rt] = kLowest;
             W.l[rt] = 0.0f;
@@ -466,12 +475,14 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
             for (int dt = 0; dt < CB; ++dt)
                 W.o[rt][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         }
-        if (SHARED && sq.prefix) {
-            vis_max = sq.bad ? 0 : sq.n;
+        if constexpr (SHARED) {
+            if (sq.prefix) {
+                vis_max = sq.bad ? 0 : sq.n;
 #pragma unroll
-            for (int off = 1; off < 16; off <<= 1)
-                vis_min = min(vis_min, __shfl_xor(vis_min, off));
-            vis_min = __builtin_amdgcn_readfirstlane(vis_min);
+                for (int off = 1; off < 16; off <<= 1)
+                    vis_min = min(vis_min, __shfl_xor(vis_min, off));
+                vis_min = __builtin_amdgcn_readfirstlane(vis_min);
+            }
         }
         const int lg = p.c.lg;
         const uint8_t *kp = p.c.key + kh * p.c.key_s_head, *vp = p.c.value + kh * p.c.value_s_head;
@@ -509,102 +520,138 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                                          bad ? 1.0f : __builtin_bit_cast(float, (uint32_t)(sc >> 32)));   // page 0's may be no number
             }
         };
-        // a KV head's scores are at most 1 GiB
+        // The wave's steps.  A ring of NB steps' codes, NB - 1 in flight while one is computed;
+        // the page ids of the next load are fetched a step before it.  Loads past the wave's
+        // last step repeat that step's: a branch around them would make every wait one for
+        // all loads.
         const int rows_all = p.gq * p.T;
-        const uint32_t sc_step = 64 * rows_all, sc_bytes = SCORES ? (uint32_t)(p.sc_cap * rows_all * 4) : 0;
-        const __amdgpu_buffer_rsrc_t scores = __builtin_amdgcn_make_buffer_rsrc(
-            SCORES ? (void *)(p.scores + (int64_t)(b * p.c.H + kh) * rows_all * p.sc_cap) : nullptr, 0, sc_bytes, 0x00027000);
-        // The wave's steps from token `tok` to `end`, of pages table[0 .. last].
-        // A ring of NB steps' codes, NB - 1 in flight while one is computed; the page
-        // ids of the next load are fetched a step before it.  Loads past the wave's
-        // last step repeat that step's: a branch around them would make every wait
-        // one for all loads.
-        auto stream = [&](const int32_t *table, int last, int vis_min, int vis_max, int tok, int end) {
-            if (tok >= end)
-                return;
+        Seq8 before{};
+        auto in_prefix = [&](int t) {   // DIRECT and SHARED: tokens of the prefix that row t sees
+            if (before.bad || sq.bad || t >= sq.tq)
+                return 0;
+            return p.causal ? max(before.n + min(sq.n - sq.tq + t + 1, 0), 0) : before.n;
+        };
+        if constexpr (MODE == kPlain) {
+            // (written out: as the lambda below, with the test for stat in the epilogue, calls that are
+            // split took 0.3 to 0.8 us more: 4 x 38,933 tokens of 8 / 2 heads 25.4 us / 24.9)
+            const int32_t *table = p.table + b * p.bt_stride;
+            const int last = (sq.n - 1) >> lg, end = min(tile1 * kUnit, vis_max);
             auto ids = [&](int tok, int (&id)[2]) {
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf)
                     id[hf] = uniform_load(table + min((tok + 16 * hf) >> lg, last));
             };
-            const int final = tok + (end - 1 - tok) / STRIDE * STRIDE;
-            RowBuf<DP, RT> ring[NB];
-            int id[NB][2];
+            int tok = tile * kUnit + 32 * wave;
+            if (tok < end) {
+                const int final = tok + (end - 1 - tok) / STRIDE * STRIDE;
+                RowBuf<DP, RT> ring[NB];
+                int id[NB][2];
 #pragma unroll
-            for (int j = 0; j < NB; ++j)
-                ids(min(tok + j * STRIDE, final), id[j]);
+                for (int j = 0; j < NB; ++j)
+                    ids(min(tok + j * STRIDE, final), id[j]);
 #pragma unroll
-            for (int j = 0; j < NB - 1; ++j)
-                load(min(tok + j * STRIDE, final), id[j], ring[j]);
-            bool more = true;
-            // LEAVE: scores go to memory as they come (1) or in bursts (2); `held` steps wait
-            constexpr int LEAVE = !SCORES ? 0 : DIRECT ? 1 : 2;
-            unsigned char *stage = (unsigned char *)&lds_o[wave][0][0];
-            const int each = 2 * sc_step, most = (int)sizeof(lds_o[0]) / each;
-            int held = 0;
-            auto burst = [&](int tok) {    // tok: where the step behind them begins
-                __builtin_amdgcn_wave_barrier();
-                const int per = each / 16, first = tok - held * STRIDE;
-                for (int c = lane; c < held * per; c += 64) {
-                    const int s = c / per, from = first + s * STRIDE;
-                    __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4 *)(stage + 16 * c), scores,
-                                                           from < p.sc_cap ? (uint32_t)(from >> 4) * sc_step + 16 * (c - s * per) : 1u << 31,
-                                                           0, 0);
-                }
-                __builtin_amdgcn_wave_barrier();
-                held = 0;
-            };
-            while (more) {
+                for (int j = 0; j < NB - 1; ++j)
+                    load(min(tok + j * STRIDE, final), id[j], ring[j]);
+                bool more = true;
+                while (more) {
 #pragma unroll
-                for (int j = 0; j < NB; ++j) {
-                    if (!more)
-                        break;
-                    load(min(tok + (NB - 1) * STRIDE, final), id[NB - 1], ring[(j + NB - 1) % NB]);
-                    ids(min(tok + NB * STRIDE, final), id[NB - 1]);
-                    uint32_t at = 0;
-                    if constexpr (LEAVE == 1)
-                        at = n < rows_all && tok < p.sc_cap ? (uint32_t)(tok >> 4) * sc_step + 64 * n + 16 * g : 1u << 31;
-                    else if constexpr (LEAVE == 2)
-                        at = n < rows_all ? held * each + 64 * n + 16 * g : 1u << 31;
-                    row_step<DP, RT, BF16, LEAVE>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min, scores, stage, at, sc_step);
-                    tok += STRIDE;
-                    more = tok < end;
-                    if constexpr (LEAVE == 2) {
-                        if (++held == most || !more)
-                            burst(tok);
+                    for (int j = 0; j < NB; ++j) {
+                        if (!more)
+                            break;
+                        load(min(tok + (NB - 1) * STRIDE, final), id[NB - 1], ring[(j + NB - 1) % NB]);
+                        ids(min(tok + NB * STRIDE, final), id[NB - 1]);
+                        row_step<DP, RT, BF16, 0>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min, __builtin_amdgcn_make_buffer_rsrc(nullptr, 0, 0, 0), nullptr, 0, 0);
+                        tok += STRIDE;
+                        more = tok < end;
                     }
                 }
             }
-        };
-        // DIRECT and SHARED: the prefix's tokens first, then the sequence's own
-        Seq8 before{};
-        auto in_prefix = [&](int t) {   // tokens of the prefix that row t sees
-            if (before.bad || sq.bad || t >= sq.tq)
-                return 0;
-            return p.causal ? max(before.n + min(sq.n - sq.tq + t + 1, 0), 0) : before.n;
-        };
-        if constexpr (DIRECT && SHARED) {
-            const int f = b / p.per;
-            before.n = p.prefix_lens[f];
-            before.bad = before.n < 0 || before.n > (int64_t)p.prefix_pages << lg || (before.n > 0 && p.c.num_pages == 0);
-            int own[RT], least = max(before.n, 0);
+        } else {
+            // a KV head's scores are at most 1 GiB
+            const uint32_t sc_step = 64 * rows_all, sc_bytes = SCORES ? (uint32_t)(p.sc_cap * rows_all * 4) : 0;
+            const __amdgpu_buffer_rsrc_t scores = __builtin_amdgcn_make_buffer_rsrc(
+                SCORES ? (void *)(p.scores + (int64_t)(b * p.c.H + kh) * rows_all * p.sc_cap) : nullptr, 0, sc_bytes, 0x00027000);
+            // from token `tok` to `end`, of pages table[0 .. last]
+            auto stream = [&](const int32_t *table, int last, int vis_min, int vis_max, int tok, int end) {
+                if (tok >= end)
+                    return;
+                auto ids = [&](int tok, int (&id)[2]) {
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const int t = (16 * rt + n) / p.gq;
-                own[rt] = W.vis[rt];
-                W.vis[rt] = in_prefix(t);
-                least = t < sq.tq ? min(least, W.vis[rt]) : least;
+                    for (int hf = 0; hf < 2; ++hf)
+                        id[hf] = uniform_load(table + min((tok + 16 * hf) >> lg, last));
+                };
+                const int final = tok + (end - 1 - tok) / STRIDE * STRIDE;
+                RowBuf<DP, RT> ring[NB];
+                int id[NB][2];
+#pragma unroll
+                for (int j = 0; j < NB; ++j)
+                    ids(min(tok + j * STRIDE, final), id[j]);
+#pragma unroll
+                for (int j = 0; j < NB - 1; ++j)
+                    load(min(tok + j * STRIDE, final), id[j], ring[j]);
+                bool more = true;
+                // LEAVE: scores go to memory as they come (1) or in bursts (2); `held` steps wait
+                constexpr int LEAVE = !SCORES ? 0 : DIRECT ? 1 : 2;
+                unsigned char *stage = (unsigned char *)&lds_o[wave][0][0];
+                const int each = 2 * sc_step, most = (int)sizeof(lds_o[0]) / each;
+                int held = 0;
+                auto burst = [&](int tok) {    // tok: where the step behind them begins
+                    __builtin_amdgcn_wave_barrier();
+                    const int per = each / 16, first = tok - held * STRIDE;
+                    for (int c = lane; c < held * per; c += 64) {
+                        const int s = c / per, from = first + s * STRIDE;
+                        __builtin_amdgcn_raw_buffer_store_b128(*(const u32x4 *)(stage + 16 * c), scores,
+                                                               from < p.sc_cap ? (uint32_t)(from >> 4) * sc_step + 16 * (c - s * per) : 1u << 31,
+                                                               0, 0);
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                    held = 0;
+                };
+                while (more) {
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) {
+                        if (!more)
+                            break;
+                        load(min(tok + (NB - 1) * STRIDE, final), id[NB - 1], ring[(j + NB - 1) % NB]);
+                        ids(min(tok + NB * STRIDE, final), id[NB - 1]);
+                        uint32_t at = 0;
+                        if constexpr (LEAVE == 1)
+                            at = n < rows_all && tok < p.sc_cap ? (uint32_t)(tok >> 4) * sc_step + 64 * n + 16 * g : 1u << 31;
+                        else if constexpr (LEAVE == 2)
+                            at = n < rows_all ? held * each + 64 * n + 16 * g : 1u << 31;
+                        row_step<DP, RT, BF16, LEAVE>(W, ring[j], tok, vis_max, p.cs, g, tok + 32 > vis_min, scores, stage, at, sc_step);
+                        tok += STRIDE;
+                        more = tok < end;
+                        if constexpr (LEAVE == 2) {
+                            if (++held == most || !more)
+                                burst(tok);
+                        }
+                    }
+                }
+            };
+            if constexpr (DIRECT && SHARED) {
+                const int f = b / p.per;
+                before.n = p.prefix_lens[f];
+                before.bad = before.n < 0 || before.n > (int64_t)p.prefix_pages << lg || (before.n > 0 && p.c.num_pages == 0);
+                int own[RT], least = max(before.n, 0);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    const int t = (16 * rt + n) / p.gq;
+                    own[rt] = W.vis[rt];
+                    W.vis[rt] = in_prefix(t);
+                    least = t < sq.tq ? min(least, W.vis[rt]) : least;
+                }
+#pragma unroll
+                for (int off = 1; off < 16; off <<= 1)
+                    least = min(least, __shfl_xor(least, off));
+                const int most = before.bad || sq.bad || sq.tq <= 0 ? 0 : before.n;
+                stream(p.prefix_table + f * p.pt_stride, (before.n - 1) >> lg, __builtin_amdgcn_readfirstlane(least), most, 32 * wave, most);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+                    W.vis[rt] = own[rt];
             }
-#pragma unroll
-            for (int off = 1; off < 16; off <<= 1)
-                least = min(least, __shfl_xor(least, off));
-            const int most = before.bad || sq.bad || sq.tq <= 0 ? 0 : before.n;
-            stream(p.prefix_table + f * p.pt_stride, (before.n - 1) >> lg, __builtin_amdgcn_readfirstlane(least), most, 32 * wave, most);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-                W.vis[rt] = own[rt];
+            stream(table8<SHARED>(p, sq, b), (sq.n - 1) >> lg, vis_min, vis_max, tile * kUnit + 32 * wave, min(tile1 * kUnit, vis_max));
         }
-        stream(table8<SHARED>(p, sq, b), (sq.n - 1) >> lg, vis_min, vis_max, tile * kUnit + 32 * wave, min(tile1 * kUnit, vis_max));
 
         // the waves' rows joined
 #pragma unroll
@@ -622,8 +669,12 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         __syncthreads();
         const bool whole = first && last_part;
         // a run may hold the whole of any number of items, and has a part of at most two others
-        const int slot = SHARED && whole ? 2 * p.n_wg + at : 2 * wg + (u == u0 ? 0 : 1);
-        const int rows = min(RM, rows8<SHARED>(p, sq, b) - r0);
+        int slot = 2 * wg + (u == u0 ? 0 : 1), rows = min(RM, p.gq * p.T - r0), at = b * per_seq + item;
+        if constexpr (SHARED) {
+            at = first_item8<true>(p, b) + item;
+            slot = whole ? 2 * p.n_wg + at : slot;
+            rows = min(RM, rows8<true>(p, sq, b) - r0);
+        }
         if (!DIRECT && first && threadIdx.x == 0)
             p.ws_tab[at] =
                 whole ? make_int2(SHARED ? slot : -1, SHARED ? -1 : 0)
@@ -652,8 +703,10 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
                 continue;
             }
             const int t = (r0 + r) / p.gq, h = kh * p.gq + (r0 + r) - t * p.gq;
-            const bool bad = sq.bad || (DIRECT && SHARED && before.bad);
-            const bool none = !bad && visible8(p, sq, t) == 0 && !(DIRECT && SHARED && in_prefix(t) > 0);
+            bool bad = sq.bad, sees = visible8(p, sq, t) != 0;
+            if constexpr (DIRECT && SHARED)
+                bad |= before.bad, sees |= in_prefix(t) > 0;
+            const bool none = !bad && !sees;
             const float inv = bad ? __builtin_nanf("") : none ? 0.0f : 1.0f / l;
             if (none)   // steps that no row masks went into its sums too, NaN among them
                 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -664,7 +717,7 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
             if (ch == 0 && p.lse)
                 p.lse[((int64_t)b * p.Hq + h) * p.T + t] =
                     bad ? __builtin_nanf("") : none ? -__builtin_inff() : (m + __builtin_log2f(l)) / kLog2e;
-            if (STAT && ch == 0 && p.stat)
+            if (MODE != kPlain && ch == 0 && p.stat)
                 p.stat[((int64_t)b * p.Hq + h) * p.T + t] = make_float2(m, inv);
             if (SCORES && DIRECT && ch == 0)
                 lds.stat[r] = make_float2(m, inv);
