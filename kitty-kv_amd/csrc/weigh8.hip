@@ -244,8 +244,8 @@ __global__ __launch_bounds__(256) void cache8_weigh_sum_kernel(Weigh8 w)
 // Up to 16 rows the scores are kept instead: reading and writing them is 8 bytes a row and
 // token where reading the keys again is head_dim, and costs products as well.  A gibibyte
 // of them at most, or of the parts' sums.  Where one launch of the row kernel has all of a
-// head's rows and tokens, it adds to the weights itself (4 rows of 512 tokens of 16 sequences
-// 8.1 us, 14.5 split; one sequence of 1,024 11.1 / 10.6).
+// head's rows and tokens, it adds to the weights itself (4 rows of 16 sequences of 512 tokens
+// 8.5 us, 14.9 split, of 1,000 13.6 / 18.1; one sequence of 512 8.1 / 11.3, of 1,024 11.4 / 11.4).
 struct WeighPlan8 {
     bool scores;
     int64_t cap;

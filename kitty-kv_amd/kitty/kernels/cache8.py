@@ -398,7 +398,9 @@ class Cache8:
         tokens of its own in the pages of block_table's row b (lens[b] may be 0; the first
         of them is row 0 of its first page).  causal: the q_lens[b] queries of sequence b
         are the last tokens of the two together; otherwise every query sees all of both.
-        Results are ``attend``'s over the two in one table but for rounding.  out may be q
+        Results are ``attend``'s over the two in one table but for rounding; for bfloat16 and
+        more than 64 rows of a prefix (its sequences' queries times the group's heads) that
+        of the softmax weights is to 11 bits, a tenth of the output's own.  out may be q
         or lie in its memory in any way.  Parts of the rows take up to a gibibyte beside
         it; calls of more run in pieces."""
         if calls_followed():
