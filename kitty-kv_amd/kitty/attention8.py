@@ -33,7 +33,10 @@ from .kernels.ops import stage_i32
 
 
 class KittyCache8:
-    """8-bit pools of `num_layers` layers and the sequences in them."""
+    """8-bit pools of `num_layers` layers and the sequences in them.
+
+    It counts their tokens and pages: what `layers[i]` writes or evicts beside it, it
+    does not know of."""
 
     def __init__(self, config: KittyConfig, num_layers: Optional[int] = None) -> None:
         self.config = config
