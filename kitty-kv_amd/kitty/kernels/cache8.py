@@ -20,6 +20,7 @@ import math
 import struct
 from typing import Optional, Tuple, Union
 
+import numpy as np
 import torch
 
 from .. import _hip
@@ -73,6 +74,23 @@ _written = torch.autograd.graph.increment_version      # what torch's own writes
 def _span(t: torch.Tensor) -> int:
     """Bytes from a tensor's first element to behind its last."""
     return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def _rows_apart(t: torch.Tensor) -> bool:
+    """Whether no two rows (of contiguous elements, the last dimension) share memory."""
+    dims, span = sorted((s, n) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1), t.shape[-1]
+    if t.numel() == 0:
+        return True
+    nested = True
+    for s, n in dims:
+        nested = nested and s >= span
+        span += (n - 1) * s
+    if nested:
+        return True
+    starts = np.zeros(1, np.int64)      # rows laid between each other, or over
+    for s, n in dims:
+        starts = (starts[:, None] + s * np.arange(n)).ravel()
+    return bool((np.diff(np.sort(starts)) >= t.shape[-1]).all())
 
 
 class Cache8:
@@ -249,7 +267,7 @@ class Cache8:
                 for t in out:
                     _need(tuple(t.shape) == shape and t.dtype == k.dtype and t.dtype in _SRC and t.stride(3) == 1,
                           f"out must be two {shape} tensors of one type with contiguous channels")
-                    _need(torch._debug_has_internal_overlap(t) != 1, "out must not share memory between its rows")
+                    _need(_rows_apart(t), "out must not share memory between its rows")
                     self._here("out", t)
                 _need(tokens == 0 or B == 0 or k.data_ptr() != v.data_ptr(), "out must not be the same memory twice")
                 dtype = k.dtype
@@ -321,7 +339,7 @@ class Cache8:
             if out is not None:
                 _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(3) == 1,
                       "out must have q's shape and dtype and contiguous channels")
-                _need(torch._debug_has_internal_overlap(out) != 1, "out must not share memory between its rows")
+                _need(_rows_apart(out), "out must not share memory between its rows")
                 self._here("out", out)
             if B == 0 or T == 0 or not self._on_device:
                 if out is None:
@@ -383,7 +401,7 @@ class Cache8:
         if out is not None:
             _need(out.shape == q.shape and out.dtype == q.dtype and out.stride(3) == 1,
                   "out must have q's shape and dtype and contiguous channels")
-            _need(torch._debug_has_internal_overlap(out) != 1, "out must not share memory between its rows")
+            _need(_rows_apart(out), "out must not share memory between its rows")
             self._here("out", out)
         return scale
 
@@ -511,7 +529,7 @@ class Cache8:
             self._i32("q_lens", q_lens, B, optional=True)
             self._check_weights(weights, B)
             _need(not weights.is_neg(), "weights must not be a negated view")
-            _need(torch._debug_has_internal_overlap(weights) != 1, "weights must not share memory between sequences or heads")
+            _need(_rows_apart(weights), "weights must not share memory between sequences or heads")
             _need(0 <= max_tokens < 1 << 31, "max_tokens must be in [0, 2^31)")
             if B == 0 or T == 0 or not self._on_device:
                 o = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out is None else out
