@@ -189,7 +189,7 @@ def test_many_pages(dev, at, place):
 
 
 @pytest.mark.parametrize("dev", DEVICES)
-@pytest.mark.parametrize("B,H,W,N", [(4500, 1, 1, 3), (9000, 2, 1, 3), (4096, 1, 1, 2), (5000, 1, 2, 20), (1500, 1, 120, 1900), (1, 3, 4090, 65000)])
+@pytest.mark.parametrize("B,H,W,N", [(4100, 1, 1, 3), (2100, 2, 1, 3), (2048, 1, 1, 2), (1100, 1, 2, 20), (500, 1, 120, 1900), (1, 3, 4090, 65000)])
 def test_many_sequences(dev, B, H, W, N):
     """Of few tokens and of many, whose written pages are more than fit one table, or than the weights' memory has
     room for; some of them clash."""
