@@ -259,12 +259,9 @@ __device__ __forceinline__ int items8(const Attend8 &p, int i)
 {
     return p.c.H * (SHARED && p.e0 + i >= p.F ? 1 : p.nrb);
 }
-template <bool SHARED>
-__device__ __forceinline__ int first_item8(const Attend8 &p, int i)
+__device__ __forceinline__ int first_item8(const Attend8 &p, int i)   // SHARED
 {
-    if (SHARED && p.e0 + i >= p.F)
-        return p.item0 + (p.e0 + i - p.F) * p.c.H;
-    return i * p.c.H * p.nrb;
+    return p.e0 + i >= p.F ? p.item0 + (p.e0 + i - p.F) * p.c.H : i * p.c.H * p.nrb;
 }
 
 template <bool SHARED>
@@ -671,7 +668,7 @@ __device__ __forceinline__ void rows_run(const Attend8 &p, int wg, int n_wg, Row
         // a run may hold the whole of any number of items, and has a part of at most two others
         int slot = 2 * wg + (u == u0 ? 0 : 1), rows = min(RM, p.gq * p.T - r0), at = b * per_seq + item;
         if constexpr (SHARED) {
-            at = first_item8<true>(p, b) + item;
+            at = first_item8(p, b) + item;
             slot = whole ? 2 * p.n_wg + at : slot;
             rows = min(RM, rows8<true>(p, sq, b) - r0);
         }
